@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define PK_ABI_VERSION 10
+#define PK_ABI_VERSION 11
 
 enum pk_dtype { PK_DTYPE_F32 = 0, PK_DTYPE_F16 = 1, PK_DTYPE_BF16 = 2 };
 
@@ -755,6 +755,155 @@ int pk_pool_reset_all(pk_pool* pool);
 int pk_pool_free_pages(const pk_pool* pool);
 int pk_pool_slot_info(const pk_pool* pool, int32_t slot, int64_t* appended, int32_t* ring_out);
 int pk_pool_free_list(const pk_pool* pool, int32_t* out, int32_t capacity);
+
+/* ---------------------------------------------------------------------------
+ * pk_page_step -- the block-table rows and the slot map of a step, built on the GPU
+ * from the streams' slots and frame counts; the page pool is kept in device memory.
+ * pk_pool_advance's counterpart for a step without host work (a recorded one), with
+ * its rings, rows and FIFO order, entry for entry.  No counterpart in the reference
+ * (its window shift is parakeet/modules/cache.py:36-45).
+ * Stream b of the batch appends n_b = lengths[b] frames, held within [0, chunk]
+ * (lengths NULL: chunk), to slot slots[b]:
+ *   the pages that slid out of its window of left + chunk frames go to the back of
+ *   the queue, pages for its frames come from the front, streams in order;
+ *   rows[b]        = {A, ring[0 .. M-1]}, A the frames before the step (as
+ *                    pk_paged_layout.rows; M = (left + chunk + page_size - 2) / page_size + 1)
+ *   slot_map[b][t] = page * page_size + row of the page for frame t < n_b, else -1
+ * A slot out of range, or named earlier in the call, is absent: rows {0, -1 ...},
+ * slot_map -1, nothing changed.
+ * queue    : int32 [num_pages], a ring of free pages; head: int32 [2] = {first
+ *            entry, entries}; appended: int64 [num_slots], frames of each slot (below
+ *            2^31); ring: int32 [num_slots][M], -1 where no page is held.  A new pool
+ *            has queue 0 .. num_pages - 1 (any order), head {0, num_pages}, appended
+ *            0, ring -1.  num_pages >= num_slots * M, so no step runs out of pages.
+ * reset    : != 0: give every page of the slots back and set appended to 0
+ *            (pk_pool_reset_slot in turn); lengths, rows and slot_map are not read.
+ * Calls on one pool are ordered by the caller (one stream, or events).
+ * num_pages * page_size < 2^31; num_slots <= PK_PAGE_STEP_MAX_SLOTS.
+ */
+#define PK_PAGE_STEP_MAX_SLOTS 131072
+typedef struct pk_page_step_args {
+  int32_t device;
+  int32_t batch;
+  int32_t num_slots;
+  int32_t num_pages;
+  int32_t page_size; /* frames per page, power of two */
+  int32_t left;
+  int32_t chunk;
+  int32_t reset;
+  int32_t* queue;
+  int32_t* head;
+  int64_t* appended;
+  int32_t* ring;
+  const int32_t* slots;
+  const int32_t* lengths;
+  int32_t* rows;
+  int32_t rows_stride;
+  int32_t* slot_map;
+  int64_t slot_map_stride;
+} pk_page_step_args;
+int pk_page_step(const pk_page_step_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_kv_append_slots -- pk_kv_append through a slot map: K and V frames to the
+ * places that slot_map names (page * page_size + row of the page), for streams
+ * that append different numbers of frames, padded or packed one after another.
+ * slot_map : int32 [batch][chunk], batch stride slot_map_stride_b; an entry below 0 or
+ *            past the layer's pages is skipped (padding, rows behind the last
+ *            stream); the others are distinct.
+ * key/value: [batch][chunk][d_model], as pk_kv_append's; packed rows are batch 1.
+ * pages    : rows is not read.
+ */
+typedef struct pk_kv_append_slots_args {
+  int32_t dtype;
+  int32_t device;
+  pk_paged_layout pages;
+  int32_t layer;
+  int32_t batch;
+  int32_t chunk;
+  const void* key;
+  int64_t key_stride_b;
+  int64_t key_stride_t;
+  const void* value;
+  int64_t value_stride_b;
+  int64_t value_stride_t;
+  const int32_t* slot_map;
+  int64_t slot_map_stride_b;
+} pk_kv_append_slots_args;
+int pk_kv_append_slots(const pk_kv_append_slots_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_adapter_plan -- the rows of a batch grouped by low-rank adapter, for
+ * pk_adapter_linear; one plan serves every layer of a step.  No counterpart in the
+ * reference.  Stream b's `frames` rows (b * frames + t) have adapter ids[b]; a number
+ * outside [0, num_adapters) is no adapter.
+ * order      : int32 [batch * frames] rows by adapter, in their own order within one,
+ *              rows without an adapter last
+ * sorted_ids : int32 [batch * frames] adapter of the row at each position, -1 none
+ * tiles      : int32 [max_tiles][4] = {adapter, first position, rows, 0}: up to 32
+ *              rows of one adapter, by adapter; {-1, 0, 0, 0} past the last one.
+ *              max_tiles >= pk_adapter_plan_tiles(...).
+ * num_adapters <= PK_ADAPTER_MAX.
+ */
+#define PK_ADAPTER_MAX 512
+#define PK_ADAPTER_MAX_RANK 128
+typedef struct pk_adapter_plan_args {
+  int32_t device;
+  int32_t batch;
+  int32_t frames;
+  int32_t num_adapters;
+  const int32_t* ids;
+  int32_t* order;
+  int32_t* sorted_ids;
+  int32_t* tiles;
+  int32_t max_tiles;
+} pk_adapter_plan_args;
+int pk_adapter_plan_tiles(int32_t batch, int32_t frames, int32_t num_adapters);
+int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_adapter_linear -- a linear layer with each row's low-rank adapter beside it:
+ *   out = act(x weight^T + bias + scale[g] (x a[g]^T) b[g]^T), g the row's adapter
+ * (rows without one: act(x weight^T + bias)).  fp32 accumulation, one rounding of
+ * the output; x a[g]^T is kept to twice the storage type's mantissa between the two
+ * products.  No counterpart in the reference (the projections are
+ * parakeet/modules/feedforward.py:20-26, attention.py:92,122).
+ * x [rows][k], weight [n][k], out [rows][n]: row strides in elements, rows 16-byte
+ * aligned; bias [n] or NULL; a [num_adapters][rank][k], b [num_adapters][n][rank]
+ * contiguous; scale fp32 [num_adapters].  order, ids, tiles: pk_adapter_plan's for
+ * these rows.  workspace: pk_adapter_workspace_bytes(rows, rank), 16-byte aligned.
+ * n and k multiples of 64, rank of 8 and at most PK_ADAPTER_MAX_RANK.
+ * activation: PK_ACT_NONE or PK_ACT_SILU.  fp32 has no product with weight here: out
+ * holds the projection with its bias on entry, weight and bias are NULL.
+ * out overlaps no operand.
+ */
+typedef struct pk_adapter_linear_args {
+  int32_t dtype;
+  int32_t device;
+  int32_t rows;
+  int32_t n;
+  int32_t k;
+  int32_t rank;
+  int32_t num_adapters;
+  int32_t activation;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;
+  const void* a;
+  const void* b;
+  const float* scale;
+  const int32_t* order;
+  const int32_t* ids;
+  const int32_t* tiles;
+  int32_t max_tiles;
+  void* workspace;
+  void* out;
+  int64_t out_stride;
+} pk_adapter_linear_args;
+int64_t pk_adapter_workspace_bytes(int32_t rows, int32_t rank);
+int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
  * pk_hbm_read_probe -- measurement only; it has no counterpart in the reference.

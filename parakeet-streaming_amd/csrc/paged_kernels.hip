@@ -1722,6 +1722,39 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const CopyK<ST> p) {
   }
 }
 
+// K/V rows to the places that a slot map names (entries outside the layer's pages are
+// skipped).
+template <typename ST>
+struct SlotsK {
+  ST* kp;  // layer slab
+  ST* vp;
+  PagesK pg;
+  const ST* k;
+  const ST* v;
+  int64_t k_sb, k_st, v_sb, v_st;
+  const int32_t* map;
+  int64_t map_sb;
+  int32_t B, T, nchunk;
+};
+
+template <typename ST>
+__global__ void __launch_bounds__(256) kv_append_slots_kernel(const SlotsK<ST> p) {
+  constexpr int VEC = Tr<ST>::VEC;
+  const int64_t total = (int64_t)p.B * p.T * p.nchunk;
+  const uint32_t places = (uint32_t)p.pg.num_pages << p.pg.page_shift;  // below 2^31, checked on the host
+  for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * blockDim.x) {
+    const int c = (int)(idx % p.nchunk);
+    const int64_t bt = idx / p.nchunk;
+    const int t = (int)(bt % p.T), b = (int)(bt / p.T);
+    const uint32_t place = (uint32_t)p.map[b * p.map_sb + t];
+    if (place >= places) continue;
+    const int64_t e = (int64_t)(place >> p.pg.page_shift) * p.pg.page_elems +
+                      ((int64_t)(place & ((1u << p.pg.page_shift) - 1u)) << p.pg.cb_shift) + page_col(p.pg, c * VEC);
+    st16(p.kp + e, ld16(p.k + b * p.k_sb + (int64_t)t * p.k_st + c * VEC));
+    st16(p.vp + e, ld16(p.v + b * p.v_sb + (int64_t)t * p.v_st + c * VEC));
+  }
+}
+
 template <typename ST>
 __global__ void __launch_bounds__(256) kv_gather_kernel(const CopyK<ST> p) {
   constexpr int VEC = Tr<ST>::VEC;
@@ -2355,10 +2388,64 @@ int copy_typed(bool gather, const pk_paged_layout& L, int layer, int B, int rows
   return check_launch(what);
 }
 
+template <typename ST>
+int append_slots_typed(const pk_kv_append_slots_args* a, hipStream_t s) {
+  const char* what = "pk_kv_append_slots";
+  constexpr int VEC = Tr<ST>::VEC;
+  if (a->batch < 0 || a->chunk < 0) return fail(PK_ERR_INVALID, "%s: need batch and chunk >= 0", what);
+  if (a->batch == 0 || a->chunk == 0) return PK_OK;
+  SlotsK<ST> p{};
+  pk_paged_layout L = a->pages;
+  L.rows = a->slot_map;  // rows is not read
+  L.rows_stride = L.max_pages + 1;
+  const int rc = pages_view(L, a->layer, VEC, (int)sizeof(ST), what, &p.pg);
+  if (rc != PK_OK) return rc;
+  if ((int64_t)L.num_pages * L.page_size >= (int64_t{1} << 31))
+    return fail(PK_ERR_INVALID, "%s: %d pages of %d frames are past a slot map's 2^31 frames", what, L.num_pages, L.page_size);
+  if (!a->key || !a->value || !aligned16(a->key) || !aligned16(a->value) || !a->slot_map)
+    return fail(PK_ERR_INVALID, "%s: K/V tensors must be non-NULL and 16-byte aligned, slot_map non-NULL", what);
+  const int64_t strides[4] = {a->key_stride_b, a->key_stride_t, a->value_stride_b, a->value_stride_t};
+  for (int64_t st : strides)
+    if (st < 0 || st % VEC != 0)
+      return fail(PK_ERR_INVALID, "%s: strides must be non-negative multiples of %d elements", what, VEC);
+  if (a->slot_map_stride_b < 0) return fail(PK_ERR_INVALID, "%s: slot_map_stride_b < 0", what);
+  const int64_t lo = layer_offset(L, a->layer);
+  p.kp = static_cast<ST*>(L.k_pool) + lo;
+  p.vp = static_cast<ST*>(L.v_pool) + lo;
+  p.k = static_cast<const ST*>(a->key);
+  p.v = static_cast<const ST*>(a->value);
+  p.k_sb = a->key_stride_b;
+  p.k_st = a->key_stride_t;
+  p.v_sb = a->value_stride_b;
+  p.v_st = a->value_stride_t;
+  p.map = a->slot_map;
+  p.map_sb = a->slot_map_stride_b;
+  p.B = a->batch;
+  p.T = a->chunk;
+  p.nchunk = L.d_model / VEC;
+  DeviceGuard dg(a->device);
+  if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
+  const int64_t total = (int64_t)p.B * p.T * p.nchunk;
+  hipLaunchKernelGGL(kv_append_slots_kernel<ST>, dim3(grid_for(total, 256)), dim3(256), 0, s, p);
+  return check_launch(what);
+}
+
 }  // namespace
 }  // namespace pk
 
 extern "C" {
+
+int pk_kv_append_slots(const pk_kv_append_slots_args* a, void* stream) {
+  pk::clear_error();
+  if (!a) return pk::fail(PK_ERR_INVALID, "pk_kv_append_slots: args is NULL");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->dtype) {
+    case PK_DTYPE_F32: return pk::append_slots_typed<float>(a, s);
+    case PK_DTYPE_F16: return pk::append_slots_typed<_Float16>(a, s);
+    case PK_DTYPE_BF16: return pk::append_slots_typed<pk::bf16_t>(a, s);
+    default: return pk::fail(PK_ERR_INVALID, "pk_kv_append_slots: unknown dtype %d", a->dtype);
+  }
+}
 
 int pk_paged_relpos_attn(const pk_attn_args* a, void* stream) {
   pk::clear_error();

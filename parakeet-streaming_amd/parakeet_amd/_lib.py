@@ -15,7 +15,7 @@ from pathlib import Path
 LIB_NAME = "libparakeet_paged.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -37,6 +37,10 @@ PRO_NORM = 1
 PRO_RESIDUAL_NORM = 2
 PRO_RESIDUAL_NORM2 = 3
 PRO_NORM_SILU = 4
+
+PAGE_STEP_MAX_SLOTS = 131072
+ADAPTER_MAX = 512
+ADAPTER_MAX_RANK = 128
 
 PCM_S16 = 0
 PCM_F32 = 1
@@ -375,6 +379,90 @@ class FePlanArgs(ctypes.Structure):
     )
 
 
+class PageStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", c_int32),
+        ("batch", c_int32),
+        ("num_slots", c_int32),
+        ("num_pages", c_int32),
+        ("page_size", c_int32),
+        ("left", c_int32),
+        ("chunk", c_int32),
+        ("reset", c_int32),
+        ("queue", c_void_p),
+        ("head", c_void_p),
+        ("appended", c_void_p),
+        ("ring", c_void_p),
+        ("slots", c_void_p),
+        ("lengths", c_void_p),
+        ("rows", c_void_p),
+        ("rows_stride", c_int32),
+        ("slot_map", c_void_p),
+        ("slot_map_stride", c_int64),
+    ]
+
+
+class KvAppendSlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("pages", PagedLayout),
+        ("layer", c_int32),
+        ("batch", c_int32),
+        ("chunk", c_int32),
+        ("key", c_void_p),
+        ("key_stride_b", c_int64),
+        ("key_stride_t", c_int64),
+        ("value", c_void_p),
+        ("value_stride_b", c_int64),
+        ("value_stride_t", c_int64),
+        ("slot_map", c_void_p),
+        ("slot_map_stride_b", c_int64),
+    ]
+
+
+class AdapterPlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", c_int32),
+        ("batch", c_int32),
+        ("frames", c_int32),
+        ("num_adapters", c_int32),
+        ("ids", c_void_p),
+        ("order", c_void_p),
+        ("sorted_ids", c_void_p),
+        ("tiles", c_void_p),
+        ("max_tiles", c_int32),
+    ]
+
+
+class AdapterLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("rows", c_int32),
+        ("n", c_int32),
+        ("k", c_int32),
+        ("rank", c_int32),
+        ("num_adapters", c_int32),
+        ("activation", c_int32),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("bias", c_void_p),
+        ("a", c_void_p),
+        ("b", c_void_p),
+        ("scale", c_void_p),
+        ("order", c_void_p),
+        ("ids", c_void_p),
+        ("tiles", c_void_p),
+        ("max_tiles", c_int32),
+        ("workspace", c_void_p),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+    ]
+
+
 # name -> (restype, argtypes); exactly the functions include/parakeet_paged.h declares
 SIGNATURES = {
     "pk_kv_append": (c_int, [POINTER(KvAppendArgs), c_void_p]),
@@ -392,6 +480,12 @@ SIGNATURES = {
     "pk_rnnt_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "pk_rnnt_greedy_step": (c_int, [POINTER(RnntArgs), c_void_p]),
     "pk_rnnt_greedy_step_static": (c_int, [POINTER(RnntArgs), c_void_p]),
+    "pk_page_step": (c_int, [POINTER(PageStepArgs), c_void_p]),
+    "pk_kv_append_slots": (c_int, [POINTER(KvAppendSlotsArgs), c_void_p]),
+    "pk_adapter_plan_tiles": (c_int, [c_int32, c_int32, c_int32]),
+    "pk_adapter_plan": (c_int, [POINTER(AdapterPlanArgs), c_void_p]),
+    "pk_adapter_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
     "pk_pool_create": (
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32, POINTER(c_int32), POINTER(c_void_p)],

@@ -1,9 +1,13 @@
-"""Host page pool: FIFO free-page queue and per-slot page rings (C++ side).
+"""Page pools: FIFO free-page queue and per-slot page rings, on the host (C++ side)
+or in device memory.
 
 Replaces the reference's slot pool / dense shift buffers
 (parakeet/engine/scheduler.py:68-104, parakeet/modules/cache.py:8-63): a slot
 owns a ring of ``max_pages`` page ids; each step frees the pages that slid out
-of its window and allocates pages for the new frames.
+of its window and allocates pages for the new frames.  :class:`PagePool` does that
+on the host, a step's rows are uploaded; :class:`DevicePagePool` does it in one
+launch, so a step needs no host work and can be recorded in a graph, and its
+streams may append fewer frames than a whole chunk.
 """
 
 from __future__ import annotations
@@ -12,8 +16,10 @@ import ctypes
 from ctypes import POINTER, c_int32, c_int64, c_void_p
 
 import numpy as np
+import torch
 
-from ._lib import check, lib
+from . import ops
+from ._lib import PAGE_STEP_MAX_SLOTS, check, lib
 
 
 def pages_per_slot(left: int, chunk: int, page_size: int) -> int:
@@ -123,3 +129,86 @@ class PagePool:
             "pk_pool_slot_info",
         )
         return int(appended.value), ring
+
+
+class DevicePagePool:
+    """A page pool in device memory: the rings, rows and FIFO order of
+    :class:`PagePool`, advanced by ``ops.page_step`` on torch's current stream.
+
+    The inspection methods (``free_pages``, ``free_list``, ``slot_info``) wait for the
+    device; nothing else does.  Steps of one pool run on one stream, or are ordered by
+    the caller's events."""
+
+    def __init__(
+        self,
+        num_slots: int,
+        page_size: int,
+        left: int,
+        chunk: int,
+        device: torch.device,
+        num_pages: int | None = None,
+        page_order=None,
+    ):
+        self.num_slots, self.page_size = int(num_slots), int(page_size)
+        self.left, self.chunk = int(left), int(chunk)
+        if self.page_size <= 0 or self.page_size & (self.page_size - 1):
+            raise ValueError(f"page_size {page_size} is not a power of two")
+        if self.left < 0 or self.chunk <= 0 or not 0 < self.num_slots <= PAGE_STEP_MAX_SLOTS:
+            raise ValueError(f"need left >= 0, chunk > 0 and 0 < num_slots <= {PAGE_STEP_MAX_SLOTS}")
+        self.max_pages = pages_per_slot(self.left, self.chunk, self.page_size)
+        self.num_pages = self.num_slots * self.max_pages if num_pages is None else int(num_pages)
+        if self.num_pages < self.num_slots * self.max_pages:
+            raise ValueError(f"{self.num_pages} pages cannot hold {self.num_slots} slots of {self.max_pages} pages each")
+        if self.num_pages * self.page_size >= 1 << 31:
+            raise ValueError(f"{self.num_pages} pages of {self.page_size} frames are past a slot map's 2^31 frames")
+        order = np.arange(self.num_pages) if page_order is None else np.asarray(page_order)
+        if order.shape != (self.num_pages,) or not np.array_equal(np.sort(order), np.arange(self.num_pages)):
+            raise ValueError(f"page_order is not a permutation of 0..{self.num_pages - 1}")
+        self.device = torch.device(device)
+        self.state = ops.PageState(
+            torch.from_numpy(order.astype(np.int32)).to(self.device),
+            torch.tensor([0, self.num_pages], dtype=torch.int32, device=self.device),
+            torch.zeros(self.num_slots, dtype=torch.int64, device=self.device),
+            torch.full((self.num_slots, self.max_pages), -1, dtype=torch.int32, device=self.device),
+            page_size=self.page_size,
+            left=self.left,
+            chunk=self.chunk,
+        )
+
+    def slots_tensor(self, slots) -> torch.Tensor:
+        """Slot numbers checked on the host (distinct, in range) and uploaded; a device
+        tensor is taken as it is (``ops.page_step`` leaves its bad entries out)."""
+        if isinstance(slots, torch.Tensor) and slots.device.type == "cuda":
+            return slots
+        s = np.ascontiguousarray(np.asarray(slots, dtype=np.int32).reshape(-1))
+        if len(np.unique(s)) != len(s) or (len(s) and (s.min() < 0 or s.max() >= self.num_slots)):
+            raise ValueError(f"slots must be distinct and in [0, {self.num_slots})")
+        return torch.from_numpy(s).to(self.device)
+
+    # -- stepping
+    def advance(self, slots, lengths: torch.Tensor | None = None, rows=None, slot_map=None):
+        """One step for ``slots`` (in order): ``(rows, slot_map)`` of ``ops.page_step``."""
+        return ops.page_step(self.state, self.slots_tensor(slots), lengths, rows=rows, slot_map=slot_map)
+
+    def reset_slot(self, slot: int) -> None:
+        self.reset_slots([int(slot)])
+
+    def reset_slots(self, slots) -> None:
+        """Every page of ``slots`` back to the queue, slot after slot."""
+        ops.page_reset(self.state, self.slots_tensor(slots))
+
+    def reset_all(self) -> None:
+        ops.page_reset(self.state, torch.arange(self.num_slots, dtype=torch.int32, device=self.device))
+
+    # -- inspection
+    def free_pages(self) -> int:
+        return int(self.state.head[1])
+
+    def free_list(self) -> np.ndarray:
+        first, n = self.state.head.tolist()
+        return self.state.queue.cpu().numpy()[(first + np.arange(n)) % self.num_pages]
+
+    def slot_info(self, slot: int) -> tuple[int, np.ndarray]:
+        if not 0 <= int(slot) < self.num_slots:
+            raise ValueError(f"slot {slot} out of range [0, {self.num_slots})")
+        return int(self.state.appended[slot]), self.state.ring[slot].cpu().numpy()
