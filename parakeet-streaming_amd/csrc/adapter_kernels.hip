@@ -45,12 +45,11 @@ struct MmaA<float> {
 // infinite, as it is where x A^T is a product of its own): a row of h is [high
 // 0..r-1 | low 0..r-1], r / 4 chunks of 16 bytes, chunk q multiplied with chunk
 // q mod r/8 of a row of B.  For ranks up to 16 both parts are one matrix instruction.
-// fp32: one part, r / 4 chunks.
+// fp32: one part, r / 4 chunks.  Where K is split over workgroups (parts > 1) a row of h
+// is the parts' rows one after another: their sum is taken by the product with B.
 template <typename ST>
 __device__ static inline int b_chunk(int q, int r) {
-  if constexpr (sizeof(ST) == 4) return q;
-  const int half = r >> 3;
-  return q >= half ? q - half : q;
+  return (int)((uint32_t)q % (uint32_t)(sizeof(ST) == 4 ? r >> 2 : r >> 3));
 }
 
 template <typename ST>
@@ -66,10 +65,11 @@ struct AdK {
   const int32_t* order;  // [M] plan: row at a position
   const int32_t* ids;    // [M] adapter at a position, -1: none
   const int4* tiles;     // {adapter, first position, rows, 0}
-  ST* h;                 // [M][2 r] (fp32: [M][r]) by position
+  ST* h;                 // [M + 1][parts][2 r] (fp32: [M + 1][parts][r]) by position, row M zeros
   ST* out;               // [M][N], stride out_s
   int64_t out_s;
   int32_t M, N, K, r, G;
+  int32_t parts, kpart;  // parts of K, columns of one (a multiple of 64)
   int32_t mtiles, xm;
 };
 
@@ -83,15 +83,28 @@ __device__ static inline int plan_row(const AdK<ST>& p, int pos) {
 constexpr int kLowWaves = 8;
 constexpr int kLowRows = 32;  // rows of a plan's tile
 
-// h of a tile: the waves split K, 16 RT ranks a workgroup.  Operands come straight from
-// memory (every byte is used once a workgroup).
+// an offset that no tensor here reaches (each is below 2^31 bytes): such a load gives zeros
+constexpr uint32_t kNowhere = 0x80000000u;
+__device__ static inline u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+
+// h of a tile: the waves split K, 16 RT ranks a workgroup, U steps of loads on their way.
+// Operands come straight from memory (every byte is used once a workgroup).
 template <typename ST, int RT>
 __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
   constexpr int V = Tr<ST>::VEC;
   constexpr int COLS = MmaA<ST>::COLS;
+  constexpr int SB = 2, kBlock = SB * COLS, U = 4;
   __shared__ f32x4_t red[kLowWaves * RT * 2 * 64];
   static_assert(2 * RT <= kLowWaves, "a wave finishes at most one sum");
+  if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {  // the row of zeros behind the last row
+    const int n = p.r * p.parts * 4 / 16;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < n; i += 64 * kLowWaves)
+      st16(reinterpret_cast<unsigned char*>(p.h) + (int64_t)p.M * n * 16 + i * 16, zero);
+  }
   const int4 tile = p.tiles[blockIdx.x];
   if ((uint32_t)tile.x >= (uint32_t)p.G) return;  // past the last tile
   if (tile.y < 0 || tile.z <= 0 || tile.z > kLowRows || tile.y > p.M - tile.z) return;  // not a plan's
@@ -99,26 +112,39 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
   const int l16 = lane & 15, kg = lane >> 4;
   const int r0 = blockIdx.y * RT * 16;
   const bool two = tile.z > 16;
-  const ST* xp[2];
+  // offsets in bytes; columns past K and a second 16 rows that the tile has not read as zero
+  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * (uint32_t)sizeof(ST));
+  const __amdgpu_buffer_rsrc_t ra = bytes_rsrc(p.a + (int64_t)tile.x * p.r * p.K, (uint32_t)p.r * p.K * (uint32_t)sizeof(ST));
+  uint32_t xo[2], ao[RT];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) xp[m] = p.x + (int64_t)plan_row(p, tile.y + min(m * 16 + l16, tile.z - 1)) * p.x_s + kg * V;
-  const ST* ap[RT];
+  for (int m = 0; m < 2; ++m)
+    xo[m] = (uint32_t)(plan_row(p, tile.y + min(m * 16 + l16, tile.z - 1)) * p.x_s + kg * V) * (uint32_t)sizeof(ST);
 #pragma unroll
-  for (int j = 0; j < RT; ++j) ap[j] = p.a + ((int64_t)tile.x * p.r + min(r0 + j * 16 + l16, p.r - 1)) * p.K + kg * V;
+  for (int j = 0; j < RT; ++j) ao[j] = (uint32_t)(min(r0 + j * 16 + l16, p.r - 1) * p.K + kg * V) * (uint32_t)sizeof(ST);
   f32x4_t acc[RT][2];
 #pragma unroll
   for (int j = 0; j < RT; ++j) acc[j][0] = acc[j][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int k = wave * COLS; k < p.K; k += kLowWaves * COLS) {
-    u32x4 af[RT], xf[2];
-    xf[0] = ld16(xp[0] + k);
-    if (two) xf[1] = ld16(xp[1] + k);
+  // a wave takes blocks of 128 bytes a row: whole lines, in adjacent steps
+  const int k0 = blockIdx.z * p.kpart, k1 = min(k0 + p.kpart, p.K);
+  for (int k = k0 + wave * kBlock; k < k1; k += U / SB * kLowWaves * kBlock) {
+    u32x4 af[U][RT], xf[U][2];
 #pragma unroll
-    for (int j = 0; j < RT; ++j) af[j] = ld16(ap[j] + k);
+    for (int u = 0; u < U; ++u) {
+      const int ku = k + u / SB * kLowWaves * kBlock + u % SB * COLS;
+      const uint32_t kb = ku < k1 ? (uint32_t)ku * (uint32_t)sizeof(ST) : kNowhere;
+      xf[u][0] = load16(rx, xo[0] + kb);
+      xf[u][1] = load16(rx, two ? xo[1] + kb : kNowhere);
 #pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      acc[j][0] = MmaA<ST>::step(af[j], xf[0], acc[j][0]);
-      if (two) acc[j][1] = MmaA<ST>::step(af[j], xf[1], acc[j][1]);
+      for (int j = 0; j < RT; ++j) af[u][j] = load16(ra, ao[j] + kb);
     }
+    __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        acc[j][0] = MmaA<ST>::step(af[u][j], xf[u][0], acc[j][0]);
+        acc[j][1] = MmaA<ST>::step(af[u][j], xf[u][1], acc[j][1]);
+      }
   }
 #pragma unroll
   for (int j = 0; j < RT; ++j)
@@ -134,7 +160,7 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
   const float sc = p.scale[tile.x];
   float f[4] = {v.x * sc, v.y * sc, v.z * sc, v.w * sc};
   if constexpr (sizeof(ST) == 4) {
-    st16(p.h + (int64_t)(tile.y + row) * p.r + c, Tr<float>::pack(f));
+    st16(p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * p.r + c, Tr<float>::pack(f));
   } else {
     float lo[4];
 #pragma unroll
@@ -142,23 +168,23 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
       const float hi = round_to<ST>(f[e]);
       lo[e] = fabsf(hi) < __builtin_inff() ? f[e] - hi : 0.f;
     }
-    ST* const q = p.h + (int64_t)(tile.y + row) * 2 * p.r + c;
+    ST* const q = p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * 2 * p.r + c;
     *reinterpret_cast<u32x2*>(q) = pack4<ST>(f);
     *reinterpret_cast<u32x2*>(q + p.r) = pack4<ST>(lo);
   }
 }
 
-// acc[m][n] += h B^T for TM x TN products of rows pos0 + 16 m and columns c0 + 16 n, one
-// pass for each adapter among the rows; of the adapters, part `wk` of WK.  Columns of a
-// product (the rows of the batch) are independent, so where only some of 16 rows have
-// the adapter the product is taken for all of them and kept for those: what a row gets
-// depends on its own adapter alone, an infinity or NaN in another's B does not reach it.
-template <typename ST, int TM, int TN, int WK>
-__device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
+// add_low where an infinity or NaN is among the operands: where only some of 16 rows have
+// an adapter its product is taken for all of them and kept for those, so that what a row
+// // gets depends on its own adapter alone, and in the same order of sums, so that the rows
+// without them keep their bits: part wk of WK are some of the adapters, or (STEPS) some
+// of each adapter's steps of 4 chunks a lane group.
+template <typename ST, int TM, int TN, int WK, bool STEPS>
+__device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
                                       f32x4_t (&acc)[TM][TN]) {
   constexpr int V = Tr<ST>::VEC;
   const int l16 = lane & 15, kg = lane >> 4;
-  const int chunks = p.r >> 2, hs = sizeof(ST) == 4 ? p.r : 2 * p.r;
+  const int chunks = (p.r >> 2) * p.parts, hs = (sizeof(ST) == 4 ? p.r : 2 * p.r) * p.parts;
   const u32x4 zero = {0u, 0u, 0u, 0u};
   const ST* hp[TM];
   uint64_t left[TM];
@@ -174,37 +200,21 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
       if (left[m]) g = __builtin_amdgcn_readlane(id[m], __builtin_ctzll(left[m]));
     if (g < 0) break;
     uint64_t has[TM];
-    bool whole = false;
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       has[m] = __ballot(id[m] == g);
       left[m] &= ~has[m];
-      whole |= has[m] == ~(uint64_t)0;
     }
-    if (WK > 1 && turn != wk) continue;
+    if (!STEPS && WK > 1 && turn != wk) continue;
     const ST* const bp = p.b + ((int64_t)g * p.N + c0 + l16) * p.r;
     auto b_of = [&](int n, int q) { return q < chunks ? ld16(bp + (int64_t)n * 16 * p.r + b_chunk<ST>(q, p.r) * V) : zero; };
-    if (whole) {
-      for (int q = kg; q - kg < chunks; q += 4) {
-        u32x4 bf[TN];
-#pragma unroll
-        for (int n = 0; n < TN; ++n) bf[n] = b_of(n, q);
-#pragma unroll
-        for (int m = 0; m < TM; ++m) {
-          if (has[m] != ~(uint64_t)0) continue;
-          const u32x4 hf = q < chunks ? ld16(hp[m] + q * V) : zero;
-#pragma unroll
-          for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(bf[n], hf, acc[m][n]);
-        }
-      }
-    }
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-      if (has[m] == 0 || has[m] == ~(uint64_t)0) continue;
+      if (has[m] == 0) continue;
       f32x4_t d[TN];
 #pragma unroll
       for (int n = 0; n < TN; ++n) d[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int q = kg; q - kg < chunks; q += 4) {
+      for (int q = (STEPS ? 4 * wk : 0) + kg; q - kg < chunks; q += STEPS ? 4 * WK : 4) {
         const u32x4 hf = q < chunks ? ld16(hp[m] + q * V) : zero;
 #pragma unroll
         for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(b_of(n, q), hf, d[n]);
@@ -217,6 +227,105 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
   }
 }
 
+// acc[m][n] = h B^T for TM x TN products of rows pos0 + 16 m and columns c0 + 16 n, summed
+// over the adapters among the rows (of these, part `wk` of WK), each with the other
+// adapters' rows of h read as zero.  Work items of one adapter and 4 chunks a lane group,
+// DEP items' loads on their way: a wave with few rows has up to 16 adapters a product,
+// and one by one each would cost a round trip to memory (0.8 us).  A zero row of h times
+// an infinity in B is a NaN in another adapter's rows: sums that are not finite are made
+// again by add_low_apart.
+template <typename ST, int TM, int TN, int WK, int DEP>
+__device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
+                                      f32x4_t (&acc)[TM][TN]) {
+  constexpr uint32_t E = sizeof(ST);
+  const int l16 = lane & 15, kg = lane >> 4;
+  const int chunks = (p.r >> 2) * p.parts;
+  const uint32_t hrow = (E == 4 ? p.r : 2 * p.r) * E * p.parts, brow = p.r * E;
+  const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
+  uint64_t left[TM];
+  uint64_t rest = 0;
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    left[m] = __ballot(id[m] >= 0);
+    rest |= left[m];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  if (!rest) return;
+  struct Item {
+    u32x4 bf[TN], hf[TM];
+    uint32_t rows;  // bit m: rows 16 m have the adapter; 0: no item
+  };
+  int g = -1, q0 = 0, turn = 0;
+  uint32_t rows = 0;
+  auto next = [&](Item& it) {
+    q0 += 4;
+    if (g < 0 || q0 >= chunks) {
+      q0 = 0;
+      bool mine = false;
+      do {
+        g = -1;
+        rows = 0;
+#pragma unroll
+        for (int m = TM - 1; m >= 0; --m)
+          if (left[m]) g = __builtin_amdgcn_readlane(id[m], __builtin_ctzll(left[m]));
+        if (g < 0) break;
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          const uint64_t has = __ballot(id[m] == g);
+          left[m] &= ~has;
+          rows |= has ? 1u << m : 0u;
+        }
+        mine = WK == 1 || turn == wk;
+        turn = turn == WK - 1 ? 0 : turn + 1;
+      } while (!mine);
+    }
+    it.rows = rows;
+    if (!rows) return;
+    const int q = q0 + kg;
+    const __amdgpu_buffer_rsrc_t rb = bytes_rsrc(p.b + (int64_t)g * p.N * p.r, (uint32_t)p.N * brow);
+    const uint32_t bo = q < chunks ? (uint32_t)(c0 + l16) * brow + (uint32_t)b_chunk<ST>(q, p.r) * 16u : kNowhere;
+#pragma unroll
+    for (int n = 0; n < TN; ++n) it.bf[n] = load16(rb, bo + (uint32_t)(n * 16) * brow);
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+      it.hf[m] = load16(rh, q < chunks && id[m] == g ? (uint32_t)(pos0 + m * 16 + l16) * hrow + (uint32_t)q * 16u : kNowhere);
+  };
+  Item it[DEP];
+#pragma unroll
+  for (int d = 0; d < DEP; ++d) next(it[d]);
+  for (bool more = true; more;) {
+#pragma unroll
+    for (int d = 0; d < DEP; ++d) {
+      if (!it[d].rows) {
+        more = false;
+        break;
+      }
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        if (!(it[d].rows >> m & 1)) continue;
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], it[d].hf[m], acc[m][n]);
+      }
+      next(it[d]);
+    }
+  }
+  bool fine = true;
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) fine &= fabsf(acc[m][n][e]) < __builtin_inff();
+  if (__ballot(!fine)) {
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    add_low_apart<ST, TM, TN, WK, false>(p, id, pos0, c0, wk, lane, acc);
+  }
+}
+
 template <int SILU>
 __device__ static inline float ad_act(float v) {
   if constexpr (SILU) return v / (1.f + __expf(-v));
@@ -225,7 +334,13 @@ __device__ static inline float ad_act(float v) {
 
 // The product with W: BM x BN outputs a workgroup, both operands staged in LDS as in
 // lin_tile_kernel, the rows of x and of the output those that the plan's order names.
-// The adapters' part is summed first, while the first stages are on their way.
+//
+// The adapters' part comes first.  Tiles of few rows (BK > 64) take it from memory while
+// the first stages are on their way (add_low).  Larger ones take it as stages before
+// those of W: for each run of rows with one adapter, 64 columns of h (rows of other
+// runs from a row of zeros) and of B_g.  A byte of either is then loaded once a
+// workgroup and in whole lines, not once a wave in halves of lines: 3584 x 1024 -> 4096 of
+// rank 64, 24 adapters, took 84 us from memory (128 x 128 tiles) and 61 so.
 template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU>
 __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
@@ -241,8 +356,14 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   constexpr int kOut = BM * OS * 2;
   constexpr int kRed = WK > 1 ? (WK - 1) * BM * BN * 4 : 0;
   constexpr int kSmem = S * kStage > kOut + kRed ? S * kStage : kOut + kRed;
-  __shared__ __align__(16) unsigned char smem[kSmem];
-  __shared__ int32_t ord[BM];
+  constexpr bool kStaged = BK == 64;
+  constexpr int RW = (BM + 63) / 64;  // 64-row words of a row mask
+  // one LDS object: with a second one the compiler keeps them apart and waits for every
+  // load to LDS in flight before an operand read
+  __shared__ __align__(16) unsigned char smem[kSmem + BM * 8 + 16];
+  int32_t* const ord = reinterpret_cast<int32_t*>(smem + kSmem);
+  int32_t* const sid = ord + BM;
+  int32_t* const odd = sid + BM;  // != 0: a sum of the adapters' part is not finite
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, kg = lane >> 4;
@@ -251,18 +372,20 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   xcd_tile(p.mtiles, p.xm, mt_i, nt_i);
   const int row0 = mt_i * BM, n0 = nt_i * BN;
 
-  // positions past the last row read the last row and store nothing
-  for (int i = threadIdx.x; i < BM; i += 64 * NW) ord[i] = plan_row(p, row0 + i);
+  // positions past the last row read the last row, have no adapter and store nothing
+  for (int i = threadIdx.x; i < BM; i += 64 * NW) {
+    ord[i] = plan_row(p, row0 + i);
+    const int g = p.ids[min(row0 + i, p.M - 1)];
+    sid[i] = row0 + i < p.M && (uint32_t)g < (uint32_t)p.G ? g : -1;
+  }
+  if (threadIdx.x == 0) *odd = 0;
+  __syncthreads();
   int id[TM];
 #pragma unroll
-  for (int m = 0; m < TM; ++m) {
-    const int pos = row0 + (wm * TM + m) * 16 + l16;
-    id[m] = pos < p.M ? p.ids[pos] : -1;
-    if ((uint32_t)id[m] >= (uint32_t)p.G) id[m] = -1;
-  }
-  __syncthreads();
+  for (int m = 0; m < TM; ++m) id[m] = sid[(wm * TM + m) * 16 + l16];
   const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * 2u);
   const __amdgpu_buffer_rsrc_t rw = bytes_rsrc(p.w, (uint32_t)((p.N - 1) * p.w_s + p.K) * 2u);
+  // chunk c of a stage: row c / CH of [x rows ; w rows], LDS position c % CH
   uint32_t off[LPS];
 #pragma unroll
   for (int i = 0; i < LPS; ++i) {
@@ -278,27 +401,13 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
       load_lds16(base < BM * CH ? rx : rw, smem + st * kStage + base * 16, off[i], k * 2);
     }
   };
+  // xs, ws of a stage times each other, for the 16-row products that `rows` names
   f32x4_t acc[TM][TN];
 #pragma unroll
   for (int m = 0; m < TM; ++m)
 #pragma unroll
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  const int iters = p.K / BK;
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s)
-    if (s < iters) issue(s, s * BK);
-  add_low<ST, TM, TN, WK>(p, id, row0 + wm * TM * 16, n0 + wn * TN * 16, wk, lane, acc);
-  int st = 0;
-  for (int it = 0; it < iters; ++it) {
-    if (it + S - 2 < iters)
-      wait_vm<(S - 2) * LPS>();
-    else
-      wait_vm<0>();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, (it + S - 1) * BK);
+  auto multiply = [&](int st, uint32_t rows) {
     const unsigned char* xs = smem + st * kStage;
     const unsigned char* ws = xs + BM * BK * 2;
 #pragma unroll
@@ -316,11 +425,145 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
         wf[n] = *reinterpret_cast<const u32x4*>(ws + r * BK * 2 + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
       }
 #pragma unroll
-      for (int m = 0; m < TM; ++m)
+      for (int m = 0; m < TM; ++m) {
+        if (!(rows >> m & 1)) continue;
 #pragma unroll
         for (int n = 0; n < TN; ++n) acc[m][n] = MmaL<ST>::k32(wf[n], xf[m], acc[m][n]);
+      }
     }
-    st = st == S - 1 ? 0 : st + 1;
+  };
+  auto wait = [&](bool last) {
+    if (!last)
+      wait_vm<(S - 2) * LPS>();
+    else
+      wait_vm<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  const int iters = p.K / BK;
+  int st = 0;
+  if constexpr (kStaged) {
+    // runs of rows with one adapter: masks of first and last rows, walked twice (the
+    // loads, S - 1 stages ahead, and the products)
+    uint64_t first[RW], last[RW];
+    int runs = 0;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+      const int i = w * 64 + lane;
+      const int g = i < BM ? sid[i] : -1;
+      first[w] = __ballot(g >= 0 && (i == 0 || sid[i - 1] != g));
+      last[w] = __ballot(g >= 0 && (i == BM - 1 || sid[i + 1] != g));
+      runs += __popcll(first[w]);
+    }
+    struct Walk {
+      uint64_t f[RW], l[RW];
+      int s, e, j;  // rows s .. e, stage j of the run
+    };
+    const int chunks = (p.r >> 2) * p.parts, nst = (chunks + 7) >> 3, total = runs * nst + iters;
+    auto step = [&](Walk& v) {
+      if (++v.j < nst) return;
+      v.j = 0;
+      v.s = v.e = BM;
+#pragma unroll
+      for (int w = RW - 1; w >= 0; --w) {
+        if (v.f[w]) v.s = w * 64 + __builtin_ctzll(v.f[w]);
+        if (v.l[w]) v.e = w * 64 + __builtin_ctzll(v.l[w]);
+      }
+#pragma unroll
+      for (int w = RW - 1; w >= 0; --w) {
+        if (v.s >> 6 == w) v.f[w] &= v.f[w] - 1;
+        if (v.e >> 6 == w) v.l[w] &= v.l[w] - 1;
+      }
+    };
+    Walk ld, mu;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+      ld.f[w] = mu.f[w] = first[w];
+      ld.l[w] = mu.l[w] = last[w];
+    }
+    ld.j = mu.j = nst;
+    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = (uint32_t)p.r * 2u;
+    const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)(p.M + 1) * hrow);
+    auto issue_low = [&](int slot) {
+      step(ld);
+      const int g = __builtin_amdgcn_readfirstlane(sid[ld.s]);
+      const __amdgpu_buffer_rsrc_t rb = bytes_rsrc(p.b + (int64_t)g * p.N * p.r, (uint32_t)p.N * brow);
+#pragma unroll
+      for (int i = 0; i < LPS; ++i) {
+        const int base = (i * NW + wave) * 64, c = base + lane;
+        const int r = c / CH, q = ld.j * 8 + ((c ^ r) & 7);
+        uint32_t o;
+        if (base < BM * CH)
+          o = r >= ld.s && r <= ld.e && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : (uint32_t)p.M * hrow;
+        else
+          o = (uint32_t)(n0 + r - BM) * brow + (uint32_t)b_chunk<ST>(q, p.r) * 16u;
+        load_lds16(base < BM * CH ? rh : rb, smem + slot * kStage + base * 16, o, 0);
+      }
+    };
+    const int nlow = runs * nst;
+    auto issue_at = [&](int slot, int it) {
+      if (it < nlow)
+        issue_low(slot);
+      else if (it < total)
+        issue(slot, (it - nlow) * BK);
+    };
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) issue_at(s, s);
+    for (int it = 0; it < nlow; ++it) {
+      wait(it + S - 2 >= total);
+      issue_at(st == 0 ? S - 1 : st - 1, it + S - 1);
+      step(mu);
+      uint32_t rows = 0;
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const int r = (wm * TM + m) * 16;
+        rows |= r <= mu.e && r + 15 >= mu.s ? 1u << m : 0u;
+      }
+      if (rows) multiply(st, rows);
+      st = st == S - 1 ? 0 : st + 1;
+    }
+    if (nlow) {
+      // a zero row of h times an infinity in another run's B is a NaN: then the part is
+      // made again with the adapters apart
+      bool fine = true;
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) fine &= fabsf(acc[m][n][e]) < __builtin_inff();
+      if (__ballot(!fine)) *odd = 1;
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stages stay in flight
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (__builtin_amdgcn_readfirstlane(*(volatile int32_t*)odd)) {
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+          for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        add_low_apart<ST, TM, TN, WK, true>(p, id, row0 + wm * TM * 16, n0 + wn * TN * 16, wk, lane, acc);
+      }
+    }
+    for (int it = nlow; it < total; ++it) {
+      wait(it + S - 2 >= total);
+      if (it + S - 1 < total) issue(st == 0 ? S - 1 : st - 1, (it - nlow + S - 1) * BK);
+      multiply(st, ~0u);
+      st = st == S - 1 ? 0 : st + 1;
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s)
+      if (s < iters) issue(s, s * BK);
+    add_low<ST, TM, TN, WK, 4>(p, id, row0 + wm * TM * 16, n0 + wn * TN * 16, wk, lane, acc);
+    for (int it = 0; it < iters; ++it) {
+      wait(it + S - 2 >= iters);
+      if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, (it + S - 1) * BK);
+      multiply(st, ~0u);
+      st = st == S - 1 ? 0 : st + 1;
+    }
   }
   __syncthreads();
   sum_parts<BM, BN, WM * WN, WK>(smem, kOut, acc, wave, lane);
@@ -362,14 +605,15 @@ __global__ void __launch_bounds__(256) adapter_add_kernel(const AdK<float> p) {
   int id[1] = {pos < p.M ? p.ids[pos] : -1};
   if ((uint32_t)id[0] >= (uint32_t)p.G) id[0] = -1;
   float* const q = p.out + (int64_t)plan_row(p, pos) * p.out_s + c0 + kg * 4;
-  f32x4_t acc[1][TN];
+  u32x4 base[TN];
 #pragma unroll
-  for (int n = 0; n < TN; ++n) acc[0][n] = __builtin_bit_cast(f32x4_t, ld16(q + n * 16));
-  add_low<float, 1, TN, 1>(p, id, blockIdx.x * 16, c0, 0, lane, acc);
+  for (int n = 0; n < TN; ++n) base[n] = ld16(q + n * 16);
+  f32x4_t acc[1][TN];
+  add_low<float, 1, TN, 1, 4>(p, id, blockIdx.x * 16, c0, 0, lane, acc);
   if (pos >= p.M) return;
 #pragma unroll
   for (int n = 0; n < TN; ++n) {
-    f32x4_t v = acc[0][n];
+    f32x4_t v = acc[0][n] + __builtin_bit_cast(f32x4_t, base[n]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = ad_act<SILU>(v[e]);
     st16(q + n * 16, __builtin_bit_cast(u32x4, v));
@@ -378,16 +622,27 @@ __global__ void __launch_bounds__(256) adapter_add_kernel(const AdK<float> p) {
 
 namespace {
 
+// workgroups over the ranks: 32 of them each, more read x again (rank 64 in one workgroup
+// takes 0.9-1.5 us longer from 1 to 3584 rows of 512 to 4096)
+int low_blocks(int r) { return (r + 31) / 32; }
+
+// Parts of K that x A^T is split into: of 1024 columns or more, up to 4, while there are
+// at most 256 workgroups (one a CU).  A tile of 32 rows x 4096 columns reads 0.5 MB, 15 us
+// for one workgroup; the product with B then takes more steps (840 x 4096 -> 1024, rank
+// 32: 38 us in one part, 32 in four).
+int k_parts(int64_t tiles, int r, int64_t k) {
+  int p = 1;
+  while (p < 4 && (int64_t)p * 2 * 1024 <= k && tiles * low_blocks(r) * p * 2 <= 256) p *= 2;
+  return p;
+}
+
 template <typename ST>
 int launch_low(const AdK<ST>& k, int max_tiles, hipStream_t s) {
-  const int rt = (k.r + 15) / 16, per = rt < 4 ? rt : 4;
-  const dim3 grid((unsigned)max_tiles, (unsigned)((rt + per - 1) / per)), block(64 * kLowWaves);
-  switch (per) {
-    case 1: hipLaunchKernelGGL((adapter_low_kernel<ST, 1>), grid, block, 0, s, k); break;
-    case 2: hipLaunchKernelGGL((adapter_low_kernel<ST, 2>), grid, block, 0, s, k); break;
-    case 3: hipLaunchKernelGGL((adapter_low_kernel<ST, 3>), grid, block, 0, s, k); break;
-    default: hipLaunchKernelGGL((adapter_low_kernel<ST, 4>), grid, block, 0, s, k); break;
-  }
+  const dim3 grid((unsigned)max_tiles, (unsigned)low_blocks(k.r), (unsigned)k.parts), block(64 * kLowWaves);
+  if (k.r <= 16)
+    hipLaunchKernelGGL((adapter_low_kernel<ST, 1>), grid, block, 0, s, k);
+  else
+    hipLaunchKernelGGL((adapter_low_kernel<ST, 2>), grid, block, 0, s, k);
   return check_launch("pk_adapter_linear");
 }
 
@@ -405,13 +660,70 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
   return check_launch("pk_adapter_linear");
 }
 
-template <typename ST, int SILU>
-int launch_product(const AdK<ST>& k, hipStream_t s) {
-  return launch_tile<ST, 64, 64, 2, 2, 2, 64, 4, SILU>(k, s);
+// The forms of the product and what a launch of each takes, as pk_linear's table has
+// them (`a` us and `s` us a 1024 columns, `m` of the latter for each further workgroup on
+// the CU, again a - 2 for each further round of `occ`), with `e` us for a step of the
+// adapters' part: a run of rows with one adapter in a tile, 16 ranks of it (from memory)
+// or 32 (staged).  Fitted to launches in a graph, 1 - 7600 rows, K and N 512 - 4096, ranks 16 and
+// 64, one adapter to one a row: on the mean 3% over the fastest form.  How many adapters
+// the rows have is not known on the host; the plan's tiles bound it.
+struct Form {
+  int bm, bn, kmul, occ;
+  float a, s, m, e;
+  bool staged;
+};
+constexpr Form kForms[] = {
+    {16, 16, 128, 4, 2.8f, 1.2f, 0.25f, 0.08f, false},   // 0
+    {16, 32, 128, 3, 3.05f, 1.37f, 0.5f, 0.13f, false},  // 1
+    {32, 32, 128, 2, 3.45f, 1.75f, 0.6f, 0.15f, false},  // 2
+    {32, 64, 128, 2, 3.6f, 2.25f, 0.95f, 0.26f, false},  // 3
+    {64, 64, 64, 2, 3.75f, 3.35f, 0.8f, 0.4f, true},     // 4
+    {64, 128, 64, 2, 4.2f, 5.5f, 0.8f, 0.5f, true},      // 5
+    {128, 128, 64, 2, 5.7f, 9.1f, 0.8f, 1.2f, true},     // 6
+    {256, 256, 64, 1, 10.0f, 28.0f, 0.f, 1.75f, true},   // 7
+};
+constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
+
+// us of a launch in form f with `adapters` among the rows, or a negative number where it
+// does not fit
+float form_cost(const Form& f, int64_t M, int64_t N, int64_t K, int r, int parts, int64_t adapters, int cus) {
+  if (N % f.bn != 0 || K % f.kmul != 0) return -1.f;
+  const int64_t tiles = (M + f.bm - 1) / f.bm * (N / f.bn);
+  const int64_t per = (tiles + cus - 1) / cus, rounds = (per + f.occ - 1) / f.occ;
+  const float c = f.s * (float)K / 1024.f;
+  const float runs = fminf(fminf((float)f.bm, (float)M), 1.f + (float)(adapters - 1) * f.bm / M);
+  const int steps = f.staged ? (r * parts + 31) / 32 : (r * parts + 15) / 16;
+  return f.a + (float)(rounds - 1) * (f.a - 2.f) + (float)rounds * c + f.m * c * (float)(per - rounds) +
+         f.e * runs * (float)steps * (float)per;
 }
 
-bool rows_ok(int64_t rows, int64_t stride, int64_t width, int vec) {
-  return stride >= 0 && stride % vec == 0 && (rows <= 1 || stride >= width) && (rows - 1) * stride + width < (int64_t{1} << 31);
+template <typename ST, int SILU>
+int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
+  int form = -1;
+  float cost = 0.f;
+  for (int i = 0; i < kNumForms; ++i) {
+    const float c = form_cost(kForms[i], k.M, k.N, k.K, k.r, k.parts, adapters, cus);
+    if (c >= 0.f && (form < 0 || c < cost)) {
+      form = i;
+      cost = c;
+    }
+  }
+  switch (form) {
+    case 0: return launch_tile<ST, 16, 16, 1, 1, 4, 128, 4, SILU>(k, s);
+    case 1: return launch_tile<ST, 16, 32, 1, 1, 4, 128, 4, SILU>(k, s);
+    case 2: return launch_tile<ST, 32, 32, 1, 1, 4, 128, 4, SILU>(k, s);
+    case 3: return launch_tile<ST, 32, 64, 1, 2, 4, 128, 3, SILU>(k, s);
+    case 4: return launch_tile<ST, 64, 64, 2, 2, 2, 64, 4, SILU>(k, s);
+    case 5: return launch_tile<ST, 64, 128, 2, 4, 1, 64, 3, SILU>(k, s);
+    case 6: return launch_tile<ST, 128, 128, 2, 2, 1, 64, 2, SILU>(k, s);
+    default: return launch_tile<ST, 256, 256, 2, 4, 1, 64, 2, SILU>(k, s);
+  }
+}
+
+// below 2^31 bytes: 32-bit offsets, and kNowhere past them
+bool rows_ok(int64_t rows, int64_t stride, int64_t width, int bytes) {
+  return stride >= 0 && stride * bytes % 16 == 0 && (rows <= 1 || stride >= width) &&
+         ((rows - 1) * stride + width) * bytes < (int64_t{1} << 31);
 }
 
 template <typename ST>
@@ -438,11 +750,12 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
     if (q != a->scale && !aligned16(q)) return fail(PK_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
   }
   if (!a->order || !a->ids) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
-  constexpr int V = Tr<ST>::VEC;
-  if (!rows_ok(a->rows, a->x_stride, a->k, V) || (!kF32 && !rows_ok(a->n, a->weight_stride, a->k, V)) ||
-      !rows_ok(a->rows, a->out_stride, a->n, V))
-    return fail(PK_ERR_INVALID, "%s: row strides must be multiples of %d elements, at least the row, and a tensor below 2^31 elements",
-                what, V);
+  constexpr int E = sizeof(ST);
+  const int parts = k_parts(a->max_tiles, a->rank, a->k);
+  if (!rows_ok(a->rows, a->x_stride, a->k, E) || (!kF32 && !rows_ok(a->n, a->weight_stride, a->k, E)) ||
+      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok((int64_t)a->rows + 1, (int64_t)a->rank * parts, (int64_t)a->rank * parts, 4) || !rows_ok(a->rank, a->k, a->k, E) ||
+      !rows_ok(a->n, a->rank, a->rank, E))
+    return fail(PK_ERR_INVALID, "%s: row strides must be multiples of 16 bytes, at least the row, and a tensor below 2^31 bytes", what);
   AdK<ST> k{};
   k.x = static_cast<const ST*>(a->x);
   k.x_s = a->x_stride;
@@ -463,6 +776,8 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   k.K = a->k;
   k.r = a->rank;
   k.G = a->num_adapters;
+  k.parts = parts;
+  k.kpart = ((k.K / 64 + k.parts - 1) / k.parts) * 64;
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   if (a->max_tiles > 0) {
@@ -478,15 +793,19 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
       hipLaunchKernelGGL(adapter_add_kernel<0>, grid, dim3(256), 0, s, k);
     return check_launch(what);
   } else {
-    return silu ? launch_product<ST, 1>(k, s) : launch_product<ST, 0>(k, s);
+    int64_t adapters = a->max_tiles - a->rows / kLowRows;  // at most
+    if (adapters < 1) adapters = 1;
+    const int cus = cu_count();
+    return silu ? launch_product<ST, 1>(k, adapters, cus, s) : launch_product<ST, 0>(k, adapters, cus, s);
   }
 }
 
 }  // namespace
 }  // namespace pk
 
-extern "C" int64_t pk_adapter_workspace_bytes(int32_t rows, int32_t rank) {
-  return rows > 0 && rank > 0 ? (int64_t)rows * rank * 4 : 0;
+extern "C" int64_t pk_adapter_workspace_bytes(int32_t rows, int32_t rank, int32_t k, int32_t max_tiles) {
+  if (rows <= 0 || rank <= 0 || k <= 0 || max_tiles < 0) return 0;
+  return ((int64_t)rows + 1) * rank * 4 * pk::k_parts(max_tiles, rank, k);
 }
 
 extern "C" int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream) {

@@ -484,7 +484,7 @@ SIGNATURES = {
     "pk_kv_append_slots": (c_int, [POINTER(KvAppendSlotsArgs), c_void_p]),
     "pk_adapter_plan_tiles": (c_int, [c_int32, c_int32, c_int32]),
     "pk_adapter_plan": (c_int, [POINTER(AdapterPlanArgs), c_void_p]),
-    "pk_adapter_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pk_adapter_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
     "pk_pool_create": (
         c_int,

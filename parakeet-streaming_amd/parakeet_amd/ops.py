@@ -1318,7 +1318,7 @@ def adapter_linear(
             out = torch.empty(shape, dtype=dt, device=dev)
         a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
         a.bias = bias.data_ptr() if bias is not None else None
-    ws = torch.empty(M * r, dtype=torch.int32, device=dev)
+    ws = torch.empty(lib().pk_adapter_workspace_bytes(M, r, k, tiles), dtype=torch.uint8, device=dev)
     a.dtype, a.device = code, dev.index if dev.index is not None else torch.cuda.current_device()
     a.rows, a.n, a.k, a.rank, a.num_adapters = M, n, k, r, G
     a.activation = _lib.ACT_SILU if silu else _lib.ACT_NONE
