@@ -778,6 +778,7 @@ int pk_pool_free_list(const pk_pool* pool, int32_t* out, int32_t capacity);
  *            0, ring -1.  num_pages >= num_slots * M, so no step runs out of pages.
  * reset    : != 0: give every page of the slots back and set appended to 0
  *            (pk_pool_reset_slot in turn); lengths, rows and slot_map are not read.
+ * workspace: pk_page_step_workspace_bytes(batch), 16-byte aligned (NULL where that is 0).
  * Calls on one pool are ordered by the caller (one stream, or events).
  * num_pages * page_size < 2^31; num_slots <= PK_PAGE_STEP_MAX_SLOTS.
  */
@@ -801,7 +802,9 @@ typedef struct pk_page_step_args {
   int32_t rows_stride;
   int32_t* slot_map;
   int64_t slot_map_stride;
+  void* workspace;
 } pk_page_step_args;
+int64_t pk_page_step_workspace_bytes(int32_t batch);
 int pk_page_step(const pk_page_step_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
@@ -843,6 +846,7 @@ int pk_kv_append_slots(const pk_kv_append_slots_args* args, void* stream);
  * tiles      : int32 [max_tiles][4] = {adapter, first position, rows, 0}: up to 32
  *              rows of one adapter, by adapter; {-1, 0, 0, 0} past the last one.
  *              max_tiles >= pk_adapter_plan_tiles(...).
+ * workspace  : pk_adapter_plan_workspace_bytes(...), 16-byte aligned (NULL where that is 0)
  * num_adapters <= PK_ADAPTER_MAX.
  */
 #define PK_ADAPTER_MAX 512
@@ -857,7 +861,9 @@ typedef struct pk_adapter_plan_args {
   int32_t* sorted_ids;
   int32_t* tiles;
   int32_t max_tiles;
+  void* workspace;
 } pk_adapter_plan_args;
+int64_t pk_adapter_plan_workspace_bytes(int32_t batch, int32_t frames, int32_t num_adapters);
 int pk_adapter_plan_tiles(int32_t batch, int32_t frames, int32_t num_adapters);
 int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream);
 

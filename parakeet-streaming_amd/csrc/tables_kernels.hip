@@ -26,6 +26,12 @@ namespace pk {
 // queue's front or is itself reached in order: all pushes, then all pops at the
 // prefix sums over the streams, give the queue that the streams one by one give.
 
+// what rows and slot map need of a stream
+struct StepOf {
+  int32_t A, slot, len;  // slot -1: absent
+  uint32_t at;           // pages taken before the stream's
+};
+
 struct PageK {
   int32_t* queue;
   int32_t* head;  // {first entry, entries}
@@ -39,31 +45,37 @@ struct PageK {
   int32_t n, S, total, M, page_shift, chunk, rows_stride;
   int32_t window;
   int32_t reset;  // give every page of the slots back instead
+  StepOf* of;  // more than kStepOne streams: [n]
+  uint32_t* front;
+  uint2* part;  // more than kStepTwo: [npad] pages given back and taken, 0 from n on
+  uint2* at;    // and those before the stream's
+  int32_t npad;
 };
 
 // inclusive sum over the 64 lanes of a wave
-__device__ static inline uint32_t wave_scan(uint32_t v) {
+template <typename T>
+__device__ static inline T wave_scan(T v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t u = (uint32_t)__shfl_up((int)v, d);
+    const T u = __shfl_up(v, d);
     if (lane >= d) v += u;
   }
   return v;
 }
 
 // exclusive sum over a workgroup of NW waves; `sum`: of all
-template <int NW>
-__device__ static inline uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t& sum) {
+template <int NW, typename T>
+__device__ static inline T block_scan(T v, T* lds, T& sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t inc = wave_scan(v);
+  const T inc = wave_scan(v);
   if (lane == 63) lds[wave] = inc;
   __syncthreads();
-  uint32_t before = 0;
+  T before = 0;
   sum = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    const uint32_t x = lds[w];
+    const T x = lds[w];
     if (w < wave) before += x;
     sum += x;
   }
@@ -72,112 +84,269 @@ __device__ static inline uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t
 }
 
 constexpr int kStepThreads = 1024;
+constexpr int kPartPad = 16;
+inline int part_pad(int n) { return (n + kPartPad - 1) / kPartPad * kPartPad; }
+// Streams of a step in one launch (64 take 7.8 us so and 8.8 in two, 128 12 and 10) and in
+// two (2048 take 12.8 us so and 15.6 in four, 4096 16.8 and 17.0, 16384 51 and 26)
+constexpr int kStepOne = 64, kStepTwo = 4096;
 
 struct StreamPages {
-  int64_t A;
+  uint32_t A;
   int32_t slot;  // -1: absent (out of range, or named before in the call)
-  int32_t len, freed, taken, lm, hm;  // ring entries of pages lo and hi
+  int32_t len, freed, taken;
+  uint32_t lo;  // first logical page held
 };
 
-__device__ static inline StreamPages stream_pages(const PageK& p, int b, const uint32_t* dup) {
-  StreamPages r{};
-  const int32_t slot = p.slots[b];
-  r.slot = -1;
-  if ((uint32_t)slot >= (uint32_t)p.S) return r;
-  if (dup[slot >> 5] >> (slot & 31) & 1) {  // rare: the first of equal slots has the step
-    for (int j = 0; j < b; ++j)
-      if (p.slots[j] == slot) return r;
-  }
-  const int64_t a = p.appended[slot];
-  r.slot = slot;
-  r.A = a > 0 ? a : 0;
-  const int32_t want = p.lengths ? p.lengths[b] : p.chunk;
-  r.len = p.reset ? 0 : min(max(want, 0), p.chunk);
-  const int64_t P = (int64_t)1 << p.page_shift, end = r.A + r.len;
-  const int64_t w0 = r.A - p.window, w1 = end - p.window;
-  const int64_t lo = w0 > 0 ? w0 >> p.page_shift : 0, lo2 = w1 > 0 ? w1 >> p.page_shift : 0;
-  const int64_t hi = (r.A + P - 1) >> p.page_shift, hi2 = (end + P - 1) >> p.page_shift;
-  r.freed = (int32_t)((p.reset ? hi : lo2) - lo);
-  r.taken = (int32_t)(hi2 - hi);
-  r.hm = (int32_t)((uint64_t)hi % (uint32_t)p.M);
-  r.lm = r.hm - (int32_t)(hi - lo);
-  if (r.lm < 0) r.lm += p.M;
-  return r;
-}
-
-__global__ void __launch_bounds__(kStepThreads) page_step_kernel(const PageK p) {
-  extern __shared__ uint32_t lds[];
-  __shared__ uint32_t sums[kStepThreads / 64];
+// Bits of the slots that the call names twice (LDS, for the workgroup).
+template <int V>
+__device__ static inline const uint32_t* mark_slots(const PageK& p, uint32_t* lds) {
   const int words = (p.S + 31) >> 5;
   uint32_t* const seen = lds;
   uint32_t* const dup = lds + words;
+  for (int i = threadIdx.x; i < 2 * words; i += kStepThreads) lds[i] = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < p.n; b0 += kStepThreads * V) {
+    int32_t s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int b = b0 + v * kStepThreads + threadIdx.x;
+      s[v] = b < p.n ? p.slots[b] : -1;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if ((uint32_t)s[v] >= (uint32_t)p.S) continue;
+      const uint32_t bit = 1u << (s[v] & 31);
+      if (atomicOr(&seen[s[v] >> 5], bit) & bit) atomicOr(&dup[s[v] >> 5], bit);
+    }
+  }
+  __syncthreads();
+  return dup;
+}
+
+// the first of equal slots has the step (rare)
+__device__ static inline bool named_before(const PageK& p, int b, int32_t slot, const uint32_t* dup) {
+  if ((uint32_t)slot < (uint32_t)p.S && (dup[slot >> 5] >> (slot & 31) & 1))
+    for (int j = 0; j < b; ++j)
+      if (p.slots[j] == slot) return true;
+  return false;
+}
+
+// n pages of a slot, ring entry r on, to place `at` of the queue on; e0: the first one's
+// number where it is at hand
+__device__ static inline void give_back(const PageK& p, int32_t slot, int n, uint32_t r, uint32_t at, const int32_t* e0) {
+  int32_t* const ring = p.ring + (int64_t)slot * p.M;
+  for (int i = 0; i < n; ++i) {
+    p.queue[at] = i == 0 && e0 ? *e0 : ring[r];
+    ring[r] = -1;
+    if (++r == (uint32_t)p.M) r = 0;
+    if (++at == (uint32_t)p.total) at = 0;
+  }
+}
+
+// dup: nullptr where equal slots are looked for later
+__device__ static inline StreamPages stream_pages(const PageK& p, int b, int32_t slot, int32_t want, int64_t a, const uint32_t* dup) {
+  StreamPages r{};
+  r.slot = -1;
+  if ((uint32_t)slot >= (uint32_t)p.S || (dup && named_before(p, b, slot, dup))) return r;
+  r.slot = slot;
+  r.A = (uint32_t)min(max(a, (int64_t)0), (int64_t)0x7fffffff);
+  r.len = p.reset ? 0 : min(max(want, 0), p.chunk);
+  const uint32_t P1 = (1u << p.page_shift) - 1u, end = r.A + r.len;  // below 2^32
+  const uint32_t lo2 = end > (uint32_t)p.window ? (end - p.window) >> p.page_shift : 0;
+  const uint32_t hi = (r.A >> p.page_shift) + ((r.A & P1) != 0), hi2 = (end >> p.page_shift) + ((end & P1) != 0);
+  r.lo = r.A > (uint32_t)p.window ? (r.A - p.window) >> p.page_shift : 0;
+  r.freed = (int32_t)((p.reset ? hi : lo2) - r.lo);
+  r.taken = (int32_t)(hi2 - hi);
+  return r;
+}
+
+// The streams' part of a step that has to be in order, by one workgroup: who is absent,
+// the sums over the streams, the pages given back, the frame counts.  1024 V streams a
+// turn, V neighbours a lane: a turn is one chain of round trips (slots, frame counts, the
+// sum over the workgroup, rings).
+template <int V>
+__device__ static inline void step_scan(const PageK& p, uint32_t* lds, uint64_t* sums, StepOf* of, uint32_t& front) {
   const int tid = threadIdx.x;
-  for (int i = tid; i < 2 * words; i += kStepThreads) lds[i] = 0;
-  const int per = (p.n + kStepThreads - 1) / kStepThreads;
-  const int b0 = min(tid * per, p.n), b1 = min(b0 + per, p.n);
-  __syncthreads();
-  for (int b = b0; b < b1; ++b) {
-    const int32_t s = p.slots[b];
-    if ((uint32_t)s >= (uint32_t)p.S) continue;
-    const uint32_t bit = 1u << (s & 31);
-    if (atomicOr(&seen[s >> 5], bit) & bit) atomicOr(&dup[s >> 5], bit);
-  }
-  __syncthreads();
-  uint32_t f = 0, t = 0;
-  for (int b = b0; b < b1; ++b) {
-    const StreamPages s = stream_pages(p, b, dup);
-    f += s.freed;
-    t += s.taken;
-  }
-  uint32_t fsum, tsum;
-  f = block_scan<kStepThreads / 64>(f, sums, fsum);
-  t = block_scan<kStepThreads / 64>(t, sums, tsum);
+  const uint32_t* dup = mark_slots<V>(p, lds);
   const uint32_t total = (uint32_t)p.total, first = (uint32_t)p.head[0] % total, count = (uint32_t)p.head[1];
-  uint32_t at = first + count % total + f;
-  for (int b = b0; b < b1; ++b) {
-    const StreamPages s = stream_pages(p, b, dup);
-    int32_t* const ring = p.ring + (int64_t)s.slot * p.M;
-    for (int i = 0; i < s.freed; ++i) {
-      int r = s.lm + i;
-      if (r >= p.M) r -= p.M;
-      p.queue[at++ % total] = ring[r];
-      ring[r] = -1;
+  const uint32_t back = (first + count % total) % total;
+  uint32_t fcarry = 0, tcarry = 0;
+  for (int b0 = 0; b0 < p.n; b0 += kStepThreads * V) {
+    const int b = b0 + tid * V;
+    int32_t slot[V], want[V];
+    int64_t a[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      slot[v] = b + v < p.n ? p.slots[b + v] : -1;
+      want[v] = p.lengths && b + v < p.n ? p.lengths[b + v] : p.chunk;
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = (uint32_t)slot[v] < (uint32_t)p.S ? p.appended[slot[v]] : 0;
+    StreamPages s[V];
+    uint64_t both = 0;  // pages given back and taken: each sum is below 2^32, two in one
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      s[v] = stream_pages(p, b + v, slot[v], want[v], a[v], dup);
+      both += (uint64_t)(uint32_t)s[v].freed << 32 | (uint32_t)s[v].taken;
+    }
+    // the first page given back of each stream, on its way while the sums meet
+    uint32_t r0[V];
+    int32_t e0[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      r0[v] = s[v].lo % (uint32_t)p.M;
+      e0[v] = s[v].freed > 0 ? p.ring[(int64_t)s[v].slot * p.M + r0[v]] : 0;
+    }
+    uint64_t all;
+    both = block_scan<kStepThreads / 64>(both, sums, all);
+    uint32_t f = fcarry + (uint32_t)(both >> 32), t = tcarry + (uint32_t)both;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (s[v].freed > 0) give_back(p, s[v].slot, s[v].freed, r0[v], (back + f) % total, &e0[v]);
+      if (of && b + v < p.n) of[b + v] = StepOf{(int32_t)s[v].A, s[v].slot, s[v].len, t};
+      if (s[v].slot >= 0) p.appended[s[v].slot] = p.reset ? 0 : (int64_t)s[v].A + s[v].len;
+      f += s[v].freed;
+      t += s[v].taken;
+    }
+    fcarry += (uint32_t)(all >> 32);
+    tcarry += (uint32_t)all;
   }
-  __syncthreads();  // every page given back is in the queue
-  at = first + t;
+  front = first;
+  if (tid == 0) {
+    p.head[0] = (int32_t)((first + tcarry) % total);
+    p.head[1] = (int32_t)(count + fcarry - tcarry);
+  }
+}
+
+// Rows and slot map of a stream by a group of 32 lanes, an entry a lane: ring entry, or the page
+// from the queue's front where the entry is one that the step takes.
+__device__ static inline void step_rows(const PageK& p, int b, const StepOf s, uint32_t front, int lane) {
+  const uint32_t total = (uint32_t)p.total;
   const int P1 = (1 << p.page_shift) - 1;
-  for (int b = b0; b < b1; ++b) {
-    const StreamPages s = stream_pages(p, b, dup);
-    int32_t* const ring = p.ring + (int64_t)s.slot * p.M;
-    for (int i = 0; i < s.taken; ++i) {
-      int r = s.hm + i;
-      if (r >= p.M) r -= p.M;
-      ring[r] = p.queue[at++ % total];
-    }
-    if (!p.reset) {
-      int32_t* const row = p.rows + (int64_t)b * p.rows_stride;
-      int32_t* const map = p.slot_map + b * p.map_stride;
-      row[0] = (int32_t)s.A;
-      for (int r = 0; r < p.M; ++r) row[1 + r] = s.slot < 0 ? -1 : ring[r];
-      const int64_t hi = (s.A + P1) >> p.page_shift;
-      for (int i = 0; i < p.chunk; ++i) {
-        const int64_t pos = s.A + i;
-        int r = s.hm + (int)((pos >> p.page_shift) - hi);  // -1: the page that A ends in
-        r = r < 0 ? r + p.M : r >= p.M ? r - p.M : r;
-        map[i] = i < s.len ? (ring[r] << p.page_shift) + (int)(pos & P1) : -1;
+  const uint32_t hi = ((uint32_t)s.A + P1) >> p.page_shift, hi2 = ((uint32_t)s.A + s.len + P1) >> p.page_shift;
+  const int hm = (int)(hi % (uint32_t)p.M), taken = s.slot < 0 ? 0 : (int)(hi2 - hi);
+  int32_t* const ring = p.ring + (int64_t)s.slot * p.M;
+  // page of the d-th logical page from hi on (-1: the one that A ends in)
+  auto page = [&](int d, int r) { return d >= 0 && d < taken ? p.queue[(front + s.at + d) % total] : s.slot < 0 ? -1 : ring[r]; };
+  int32_t* const row = p.rows + (int64_t)b * p.rows_stride;
+  for (int i = lane; i < 1 + p.M; i += 32) {
+    const int r = i - 1, d = r >= hm ? r - hm : r - hm + p.M;
+    const int v = i == 0 ? s.A : page(d, r);
+    row[i] = v;
+    if (i > 0 && d < taken) ring[r] = v;
+  }
+  int32_t* const map = p.slot_map + b * p.map_stride;
+  for (int t = lane; t < p.chunk; t += 32) {
+    const uint32_t pos = (uint32_t)s.A + t;
+    const int d = (int)((pos >> p.page_shift) - hi);
+    int r = hm + d;
+    r = r < 0 ? r + p.M : r >= p.M ? r - p.M : r;
+    map[t] = t < s.len ? (page(d, r) << p.page_shift) + (int)(pos & P1) : -1;
+  }
+}
+
+// A step of up to kStepOne streams, and a reset, in one launch: bound by its chain of
+// round trips to memory (slots, frame counts, rings, queue).
+__global__ void __launch_bounds__(kStepThreads) page_step_kernel(const PageK p) {
+  extern __shared__ uint32_t lds[];
+  __shared__ uint64_t sums[kStepThreads / 64];
+  __shared__ StepOf of[kStepOne];
+  uint32_t front;
+  step_scan<1>(p, lds, sums, p.reset ? nullptr : of, front);
+  if (p.reset) return;
+  __syncthreads();  // every page given back is in the queue
+  for (int b = threadIdx.x >> 5; b < p.n; b += kStepThreads / 32) step_rows(p, b, of[b], front, threadIdx.x & 31);
+}
+
+// More streams: the part in order by one workgroup, rows and slot map by all of them in a
+// second launch.
+__global__ void __launch_bounds__(kStepThreads) page_scan_kernel(const PageK p) {
+  extern __shared__ uint32_t lds[];
+  __shared__ uint64_t sums[kStepThreads / 64];
+  uint32_t front;
+  step_scan<4>(p, lds, sums, p.of, front);
+  if (threadIdx.x == 0) *p.front = front;
+}
+__global__ void __launch_bounds__(256) page_rows_kernel(const PageK p) {
+  const int b = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (b < p.n) step_rows(p, b, p.of[b], *p.front, threadIdx.x & 31);
+}
+
+// Thousands of streams: one CU's scattered reads (0.6 a ns) of their frame counts and
+// rings would be the step (16384 streams: 44 us), so only the sums are one workgroup's:
+// what each stream gives and takes, their sums, the pages given back, the rows, a launch
+// each.
+__global__ void __launch_bounds__(256) page_part_kernel(const PageK p) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= p.n) {
+    if (b < p.npad) p.part[b] = uint2{0, 0};
+    return;
+  }
+  const int32_t slot = p.slots[b], want = p.lengths ? p.lengths[b] : p.chunk;
+  const StreamPages s = stream_pages(p, b, slot, want, (uint32_t)slot < (uint32_t)p.S ? p.appended[slot] : 0, nullptr);
+  p.of[b] = StepOf{(int32_t)s.A, s.slot, s.len, 0};
+  p.part[b] = uint2{(uint32_t)s.freed, (uint32_t)s.taken};
+}
+
+// V neighbouring streams a lane, 16384 a turn: a turn is one chain of round trips
+__global__ void __launch_bounds__(kStepThreads) page_sums_kernel(const PageK p) {
+  constexpr int V = kPartPad;
+  extern __shared__ uint32_t lds[];
+  __shared__ uint64_t sums[kStepThreads / 64];
+  const uint32_t* dup = mark_slots<V>(p, lds);
+  uint32_t twice = 0;
+  for (int i = threadIdx.x; i < (p.S + 31) >> 5; i += kStepThreads) twice |= dup[i];
+  if (__syncthreads_or(twice)) {
+    for (int b = threadIdx.x; b < p.n; b += kStepThreads)
+      if (named_before(p, b, p.slots[b], dup)) {
+        p.part[b] = uint2{0, 0};
+        p.of[b] = StepOf{0, -1, 0, 0};
+      }
+    __syncthreads();
+  }
+  const uint32_t total = (uint32_t)p.total, first = (uint32_t)p.head[0] % total, count = (uint32_t)p.head[1];
+  uint64_t carry = 0;
+  for (int b0 = 0; b0 < p.n; b0 += kStepThreads * V) {
+    const int b = b0 + threadIdx.x * V;
+    u32x4 s[V / 2];
+    uint64_t run = 0, all;
+#pragma unroll
+    for (int v = 0; v < V / 2; ++v) s[v] = b < p.n ? ld16(p.part + b + v * 2) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int v = 0; v < V / 2; ++v) run += (uint64_t)(s[v].x + s[v].z) << 32 | (s[v].y + s[v].w);
+    run = block_scan<kStepThreads / 64>(run, sums, all) + carry;
+    uint32_t f = (uint32_t)(run >> 32), t = (uint32_t)run;
+    if (b < p.n) {
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        const u32x4 at = {f, t, f + s[v].x, t + s[v].y};
+        st16(p.at + b + v * 2, at);
+        f += s[v].x + s[v].z;
+        t += s[v].y + s[v].w;
       }
     }
+    carry += all;
   }
-  __syncthreads();  // every stream's frame count was read
-  for (int b = b0; b < b1; ++b) {
-    const StreamPages s = stream_pages(p, b, dup);
-    if (s.slot >= 0) p.appended[s.slot] = p.reset ? 0 : s.A + s.len;
+  if (threadIdx.x == 0) {
+    p.front[0] = first;
+    p.front[1] = (first + count % total) % total;
+    p.head[0] = (int32_t)((first + (uint32_t)carry) % total);
+    p.head[1] = (int32_t)(count + (uint32_t)(carry >> 32) - (uint32_t)carry);
   }
-  if (tid == 0) {
-    p.head[0] = (int32_t)((first + tsum) % total);
-    p.head[1] = (int32_t)(count + fsum - tsum);
+}
+
+__global__ void __launch_bounds__(256) page_back_kernel(const PageK p) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= p.n) return;
+  const StepOf s = p.of[b];
+  if (s.slot < 0) return;
+  const uint2 part = p.part[b], at = p.at[b];
+  if (part.x) {
+    const uint32_t A = (uint32_t)s.A, lo = A > (uint32_t)p.window ? (A - p.window) >> p.page_shift : 0;
+    give_back(p, s.slot, part.x, lo % (uint32_t)p.M, (p.front[1] + at.x) % (uint32_t)p.total, nullptr);
   }
+  p.of[b].at = at.y;
+  p.appended[s.slot] = (int64_t)(uint32_t)s.A + s.len;
 }
 
 // ---------------------------------------------------------------------------
@@ -190,7 +359,8 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(const PageK p) 
 // without an adapter are bucket G.
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr int kPlanTile = 32;  // rows of a tile
+constexpr int kPlanTile = 32;    // rows of a tile
+constexpr int kPlanOne = 4096;   // rows of a plan in one launch
 
 struct PlanK {
   const int32_t* ids;
@@ -198,7 +368,24 @@ struct PlanK {
   int32_t* sorted;
   int4* tiles;
   int32_t B, T, G, max_tiles, bits;
+  int2* by;  // {stream, adapter} by position, where rows and tiles are a second launch's
+  uint32_t* tab;  // its tables: start [G + 1], tile0 [G + 1]
 };
+
+// rows of a tile t: the adapter whose tiles it is among (bisection over their first tiles)
+__device__ static inline int4 plan_tile(const PlanK& p, const uint32_t* start, const uint32_t* tile0, int t) {
+  if ((uint32_t)t >= tile0[p.G]) return int4{-1, 0, 0, 0};
+  int lo = 0, hi = p.G;  // tile0[lo] <= t < tile0[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile0[mid] <= (uint32_t)t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int off = (t - (int)tile0[lo]) * kPlanTile;
+  return int4{lo, (int)start[lo] * p.T + off, min(kPlanTile, (int)(start[lo + 1] - start[lo]) * p.T - off), 0};
+}
 
 __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const PlanK p) {
   extern __shared__ uint32_t lds[];
@@ -259,32 +446,35 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const PlanK 
     if (in && (same >> lane) == 1) *h = base + __popcll(same);  // the last of the equal ones
     wave_lds_sync();
     if (in) {
-      const int64_t at = (int64_t)(base + __popcll(same & below)) * p.T;
-      for (int t = 0; t < p.T; ++t) {
-        p.order[at + t] = (b + lane) * p.T + t;
-        p.sorted[at + t] = has ? id : -1;
+      const int32_t at = (int32_t)(base + __popcll(same & below));
+      if (p.by) {
+        p.by[at] = int2{b + lane, has ? id : -1};
+      } else {
+        for (int t = 0; t < p.T; ++t) {
+          p.order[at * p.T + t] = (b + lane) * p.T + t;
+          p.sorted[at * p.T + t] = has ? id : -1;
+        }
       }
     }
   }
-  // tile t: the adapter whose tiles it is among (bisection over their first tiles)
-  for (int t = tid; t < p.max_tiles; t += kPlanThreads) {
-    int4 v = {-1, 0, 0, 0};
-    if ((uint32_t)t < tcarry) {
-      int lo = 0, hi = p.G;  // tile0[lo] <= t < tile0[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tile0[mid] <= (uint32_t)t)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      const int off = (t - (int)tile0[lo]) * kPlanTile;
-      v.x = lo;
-      v.y = (int)start[lo] * p.T + off;
-      v.z = min(kPlanTile, (int)(start[lo + 1] - start[lo]) * p.T - off);
-    }
-    p.tiles[t] = v;
+  if (p.by) {
+    for (int i = tid; i < 2 * G1; i += kPlanThreads) p.tab[i] = i < G1 ? start[i] : tile0[i - G1];
+    return;
   }
+  for (int t = tid; t < p.max_tiles; t += kPlanThreads) p.tiles[t] = plan_tile(p, start, tile0, t);
+}
+
+// Many rows: theirs and the tiles in a second launch, by all CUs (57344 rows in 512 buckets:
+// one workgroup stores 0.5 MB in 50 us).
+__global__ void __launch_bounds__(256) adapter_rows_kernel(const PlanK p) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < p.B * p.T) {
+    const int s = i / p.T;
+    const int2 v = p.by[s];
+    p.order[i] = v.x * p.T + (i - s * p.T);
+    p.sorted[i] = v.y;
+  }
+  if (i < p.max_tiles) p.tiles[i] = plan_tile(p, p.tab, p.tab + p.G + 1, i);
 }
 
 namespace {
@@ -318,6 +508,9 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
     if (a->rows_stride < 1 + M || a->slot_map_stride < a->chunk)
       return fail(PK_ERR_INVALID, "%s: need rows_stride >= %d and slot_map_stride >= %d", what, 1 + M, a->chunk);
   }
+  const bool two = !a->reset && a->batch > kStepOne;
+  if (two && (!a->workspace || !aligned16(a->workspace)))
+    return fail(PK_ERR_INVALID, "%s: workspace must be non-NULL and 16-byte aligned for %d streams", what, a->batch);
   PageK k{};
   k.queue = a->queue;
   k.head = a->head;
@@ -337,10 +530,29 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
   k.rows_stride = a->rows_stride;
   k.window = a->left + a->chunk;
   k.reset = a->reset ? 1 : 0;
+  if (two) {
+    k.of = static_cast<StepOf*>(a->workspace);
+    k.front = reinterpret_cast<uint32_t*>(k.of + k.n);
+    k.part = reinterpret_cast<uint2*>(k.of + k.n + 1);
+    k.npad = part_pad(k.n);
+    k.at = k.part + k.npad;
+  }
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const size_t bits = (size_t)((k.S + 31) / 32) * 8;
-  hipLaunchKernelGGL(page_step_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
+  if (!two) {
+    hipLaunchKernelGGL(page_step_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
+    return check_launch(what);
+  }
+  const dim3 all((unsigned)((k.npad + 255) / 256));
+  if (k.n <= kStepTwo) {
+    hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
+  } else {
+    hipLaunchKernelGGL(page_part_kernel, all, dim3(256), 0, s, k);
+    hipLaunchKernelGGL(page_sums_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
+    hipLaunchKernelGGL(page_back_kernel, all, dim3(256), 0, s, k);
+  }
+  hipLaunchKernelGGL(page_rows_kernel, dim3((unsigned)((k.n + 7) / 8)), dim3(256), 0, s, k);
   return check_launch(what);
 }
 
@@ -366,15 +578,29 @@ int adapter_plan(const pk_adapter_plan_args* a, hipStream_t s) {
   k.G = a->num_adapters;
   k.max_tiles = a->max_tiles;
   while ((1 << k.bits) <= k.G) ++k.bits;
+  if (pk_adapter_plan_workspace_bytes(k.B, k.T, k.G) > 0) {
+    if (!a->workspace || !aligned16(a->workspace))
+      return fail(PK_ERR_INVALID, "%s: workspace must be non-NULL and 16-byte aligned for %d rows", what, k.B * k.T);
+    k.by = static_cast<int2*>(a->workspace);
+    k.tab = reinterpret_cast<uint32_t*>(k.by + k.B);
+  }
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const size_t lds = sizeof(uint32_t) * ((size_t)kPlanWaves * (k.G + 1) + 2 * (k.G + 2));
   hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanThreads), lds, s, k);
+  int rc = check_launch(what);
+  if (rc != PK_OK || !k.by) return rc;
+  const int rows = k.B * k.T > k.max_tiles ? k.B * k.T : k.max_tiles;
+  hipLaunchKernelGGL(adapter_rows_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, k);
   return check_launch(what);
 }
 
 }  // namespace
 }  // namespace pk
+
+extern "C" int64_t pk_page_step_workspace_bytes(int32_t batch) {
+  return batch > pk::kStepOne ? ((int64_t)batch + 1) * sizeof(pk::StepOf) + (int64_t)pk::part_pad(batch) * 2 * sizeof(uint2) : 0;
+}
 
 extern "C" int pk_page_step(const pk_page_step_args* args, void* stream) {
   pk::clear_error();
@@ -385,6 +611,11 @@ extern "C" int pk_page_step(const pk_page_step_args* args, void* stream) {
 extern "C" int pk_adapter_plan_tiles(int32_t batch, int32_t frames, int32_t num_adapters) {
   if (batch <= 0 || frames <= 0 || num_adapters <= 0) return 0;
   return (int)((int64_t)batch * frames / pk::kPlanTile + (num_adapters < batch ? num_adapters : batch));
+}
+
+extern "C" int64_t pk_adapter_plan_workspace_bytes(int32_t batch, int32_t frames, int32_t num_adapters) {
+  if (batch <= 0 || frames <= 0 || num_adapters <= 0 || (int64_t)batch * frames <= pk::kPlanOne) return 0;
+  return (int64_t)batch * sizeof(int2) + 2 * ((int64_t)num_adapters + 1) * sizeof(uint32_t);
 }
 
 extern "C" int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream) {

@@ -399,6 +399,7 @@ class PageStepArgs(ctypes.Structure):
         ("rows_stride", c_int32),
         ("slot_map", c_void_p),
         ("slot_map_stride", c_int64),
+        ("workspace", c_void_p),
     ]
 
 
@@ -432,6 +433,7 @@ class AdapterPlanArgs(ctypes.Structure):
         ("sorted_ids", c_void_p),
         ("tiles", c_void_p),
         ("max_tiles", c_int32),
+        ("workspace", c_void_p),
     ]
 
 
@@ -480,9 +482,11 @@ SIGNATURES = {
     "pk_rnnt_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "pk_rnnt_greedy_step": (c_int, [POINTER(RnntArgs), c_void_p]),
     "pk_rnnt_greedy_step_static": (c_int, [POINTER(RnntArgs), c_void_p]),
+    "pk_page_step_workspace_bytes": (c_int64, [c_int32]),
     "pk_page_step": (c_int, [POINTER(PageStepArgs), c_void_p]),
     "pk_kv_append_slots": (c_int, [POINTER(KvAppendSlotsArgs), c_void_p]),
     "pk_adapter_plan_tiles": (c_int, [c_int32, c_int32, c_int32]),
+    "pk_adapter_plan_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "pk_adapter_plan": (c_int, [POINTER(AdapterPlanArgs), c_void_p]),
     "pk_adapter_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),

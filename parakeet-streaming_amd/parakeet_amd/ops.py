@@ -1085,9 +1085,24 @@ def subsample(
 # the tables of a batch, built on the device
 
 
-def _i32(t: torch.Tensor, name: str, shape: tuple) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+_INT32 = torch.int32
+
+
+def _i32(t: torch.Tensor, name: str, shape: tuple) -> int:
+    """The address of a contiguous int32 tensor of ``shape``."""
+    if t.dtype is not _INT32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _on(dev: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {name} is on {t.device}, not {dev}")
+
+
+def _index(dev: torch.device) -> int:
+    return torch.cuda.current_device() if dev.index is None else dev.index
 
 
 @dataclass
@@ -1109,29 +1124,21 @@ class PageState:
     def max_pages(self) -> int:
         return (self.left + self.chunk + self.page_size - 2) // self.page_size + 1
 
-    def _args(self) -> tuple[PageStepArgs, torch.device]:
-        if self.page_size <= 0 or self.left < 0 or self.chunk <= 0:
-            raise ValueError(f"need page_size > 0, left >= 0 and chunk > 0, got {self.page_size}, {self.left}, {self.chunk}")
-        S = self.appended.shape[0] if self.appended.dim() == 1 else -1
-        if S <= 0 or self.appended.dtype != torch.int64 or not self.appended.is_contiguous():
-            raise ValueError(f"appended must be contiguous int64 [num_slots], got {tuple(self.appended.shape)} {self.appended.dtype}")
-        _i32(self.queue, "queue", (self.queue.numel(),))
-        _i32(self.head, "head", (2,))
-        _i32(self.ring, "ring", (S, self.max_pages))
+    def _args(self) -> tuple[PageStepArgs, torch.device, int]:
+        P, left, chunk, A = self.page_size, self.left, self.chunk, self.appended
+        if P <= 0 or left < 0 or chunk <= 0:
+            raise ValueError(f"need page_size > 0, left >= 0 and chunk > 0, got {P}, {left}, {chunk}")
+        if A.dim() != 1 or A.dtype is not torch.int64 or not A.is_contiguous():
+            raise ValueError(f"appended must be contiguous int64 [num_slots], got {tuple(A.shape)} {A.dtype}")
+        M = self.max_pages
         a = PageStepArgs()
-        a.num_slots, a.num_pages = S, self.queue.numel()
-        a.page_size, a.left, a.chunk = self.page_size, self.left, self.chunk
-        a.queue, a.head, a.appended, a.ring = self.queue.data_ptr(), self.head.data_ptr(), self.appended.data_ptr(), self.ring.data_ptr()
-        dev = _require_device(self.queue, self.head, self.appended, self.ring)
-        a.device = dev.index if dev.index is not None else torch.cuda.current_device()
-        return a, dev
-
-
-def _vector(t: torch.Tensor, name: str, n: int, dev: torch.device) -> int:
-    _i32(t, name, (n,))
-    if t.device != dev:
-        raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    return t.data_ptr()
+        a.num_slots, a.num_pages = S, N = A.shape[0], self.queue.numel()
+        a.page_size, a.left, a.chunk = P, left, chunk
+        a.queue, a.head = _i32(self.queue, "queue", (N,)), _i32(self.head, "head", (2,))
+        a.appended, a.ring = A.data_ptr(), _i32(self.ring, "ring", (S, M))
+        dev = _require_device(A, self.queue, self.head, self.ring)
+        a.device = _index(dev)
+        return a, dev, M
 
 
 def page_step(
@@ -1151,32 +1158,37 @@ def page_step(
     a stream's frames) for :func:`kv_append_slots`.  A slot out of range or named
     earlier in the call is absent (rows {0, -1 ...}, slot_map -1, nothing changed).
     No host work and no synchronisation: a step may be recorded in a graph."""
-    a, dev = state._args()
+    a, dev, M = state._args()
     if slots.dim() != 1:
         raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
-    B, M = slots.shape[0], state.max_pages
-    a.batch, a.slots = B, _vector(slots, "slots", B, dev)
-    a.lengths = None if lengths is None else _vector(lengths, "lengths", B, dev)
+    B, T = slots.shape[0], state.chunk
+    a.batch, a.slots = B, _i32(slots, "slots", (B,))
+    if lengths is not None:
+        a.lengths = _i32(lengths, "lengths", (B,))
     if rows is None:
-        rows = torch.empty((B, 1 + M), dtype=torch.int32, device=dev)
+        rows = torch.empty((B, 1 + M), dtype=_INT32, device=dev)
     if slot_map is None:
-        slot_map = torch.empty((B, state.chunk), dtype=torch.int32, device=dev)
-    _i32(rows, "rows", (B, 1 + M))
-    _i32(slot_map, "slot_map", (B, state.chunk))
-    if rows.device != dev or slot_map.device != dev:
-        raise ValueError(f"rows and slot_map must be on {dev}")
-    a.rows, a.rows_stride, a.slot_map, a.slot_map_stride = rows.data_ptr(), 1 + M, slot_map.data_ptr(), state.chunk
-    check(lib().pk_page_step(ctypes.byref(a), _stream(dev)), "pk_page_step")
+        slot_map = torch.empty((B, T), dtype=_INT32, device=dev)
+    a.rows, a.slot_map = _i32(rows, "rows", (B, 1 + M)), _i32(slot_map, "slot_map", (B, T))
+    _on(dev, slots=slots, lengths=lengths, rows=rows, slot_map=slot_map)
+    a.rows_stride, a.slot_map_stride = 1 + M, T
+    L = lib()
+    n = L.pk_page_step_workspace_bytes(B)
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+    check(L.pk_page_step(ctypes.byref(a), _stream(dev)), "pk_page_step")
     return rows, slot_map
 
 
 def page_reset(state: PageState, slots: torch.Tensor) -> None:
     """Gives every page of ``slots`` (int32 [B]) back to the queue, slot after slot, and
     sets their frame counts to 0 (``PagePool.reset_slot``)."""
-    a, dev = state._args()
+    a, dev, _ = state._args()
     if slots.dim() != 1:
         raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
-    a.batch, a.slots, a.reset = slots.shape[0], _vector(slots, "slots", slots.shape[0], dev), 1
+    a.batch, a.slots, a.reset = slots.shape[0], _i32(slots, "slots", (slots.shape[0],)), 1
+    _on(dev, slots=slots)
     check(lib().pk_page_step(ctypes.byref(a), _stream(dev)), "pk_page_step")
 
 
@@ -1185,31 +1197,31 @@ def kv_append_slots(pages: PagedKV, layer: int, key: torch.Tensor, value: torch.
     names: page * page_size + row of the page, below 0 for a row that is not written
     (:func:`page_step`'s map for [B, T, D]; packed rows [N, D] take its valid entries one
     after another).  Places of one call are distinct.  ``pages.rows`` is not read."""
-    kp = pages.k_pool
-    D = kp.shape[3] if kp.dim() == 4 else 0
-    lead = tuple(slot_map.shape)
-    if len(lead) not in (1, 2) or slot_map.dtype != torch.int32 or (slot_map.numel() and slot_map.stride(-1) != 1):
-        raise ValueError(f"slot_map must be int32 [N] or [B, T] with unit inner stride, got {lead} {slot_map.dtype}")
+    kp, lead = pages.k_pool, slot_map.shape
+    dt, D, packed = kp.dtype, kp.shape[-1], len(lead) == 1
+    if not 1 <= len(lead) <= 2 or slot_map.dtype is not _INT32 or (slot_map.stride(-1) != 1 and slot_map.numel()):
+        raise ValueError(f"slot_map must be int32 [N] or [B, T] with unit inner stride, got {tuple(lead)} {slot_map.dtype}")
     for name, t in (("key", key), ("value", value)):
-        if tuple(t.shape) != (*lead, D):
+        if t.shape != (*lead, D):
             raise ValueError(f"{name}: expected shape {(*lead, D)}, got {tuple(t.shape)}")
-        if t.dtype != kp.dtype:
-            raise TypeError(f"{name}: dtype {t.dtype} != {kp.dtype}")
+        if t.dtype is not dt:
+            raise TypeError(f"{name}: dtype {t.dtype} != {dt}")
         if t.stride(-1) != 1 and t.numel():
             raise ValueError(f"{name}: last dimension must be contiguous")
-    dev = _require_device(key, value, kp, pages.v_pool, slot_map)
-    a = KvAppendSlotsArgs()
-    a.dtype = dtype_code(kp.dtype)
-    a.device = dev.index if dev.index is not None else torch.cuda.current_device()
-    a.pages = pages.layout()
-    a.layer = int(layer)
+    dev = _require_device(kp, pages.v_pool, key, value, slot_map)
     if slot_map.numel() == 0:
         return
-    packed = len(lead) == 1
-    a.batch, a.chunk = (1, lead[0]) if packed else lead
-    a.key, a.key_stride_b, a.key_stride_t = key.data_ptr(), 0 if packed else key.stride(0), key.stride(-2)
-    a.value, a.value_stride_b, a.value_stride_t = value.data_ptr(), 0 if packed else value.stride(0), value.stride(-2)
-    a.slot_map, a.slot_map_stride_b = slot_map.data_ptr(), 0 if packed else slot_map.stride(0)
+    a = KvAppendSlotsArgs()
+    a.dtype, a.device, a.pages, a.layer = dtype_code(dt), _index(dev), pages.layout(), int(layer)
+    a.key, a.value, a.slot_map = key.data_ptr(), value.data_ptr(), slot_map.data_ptr()
+    if packed:
+        a.batch, a.chunk = 1, lead[0]
+        a.key_stride_t, a.value_stride_t = key.stride(0), value.stride(0)
+    else:
+        a.batch, a.chunk = lead
+        a.key_stride_b, a.key_stride_t, _ = key.stride()
+        a.value_stride_b, a.value_stride_t, _ = value.stride()
+        a.slot_map_stride_b = slot_map.stride(0)
     check(lib().pk_kv_append_slots(ctypes.byref(a), _stream(dev)), "pk_kv_append_slots")
 
 
@@ -1233,24 +1245,26 @@ def adapter_plan(ids: torch.Tensor, frames: int = 1, *, num_adapters: int) -> Ad
     """Groups the rows of a batch [B, frames, ...] by the streams' adapters ``ids`` (int32
     [B]; a number outside 0 .. num_adapters - 1 is no adapter).  One launch; the plan
     serves every layer of the step."""
-    if ids.dim() != 1 or ids.dtype != torch.int32 or not ids.is_contiguous():
-        raise ValueError(f"ids must be contiguous int32 [B], got {tuple(ids.shape)} {ids.dtype}")
-    dev = _require_device(ids)
+    if ids.dim() != 1:
+        raise ValueError(f"ids must be int32 [B], got {tuple(ids.shape)}")
     B, T, G = ids.shape[0], int(frames), int(num_adapters)
-    if T <= 0 or G <= 0 or B * T >= 1 << 31:
+    at, M = _i32(ids, "ids", (B,)), B * T
+    dev = _require_device(ids)
+    if T <= 0 or G <= 0 or M >= 1 << 31:
         raise ValueError(f"need frames and num_adapters > 0 and fewer than 2^31 rows, got {B} x {T}, {G}")
-    M = B * T
-    tiles = M // 32 + min(G, B)
+    n = M // 32 + min(G, B)
     a = AdapterPlanArgs()
-    a.device = dev.index if dev.index is not None else torch.cuda.current_device()
-    a.batch, a.frames, a.num_adapters, a.max_tiles = B, T, G, tiles
+    a.device, a.batch, a.frames, a.num_adapters, a.max_tiles = _index(dev), B, T, G, n
     p = AdapterPlan(
-        torch.empty(M, dtype=torch.int32, device=dev),
-        torch.empty(M, dtype=torch.int32, device=dev),
-        torch.empty((tiles, 4), dtype=torch.int32, device=dev),
+        torch.empty(M, dtype=_INT32, device=dev), torch.empty(M, dtype=_INT32, device=dev), torch.empty((n, 4), dtype=_INT32, device=dev)
     )
-    a.ids, a.order, a.sorted_ids, a.tiles = ids.data_ptr(), p.order.data_ptr(), p.ids.data_ptr(), p.tiles.data_ptr()
-    check(lib().pk_adapter_plan(ctypes.byref(a), _stream(dev)), "pk_adapter_plan")
+    a.ids, a.order, a.sorted_ids, a.tiles = at, p.order.data_ptr(), p.ids.data_ptr(), p.tiles.data_ptr()
+    L = lib()
+    n = L.pk_adapter_plan_workspace_bytes(B, T, G)
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+    check(L.pk_adapter_plan(ctypes.byref(a), _stream(dev)), "pk_adapter_plan")
     return p
 
 
@@ -1279,8 +1293,8 @@ def adapter_linear(
     stream beside it.  fp16 and bf16: two launches, one rounding of the output; fp32:
     torch's linear, then two launches.  x [..., K], weight [N, K], bias [N] or None; N
     and K multiples of 64, ranks of 8 up to 128.  No gradients."""
-    A, Bm, scale = adapters.a, adapters.b, adapters.scale
-    dt, dev = x.dtype, _require_device(x, weight, A, Bm, scale, plan.order, plan.ids, plan.tiles)
+    A, Bm, scale, tiles = adapters.a, adapters.b, adapters.scale, plan.tiles
+    dt, dev = x.dtype, _require_device(x, weight, A, Bm, scale, plan.order, plan.ids, tiles)
     code = dtype_code(dt)
     if x.dim() == 0 or weight.dim() != 2:
         raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
@@ -1288,43 +1302,43 @@ def adapter_linear(
     n, k = weight.shape
     G, r = A.shape[:2] if A.dim() == 3 else (0, 0)
     if (
-        tuple(A.shape) != (G, r, k) or tuple(Bm.shape) != (G, n, r) or A.dtype != dt or Bm.dtype != dt
+        A.shape != (G, r, k) or Bm.shape != (G, n, r) or A.dtype is not dt or Bm.dtype is not dt
         or not A.is_contiguous() or not Bm.is_contiguous()
     ):
         raise ValueError(f"adapters must be contiguous a [G, r, {k}] and b [G, {n}, r] of {dt}, got {tuple(A.shape)} {A.dtype} and "
                          f"{tuple(Bm.shape)} {Bm.dtype}")
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (G,) or not scale.is_contiguous():
+    if scale.dtype is not torch.float32 or scale.shape != (G,) or not scale.is_contiguous():
         raise ValueError(f"scale must be contiguous float32 [{G}], got {tuple(scale.shape)} {scale.dtype}")
     if k % 64 or n % 64 or k == 0 or n == 0 or r % 8 or not 0 < r <= _lib.ADAPTER_MAX_RANK or not 0 < G <= _lib.ADAPTER_MAX:
         raise NotImplementedError(f"built for widths of multiples of 64, ranks of multiples of 8 up to {_lib.ADAPTER_MAX_RANK} and up to "
                                   f"{_lib.ADAPTER_MAX} adapters; got {k} -> {n}, rank {r}, {G} adapters")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, A, Bm, scale)):
+    if (
+        x.requires_grad or weight.requires_grad or A.requires_grad or Bm.requires_grad or scale.requires_grad
+        or (bias is not None and bias.requires_grad)
+    ) and torch.is_grad_enabled():
         raise RuntimeError("adapter_linear has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
-    M = x.numel() // k
-    _i32(plan.order, "plan.order", (M,))
-    _i32(plan.ids, "plan.ids", (M,))
-    tiles = plan.tiles.shape[0] if plan.tiles.dim() == 2 else -1
-    _i32(plan.tiles, "plan.tiles", (tiles, 4))
+    M, T = x.numel() // k, tiles.shape[0] if tiles.dim() == 2 else -1
+    a = AdapterLinearArgs()
+    a.order, a.ids = _i32(plan.order, "plan.order", (M,)), _i32(plan.ids, "plan.ids", (M,))
+    a.tiles, a.max_tiles = _i32(tiles, "plan.tiles", (T, 4)), T
     x = _aligned_rows(x)
     shape = (*x.shape[:-1], n)
-    if out is not None and (tuple(out.shape) != shape or out.dtype != dt or out.device != dev or not out.is_contiguous()):
+    if out is not None and (out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
-    a = AdapterLinearArgs()
-    if dt == torch.float32:
+    if dt is torch.float32:
         y = torch.nn.functional.linear(x, weight, bias)
         out = y if out is None else out.copy_(y)
     else:
         if out is None:
             out = torch.empty(shape, dtype=dt, device=dev)
         a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
-        a.bias = bias.data_ptr() if bias is not None else None
-    ws = torch.empty(lib().pk_adapter_workspace_bytes(M, r, k, tiles), dtype=torch.uint8, device=dev)
-    a.dtype, a.device = code, dev.index if dev.index is not None else torch.cuda.current_device()
-    a.rows, a.n, a.k, a.rank, a.num_adapters = M, n, k, r, G
+        if bias is not None:
+            a.bias = bias.data_ptr()
+    L = lib()
+    ws = torch.empty(L.pk_adapter_workspace_bytes(M, r, k, T), dtype=torch.uint8, device=dev)
+    a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters = code, _index(dev), M, n, k, r, G
     a.activation = _lib.ACT_SILU if silu else _lib.ACT_NONE
-    a.x, a.x_stride = x.data_ptr(), k
-    a.a, a.b, a.scale = A.data_ptr(), Bm.data_ptr(), scale.data_ptr()
-    a.order, a.ids, a.tiles, a.max_tiles = plan.order.data_ptr(), plan.ids.data_ptr(), plan.tiles.data_ptr(), tiles
-    a.workspace, a.out, a.out_stride = ws.data_ptr(), out.data_ptr(), n
-    check(lib().pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
+    a.x, a.x_stride, a.out, a.out_stride = x.data_ptr(), k, out.data_ptr(), n
+    a.a, a.b, a.scale, a.workspace = A.data_ptr(), Bm.data_ptr(), scale.data_ptr(), ws.data_ptr()
+    check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out
