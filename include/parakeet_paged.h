@@ -881,9 +881,7 @@ int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream);
  * aligned.
  * n and k multiples of 64, rank of 8 and at most PK_ADAPTER_MAX_RANK.
  * x, weight, out, the workspace and one adapter's a and b are each below 2^31 bytes.
- * activation: PK_ACT_NONE or PK_ACT_SILU.  fp32 has no product with weight here: out
- * holds the projection with its bias on entry, weight and bias are NULL.
- * out overlaps no operand.
+ * activation: PK_ACT_NONE or PK_ACT_SILU.  out overlaps no operand.
  */
 typedef struct pk_adapter_linear_args {
   int32_t dtype;

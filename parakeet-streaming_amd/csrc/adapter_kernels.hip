@@ -5,7 +5,6 @@
 //   adapter_low_kernel   h = scale_g x A_g^T, a tile of rows of one adapter a workgroup
 //   adapter_tile_kernel  the product with W over rows in the plan's order, the
 //                        h B_g^T of the tile's adapters added to its sums
-//   adapter_add_kernel   fp32: h B_g^T added to a projection that is there
 //
 // Rows are taken in the order of an adapter plan (equal adapters side by side), so 16
 // rows of a matrix instruction have few adapters: with streams of 2 frames in their
@@ -346,17 +345,18 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 #pragma clang fp contract(off)
   constexpr int NW = WM * WN * WK;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int CH = BK / 8;
-  constexpr int kStage = (BM + BN) * BK * 2;
+  constexpr int E = sizeof(ST), V = 16 / E;
+  constexpr int ROW = BK * E, CH = ROW / 16;  // bytes and 16-byte chunks of a row's stage
+  constexpr int kStage = (BM + BN) * ROW;
   constexpr int LPS = kStage / 1024 / NW;
-  static_assert(BK % 64 == 0, "the permutation stays within a row's stage: whole groups of 8 chunks");
+  static_assert(ROW % 128 == 0, "the permutation stays within a row's stage: whole groups of 8 chunks");
   static_assert(kStage % (1024 * NW) == 0 && (BM * CH) % 64 == 0, "whole waves of chunks");
-  constexpr int KS = BK / 32 / WK;
-  constexpr int OS = BN + 8;
-  constexpr int kOut = BM * OS * 2;
+  constexpr int KS = CH / 4 / WK;  // steps of 4 chunks a lane group a wave does a stage
+  constexpr int OS = BN + V;       // LDS row stride of the staged output
+  constexpr int kOut = BM * OS * E;
   constexpr int kRed = WK > 1 ? (WK - 1) * BM * BN * 4 : 0;
   constexpr int kSmem = S * kStage > kOut + kRed ? S * kStage : kOut + kRed;
-  constexpr bool kStaged = BK == 64;
+  constexpr bool kStaged = CH == 8;
   constexpr int RW = (BM + 63) / 64;  // 64-row words of a row mask
   // one LDS object: with a second one the compiler keeps them apart and waits for every
   // load to LDS in flight before an operand read
@@ -383,8 +383,8 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   int id[TM];
 #pragma unroll
   for (int m = 0; m < TM; ++m) id[m] = sid[(wm * TM + m) * 16 + l16];
-  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * 2u);
-  const __amdgpu_buffer_rsrc_t rw = bytes_rsrc(p.w, (uint32_t)((p.N - 1) * p.w_s + p.K) * 2u);
+  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * E);
+  const __amdgpu_buffer_rsrc_t rw = bytes_rsrc(p.w, (uint32_t)((p.N - 1) * p.w_s + p.K) * E);
   // chunk c of a stage: row c / CH of [x rows ; w rows], LDS position c % CH
   uint32_t off[LPS];
 #pragma unroll
@@ -392,13 +392,13 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     const int c = (i * NW + wave) * 64 + lane;
     const int r = c / CH, pos = c % CH;
     const int ch = (pos & ~7) | ((pos ^ r) & 7);
-    off[i] = r < BM ? (uint32_t)(ord[r] * p.x_s + ch * 8) * 2u : (uint32_t)((n0 + r - BM) * p.w_s + ch * 8) * 2u;
+    off[i] = r < BM ? (uint32_t)(ord[r] * p.x_s + ch * V) * E : (uint32_t)((n0 + r - BM) * p.w_s + ch * V) * E;
   }
   auto issue = [&](int st, int k) {
 #pragma unroll
     for (int i = 0; i < LPS; ++i) {
       const int base = (i * NW + wave) * 64;
-      load_lds16(base < BM * CH ? rx : rw, smem + st * kStage + base * 16, off[i], k * 2);
+      load_lds16(base < BM * CH ? rx : rw, smem + st * kStage + base * 16, off[i], k * E);
     }
   };
   // xs, ws of a stage times each other, for the 16-row products that `rows` names
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](int st, uint32_t rows) {
     const unsigned char* xs = smem + st * kStage;
-    const unsigned char* ws = xs + BM * BK * 2;
+    const unsigned char* ws = xs + BM * ROW;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int ch = (wk * KS + s) * 4 + kg;
@@ -417,18 +417,18 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 #pragma unroll
       for (int m = 0; m < TM; ++m) {
         const int r = (wm * TM + m) * 16 + l16;
-        xf[m] = *reinterpret_cast<const u32x4*>(xs + r * BK * 2 + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+        xf[m] = *reinterpret_cast<const u32x4*>(xs + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
       }
 #pragma unroll
       for (int n = 0; n < TN; ++n) {
         const int r = (wn * TN + n) * 16 + l16;
-        wf[n] = *reinterpret_cast<const u32x4*>(ws + r * BK * 2 + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+        wf[n] = *reinterpret_cast<const u32x4*>(ws + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
       }
 #pragma unroll
       for (int m = 0; m < TM; ++m) {
         if (!(rows >> m & 1)) continue;
 #pragma unroll
-        for (int n = 0; n < TN; ++n) acc[m][n] = MmaL<ST>::k32(wf[n], xf[m], acc[m][n]);
+        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(wf[n], xf[m], acc[m][n]);
       }
     }
   };
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
       ld.l[w] = mu.l[w] = last[w];
     }
     ld.j = mu.j = nst;
-    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = (uint32_t)p.r * 2u;
+    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = (uint32_t)p.r * E;
     const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)(p.M + 1) * hrow);
     auto issue_low = [&](int slot) {
       step(ld);
@@ -582,41 +582,18 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
         float f[4] = {acc[m][n].x, acc[m][n].y, acc[m][n].z, acc[m][n].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[e] = ad_act<SILU>(f[e] + b[e]);
-        *reinterpret_cast<u32x2*>(os + ((wm * TM + m) * 16 + l16) * OS + c) = pack4<ST>(f);
+        ST* const o = os + ((wm * TM + m) * 16 + l16) * OS + c;
+        if constexpr (E == 4)
+          *reinterpret_cast<u32x4*>(o) = Tr<float>::pack(f);
+        else
+          *reinterpret_cast<u32x2*>(o) = pack4<ST>(f);
       }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BM * BN / 8; i += 64 * NW) {
-    const int r = i / (BN / 8), c = (i % (BN / 8)) * 8;
+  for (int i = threadIdx.x; i < BM * BN / V; i += 64 * NW) {
+    const int r = i / (BN / V), c = (i % (BN / V)) * V;
     if (row0 + r < p.M) st16(p.out + (int64_t)ord[r] * p.out_s + n0 + c, *reinterpret_cast<const u32x4*>(os + r * OS + c));
-  }
-}
-
-// fp32: out = act(out + h B^T), 16 rows x 64 columns a wave, out read in the layout of
-// the matrix instruction's sums (4 columns of a row a lane).
-template <int SILU>
-__global__ void __launch_bounds__(256) adapter_add_kernel(const AdK<float> p) {
-  constexpr int TN = 4;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l16 = lane & 15, kg = lane >> 4;
-  const int pos = blockIdx.x * 16 + l16, c0 = (blockIdx.y * 4 + wave) * TN * 16;
-  if (c0 >= p.N) return;  // the whole wave; no barrier below
-  int id[1] = {pos < p.M ? p.ids[pos] : -1};
-  if ((uint32_t)id[0] >= (uint32_t)p.G) id[0] = -1;
-  float* const q = p.out + (int64_t)plan_row(p, pos) * p.out_s + c0 + kg * 4;
-  u32x4 base[TN];
-#pragma unroll
-  for (int n = 0; n < TN; ++n) base[n] = ld16(q + n * 16);
-  f32x4_t acc[1][TN];
-  add_low<float, 1, TN, 1, 4>(p, id, blockIdx.x * 16, c0, 0, lane, acc);
-  if (pos >= p.M) return;
-#pragma unroll
-  for (int n = 0; n < TN; ++n) {
-    f32x4_t v = acc[0][n] + __builtin_bit_cast(f32x4_t, base[n]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = ad_act<SILU>(v[e]);
-    st16(q + n * 16, __builtin_bit_cast(u32x4, v));
   }
 }
 
@@ -656,53 +633,56 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
     grid = dim3(8u, (unsigned)(k.mtiles / k.xm), (unsigned)(nt / (8 / k.xm)));
   else
     k.xm = 0;
-  hipLaunchKernelGGL((adapter_tile_kernel<ST, BM, BN, WM, WN, WK, BK, S, SILU>), grid, dim3(64 * WM * WN * WK), 0, s, k);
+  // BK columns of 16-bit types; of fp32 half as many, the same bytes
+  hipLaunchKernelGGL((adapter_tile_kernel<ST, BM, BN, WM, WN, WK, BK * 2 / (int)sizeof(ST), S, SILU>), grid, dim3(64 * WM * WN * WK), 0, s, k);
   return check_launch("pk_adapter_linear");
 }
 
-// The forms of the product and what a launch of each takes, as pk_linear's table has
-// them (`a` us and `s` us a 1024 columns, `m` of the latter for each further workgroup on
-// the CU, again a - 2 for each further round of `occ`), with `e` us for a step of the
-// adapters' part: a run of rows with one adapter in a tile, 16 ranks of it (from memory)
-// or 32 (staged).  Fitted to launches in a graph, 1 - 7600 rows, K and N 512 - 4096, ranks 16 and
-// 64, one adapter to one a row: on the mean 3% over the fastest form.  How many adapters
-// the rows have is not known on the host; the plan's tiles bound it.
+// The forms of the product and what a launch of each takes: `a` us and `s` us a 1024
+// columns for a workgroup alone on its CU, `m` of the latter for each further one beside
+// it (`occ` fit), again a - 2 for each further round, and `e` us for a step of the adapters'
+// part: a run of rows with one adapter in a tile, 16 ranks of it (from memory) or 32
+// (staged).  Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks
+// 16 and 64, from one adapter to one for every second row: the cheapest by it is the
+// fastest form or within 10%, on the mean 0.2%.  How many adapters the rows have is not
+// known on the host; the plan's tiles bound it.
 struct Form {
-  int bm, bn, kmul, occ;
-  float a, s, m, e;
+  int bm, bn, occ;
   bool staged;
 };
-constexpr Form kForms[] = {
-    {16, 16, 128, 4, 2.8f, 1.2f, 0.25f, 0.08f, false},   // 0
-    {16, 32, 128, 3, 3.05f, 1.37f, 0.5f, 0.13f, false},  // 1
-    {32, 32, 128, 2, 3.45f, 1.75f, 0.6f, 0.15f, false},  // 2
-    {32, 64, 128, 2, 3.6f, 2.25f, 0.95f, 0.26f, false},  // 3
-    {64, 64, 64, 2, 3.75f, 3.35f, 0.8f, 0.4f, true},     // 4
-    {64, 128, 64, 2, 4.2f, 5.5f, 0.8f, 0.5f, true},      // 5
-    {128, 128, 64, 2, 5.7f, 9.1f, 0.8f, 1.2f, true},     // 6
-    {256, 256, 64, 1, 10.0f, 28.0f, 0.f, 1.75f, true},   // 7
+struct FormCost {
+  float a, s, m, e;
 };
-constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
+constexpr Form kForms[] = {{16, 16, 4, false}, {16, 32, 3, false}, {32, 32, 2, false},  {32, 64, 2, false},
+                           {64, 64, 2, true},  {64, 128, 2, true}, {128, 128, 2, true}, {256, 256, 1, true}};
+constexpr FormCost kCost16[] = {{3.51f, 1.92f, 0.17f, 0.04f}, {3.59f, 2.39f, 0.15f, 0.05f}, {4.49f, 2.67f, 0.27f, 0.07f},
+                                {3.16f, 5.20f, 0.21f, 0.14f}, {3.49f, 5.02f, 0.26f, 0.42f}, {3.67f, 6.63f, 0.35f, 0.50f},
+                                {5.43f, 9.87f, 0.f, 1.12f},   {10.24f, 17.88f, 0.f, 2.12f}};
+// fp32 (256 x 256 outputs of it do not fit LDS)
+constexpr FormCost kCost32[] = {{3.24f, 4.58f, 0.18f, 0.03f},  {3.57f, 5.97f, 0.17f, 0.06f},  {3.68f, 7.82f, 0.25f, 0.10f},
+                                {2.30f, 15.64f, 0.17f, 0.19f}, {4.17f, 18.60f, 0.65f, 0.53f}, {3.89f, 34.59f, 0.63f, 0.59f},
+                                {7.66f, 67.55f, 0.61f, 1.45f}};
 
 // us of a launch in form f with `adapters` among the rows, or a negative number where it
-// does not fit
-float form_cost(const Form& f, int64_t M, int64_t N, int64_t K, int r, int parts, int64_t adapters, int cus) {
-  if (N % f.bn != 0 || K % f.kmul != 0) return -1.f;
+// does not fit (a stage of 128 bytes a row, 256 where the adapters are not staged)
+float form_cost(const Form& f, const FormCost& c, int64_t M, int64_t N, int64_t K, int elem, int r, int parts, int64_t adapters, int cus) {
+  if (N % f.bn != 0 || K * elem % (f.staged ? 128 : 256) != 0) return -1.f;
   const int64_t tiles = (M + f.bm - 1) / f.bm * (N / f.bn);
   const int64_t per = (tiles + cus - 1) / cus, rounds = (per + f.occ - 1) / f.occ;
-  const float c = f.s * (float)K / 1024.f;
+  const float k = c.s * (float)K / 1024.f;
   const float runs = fminf(fminf((float)f.bm, (float)M), 1.f + (float)(adapters - 1) * f.bm / M);
   const int steps = f.staged ? (r * parts + 31) / 32 : (r * parts + 15) / 16;
-  return f.a + (float)(rounds - 1) * (f.a - 2.f) + (float)rounds * c + f.m * c * (float)(per - rounds) +
-         f.e * runs * (float)steps * (float)per;
+  return c.a + (float)(rounds - 1) * (c.a - 2.f) + (float)rounds * k + c.m * k * (float)(per - rounds) +
+         c.e * runs * (float)steps * (float)per;
 }
 
 template <typename ST, int SILU>
 int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
   int form = -1;
   float cost = 0.f;
-  for (int i = 0; i < kNumForms; ++i) {
-    const float c = form_cost(kForms[i], k.M, k.N, k.K, k.r, k.parts, adapters, cus);
+  constexpr int kBuilt = sizeof(ST) == 4 ? sizeof(kCost32) / sizeof(kCost32[0]) : sizeof(kCost16) / sizeof(kCost16[0]);
+  for (int i = 0; i < kBuilt; ++i) {
+    const float c = form_cost(kForms[i], sizeof(ST) == 4 ? kCost32[i] : kCost16[i], k.M, k.N, k.K, sizeof(ST), k.r, k.parts, adapters, cus);
     if (c >= 0.f && (form < 0 || c < cost)) {
       form = i;
       cost = c;
@@ -716,7 +696,9 @@ int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
     case 4: return launch_tile<ST, 64, 64, 2, 2, 2, 64, 4, SILU>(k, s);
     case 5: return launch_tile<ST, 64, 128, 2, 4, 1, 64, 3, SILU>(k, s);
     case 6: return launch_tile<ST, 128, 128, 2, 2, 1, 64, 2, SILU>(k, s);
-    default: return launch_tile<ST, 256, 256, 2, 4, 1, 64, 2, SILU>(k, s);
+    default:
+      if constexpr (sizeof(ST) == 2) return launch_tile<ST, 256, 256, 2, 4, 1, 64, 2, SILU>(k, s);
+      return fail(PK_ERR_UNSUPPORTED, "pk_adapter_linear: no form for %d -> %d", k.K, k.N);
   }
 }
 
@@ -729,7 +711,6 @@ bool rows_ok(int64_t rows, int64_t stride, int64_t width, int bytes) {
 template <typename ST>
 int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   const char* what = "pk_adapter_linear";
-  constexpr bool kF32 = sizeof(ST) == 4;
   if (a->rows < 0) return fail(PK_ERR_INVALID, "%s: rows %d < 0", what, a->rows);
   if (a->n <= 0 || a->n % 64 != 0 || a->k <= 0 || a->k % 64 != 0)
     return fail(PK_ERR_UNSUPPORTED, "%s: n %d and k %d must be multiples of 64", what, a->n, a->k);
@@ -741,10 +722,7 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
     return fail(PK_ERR_INVALID, "%s: activation %d must be none or SiLU", what, a->activation);
   if (a->max_tiles < 0) return fail(PK_ERR_INVALID, "%s: max_tiles %d < 0", what, a->max_tiles);
   if (a->rows == 0) return PK_OK;
-  if (kF32 && (a->weight || a->bias))
-    return fail(PK_ERR_INVALID, "%s: fp32 adds to a projection that out holds; weight and bias must be NULL", what);
-  const void* ptrs[9] = {a->x,     a->a,  a->b,         kF32 ? a->x : a->weight, a->bias ? a->bias : a->x,
-                         a->tiles, a->out, a->workspace, a->scale};
+  const void* ptrs[9] = {a->x, a->a, a->b, a->weight, a->bias ? a->bias : a->x, a->tiles, a->out, a->workspace, a->scale};
   for (const void* q : ptrs) {
     if (!q) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
     if (q != a->scale && !aligned16(q)) return fail(PK_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
@@ -752,7 +730,7 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   if (!a->order || !a->ids) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
   constexpr int E = sizeof(ST);
   const int parts = k_parts(a->max_tiles, a->rank, a->k);
-  if (!rows_ok(a->rows, a->x_stride, a->k, E) || (!kF32 && !rows_ok(a->n, a->weight_stride, a->k, E)) ||
+  if (!rows_ok(a->rows, a->x_stride, a->k, E) || !rows_ok(a->n, a->weight_stride, a->k, E) ||
       !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok((int64_t)a->rows + 1, (int64_t)a->rank * parts, (int64_t)a->rank * parts, 4) || !rows_ok(a->rank, a->k, a->k, E) ||
       !rows_ok(a->n, a->rank, a->rank, E))
     return fail(PK_ERR_INVALID, "%s: row strides must be multiples of 16 bytes, at least the row, and a tensor below 2^31 bytes", what);
@@ -784,20 +762,10 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
     const int rc = launch_low(k, a->max_tiles, s);
     if (rc != PK_OK) return rc;
   }
-  const bool silu = a->activation == PK_ACT_SILU;
-  if constexpr (kF32) {
-    const dim3 grid((unsigned)((k.M + 15) / 16), (unsigned)((k.N + 255) / 256));
-    if (silu)
-      hipLaunchKernelGGL(adapter_add_kernel<1>, grid, dim3(256), 0, s, k);
-    else
-      hipLaunchKernelGGL(adapter_add_kernel<0>, grid, dim3(256), 0, s, k);
-    return check_launch(what);
-  } else {
-    int64_t adapters = a->max_tiles - a->rows / kLowRows;  // at most
-    if (adapters < 1) adapters = 1;
-    const int cus = cu_count();
-    return silu ? launch_product<ST, 1>(k, adapters, cus, s) : launch_product<ST, 0>(k, adapters, cus, s);
-  }
+  int64_t adapters = a->max_tiles - a->rows / kLowRows;  // at most
+  if (adapters < 1) adapters = 1;
+  const int cus = cu_count();
+  return a->activation == PK_ACT_SILU ? launch_product<ST, 1>(k, adapters, cus, s) : launch_product<ST, 0>(k, adapters, cus, s);
 }
 
 }  // namespace

@@ -1290,9 +1290,8 @@ def adapter_linear(
 ) -> torch.Tensor:
     """``x @ weight.T + bias + scale[g] * (x @ a[g].T) @ b[g].T``, g the adapter of x's row in
     ``plan``, and SiLU of it: a shared projection with the low-rank adapter of each
-    stream beside it.  fp16 and bf16: two launches, one rounding of the output; fp32:
-    torch's linear, then two launches.  x [..., K], weight [N, K], bias [N] or None; N
-    and K multiples of 64, ranks of 8 up to 128.  No gradients."""
+    stream beside it, in two launches, the output rounded once.  x [..., K], weight
+    [N, K], bias [N] or None; N and K multiples of 64, ranks of 8 up to 128.  No gradients."""
     A, Bm, scale, tiles = adapters.a, adapters.b, adapters.scale, plan.tiles
     dt, dev = x.dtype, _require_device(x, weight, A, Bm, scale, plan.order, plan.ids, tiles)
     code = dtype_code(dt)
@@ -1325,20 +1324,16 @@ def adapter_linear(
     shape = (*x.shape[:-1], n)
     if out is not None and (out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
-    if dt is torch.float32:
-        y = torch.nn.functional.linear(x, weight, bias)
-        out = y if out is None else out.copy_(y)
-    else:
-        if out is None:
-            out = torch.empty(shape, dtype=dt, device=dev)
-        a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
-        if bias is not None:
-            a.bias = bias.data_ptr()
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+    if bias is not None:
+        a.bias = bias.data_ptr()
     L = lib()
     ws = torch.empty(L.pk_adapter_workspace_bytes(M, r, k, T), dtype=torch.uint8, device=dev)
     a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters = code, _index(dev), M, n, k, r, G
     a.activation = _lib.ACT_SILU if silu else _lib.ACT_NONE
     a.x, a.x_stride, a.out, a.out_stride = x.data_ptr(), k, out.data_ptr(), n
+    a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
     a.a, a.b, a.scale, a.workspace = A.data_ptr(), Bm.data_ptr(), scale.data_ptr(), ws.data_ptr()
     check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out

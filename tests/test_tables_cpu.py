@@ -152,7 +152,7 @@ def test_adapter_linear_refusals():
     for field, value, code in (("n", 100, unsupported), ("k", 96, unsupported), ("rank", 12, unsupported), ("rank", 136, unsupported), ("rank", 0, unsupported),
                                ("num_adapters", 0, unsupported), ("num_adapters", 513, unsupported), ("activation", 2, bad), ("rows", -1, bad),
                                ("max_tiles", -1, bad), ("x", at + 8, bad), ("order", None, bad), ("x_stride", 132, bad), ("weight_stride", 64, bad),
-                               ("out_stride", 120, bad), ("out_stride", 1 << 30, bad), ("dtype", 5, bad), ("dtype", _lib.DTYPE_F32, bad)):
+                               ("out_stride", 120, bad), ("out_stride", 1 << 30, bad), ("dtype", 5, bad), ("weight", None, bad)):
         keep = getattr(a, field)
         setattr(a, field, value)
         assert L.pk_adapter_linear(ctypes.byref(a), None) == code, (field, value)
