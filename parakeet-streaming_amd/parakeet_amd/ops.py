@@ -1095,12 +1095,6 @@ def _i32(t: torch.Tensor, name: str, shape: tuple) -> int:
     return t.data_ptr()
 
 
-def _on(dev: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {name} is on {t.device}, not {dev}")
-
-
 def _index(dev: torch.device) -> int:
     return torch.cuda.current_device() if dev.index is None else dev.index
 
@@ -1124,21 +1118,25 @@ class PageState:
     def max_pages(self) -> int:
         return (self.left + self.chunk + self.page_size - 2) // self.page_size + 1
 
-    def _args(self) -> tuple[PageStepArgs, torch.device, int]:
-        P, left, chunk, A = self.page_size, self.left, self.chunk, self.appended
+    def _args(self, slots: torch.Tensor) -> tuple[PageStepArgs, torch.device, int, int]:
+        """The arguments that a step and a reset of ``slots`` share, the device, the ring
+        entries and the batch."""
+        P, left, chunk, A, queue, head, ring = self.page_size, self.left, self.chunk, self.appended, self.queue, self.head, self.ring
         if P <= 0 or left < 0 or chunk <= 0:
             raise ValueError(f"need page_size > 0, left >= 0 and chunk > 0, got {P}, {left}, {chunk}")
         if A.dim() != 1 or A.dtype is not torch.int64 or not A.is_contiguous():
             raise ValueError(f"appended must be contiguous int64 [num_slots], got {tuple(A.shape)} {A.dtype}")
-        M = self.max_pages
+        if slots.dim() != 1:
+            raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
+        M = (left + chunk + P - 2) // P + 1
         a = PageStepArgs()
-        a.num_slots, a.num_pages = S, N = A.shape[0], self.queue.numel()
+        a.num_slots, a.num_pages, a.batch = S, N, B = A.shape[0], queue.numel(), slots.shape[0]
         a.page_size, a.left, a.chunk = P, left, chunk
-        a.queue, a.head = _i32(self.queue, "queue", (N,)), _i32(self.head, "head", (2,))
-        a.appended, a.ring = A.data_ptr(), _i32(self.ring, "ring", (S, M))
-        dev = _require_device(A, self.queue, self.head, self.ring)
+        a.queue, a.head = _i32(queue, "queue", (N,)), _i32(head, "head", (2,))
+        a.appended, a.ring, a.slots = A.data_ptr(), _i32(ring, "ring", (S, M)), _i32(slots, "slots", (B,))
+        dev = _require_device(A, queue, head, ring, slots)
         a.device = _index(dev)
-        return a, dev, M
+        return a, dev, M, B
 
 
 def page_step(
@@ -1158,19 +1156,16 @@ def page_step(
     a stream's frames) for :func:`kv_append_slots`.  A slot out of range or named
     earlier in the call is absent (rows {0, -1 ...}, slot_map -1, nothing changed).
     No host work and no synchronisation: a step may be recorded in a graph."""
-    a, dev, M = state._args()
-    if slots.dim() != 1:
-        raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
-    B, T = slots.shape[0], state.chunk
-    a.batch, a.slots = B, _i32(slots, "slots", (B,))
+    a, dev, M, B = state._args(slots)
+    T = state.chunk
     if lengths is not None:
         a.lengths = _i32(lengths, "lengths", (B,))
     if rows is None:
-        rows = torch.empty((B, 1 + M), dtype=_INT32, device=dev)
+        rows = slots.new_empty((B, 1 + M))
     if slot_map is None:
-        slot_map = torch.empty((B, T), dtype=_INT32, device=dev)
+        slot_map = slots.new_empty((B, T))
     a.rows, a.slot_map = _i32(rows, "rows", (B, 1 + M)), _i32(slot_map, "slot_map", (B, T))
-    _on(dev, slots=slots, lengths=lengths, rows=rows, slot_map=slot_map)
+    _require_device(slots, rows, slot_map, slots if lengths is None else lengths)
     a.rows_stride, a.slot_map_stride = 1 + M, T
     L = lib()
     n = L.pk_page_step_workspace_bytes(B)
@@ -1184,11 +1179,8 @@ def page_step(
 def page_reset(state: PageState, slots: torch.Tensor) -> None:
     """Gives every page of ``slots`` (int32 [B]) back to the queue, slot after slot, and
     sets their frame counts to 0 (``PagePool.reset_slot``)."""
-    a, dev, _ = state._args()
-    if slots.dim() != 1:
-        raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
-    a.batch, a.slots, a.reset = slots.shape[0], _i32(slots, "slots", (slots.shape[0],)), 1
-    _on(dev, slots=slots)
+    a, dev, _, _ = state._args(slots)
+    a.reset = 1
     check(lib().pk_page_step(ctypes.byref(a), _stream(dev)), "pk_page_step")
 
 
@@ -1255,9 +1247,7 @@ def adapter_plan(ids: torch.Tensor, frames: int = 1, *, num_adapters: int) -> Ad
     n = M // 32 + min(G, B)
     a = AdapterPlanArgs()
     a.device, a.batch, a.frames, a.num_adapters, a.max_tiles = _index(dev), B, T, G, n
-    p = AdapterPlan(
-        torch.empty(M, dtype=_INT32, device=dev), torch.empty(M, dtype=_INT32, device=dev), torch.empty((n, 4), dtype=_INT32, device=dev)
-    )
+    p = AdapterPlan(ids.new_empty(M), ids.new_empty(M), ids.new_empty((n, 4)))
     a.ids, a.order, a.sorted_ids, a.tiles = at, p.order.data_ptr(), p.ids.data_ptr(), p.tiles.data_ptr()
     L = lib()
     n = L.pk_adapter_plan_workspace_bytes(B, T, G)
@@ -1325,7 +1315,7 @@ def adapter_linear(
     if out is not None and (out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = x.new_empty(shape)
     if bias is not None:
         a.bias = bias.data_ptr()
     L = lib()
