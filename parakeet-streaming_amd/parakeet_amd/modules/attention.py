@@ -118,8 +118,9 @@ class ConformerAttention(nn.Module):
     def forward(self, x: Tensor, pos_emb: Tensor, attn_mask: Tensor, cache: ModelCache = None):
         return self.attend(ops.module_linear(x, self.qkv), pos_emb, attn_mask, cache)
 
-    def attend(self, qkv: Tensor, pos_emb: Tensor, attn_mask: Tensor, cache: ModelCache = None):
-        """:meth:`forward` from the qkv projection's output [B, T, 3 D]."""
+    def attend(self, qkv: Tensor, pos_emb: Tensor, attn_mask: Tensor, cache: ModelCache = None, project=None):
+        """:meth:`forward` from the qkv projection's output [B, T, 3 D]; ``project``: what
+        stands for ``linear_out``."""
         B, T = qkv.shape[:2]
         query, key, value = qkv.chunk(3, dim=-1)
         # [1, P, D] is one table for every stream; [B, P, D] gives each stream
@@ -138,7 +139,8 @@ class ConformerAttention(nn.Module):
             out = ops.paged_relpos_attn(
                 query, key, value, pos, bias_u, bias_v, mask, num_heads=self.num_heads, left=0, pages=None, append=False
             )
-        return ops.module_linear(out.reshape(B, T, self.num_heads * self.d_k), self.linear_out)
+        out = out.reshape(B, T, self.num_heads * self.d_k)
+        return ops.module_linear(out, self.linear_out) if project is None else project(out)
 
 
 __all__ = ["ConformerAttention", "PositionalEncoding"]

@@ -28,7 +28,7 @@ import torch
 from torch import Tensor
 
 from .. import ops
-from ..pool import PagePool
+from ..pool import DevicePagePool, PagePool
 
 
 class _RowStaging:
@@ -64,8 +64,12 @@ class ModelCache:
     parakeet/modules/cache.py:7-77.
 
     Extra keyword-only arguments: ``page_size`` (frames per page, power of two),
-    ``num_pages`` (pool size, default ``batch_size * max_pages``) and
-    ``page_order`` (initial free-queue order, default 0..num_pages-1).
+    ``num_pages`` (pool size, default ``batch_size * max_pages``),
+    ``page_order`` (initial free-queue order, default 0..num_pages-1) and
+    ``device_pages``: the page pool is kept in device memory
+    (:class:`~parakeet_amd.pool.DevicePagePool`, the same rings and rows) and a step opens
+    with one launch, without host page work and upload; ``EncoderStepGraph`` then
+    records it with the step.
     """
 
     def __init__(
@@ -81,6 +85,7 @@ class ModelCache:
         page_size: int = 16,
         num_pages: int | None = None,
         page_order=None,
+        device_pages: bool = False,
     ):
         super().__init__()
         self.left_attn = int(attn_context_size[0])
@@ -93,13 +98,16 @@ class ModelCache:
         self.chunk = self.right_attn + 1
         device = torch.device(device) if device is not None else torch.device("cpu")
         dtype = dtype if dtype is not None else torch.get_default_dtype()
-        self.pool = PagePool(
+        self.device_pages = bool(device_pages)
+        kind = {"device": device} if self.device_pages else {}
+        self.pool = (DevicePagePool if self.device_pages else PagePool)(
             num_slots=batch_size,
             page_size=page_size,
             left=self.left_attn,
             chunk=self.chunk,
             num_pages=num_pages,
             page_order=page_order,
+            **kind,
         )
         self.page_size = self.pool.page_size
         self.max_pages = self.pool.max_pages
@@ -132,6 +140,7 @@ class ModelCache:
         self._slot_index = None if self._prefix else up(self._slots.astype(np.int64))
         self._slots_i32 = up(self._slots.copy())
         self._rows = torch.zeros((n, 1 + self.max_pages), dtype=torch.int32, device=dev)
+        self._places = torch.empty((n, self.chunk), dtype=torch.int32, device=dev) if self.device_pages else None
         self._seen: set[int] = set()
         self._step_open = False
         self._recording = False
@@ -148,6 +157,7 @@ class ModelCache:
             "num_layers",
             "embed_dim",
             "chunk",
+            "device_pages",
             "pool",
             "page_size",
             "max_pages",
@@ -205,7 +215,9 @@ class ModelCache:
 
     def _open_step(self) -> None:
         base = self._base
-        if self._rows.device.type == "cuda":
+        if self.device_pages:
+            self._advance_pages()
+        elif self._rows.device.type == "cuda":
             if base._staging is None:
                 base._staging = _RowStaging(max(1, base.pool.num_slots), 1 + self.max_pages)
             base._staging.upload(self.pool, self._slots, self._rows)
@@ -214,6 +226,16 @@ class ModelCache:
             self._rows.copy_(torch.from_numpy(rows))
         self._seen = set()
         self._step_open = True
+
+    def _advance_pages(self) -> None:
+        self.pool.advance(self._slots_i32, rows=self._rows, slot_map=self._places)
+
+    def open_recorded_step(self) -> None:
+        """Inside :meth:`recording`: the opening of the step as a launch of the recording
+        (``device_pages``), instead of an :meth:`open_step` before each replay."""
+        if not (self._recording and self.device_pages):
+            raise RuntimeError("paged cache: only a recording with device_pages opens its own step")
+        self._advance_pages()
 
     def open_step(self) -> None:
         """Opens the next step now -- the host page work for the batch and the

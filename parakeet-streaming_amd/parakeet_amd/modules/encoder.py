@@ -34,6 +34,7 @@ from torch import Tensor, nn
 from torch.nn import functional as F
 
 from .. import ops
+from .adapters import EncoderAdapters, StepAdapters
 from .attention import ConformerAttention, PositionalEncoding
 from .cache import ConvCacheRef, ModelCache, StreamingState
 from .frontend import ConvSubsampling
@@ -170,7 +171,9 @@ class ConformerLayer(nn.Module):
         self.feed_forward2 = ConformerFeedForward(hidden_size, d_ff, dropout, use_bias)
         self.norm_out = nn.LayerNorm(hidden_size)
 
-    def forward(self, x: Tensor, pos_emb: Tensor, pad_mask: Tensor, attn_mask: Tensor, cache: ModelCache):
+    def forward(self, x: Tensor, pos_emb: Tensor, pad_mask: Tensor, attn_mask: Tensor, cache: ModelCache, adapters: StepAdapters | None = None):
+        if adapters is not None:
+            return self.adapted_step(x, pos_emb, pad_mask, attn_mask, cache, adapters)
         if self.fuses(x, cache):
             return self.finish(self.fused_step(x, pos_emb, pad_mask, attn_mask, cache))
         # each residual update and the LayerNorm that reads it are one step
@@ -183,6 +186,23 @@ class ConformerLayer(nn.Module):
         residual, h = self.residual_norm(residual, conv_out, self.norm_feed_forward2, 1.0, in_place=True)
         _, out = self.residual_norm(residual, self.feed_forward2(h), self.norm_out, 0.5, in_place=True)
         return out
+
+    def adapted_step(self, x: Tensor, pos_emb: Tensor, pad_mask: Tensor, attn_mask: Tensor, cache: ModelCache, adapters: StepAdapters):
+        """:meth:`forward` module by module, the feed-forward and attention projections
+        with each stream's low-rank adapter beside them."""
+        i, attn = self.layer_idx, self.self_attn
+        if not ops.plain_module(attn, ConformerAttention):
+            raise NotImplementedError("adapters beside a replaced or hooked attention module")
+        y = adapters.feed_forward(i, "feed_forward1", self.feed_forward1, self.norm_feed_forward1(x))
+        residual, h = self.residual_norm(x, y, self.norm_self_att, 0.5)
+        qkv = adapters.linear(i, "self_attn.qkv", attn.qkv, h)
+        y = attn.attend(qkv, pos_emb, attn_mask, cache, project=lambda o: adapters.linear(i, "self_attn.linear_out", attn.linear_out, o))
+        residual, h = self.residual_norm(residual, y, self.norm_conv, 1.0, in_place=True)
+        y, conv_cache = self.conv(h, pad_mask=pad_mask, cache=cache.conv_ref(i))
+        cache.update_conv_cache(i, conv_cache)
+        residual, h = self.residual_norm(residual, y, self.norm_feed_forward2, 1.0, in_place=True)
+        y = adapters.feed_forward(i, "feed_forward2", self.feed_forward2, h)
+        return self.residual_norm(residual, y, self.norm_out, 0.5, in_place=True)[1]
 
     def fuses(self, x: Tensor, cache) -> bool:
         """Whether :meth:`fused_step` is this layer's step on ``x``: every module
@@ -353,7 +373,14 @@ class ConformerEncoder(nn.Module):
             chunk_size=self.att_context_size[1] + 1,
         )
 
-    def forward(self, x: Tensor, state: StreamingState, length: Tensor | None = None, bypass_pre_encode: bool = False):
+    def forward(
+        self,
+        x: Tensor,
+        state: StreamingState,
+        length: Tensor | None = None,
+        bypass_pre_encode: bool = False,
+        adapters: StepAdapters | None = None,
+    ):
         cache_lengths = state.cache_lengths
         if not isinstance(cache_lengths, Tensor):
             cache_lengths = torch.full((x.size(0),), int(cache_lengths), dtype=torch.int64, device=x.device)
@@ -371,6 +398,9 @@ class ConformerEncoder(nn.Module):
         # a layer's last residual update and norm run in the next layer's first launch
         pend = None
         for layer in self.layers:
+            if adapters is not None:
+                x = layer(x, pos_emb=pos_emb, pad_mask=pad_mask, attn_mask=att_mask, cache=state.cache, adapters=adapters)
+                continue
             y = x if pend is None else pend.x
             if ops.plain_module(layer, ConformerLayer) and layer.fuses(y, state.cache):
                 pend = layer.fused_step(x if pend is None else pend, pos_emb, pad_mask, att_mask, state.cache)
@@ -406,9 +436,21 @@ class EncoderStepGraph:
     ``length`` is the per-stream frame count of every step ([B] int64; the engine
     feeds whole chunks, parakeet/engine/sequence.py:137-146).  The returned
     [B, D, T] tensor is a fixed buffer that the next call overwrites.
+
+    With ``device_pages`` in the cache the step's page work is a launch of the
+    recording: a replay needs no host page work and no upload.  ``adapters``: the
+    batch's streams run with their low-rank adapters, numbers ``adapter_ids`` (int32
+    [B] on the device, read at each step, so another batch's are copied into it).
     """
 
-    def __init__(self, encoder: ConformerEncoder, state: StreamingState, length: Tensor):
+    def __init__(
+        self,
+        encoder: ConformerEncoder,
+        state: StreamingState,
+        length: Tensor,
+        adapters: EncoderAdapters | None = None,
+        adapter_ids: Tensor | None = None,
+    ):
         cache = state.cache
         if not isinstance(cache, ModelCache):
             raise TypeError("state.cache must be the paged ModelCache")
@@ -419,6 +461,11 @@ class EncoderStepGraph:
         dev = cache.k_pages.device
         if not isinstance(length, Tensor) or tuple(length.shape) != (B,):
             raise ValueError(f"length must be a [{B}] tensor")
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters and adapter_ids go together")
+        if adapter_ids is not None and (tuple(adapter_ids.shape) != (B,) or adapter_ids.dtype != torch.int32 or adapter_ids.device != dev):
+            raise ValueError(f"adapter_ids must be int32 [{B}] on {dev}")
+        self.adapters, self.adapter_ids = adapters, adapter_ids
         self.encoder = encoder
         self.state = state
         self.length = length.to(device=dev, dtype=torch.int64).clone()
@@ -431,13 +478,16 @@ class EncoderStepGraph:
         if tuple(x.shape) != self.shape:
             raise ValueError(f"x must be {self.shape}, got {tuple(x.shape)}")
         cache = self.state.cache
-        cache.open_step()
+        if self.graph is None or not cache.device_pages:
+            cache.open_step()
         if self.graph is None:
             self.x = x.detach().clone()
-            out, _ = self.encoder(self.x, self.state, length=self.length)
+            out = self._step()
             graph = torch.cuda.CUDAGraph()
             with cache.recording(), torch.cuda.graph(graph):
-                self.out, _ = self.encoder(self.x, self.state, length=self.length)
+                if cache.device_pages:
+                    cache.open_recorded_step()
+                self.out = self._step()
             self.graph = graph
             return out
         self.x.copy_(x)
@@ -445,6 +495,10 @@ class EncoderStepGraph:
             layer.self_attn.refresh_projected_pos()
         self.graph.replay()
         return self.out
+
+    def _step(self) -> Tensor:
+        step = None if self.adapters is None else self.adapters.step(self.adapter_ids, self.shape[1])
+        return self.encoder(self.x, self.state, length=self.length, **({} if step is None else {"adapters": step}))[0]
 
 
 __all__ = [
