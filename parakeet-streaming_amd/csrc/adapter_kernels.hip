@@ -88,15 +88,21 @@ __device__ static inline u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t o
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
 }
 
-// h of a tile: the waves split K, 16 RT ranks a workgroup, U steps of loads on their way.
-// Operands come straight from memory (every byte is used once a workgroup).
-template <typename ST, int RT>
+// h of a tile: its 32 rows of x and 16 RT rows of A through LDS, 512 bytes of each a
+// stage, S stages on their way (whole lines; read straight from memory as matrix
+// operands, 16 rows of 64 bytes an instruction, a CU moved 16-34 GB/s).  The waves take
+// a step of 4 chunks a lane group of each stage and their sums meet at the end.  Columns past
+// the part's end are loaded from its start and not multiplied.
+template <typename ST, int RT, int S>
 __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
-  constexpr int V = Tr<ST>::VEC;
-  constexpr int COLS = MmaA<ST>::COLS;
-  constexpr int SB = 2, kBlock = SB * COLS, U = 4;
-  __shared__ f32x4_t red[kLowWaves * RT * 2 * 64];
+  constexpr int E = sizeof(ST), V = 16 / E, COLS = MmaA<ST>::COLS;
+  constexpr int CH = 4 * kLowWaves, ROW = CH * 16, BK = ROW / E;  // a wave's step each
+  constexpr int NR = kLowRows + 16 * RT, kStage = NR * ROW;
+  constexpr int LPS = NR * CH / 64 / kLowWaves;
+  static_assert(NR * CH % (64 * kLowWaves) == 0 && BK == COLS * kLowWaves, "whole waves of chunks, a step a wave");
+  constexpr int kRed = kLowWaves * RT * 2 * 64 * 16;
+  __shared__ __align__(16) unsigned char smem[S * kStage > kRed ? S * kStage : kRed];
   static_assert(2 * RT <= kLowWaves, "a wave finishes at most one sum");
   if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {  // the row of zeros behind the last row
     const int n = p.r * p.parts * 4 / 16;
@@ -110,41 +116,59 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, kg = lane >> 4;
   const int r0 = blockIdx.y * RT * 16;
-  const bool two = tile.z > 16;
-  // offsets in bytes; columns past K and a second 16 rows that the tile has not read as zero
-  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * (uint32_t)sizeof(ST));
-  const __amdgpu_buffer_rsrc_t ra = bytes_rsrc(p.a + (int64_t)tile.x * p.r * p.K, (uint32_t)p.r * p.K * (uint32_t)sizeof(ST));
-  uint32_t xo[2], ao[RT];
+  const int k0 = blockIdx.z * p.kpart, k1 = min(k0 + p.kpart, p.K), iters = (k1 - k0 + BK - 1) / BK;
+  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * E);
+  const __amdgpu_buffer_rsrc_t ra = bytes_rsrc(p.a + (int64_t)tile.x * p.r * p.K, (uint32_t)p.r * p.K * E);
+  // chunk c of a stage: row c / CH of [x rows ; A rows], LDS position c % CH; rows past the
+  // tile's and ranks past the last are loaded again
+  uint32_t off[LPS], col[LPS];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-    xo[m] = (uint32_t)(plan_row(p, tile.y + min(m * 16 + l16, tile.z - 1)) * p.x_s + kg * V) * (uint32_t)sizeof(ST);
+  for (int i = 0; i < LPS; ++i) {
+    const int c = (i * kLowWaves + wave) * 64 + lane;
+    const int r = c / CH, pos = c % CH;
+    col[i] = ((pos & ~7) | ((pos ^ r) & 7)) * V;
+    off[i] = r < kLowRows ? (uint32_t)(plan_row(p, tile.y + min(r, tile.z - 1)) * p.x_s) * E
+                          : (uint32_t)(min(r0 + r - kLowRows, p.r - 1) * p.K) * E;
+  }
+  auto issue = [&](int st, int k) {
 #pragma unroll
-  for (int j = 0; j < RT; ++j) ao[j] = (uint32_t)(min(r0 + j * 16 + l16, p.r - 1) * p.K + kg * V) * (uint32_t)sizeof(ST);
+    for (int i = 0; i < LPS; ++i) {
+      const int base = (i * kLowWaves + wave) * 64;
+      const uint32_t at = k + (int)col[i] < k1 ? (uint32_t)k + col[i] : (uint32_t)k0;
+      load_lds16(base < kLowRows * CH ? rx : ra, smem + st * kStage + base * 16, off[i] + at * E, 0);
+    }
+  };
   f32x4_t acc[RT][2];
 #pragma unroll
   for (int j = 0; j < RT; ++j) acc[j][0] = acc[j][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // a wave takes blocks of 128 bytes a row: whole lines, in adjacent steps
-  const int k0 = blockIdx.z * p.kpart, k1 = min(k0 + p.kpart, p.K);
-  for (int k = k0 + wave * kBlock; k < k1; k += U / SB * kLowWaves * kBlock) {
-    u32x4 af[U][RT], xf[U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int ku = k + u / SB * kLowWaves * kBlock + u % SB * COLS;
-      const uint32_t kb = ku < k1 ? (uint32_t)ku * (uint32_t)sizeof(ST) : kNowhere;
-      xf[u][0] = load16(rx, xo[0] + kb);
-      xf[u][1] = load16(rx, two ? xo[1] + kb : kNowhere);
-#pragma unroll
-      for (int j = 0; j < RT; ++j) af[u][j] = load16(ra, ao[j] + kb);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
-#pragma unroll
-    for (int u = 0; u < U; ++u)
+  for (int s = 0; s < S - 1; ++s)
+    if (s < iters) issue(s, k0 + s * BK);
+  int st = 0;
+  for (int it = 0; it < iters; ++it) {
+    if (it + S - 2 < iters)
+      wait_vm<(S - 2) * LPS>();
+    else
+      wait_vm<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, k0 + (it + S - 1) * BK);
+    if (k0 + it * BK + wave * COLS < k1) {
+      const int ch = wave * 4 + kg;
+      auto frag = [&](int r) { return *reinterpret_cast<const u32x4*>(smem + st * kStage + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16); };
+      const u32x4 xf[2] = {frag(l16), frag(16 + l16)};
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        acc[j][0] = MmaA<ST>::step(af[u][j], xf[u][0], acc[j][0]);
-        acc[j][1] = MmaA<ST>::step(af[u][j], xf[u][1], acc[j][1]);
+        const u32x4 af = frag(kLowRows + j * 16 + l16);
+        acc[j][0] = MmaA<ST>::step(af, xf[0], acc[j][0]);
+        acc[j][1] = MmaA<ST>::step(af, xf[1], acc[j][1]);
       }
+    }
+    st = st == S - 1 ? 0 : st + 1;
   }
+  __syncthreads();  // the stages are read
+  f32x4_t* const red = reinterpret_cast<f32x4_t*>(smem);
 #pragma unroll
   for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -599,27 +623,24 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 
 namespace {
 
-// workgroups over the ranks: 32 of them each, more read x again (rank 64 in one workgroup
-// takes 0.9-1.5 us longer from 1 to 3584 rows of 512 to 4096)
-int low_blocks(int r) { return (r + 31) / 32; }
+// workgroups over the ranks, 64 of them each
+int low_blocks(int r) { return (r + 63) / 64; }
 
-// Parts of K that x A^T is split into: of 1024 columns or more, up to 4, while there are
-// at most 256 workgroups (one a CU).  A tile of 32 rows x 4096 columns reads 0.5 MB, 15 us
-// for one workgroup; the product with B then takes more steps (840 x 4096 -> 1024, rank
-// 32: 38 us in one part, 32 in four).
-int k_parts(int64_t tiles, int r, int64_t k) {
-  int p = 1;
-  while (p < 4 && (int64_t)p * 2 * 1024 <= k && tiles * low_blocks(r) * p * 2 <= 256) p *= 2;
-  return p;
-}
+// Parts of K that x A^T is split into: two, of 1024 columns or more, while there are at most
+// 256 workgroups (one a CU): 32 x 2 rows 4096 -> 1024 take 16.3 us so and 18.1 in one part; the
+// product with B then takes twice the steps (840 rows of rank 64: 38.5 and 38.7; in four
+// parts 43.3).
+int k_parts(int64_t tiles, int r, int64_t k) { return k >= 2048 && tiles * low_blocks(r) * 2 <= 256 ? 2 : 1; }
 
 template <typename ST>
 int launch_low(const AdK<ST>& k, int max_tiles, hipStream_t s) {
   const dim3 grid((unsigned)max_tiles, (unsigned)low_blocks(k.r), (unsigned)k.parts), block(64 * kLowWaves);
   if (k.r <= 16)
-    hipLaunchKernelGGL((adapter_low_kernel<ST, 1>), grid, block, 0, s, k);
+    hipLaunchKernelGGL((adapter_low_kernel<ST, 1, 4>), grid, block, 0, s, k);
+  else if (k.r <= 32)
+    hipLaunchKernelGGL((adapter_low_kernel<ST, 2, 4>), grid, block, 0, s, k);
   else
-    hipLaunchKernelGGL((adapter_low_kernel<ST, 2>), grid, block, 0, s, k);
+    hipLaunchKernelGGL((adapter_low_kernel<ST, 4, 3>), grid, block, 0, s, k);
   return check_launch("pk_adapter_linear");
 }
 
