@@ -1122,21 +1122,34 @@ class PageState:
         """The arguments that a step and a reset of ``slots`` share, the device, the ring
         entries and the batch."""
         P, left, chunk, A, queue, head, ring = self.page_size, self.left, self.chunk, self.appended, self.queue, self.head, self.ring
+        M = (left + chunk + P - 2) // P + 1 if P > 0 else 0
+        dev = A.device
+        S, B = A.numel(), slots.numel()
+        if not (
+            dev.type == "cuda" and M > 0 and left >= 0 and chunk > 0
+            and A.dtype is torch.int64 and queue.dtype is _INT32 and head.dtype is _INT32 and ring.dtype is _INT32 and slots.dtype is _INT32
+            and A.shape == (S,) and head.shape == (2,) and ring.shape == (S, M) and slots.shape == (B,)
+            and queue.device == dev and head.device == dev and ring.device == dev and slots.device == dev
+            and A.is_contiguous() and queue.is_contiguous() and head.is_contiguous() and ring.is_contiguous() and slots.is_contiguous()
+        ):
+            self._refuse(slots)
+        a = PageStepArgs()
+        a.device, a.batch, a.num_slots, a.num_pages, a.page_size, a.left, a.chunk = _index(dev), B, S, queue.numel(), P, left, chunk
+        a.queue, a.head, a.appended, a.ring, a.slots = queue.data_ptr(), head.data_ptr(), A.data_ptr(), ring.data_ptr(), slots.data_ptr()
+        return a, dev, M, B
+
+    def _refuse(self, slots: torch.Tensor) -> None:
+        """Says what a step does not take of the state and the slots."""
+        P, left, chunk, A = self.page_size, self.left, self.chunk, self.appended
         if P <= 0 or left < 0 or chunk <= 0:
             raise ValueError(f"need page_size > 0, left >= 0 and chunk > 0, got {P}, {left}, {chunk}")
         if A.dim() != 1 or A.dtype is not torch.int64 or not A.is_contiguous():
             raise ValueError(f"appended must be contiguous int64 [num_slots], got {tuple(A.shape)} {A.dtype}")
-        if slots.dim() != 1:
-            raise ValueError(f"slots must be int32 [B], got {tuple(slots.shape)}")
-        M = (left + chunk + P - 2) // P + 1
-        a = PageStepArgs()
-        a.num_slots, a.num_pages, a.batch = S, N, B = A.shape[0], queue.numel(), slots.shape[0]
-        a.page_size, a.left, a.chunk = P, left, chunk
-        a.queue, a.head = _i32(queue, "queue", (N,)), _i32(head, "head", (2,))
-        a.appended, a.ring, a.slots = A.data_ptr(), _i32(ring, "ring", (S, M)), _i32(slots, "slots", (B,))
-        dev = _require_device(A, queue, head, ring, slots)
-        a.device = _index(dev)
-        return a, dev, M, B
+        _i32(self.queue, "queue", (self.queue.numel(),) if self.queue.dim() == 1 else tuple(self.queue.shape))
+        _i32(self.head, "head", (2,))
+        _i32(self.ring, "ring", (A.shape[0], self.max_pages))
+        _i32(slots, "slots", (slots.numel(),))
+        _require_device(A, self.queue, self.head, self.ring, slots)
 
 
 def page_step(
@@ -1160,13 +1173,17 @@ def page_step(
     T = state.chunk
     if lengths is not None:
         a.lengths = _i32(lengths, "lengths", (B,))
+        _require_device(slots, lengths)
     if rows is None:
         rows = slots.new_empty((B, 1 + M))
+    else:
+        _require_device(slots, rows)
     if slot_map is None:
         slot_map = slots.new_empty((B, T))
-    a.rows, a.slot_map = _i32(rows, "rows", (B, 1 + M)), _i32(slot_map, "slot_map", (B, T))
-    _require_device(slots, rows, slot_map, slots if lengths is None else lengths)
-    a.rows_stride, a.slot_map_stride = 1 + M, T
+    else:
+        _require_device(slots, slot_map)
+    a.rows, a.rows_stride = _i32(rows, "rows", (B, 1 + M)), 1 + M
+    a.slot_map, a.slot_map_stride = _i32(slot_map, "slot_map", (B, T)), T
     L = lib()
     n = L.pk_page_step_workspace_bytes(B)
     if n:
@@ -1282,48 +1299,72 @@ def adapter_linear(
     ``plan``, and SiLU of it: a shared projection with the low-rank adapter of each
     stream beside it, in two launches, the output rounded once.  x [..., K], weight
     [N, K], bias [N] or None; N and K multiples of 64, ranks of 8 up to 128.  No gradients."""
-    A, Bm, scale, tiles = adapters.a, adapters.b, adapters.scale, plan.tiles
-    dt, dev = x.dtype, _require_device(x, weight, A, Bm, scale, plan.order, plan.ids, tiles)
-    code = dtype_code(dt)
-    if x.dim() == 0 or weight.dim() != 2:
-        raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    _check_linear(dt, dev, x, weight, bias)
-    n, k = weight.shape
+    A, Bm, scale, order, ids, tiles = adapters.a, adapters.b, adapters.scale, plan.order, plan.ids, plan.tiles
+    dt, dev, ws, xs = x.dtype, x.device, weight.shape, x.shape
+    n, k = ws if len(ws) == 2 else (0, 0)
     G, r = A.shape[:2] if A.dim() == 3 else (0, 0)
-    if (
-        A.shape != (G, r, k) or Bm.shape != (G, n, r) or A.dtype is not dt or Bm.dtype is not dt
-        or not A.is_contiguous() or not Bm.is_contiguous()
+    M = x.numel() // k if k else 0
+    T = tiles.shape[0] if tiles.dim() else 0
+    if not (
+        dev.type == "cuda" and xs and xs[-1] == k and 0 < r <= _lib.ADAPTER_MAX_RANK and 0 < G <= _lib.ADAPTER_MAX
+        and not (k % 64 or n % 64 or r % 8 or n == 0)
+        and A.shape == (G, r, k) and Bm.shape == (G, n, r) and scale.shape == (G,)
+        and order.shape == (M,) and ids.shape == (M,) and tiles.shape == (T, 4)
+        and weight.dtype is dt and A.dtype is dt and Bm.dtype is dt and scale.dtype is torch.float32
+        and order.dtype is _INT32 and ids.dtype is _INT32 and tiles.dtype is _INT32
+        and weight.device == dev and A.device == dev and Bm.device == dev and scale.device == dev
+        and order.device == dev and ids.device == dev and tiles.device == dev
+        and weight.stride(1) == 1 and A.is_contiguous() and Bm.is_contiguous() and scale.is_contiguous()
+        and order.is_contiguous() and ids.is_contiguous() and tiles.is_contiguous()
+        and (bias is None or (bias.shape == (n,) and bias.dtype is dt and bias.device == dev and bias.is_contiguous()))
     ):
-        raise ValueError(f"adapters must be contiguous a [G, r, {k}] and b [G, {n}, r] of {dt}, got {tuple(A.shape)} {A.dtype} and "
-                         f"{tuple(Bm.shape)} {Bm.dtype}")
-    if scale.dtype is not torch.float32 or scale.shape != (G,) or not scale.is_contiguous():
-        raise ValueError(f"scale must be contiguous float32 [{G}], got {tuple(scale.shape)} {scale.dtype}")
-    if k % 64 or n % 64 or k == 0 or n == 0 or r % 8 or not 0 < r <= _lib.ADAPTER_MAX_RANK or not 0 < G <= _lib.ADAPTER_MAX:
-        raise NotImplementedError(f"built for widths of multiples of 64, ranks of multiples of 8 up to {_lib.ADAPTER_MAX_RANK} and up to "
-                                  f"{_lib.ADAPTER_MAX} adapters; got {k} -> {n}, rank {r}, {G} adapters")
+        _refuse_adapter_linear(x, weight, bias, adapters, plan)
     if (
         x.requires_grad or weight.requires_grad or A.requires_grad or Bm.requires_grad or scale.requires_grad
         or (bias is not None and bias.requires_grad)
     ) and torch.is_grad_enabled():
         raise RuntimeError("adapter_linear has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
-    M, T = x.numel() // k, tiles.shape[0] if tiles.dim() == 2 else -1
-    a = AdapterLinearArgs()
-    a.order, a.ids = _i32(plan.order, "plan.order", (M,)), _i32(plan.ids, "plan.ids", (M,))
-    a.tiles, a.max_tiles = _i32(tiles, "plan.tiles", (T, 4)), T
     x = _aligned_rows(x)
-    shape = (*x.shape[:-1], n)
-    if out is not None and (out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous()):
-        raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
+    shape = (*xs[:-1], n)
     if out is None:
         out = x.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
+    L = lib()
+    space = torch.empty(L.pk_adapter_workspace_bytes(M, r, k, T), dtype=torch.uint8, device=dev)
+    a = AdapterLinearArgs()
+    a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters, a.max_tiles = dtype_code(dt), _index(dev), M, n, k, r, G, T
+    if silu:
+        a.activation = _lib.ACT_SILU
     if bias is not None:
         a.bias = bias.data_ptr()
-    L = lib()
-    ws = torch.empty(L.pk_adapter_workspace_bytes(M, r, k, T), dtype=torch.uint8, device=dev)
-    a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters = code, _index(dev), M, n, k, r, G
-    a.activation = _lib.ACT_SILU if silu else _lib.ACT_NONE
-    a.x, a.x_stride, a.out, a.out_stride = x.data_ptr(), k, out.data_ptr(), n
-    a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
-    a.a, a.b, a.scale, a.workspace = A.data_ptr(), Bm.data_ptr(), scale.data_ptr(), ws.data_ptr()
+    a.x, a.x_stride, a.weight, a.weight_stride, a.out, a.out_stride = x.data_ptr(), k, weight.data_ptr(), weight.stride(0), out.data_ptr(), n
+    a.a, a.b, a.scale, a.workspace = A.data_ptr(), Bm.data_ptr(), scale.data_ptr(), space.data_ptr()
+    a.order, a.ids, a.tiles = order.data_ptr(), ids.data_ptr(), tiles.data_ptr()
     check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out
+
+
+def _refuse_adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, adapters: Adapters, plan: AdapterPlan) -> None:
+    """Says what :func:`adapter_linear` does not take of a call."""
+    A, Bm, scale = adapters.a, adapters.b, adapters.scale
+    dt, dev = x.dtype, _require_device(x, weight, A, Bm, scale, plan.order, plan.ids, plan.tiles)
+    dtype_code(dt)
+    if x.dim() == 0 or weight.dim() != 2:
+        raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _check_linear(dt, dev, x, weight, bias)
+    n, k = weight.shape
+    G, r = A.shape[:2] if A.dim() == 3 else (0, 0)
+    if A.shape != (G, r, k) or Bm.shape != (G, n, r) or A.dtype != dt or Bm.dtype != dt or not A.is_contiguous() or not Bm.is_contiguous():
+        raise ValueError(f"adapters must be contiguous a [G, r, {k}] and b [G, {n}, r] of {dt}, got {tuple(A.shape)} {A.dtype} and "
+                         f"{tuple(Bm.shape)} {Bm.dtype}")
+    if scale.dtype != torch.float32 or scale.shape != (G,) or not scale.is_contiguous():
+        raise ValueError(f"scale must be contiguous float32 [{G}], got {tuple(scale.shape)} {scale.dtype}")
+    if k % 64 or n % 64 or k == 0 or n == 0 or r % 8 or not 0 < r <= _lib.ADAPTER_MAX_RANK or not 0 < G <= _lib.ADAPTER_MAX:
+        raise NotImplementedError(f"built for widths of multiples of 64, ranks of multiples of 8 up to {_lib.ADAPTER_MAX_RANK} and up to "
+                                  f"{_lib.ADAPTER_MAX} adapters; got {k} -> {n}, rank {r}, {G} adapters")
+    M = x.numel() // k
+    _i32(plan.order, "plan.order", (M,))
+    _i32(plan.ids, "plan.ids", (M,))
+    _i32(plan.tiles, "plan.tiles", (plan.tiles.shape[0] if plan.tiles.dim() else 0, 4))
+    raise ValueError(f"adapter_linear does not take x {tuple(x.shape)}, weight {tuple(weight.shape)} with strides {weight.stride()}")
