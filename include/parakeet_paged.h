@@ -877,8 +877,8 @@ int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream);
  * x [rows][k], weight [n][k], out [rows][n]: row strides in elements, rows 16-byte
  * aligned; bias [n] or NULL; a [num_adapters][rank][k], b [num_adapters][n][rank]
  * contiguous; scale fp32 [num_adapters].  order, ids, tiles: pk_adapter_plan's for
- * these rows.  workspace: pk_adapter_workspace_bytes(rows, rank, k, max_tiles), 16-byte
- * aligned.
+ * these rows.  workspace: pk_adapter_workspace_bytes(...) on the call's device, 16-byte
+ * aligned (NULL where that is 0: few rows with few adapters take one launch).
  * n and k multiples of 64, rank of 8 and at most PK_ADAPTER_MAX_RANK.
  * x, weight, out, the workspace and one adapter's a and b are each below 2^31 bytes.
  * activation: PK_ACT_NONE or PK_ACT_SILU.  out overlaps no operand.
@@ -908,7 +908,7 @@ typedef struct pk_adapter_linear_args {
   void* out;
   int64_t out_stride;
 } pk_adapter_linear_args;
-int64_t pk_adapter_workspace_bytes(int32_t rows, int32_t rank, int32_t k, int32_t max_tiles);
+int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles);
 int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------

@@ -88,6 +88,24 @@ __device__ static inline u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t o
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
 }
 
+// 4 ranks of a row of h, scaled, at q (their low parts r elements on)
+template <typename ST>
+__device__ static inline void store_low(f32x4_t v, float sc, ST* q, int r) {
+  float f[4] = {v.x * sc, v.y * sc, v.z * sc, v.w * sc};
+  if constexpr (sizeof(ST) == 4) {
+    st16(q, Tr<float>::pack(f));
+  } else {
+    float lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float hi = round_to<ST>(f[e]);
+      lo[e] = fabsf(hi) < __builtin_inff() ? f[e] - hi : 0.f;
+    }
+    *reinterpret_cast<u32x2*>(q) = pack4<ST>(f);
+    *reinterpret_cast<u32x2*>(q + r) = pack4<ST>(lo);
+  }
+}
+
 // h of a tile: its 32 rows of x and 16 RT rows of A through LDS, 512 bytes of each a
 // stage, S stages on their way (whole lines; read straight from memory as matrix
 // operands, 16 rows of 64 bytes an instruction, a CU moved 16-34 GB/s).  The waves take
@@ -180,21 +198,7 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
 #pragma unroll
   for (int w = 1; w < kLowWaves; ++w) v += red[(w * RT * 2 + wave) * 64 + lane];
   if (row >= tile.z || c >= p.r) return;  // r is a multiple of 8, c of 4
-  const float sc = p.scale[tile.x];
-  float f[4] = {v.x * sc, v.y * sc, v.z * sc, v.w * sc};
-  if constexpr (sizeof(ST) == 4) {
-    st16(p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * p.r + c, Tr<float>::pack(f));
-  } else {
-    float lo[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float hi = round_to<ST>(f[e]);
-      lo[e] = fabsf(hi) < __builtin_inff() ? f[e] - hi : 0.f;
-    }
-    ST* const q = p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * 2 * p.r + c;
-    *reinterpret_cast<u32x2*>(q) = pack4<ST>(f);
-    *reinterpret_cast<u32x2*>(q + p.r) = pack4<ST>(lo);
-  }
+  store_low<ST>(v, p.scale[tile.x], p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * (sizeof(ST) == 4 ? p.r : 2 * p.r) + c, p.r);
 }
 
 // whether every sum is finite: an infinity or NaN times zero is a NaN
@@ -362,6 +366,46 @@ template <int SILU>
 __device__ static inline float ad_act(float v) {
   if constexpr (SILU) return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
   return v;
+}
+
+// A tile's output: sums of the parts of K, bias and activation, then through LDS (smem,
+// free when every wave is here) to whole 16-byte chunks of the rows that `ord` names.
+template <typename ST, int BM, int BN, int WM, int WN, int WK, int TM, int TN, int SILU>
+__device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f32x4_t (&acc)[TM][TN], const int32_t* ord, int row0, int n0,
+                                        int wave, int lane) {
+  constexpr int E = sizeof(ST), V = 16 / E;
+  constexpr int OS = BN + V;  // LDS row stride of the staged output
+  const int l16 = lane & 15, kg = lane >> 4;
+  const int wk = wave / (WM * WN), wm = (wave / WN) % WM, wn = wave % WN;
+  sum_parts<BM, BN, WM * WN, WK>(smem, BM * OS * E, acc, wave, lane);
+  ST* const os = reinterpret_cast<ST*>(smem);
+  if (wk == 0) {
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+      const int c = (wn * TN + n) * 16 + kg * 4;
+      float b[4] = {0.f, 0.f, 0.f, 0.f};
+      if (p.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = from_st(p.bias[n0 + c + e]);
+      }
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        float f[4] = {acc[m][n].x, acc[m][n].y, acc[m][n].z, acc[m][n].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = ad_act<SILU>(f[e] + b[e]);
+        ST* const o = os + ((wm * TM + m) * 16 + l16) * OS + c;
+        if constexpr (E == 4)
+          *reinterpret_cast<u32x4*>(o) = Tr<float>::pack(f);
+        else
+          *reinterpret_cast<u32x2*>(o) = pack4<ST>(f);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < BM * BN / V; i += 64 * WM * WN * WK) {
+    const int r = i / (BN / V), c = (i % (BN / V)) * V;
+    if (row0 + r < p.M) st16(p.out + (int64_t)ord[r] * p.out_s + n0 + c, *reinterpret_cast<const u32x4*>(os + r * OS + c));
+  }
 }
 
 // The product with W: BM x BN outputs a workgroup, both operands staged in LDS as in
@@ -595,35 +639,184 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     }
   }
   __syncthreads();
-  sum_parts<BM, BN, WM * WN, WK>(smem, kOut, acc, wave, lane);
-  ST* const os = reinterpret_cast<ST*>(smem);
-  if (wk == 0) {
-#pragma unroll
-    for (int n = 0; n < TN; ++n) {
-      const int c = (wn * TN + n) * 16 + kg * 4;
-      float b[4] = {0.f, 0.f, 0.f, 0.f};
-      if (p.bias) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = from_st(p.bias[n0 + c + e]);
-      }
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        float f[4] = {acc[m][n].x, acc[m][n].y, acc[m][n].z, acc[m][n].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = ad_act<SILU>(f[e] + b[e]);
-        ST* const o = os + ((wm * TM + m) * 16 + l16) * OS + c;
-        if constexpr (E == 4)
-          *reinterpret_cast<u32x4*>(o) = Tr<float>::pack(f);
-        else
-          *reinterpret_cast<u32x2*>(o) = pack4<ST>(f);
-      }
-    }
+  store_out<ST, BM, BN, WM, WN, WK, TM, TN, SILU>(p, smem, acc, ord, row0, n0, wave, lane);
+}
+
+// Few rows, in one launch: 16 rows x BN outputs a workgroup, their x whole in LDS, where h of
+// the tile's adapters is made while the first stages of W are on their way.  Every
+// workgroup of a row tile makes the same h again and reads its adapters' A, which is less
+// than a launch of its own (3.3 us of the host's, 4 of the GPU's) while a tile has few
+// adapters.  RW: bytes of a row of x.
+template <typename ST, int RW, int RT, int BN, int WN, int WK, int BKB, int S, int SILU>
+__global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST> p) {
+#pragma clang fp contract(off)
+  constexpr int E = sizeof(ST), V = 16 / E, COLS = MmaA<ST>::COLS;
+  constexpr int K = RW / E, BK = BKB / E, CH = BKB / 16;
+  constexpr int NW = WN * WK, BM = 16, TN = BN / WN / 16;
+  constexpr int kAct = BM * RW, kStage = BN * BKB;
+  constexpr int LPS = kStage / 1024 / NW, LPX = kAct / 1024 / NW;
+  constexpr int KS = CH / 4 / WK, iters = K / BK;
+  static_assert(NW == 8 && BKB % 128 == 0 && RW % BKB == 0 && kStage % (1024 * NW) == 0 && kAct % (1024 * NW) == 0 && KS > 0, "whole waves of chunks");
+  constexpr int U = 4, AS = K / COLS / NW;  // steps of K a wave does for h, U of them on their way
+  static_assert(K % (COLS * NW) == 0, "whole steps a wave");
+  constexpr int OS = BN + V, kOut = BM * OS * E, kRed = (WK - 1) * BM * BN * 4;
+  constexpr int kLow = NW * RT * 1024, kH = BM * RT * 64;
+  constexpr int kMain = kAct + S * kStage > kOut + kRed ? kAct + S * kStage : kOut + kRed;
+  __shared__ __align__(16) unsigned char smem[kMain + kLow + kH + BM * 8];
+  f32x4_t* const red = reinterpret_cast<f32x4_t*>(smem + kMain);
+  unsigned char* const hs = smem + kMain + kLow;  // [16] rows of h
+  int32_t* const ord = reinterpret_cast<int32_t*>(hs + kH);
+  int32_t* const sid = ord + BM;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, kg = lane >> 4;
+  const int wk = wave / WN, wn = wave % WN;
+  int mt_i, nt_i;
+  xcd_tile(p.mtiles, p.xm, mt_i, nt_i);
+  const int row0 = mt_i * BM, n0 = nt_i * BN;
+  if (threadIdx.x < BM) {
+    const int pos = row0 + threadIdx.x;
+    ord[threadIdx.x] = plan_row(p, pos);
+    const int g = p.ids[min(pos, p.M - 1)];
+    sid[threadIdx.x] = pos < p.M && (uint32_t)g < (uint32_t)p.G ? g : -1;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BM * BN / V; i += 64 * NW) {
-    const int r = i / (BN / V), c = (i % (BN / V)) * V;
-    if (row0 + r < p.M) st16(p.out + (int64_t)ord[r] * p.out_s + n0 + c, *reinterpret_cast<const u32x4*>(os + r * OS + c));
+  const int id = sid[l16];
+  const __amdgpu_buffer_rsrc_t rx = bytes_rsrc(p.x, (uint32_t)((p.M - 1) * p.x_s + p.K) * E);
+  const __amdgpu_buffer_rsrc_t rw = bytes_rsrc(p.w, (uint32_t)((p.N - 1) * p.w_s + p.K) * E);
+  unsigned char* const ring = smem + kAct;
+#pragma unroll
+  for (int i = 0; i < LPX; ++i) {
+    const int c = (i * NW + wave) * 64 + lane, r = c / (RW / 16), pos = c % (RW / 16);
+    load_lds16(rx, smem + (i * NW + wave) * 1024, (uint32_t)(ord[r] * p.x_s) * E + (uint32_t)(((pos & ~7) | ((pos ^ r) & 7)) * 16), 0);
   }
+  uint32_t off[LPS];
+#pragma unroll
+  for (int i = 0; i < LPS; ++i) {
+    const int c = (i * NW + wave) * 64 + lane, r = c / CH, pos = c % CH;
+    off[i] = (uint32_t)((n0 + r) * p.w_s) * E + (uint32_t)(((pos & ~7) | ((pos ^ r) & 7)) * 16);
+  }
+  auto issue = [&](int st, int it) {
+#pragma unroll
+    for (int i = 0; i < LPS; ++i) load_lds16(rw, ring + st * kStage + (i * NW + wave) * 1024, off[i], it * BKB);
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < iters) issue(s, s);
+  auto x_frag = [&](int ch) { return *reinterpret_cast<const u32x4*>(smem + l16 * RW + ((ch & ~7) | ((ch ^ l16) & 7)) * 16); };
+  auto meet = [&]() {  // the waves' LDS stores are done; loads to LDS stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  f32x4_t acc[1][TN];
+#pragma unroll
+  for (int n = 0; n < TN; ++n) acc[0][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const uint32_t arow = (uint32_t)p.r * E, chunks = p.r >> 2;
+  uint32_t left = (uint32_t)(__ballot(id >= 0) & 0xffff);
+  int turn = 0;
+  bool first = true;
+  while (left) {
+    const int g = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    const bool mine = id == g;
+    left &= ~(uint32_t)(__ballot(mine) & 0xffff);
+    const __amdgpu_buffer_rsrc_t ra = bytes_rsrc(p.a + (int64_t)g * p.r * K, arow * K);
+    const __amdgpu_buffer_rsrc_t rb = bytes_rsrc(p.b + (int64_t)g * p.N * p.r, (uint32_t)p.N * arow);
+    f32x4_t h[RT];
+#pragma unroll
+    for (int j = 0; j < RT; ++j) h[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s0 = 0; s0 < AS; s0 += U) {
+      u32x4 af[U][RT];
+#pragma unroll
+      for (int u = 0; u < U && s0 + u < AS; ++u)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+          af[u][j] = load16(ra, (uint32_t)(min(j * 16 + l16, p.r - 1) * K + ((s0 + u) * NW + wave) * COLS) * E + kg * 16u);
+      if (first) {  // the rows of x are in for every wave
+        wait_vm<0>();
+        meet();
+        first = false;
+      }
+#pragma unroll
+      for (int u = 0; u < U && s0 + u < AS; ++u)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) h[j] = MmaA<ST>::step(af[u][j], x_frag(((s0 + u) * NW + wave) * 4 + kg), h[j]);
+    }
+    // this adapter's B for the wave's columns, on its way while the sums meet
+    u32x4 bf[RT][TN];
+    const bool turn_mine = turn == wk;
+    turn = turn == WK - 1 ? 0 : turn + 1;
+    if (turn_mine) {
+#pragma unroll
+      for (int q = 0; q < RT; ++q)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+          const uint32_t c = q * 4 + kg;  // 16 ranks a step
+          bf[q][n] = load16(rb, c < chunks ? (uint32_t)(n0 + (wn * TN + n) * 16 + l16) * arow + (uint32_t)b_chunk<ST>(c, p.r) * 16u : kNowhere);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j) red[(wave * RT + j) * 64 + lane] = h[j];
+    meet();
+    if (wave < RT) {
+      f32x4_t v = red[wave * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v += red[(w * RT + wave) * 64 + lane];
+      const int c = wave * 16 + kg * 4;
+      if (mine && c < p.r) store_low<ST>(v, p.scale[g], reinterpret_cast<ST*>(hs + l16 * (RT * 64)) + c, p.r);
+    }
+    meet();
+    if (turn_mine) {
+      f32x4_t d[TN];
+#pragma unroll
+      for (int n = 0; n < TN; ++n) d[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < RT; ++q) {
+        const uint32_t c = q * 4 + kg;
+        u32x4 hf = {0u, 0u, 0u, 0u};
+        if (mine && c < chunks) hf = *reinterpret_cast<const u32x4*>(hs + l16 * (RT * 64) + c * 16);
+#pragma unroll
+        for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(bf[q][n], hf, d[n]);
+      }
+      // columns (rows of the batch) are independent: kept for the adapter's own rows
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][n][e] = mine ? d[n][e] : acc[0][n][e];
+    }
+  }
+
+  int st = 0;
+#pragma unroll 1
+  for (int it = 0; it < iters; ++it) {
+    if (!first && it + S - 2 < iters)
+      wait_vm<(S - 2) * LPS>();
+    else
+      wait_vm<0>();
+    first = false;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, it + S - 1);
+    const unsigned char* ws = ring + st * kStage;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int ch = (wk * KS + s) * 4 + kg;
+      const u32x4 xf = x_frag(it * CH + ch);
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        const int r = (wn * TN + n) * 16 + l16;
+        const u32x4 wf = *reinterpret_cast<const u32x4*>(ws + r * BKB + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+        acc[0][n] = MmaA<ST>::step(wf, xf, acc[0][n]);
+      }
+    }
+    st = st == S - 1 ? 0 : st + 1;
+  }
+  __syncthreads();
+  store_out<ST, BM, BN, 1, WN, WK, 1, TN, SILU>(p, smem, acc, ord, row0, n0, wave, lane);
 }
 
 namespace {
@@ -728,6 +921,50 @@ int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
   }
 }
 
+template <typename ST, int RW, int RT, int BN, int WN, int WK, int BKB, int S, int SILU>
+int launch_few_t(AdK<ST> k, hipStream_t s) {
+  k.mtiles = (k.M + 15) / 16;
+  const int nt = k.N / BN;
+  k.xm = xcd_split(k.mtiles, nt, 16, BN);
+  dim3 grid((unsigned)(k.mtiles * nt));
+  if (k.xm > 0) grid = dim3(8u, (unsigned)(k.mtiles / k.xm), (unsigned)(nt / (8 / k.xm)));
+  hipLaunchKernelGGL((adapter_few_kernel<ST, RW, RT, BN, WN, WK, BKB, S, SILU>), grid, dim3(64 * WN * WK), 0, s, k);
+  return check_launch("pk_adapter_linear");
+}
+
+template <typename ST, int RW, int RT, int SILU>
+int launch_few_n(const AdK<ST>& k, int bn, hipStream_t s) {
+  if (bn == 16) return launch_few_t<ST, RW, RT, 16, 1, 8, 1024, 2, SILU>(k, s);
+  if (bn == 32) return launch_few_t<ST, RW, RT, 32, 1, 8, 1024, 2, SILU>(k, s);
+  if (bn == 64) return launch_few_t<ST, RW, RT, 64, 2, 4, 256, 3, SILU>(k, s);
+  return launch_few_t<ST, RW, RT, 128, 4, 2, 256, 3, SILU>(k, s);
+}
+
+template <typename ST, int SILU>
+int launch_few(const AdK<ST>& k, int bn, hipStream_t s) {
+  const bool wide = k.K * (int)sizeof(ST) == 2048;
+  if (k.r <= 16) return wide ? launch_few_n<ST, 2048, 1, SILU>(k, bn, s) : launch_few_n<ST, 1024, 1, SILU>(k, bn, s);
+  return wide ? launch_few_n<ST, 2048, 2, SILU>(k, bn, s) : launch_few_n<ST, 1024, 2, SILU>(k, bn, s);
+}
+
+// adapters that the rows of a plan with so many tiles have at most
+int64_t most_adapters(int64_t rows, int64_t max_tiles) { return max_tiles - rows / kLowRows > 1 ? max_tiles - rows / kLowRows : 1; }
+
+// Outputs a workgroup of the few-row form: the fewest that give no CU a second tile; 0
+// where two launches are as fast.  The line is what a tile's adapters (as many as the
+// plan may have) take of A, 96 KB.  In a graph, few-row form and two launches, 128 rows 512 ->
+// 2048 bf16: rank 16, one adapter (16 KB) 7.8 us and 10.0, 3 a tile (46 KB) 9.0 and 10.4, 5 (78
+// KB) 12.8 and 10.7, rank 32, 3 a tile (93 KB) 11.7 and 10.9; called one by one the second
+// launch is 3.3 us of the host's besides.
+int few_form(int64_t M, int64_t N, int64_t row_bytes, int r, int64_t adapters, int cus) {
+  if ((row_bytes != 1024 && row_bytes != 2048) || r > 32) return 0;
+  const float runs = fminf(fminf(16.f, (float)M), 1.f + (float)(adapters - 1) * 16.f / M);
+  if (runs * (float)r * (float)row_bytes > 96.f * 1024.f) return 0;
+  for (int bn = 16; bn <= 128; bn *= 2)
+    if (N % bn == 0 && (M + 15) / 16 * (N / bn) <= cus) return bn;
+  return 0;
+}
+
 // below 2^31 bytes: 32-bit offsets, and kNowhere past them
 bool rows_ok(int64_t rows, int64_t stride, int64_t width, int bytes) {
   return stride >= 0 && stride * bytes % 16 == 0 && (rows <= 1 || stride >= width) &&
@@ -748,7 +985,9 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
     return fail(PK_ERR_INVALID, "%s: activation %d must be none or SiLU", what, a->activation);
   if (a->max_tiles < 0) return fail(PK_ERR_INVALID, "%s: max_tiles %d < 0", what, a->max_tiles);
   if (a->rows == 0) return PK_OK;
-  const void* ptrs[9] = {a->x, a->a, a->b, a->weight, a->bias ? a->bias : a->x, a->tiles, a->out, a->workspace, a->scale};
+  const int few = few_form(a->rows, a->n, (int64_t)a->k * sizeof(ST), a->rank, most_adapters(a->rows, a->max_tiles), cu_count());
+  const void* ptrs[9] = {a->x,     a->a,   a->b, a->weight, a->bias ? a->bias : a->x,
+                         a->tiles, a->out, few ? a->x : a->workspace, a->scale};
   for (const void* q : ptrs) {
     if (!q) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
     if (q != a->scale && !aligned16(q)) return fail(PK_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
@@ -784,21 +1023,23 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   k.kpart = ((k.K / 64 + k.parts - 1) / k.parts) * 64;
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
+  const int64_t adapters = most_adapters(k.M, a->max_tiles);
+  const int cus = cu_count();
+  if (few) return a->activation == PK_ACT_SILU ? launch_few<ST, 1>(k, few, s) : launch_few<ST, 0>(k, few, s);
   if (a->max_tiles > 0) {
     const int rc = launch_low(k, a->max_tiles, s);
     if (rc != PK_OK) return rc;
   }
-  int64_t adapters = a->max_tiles - a->rows / kLowRows;  // at most
-  if (adapters < 1) adapters = 1;
-  const int cus = cu_count();
   return a->activation == PK_ACT_SILU ? launch_product<ST, 1>(k, adapters, cus, s) : launch_product<ST, 0>(k, adapters, cus, s);
 }
 
 }  // namespace
 }  // namespace pk
 
-extern "C" int64_t pk_adapter_workspace_bytes(int32_t rows, int32_t rank, int32_t k, int32_t max_tiles) {
-  if (rows <= 0 || rank <= 0 || k <= 0 || max_tiles < 0) return 0;
+extern "C" int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles) {
+  if (rows <= 0 || n <= 0 || rank <= 0 || k <= 0 || max_tiles < 0) return 0;
+  const int64_t row = (int64_t)k * (dtype == PK_DTYPE_F32 ? 4 : 2);
+  if (pk::few_form(rows, n, row, rank, pk::most_adapters(rows, max_tiles), pk::cu_count())) return 0;
   return ((int64_t)rows + 1) * rank * 4 * pk::k_parts(max_tiles, rank, k);
 }
 

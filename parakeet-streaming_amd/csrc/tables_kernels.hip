@@ -47,9 +47,8 @@ struct PageK {
   int32_t reset;  // give every page of the slots back instead
   StepOf* of;  // more than kStepOne streams: [n]
   uint32_t* front;
-  uint2* part;  // more than kStepTwo: [npad] pages given back and taken, 0 from n on
-  uint2* at;    // and those before the stream's
-  int32_t npad;
+  uint2* part;  // more than kStepTwo: [n] pages given back and taken
+  uint2* sum;   // and of each 256 streams, then of those before them
 };
 
 // inclusive sum over the 64 lanes of a wave
@@ -84,11 +83,9 @@ __device__ static inline T block_scan(T v, T* lds, T& sum) {
 }
 
 constexpr int kStepThreads = 1024;
-constexpr int kPartPad = 16;
-inline int part_pad(int n) { return (n + kPartPad - 1) / kPartPad * kPartPad; }
-// Streams of a step in one launch (64 take 7.8 us so and 8.8 in two, 128 12 and 10) and in
-// two (2048 take 12.8 us so and 15.6 in four, 4096 16.8 and 17.0, 16384 51 and 26)
-constexpr int kStepOne = 64, kStepTwo = 4096;
+// Streams of a step in one launch (64 take 8.0 us in a graph so and 8.8 in two, 128 12 and
+// 10.1) and in two (2048 take 12.7 us so and 15.3 in four, 4096 16.8 and 15.7, 16384 51 and 18)
+constexpr int kStepOne = 64, kStepTwo = 3500;
 
 struct StreamPages {
   uint32_t A;
@@ -273,58 +270,52 @@ __global__ void __launch_bounds__(256) page_rows_kernel(const PageK p) {
 }
 
 // Thousands of streams: one CU's scattered reads (0.6 a ns) of their frame counts and
-// rings would be the step (16384 streams: 44 us), so only the sums are one workgroup's:
-// what each stream gives and takes, their sums, the pages given back, the rows, a launch
-// each.
-__global__ void __launch_bounds__(256) page_part_kernel(const PageK p) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b >= p.n) {
-    if (b < p.npad) p.part[b] = uint2{0, 0};
-    return;
-  }
-  const int32_t slot = p.slots[b], want = p.lengths ? p.lengths[b] : p.chunk;
+// rings, and its share of the memory's rate, would be the step (16384 streams: 44 us). So a
+// workgroup sums what its 256 streams give and take, one workgroup sums the sums and looks
+// for equal slots, the pages go back, the rows are written, a launch each.
+constexpr int kPartThreads = 256;
+
+__global__ void __launch_bounds__(kPartThreads) page_part_kernel(const PageK p) {
+  __shared__ uint64_t sums[kPartThreads / 64];
+  const int b = blockIdx.x * kPartThreads + threadIdx.x;
+  const int32_t slot = b < p.n ? p.slots[b] : -1, want = p.lengths && b < p.n ? p.lengths[b] : p.chunk;
   const StreamPages s = stream_pages(p, b, slot, want, (uint32_t)slot < (uint32_t)p.S ? p.appended[slot] : 0, nullptr);
-  p.of[b] = StepOf{(int32_t)s.A, s.slot, s.len, 0};
-  p.part[b] = uint2{(uint32_t)s.freed, (uint32_t)s.taken};
+  uint64_t all;
+  block_scan<kPartThreads / 64>((uint64_t)(uint32_t)s.freed << 32 | (uint32_t)s.taken, sums, all);
+  if (b < p.n) {
+    p.of[b] = StepOf{(int32_t)s.A, s.slot, s.len, 0};
+    p.part[b] = uint2{(uint32_t)s.freed, (uint32_t)s.taken};
+  }
+  if (threadIdx.x == 0) p.sum[blockIdx.x] = uint2{(uint32_t)(all >> 32), (uint32_t)all};
 }
 
-// V neighbouring streams a lane, 16384 a turn: a turn is one chain of round trips
 __global__ void __launch_bounds__(kStepThreads) page_sums_kernel(const PageK p) {
-  constexpr int V = kPartPad;
   extern __shared__ uint32_t lds[];
   __shared__ uint64_t sums[kStepThreads / 64];
-  const uint32_t* dup = mark_slots<V>(p, lds);
+  const uint32_t* dup = mark_slots<16>(p, lds);
   uint32_t twice = 0;
   for (int i = threadIdx.x; i < (p.S + 31) >> 5; i += kStepThreads) twice |= dup[i];
   if (__syncthreads_or(twice)) {
     for (int b = threadIdx.x; b < p.n; b += kStepThreads)
       if (named_before(p, b, p.slots[b], dup)) {
+        const uint2 s = p.part[b];
+        atomicSub(&p.sum[b / kPartThreads].x, s.x);
+        atomicSub(&p.sum[b / kPartThreads].y, s.y);
         p.part[b] = uint2{0, 0};
         p.of[b] = StepOf{0, -1, 0, 0};
       }
+    __threadfence();
     __syncthreads();
   }
   const uint32_t total = (uint32_t)p.total, first = (uint32_t)p.head[0] % total, count = (uint32_t)p.head[1];
+  const int blocks = (p.n + kPartThreads - 1) / kPartThreads;
   uint64_t carry = 0;
-  for (int b0 = 0; b0 < p.n; b0 += kStepThreads * V) {
-    const int b = b0 + threadIdx.x * V;
-    u32x4 s[V / 2];
-    uint64_t run = 0, all;
-#pragma unroll
-    for (int v = 0; v < V / 2; ++v) s[v] = b < p.n ? ld16(p.part + b + v * 2) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int v = 0; v < V / 2; ++v) run += (uint64_t)(s[v].x + s[v].z) << 32 | (s[v].y + s[v].w);
-    run = block_scan<kStepThreads / 64>(run, sums, all) + carry;
-    uint32_t f = (uint32_t)(run >> 32), t = (uint32_t)run;
-    if (b < p.n) {
-#pragma unroll
-      for (int v = 0; v < V / 2; ++v) {
-        const u32x4 at = {f, t, f + s[v].x, t + s[v].y};
-        st16(p.at + b + v * 2, at);
-        f += s[v].x + s[v].z;
-        t += s[v].y + s[v].w;
-      }
-    }
+  for (int i0 = 0; i0 < blocks; i0 += kStepThreads) {
+    const int i = i0 + threadIdx.x;
+    const uint2 s = i < blocks ? p.sum[i] : uint2{0, 0};
+    uint64_t all;
+    const uint64_t at = block_scan<kStepThreads / 64>((uint64_t)s.x << 32 | s.y, sums, all) + carry;
+    if (i < blocks) p.sum[i] = uint2{(uint32_t)(at >> 32), (uint32_t)at};
     carry += all;
   }
   if (threadIdx.x == 0) {
@@ -335,17 +326,19 @@ __global__ void __launch_bounds__(kStepThreads) page_sums_kernel(const PageK p) 
   }
 }
 
-__global__ void __launch_bounds__(256) page_back_kernel(const PageK p) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b >= p.n) return;
-  const StepOf s = p.of[b];
+__global__ void __launch_bounds__(kPartThreads) page_back_kernel(const PageK p) {
+  __shared__ uint64_t sums[kPartThreads / 64];
+  const int b = blockIdx.x * kPartThreads + threadIdx.x;
+  const StepOf s = b < p.n ? p.of[b] : StepOf{0, -1, 0, 0};
+  const uint2 part = b < p.n ? p.part[b] : uint2{0, 0}, base = p.sum[blockIdx.x];
+  uint64_t all;
+  const uint64_t at = block_scan<kPartThreads / 64>((uint64_t)part.x << 32 | part.y, sums, all);
   if (s.slot < 0) return;
-  const uint2 part = p.part[b], at = p.at[b];
   if (part.x) {
     const uint32_t A = (uint32_t)s.A, lo = A > (uint32_t)p.window ? (A - p.window) >> p.page_shift : 0;
-    give_back(p, s.slot, part.x, lo % (uint32_t)p.M, (p.front[1] + at.x) % (uint32_t)p.total, nullptr);
+    give_back(p, s.slot, part.x, lo % (uint32_t)p.M, (p.front[1] + base.x + (uint32_t)(at >> 32)) % (uint32_t)p.total, nullptr);
   }
-  p.of[b].at = at.y;
+  p.of[b].at = base.y + (uint32_t)at;
   p.appended[s.slot] = (int64_t)(uint32_t)s.A + s.len;
 }
 
@@ -534,8 +527,7 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
     k.of = static_cast<StepOf*>(a->workspace);
     k.front = reinterpret_cast<uint32_t*>(k.of + k.n);
     k.part = reinterpret_cast<uint2*>(k.of + k.n + 1);
-    k.npad = part_pad(k.n);
-    k.at = k.part + k.npad;
+    k.sum = k.part + k.n;
   }
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
@@ -544,13 +536,13 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
     hipLaunchKernelGGL(page_step_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
     return check_launch(what);
   }
-  const dim3 all((unsigned)((k.npad + 255) / 256));
+  const dim3 all((unsigned)((k.n + kPartThreads - 1) / kPartThreads));
   if (k.n <= kStepTwo) {
     hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
   } else {
-    hipLaunchKernelGGL(page_part_kernel, all, dim3(256), 0, s, k);
+    hipLaunchKernelGGL(page_part_kernel, all, dim3(kPartThreads), 0, s, k);
     hipLaunchKernelGGL(page_sums_kernel, dim3(1), dim3(kStepThreads), bits, s, k);
-    hipLaunchKernelGGL(page_back_kernel, all, dim3(256), 0, s, k);
+    hipLaunchKernelGGL(page_back_kernel, all, dim3(kPartThreads), 0, s, k);
   }
   hipLaunchKernelGGL(page_rows_kernel, dim3((unsigned)((k.n + 7) / 8)), dim3(256), 0, s, k);
   return check_launch(what);
@@ -599,7 +591,9 @@ int adapter_plan(const pk_adapter_plan_args* a, hipStream_t s) {
 }  // namespace pk
 
 extern "C" int64_t pk_page_step_workspace_bytes(int32_t batch) {
-  return batch > pk::kStepOne ? ((int64_t)batch + 1) * sizeof(pk::StepOf) + (int64_t)pk::part_pad(batch) * 2 * sizeof(uint2) : 0;
+  if (batch <= pk::kStepOne) return 0;
+  const int64_t blocks = ((int64_t)batch + pk::kPartThreads - 1) / pk::kPartThreads;
+  return ((int64_t)batch + 1) * sizeof(pk::StepOf) + (batch > pk::kStepTwo ? (batch + blocks) * (int64_t)sizeof(uint2) : 0);
 }
 
 extern "C" int pk_page_step(const pk_page_step_args* args, void* stream) {

@@ -488,7 +488,7 @@ SIGNATURES = {
     "pk_adapter_plan_tiles": (c_int, [c_int32, c_int32, c_int32]),
     "pk_adapter_plan_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "pk_adapter_plan": (c_int, [POINTER(AdapterPlanArgs), c_void_p]),
-    "pk_adapter_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "pk_adapter_workspace_bytes": (c_int64, [c_int32] * 6),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
     "pk_pool_create": (
         c_int,

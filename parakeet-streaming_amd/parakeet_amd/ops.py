@@ -1331,15 +1331,18 @@ def adapter_linear(
     elif out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
     L = lib()
-    space = torch.empty(L.pk_adapter_workspace_bytes(M, r, k, T), dtype=torch.uint8, device=dev)
-    a = AdapterLinearArgs()
-    a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters, a.max_tiles = dtype_code(dt), _index(dev), M, n, k, r, G, T
+    a, code = AdapterLinearArgs(), dtype_code(dt)
+    space = L.pk_adapter_workspace_bytes(code, M, n, k, r, T)
+    if space:
+        space = torch.empty(space, dtype=torch.uint8, device=dev)
+        a.workspace = space.data_ptr()
+    a.dtype, a.device, a.rows, a.n, a.k, a.rank, a.num_adapters, a.max_tiles = code, _index(dev), M, n, k, r, G, T
     if silu:
         a.activation = _lib.ACT_SILU
     if bias is not None:
         a.bias = bias.data_ptr()
     a.x, a.x_stride, a.weight, a.weight_stride, a.out, a.out_stride = x.data_ptr(), k, weight.data_ptr(), weight.stride(0), out.data_ptr(), n
-    a.a, a.b, a.scale, a.workspace = A.data_ptr(), Bm.data_ptr(), scale.data_ptr(), space.data_ptr()
+    a.a, a.b, a.scale = A.data_ptr(), Bm.data_ptr(), scale.data_ptr()
     a.order, a.ids, a.tiles = order.data_ptr(), ids.data_ptr(), tiles.data_ptr()
     check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out

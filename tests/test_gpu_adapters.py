@@ -71,7 +71,7 @@ def _run(x, w, bias, ad, ids, silu=False, **kw):
 @pytest.mark.parametrize("B,T,K,N,r,G", [
     (1, 1, 512, 512, 8, 1), (1, 2, 512, 2048, 16, 8), (5, 3, 64, 64, 8, 2), (17, 1, 640, 640, 24, 40), (61, 1, 1024, 1024, 16, 64),
     (40, 14, 512, 512, 32, 6), (128, 2, 512, 2048, 64, 20), (60, 14, 1024, 1024, 128, 4), (3, 14, 4096, 1024, 48, 3), (33, 1, 192, 320, 40, 512),
-    (700, 1, 256, 128, 8, 300),
+    (700, 1, 256, 128, 8, 300), (9, 14, 512, 64, 24, 3), (37, 3, 1024, 192, 32, 1), (150, 2, 512, 2048, 16, 16), (5, 1, 256, 64, 32, 2),
 ])
 def test_against_64_bits(cuda, dtype, B, T, K, N, r, G):
     x, w, bias, ad, ids = _make(cuda, B, T, K, N, r, G, dtype, seed=B + K, bias=B % 2 == 1)

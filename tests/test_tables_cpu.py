@@ -159,7 +159,7 @@ def test_adapter_linear_refusals():
         setattr(a, field, keep)
     a.rows = 0
     assert L.pk_adapter_linear(ctypes.byref(a), None) == _lib.PK_OK
-    assert L.pk_adapter_workspace_bytes(10, 16, 512, 4) >= 640 and L.pk_adapter_workspace_bytes(0, 16, 512, 4) == 0
+    assert L.pk_adapter_workspace_bytes(_lib.DTYPE_F16, 2000, 2048, 640, 16, 90) >= 2000 * 64 and L.pk_adapter_workspace_bytes(_lib.DTYPE_F16, 0, 64, 512, 16, 4) == 0
 
 
 def test_cpu_tensors_are_refused():
