@@ -1297,8 +1297,10 @@ def adapter_linear(
 ) -> torch.Tensor:
     """``x @ weight.T + bias + scale[g] * (x @ a[g].T) @ b[g].T``, g the adapter of x's row in
     ``plan``, and SiLU of it: a shared projection with the low-rank adapter of each
-    stream beside it, in two launches, the output rounded once.  x [..., K], weight
-    [N, K], bias [N] or None; N and K multiples of 64, ranks of 8 up to 128.  No gradients."""
+    stream beside it, the output rounded once.  Two launches, or one for few rows of few
+    adapters.  x [..., K], weight [N, K], bias [N] or None; N and K multiples of 64, ranks
+    of 8 up to 128; ``out`` overlaps no operand.  What a row gets depends on its own
+    adapter alone.  No gradients."""
     A, Bm, scale, order, ids, tiles = adapters.a, adapters.b, adapters.scale, plan.order, plan.ids, plan.tiles
     dt, dev, ws, xs = x.dtype, x.device, weight.shape, x.shape
     n, k = ws if len(ws) == 2 else (0, 0)
@@ -1328,8 +1330,12 @@ def adapter_linear(
     shape = (*xs[:-1], n)
     if out is None:
         out = x.new_empty(shape)
-    elif out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
+    else:
+        if out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous {shape} of {dt} on {dev}")
+        # workgroups read x, the weights and the banks after others have written
+        if any(_overlap(out, t) for t in (x, weight, A, Bm, scale, order, ids, tiles, bias) if t is not None):
+            raise ValueError("out must not overlap an operand")
     L = lib()
     a, code = AdapterLinearArgs(), dtype_code(dt)
     space = L.pk_adapter_workspace_bytes(code, M, n, k, r, T)
@@ -1346,6 +1352,14 @@ def adapter_linear(
     a.order, a.ids, a.tiles = order.data_ptr(), ids.data_ptr(), tiles.data_ptr()
     check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory spans of two tensors (no negative strides) meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    end = lambda t: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()  # noqa: E731
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def _refuse_adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, adapters: Adapters, plan: AdapterPlan) -> None:

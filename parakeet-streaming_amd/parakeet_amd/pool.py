@@ -136,8 +136,8 @@ class DevicePagePool:
     :class:`PagePool`, advanced by ``ops.page_step`` on torch's current stream.
 
     The inspection methods (``free_pages``, ``free_list``, ``slot_info``) wait for the
-    device; nothing else does.  Steps of one pool run on one stream, or are ordered by
-    the caller's events."""
+    device; nothing else does.  Steps and resets of one pool run on one stream, or are
+    ordered by the caller's events (threads included: there is no lock)."""
 
     def __init__(
         self,
@@ -183,7 +183,9 @@ class DevicePagePool:
         s = np.ascontiguousarray(np.asarray(slots, dtype=np.int32).reshape(-1))
         if len(np.unique(s)) != len(s) or (len(s) and (s.min() < 0 or s.max() >= self.num_slots)):
             raise ValueError(f"slots must be distinct and in [0, {self.num_slots})")
-        return torch.from_numpy(s).to(self.device)
+        t = torch.from_numpy(s)
+        # from pinned memory, without waiting (torch keeps it until the copy has run)
+        return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
     # -- stepping
     def advance(self, slots, lengths: torch.Tensor | None = None, rows=None, slot_map=None):

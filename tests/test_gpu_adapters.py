@@ -101,10 +101,10 @@ def test_mixtures(cuda, dtype, how):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,T", [(40, 1), (9, 14), (200, 2)])
-def test_an_adapter_reaches_its_own_rows_alone(cuda, dtype, B, T):
+@pytest.mark.parametrize("B,T,K,r", [(40, 1, 256, 16), (9, 14, 256, 16), (200, 2, 256, 16), (30, 1, 512, 16), (11, 14, 512, 8), (300, 14, 512, 32)])
+def test_an_adapter_reaches_its_own_rows_alone(cuda, dtype, B, T, K, r):
     """Infinities and NaN in one adapter, or in one row, leave the other rows as they are."""
-    x, w, bias, ad, _ = _make(cuda, B, T, 256, 128, 16, 4, dtype)
+    x, w, bias, ad, _ = _make(cuda, B, T, K, 128, r, 4, dtype)
     ids = (torch.arange(B, device=cuda) * 7 % 5 - 1).to(torch.int32)
     clean = _run(x, w, bias, ad, ids)
     for what in ("a", "b", "scale"):
@@ -222,6 +222,10 @@ def test_refusals(cuda):
         call(ad=ops.Adapters(ad.a.cpu(), ad.b, ad.scale))
     with pytest.raises(ValueError, match="out must"):
         call(out=torch.empty(6, 2, 32, dtype=torch.float16, device=cuda))
+    y, v, c, b2, _ = _make(cuda, 6, 2, 64, 64, 8, 2, torch.float16)
+    for over in (y, v[:12].view(6, 2, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            call(x=y, w=v, bias=c, ad=b2, out=over)
     with pytest.raises(RuntimeError, match="no backward"):
         call(w=w.clone().requires_grad_())
     with pytest.raises(TypeError):

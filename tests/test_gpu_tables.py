@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from parakeet_amd import ops
+from parakeet_amd import _lib, ops
 from parakeet_amd.pool import DevicePagePool, PagePool
 from tests._tables_model import RaggedPool, plan_model
 
@@ -80,6 +80,39 @@ def test_ragged_steps_match_the_model(cuda, n, slots, left, chunk, P):
             dev.reset_slots(_up(gone, cuda))
             model.reset(gone.tolist())
     _same_pool(dev, model)
+
+
+def test_the_most_slots(cuda):
+    """Every slot of the largest pool in one step, twice, against array arithmetic."""
+    S, P, left, chunk = _lib.PAGE_STEP_MAX_SLOTS, 16, 14, 9
+    dev = DevicePagePool(S, P, left, chunk, cuda)
+    rng = np.random.default_rng(2)
+    A, taken = np.zeros(S, dtype=np.int64), 0
+    first = None
+    for step in range(2):
+        slots, lengths = rng.permutation(S), rng.integers(0, chunk + 1, S)
+        rows, place = (t.cpu().numpy() for t in dev.advance(_up(slots, cuda), _up(lengths, cuda)))
+        a = A[slots]
+        np.testing.assert_array_equal(rows[:, 0], a)
+        # no window has moved past a page yet: pages come in order of the streams
+        need = (a + lengths + P - 1) // P - (a + P - 1) // P
+        at = taken + np.cumsum(need) - need
+        if step == 0:
+            np.testing.assert_array_equal(rows[:, 1], np.where(need > 0, at, -1))
+            first = np.full(S, -1)
+            first[slots] = rows[:, 1]
+        else:
+            old = np.where(first[slots] >= 0, first[slots], np.where(need > 0, at, -1))
+            np.testing.assert_array_equal(rows[:, 1], old)
+            np.testing.assert_array_equal(rows[:, 2], np.where(a + lengths > P, at + need - 1, -1))
+        t = np.arange(chunk)[None, :]
+        pos = a[:, None] + t
+        want = np.take_along_axis(rows[:, 1:], pos // P % dev.max_pages, 1) * P + pos % P
+        np.testing.assert_array_equal(place, np.where(t < lengths[:, None], want, -1))
+        taken += int(need.sum())
+        A[slots] = a + lengths
+    assert dev.free_pages() == dev.num_pages - taken
+    assert dev.state.head.tolist() == [taken % dev.num_pages, dev.num_pages - taken]
 
 
 def test_every_slot_the_same(cuda):
