@@ -216,10 +216,9 @@ __device__ static inline bool all_finite(const f32x4_t (&acc)[TM][TN]) {
 
 // add_low where an infinity or NaN is among the operands: where only some of 16 rows have
 // an adapter its product is taken for all of them and kept for those, so that what a row
-// // gets depends on its own adapter alone, and in the same order of sums, so that the rows
-// without them keep their bits: part wk of WK are some of the adapters, or (STEPS) some
-// of each adapter's steps of 4 chunks a lane group.
-template <typename ST, int TM, int TN, int WK, bool STEPS>
+// gets depends on its own adapter alone, and in the same order of sums, so that the rows
+// without them keep their bits.
+template <typename ST, int TM, int TN, int WK>
 __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
                                       f32x4_t (&acc)[TM][TN]) {
   constexpr int V = Tr<ST>::VEC;
@@ -245,7 +244,7 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
       has[m] = __ballot(id[m] == g);
       left[m] &= ~has[m];
     }
-    if (!STEPS && WK > 1 && turn != wk) continue;
+    if (WK > 1 && turn != wk) continue;
     const ST* const bp = p.b + ((int64_t)g * p.N + c0 + l16) * p.r;
     auto b_of = [&](int n, int q) { return q < chunks ? ld16(bp + (int64_t)n * 16 * p.r + b_chunk<ST>(q, p.r) * V) : zero; };
 #pragma unroll
@@ -254,7 +253,7 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
       f32x4_t d[TN];
 #pragma unroll
       for (int n = 0; n < TN; ++n) d[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int q = (STEPS ? 4 * wk : 0) + kg; q - kg < chunks; q += STEPS ? 4 * WK : 4) {
+      for (int q = kg; q - kg < chunks; q += 4) {
         const u32x4 hf = q < chunks ? ld16(hp[m] + q * V) : zero;
 #pragma unroll
         for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(b_of(n, q), hf, d[n]);
@@ -267,41 +266,36 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
   }
 }
 
-// acc[m][n] = h B^T for TM x TN products of rows pos0 + 16 m and columns c0 + 16 n, summed
-// over the adapters among the rows (of these, part `wk` of WK), each with the other
-// adapters' rows of h read as zero.  Work items of one adapter and 4 chunks a lane group,
-// DEP items' loads on their way: a wave with few rows has up to 16 adapters a product,
-// and one by one each would cost a round trip to memory (0.8 us).  A zero row of h times
-// an infinity in B is a NaN in another adapter's rows: sums that are not finite are made
-// again by add_low_apart.
-template <typename ST, int TM, int TN, int WK, int DEP>
-__device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
-                                      f32x4_t (&acc)[TM][TN]) {
+// acc[m][n] += h B^T for TM x TN products of rows pos0 + 16 m and columns c0 + 16 n, over
+// chunks qa .. qb of h, summed over the adapters among the rows (of these, part `wk` of
+// WK), each with the other adapters' rows of h read as zero.  Work items of one adapter and
+// 4 chunks a lane group, DEP items' loads on their way: a wave with few rows has up to 16
+// adapters a product, and one by one each would cost a round trip to memory (0.8 us).
+// LDS: the chunks of h are at hs, kLowRow bytes a row from local row lr0 on, once `ready` has
+// waited for them; else they are read with B's.  A zero row of h times an infinity in B is
+// a NaN in another adapter's rows: the caller makes sums that are not finite again.
+constexpr int kLowChunks = 16, kLowRow = kLowChunks * 16;
+template <typename ST, int TM, int TN, int WK, int DEP, bool LDS, typename Ready>
+__device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane, const unsigned char* hs,
+                                      int lr0, int qa, int qb, Ready ready, f32x4_t (&acc)[TM][TN]) {
   constexpr uint32_t E = sizeof(ST);
   const int l16 = lane & 15, kg = lane >> 4;
-  const int chunks = (p.r >> 2) * p.parts;
-  const uint32_t hrow = (E == 4 ? p.r : 2 * p.r) * E * p.parts, brow = p.r * E;
+  const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = p.r * E;
   const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
   uint64_t left[TM];
-  uint64_t rest = 0;
 #pragma unroll
-  for (int m = 0; m < TM; ++m) {
-    left[m] = __ballot(id[m] >= 0);
-    rest |= left[m];
-#pragma unroll
-    for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  if (!rest) return;
+  for (int m = 0; m < TM; ++m) left[m] = __ballot(id[m] >= 0);
   struct Item {
-    u32x4 bf[TN], hf[TM];
+    u32x4 bf[TN], hf[LDS ? 1 : TM];
     uint32_t rows;  // bit m: rows 16 m have the adapter; 0: no item
+    int g, q;
   };
   int g = -1, q0 = 0, turn = 0;
   uint32_t rows = 0;
   auto next = [&](Item& it) {
     q0 += 4;
-    if (g < 0 || q0 >= chunks) {
-      q0 = 0;
+    if (g < 0 || q0 >= qb) {
+      q0 = qa;
       bool mine = false;
       do {
         g = -1;
@@ -321,19 +315,24 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
       } while (!mine);
     }
     it.rows = rows;
+    it.g = g;
+    it.q = q0;
     if (!rows) return;
     const int q = q0 + kg;
     const __amdgpu_buffer_rsrc_t rb = bytes_rsrc(p.b + (int64_t)g * p.N * p.r, (uint32_t)p.N * brow);
-    const uint32_t bo = q < chunks ? (uint32_t)(c0 + l16) * brow + (uint32_t)b_chunk<ST>(q, p.r) * 16u : kNowhere;
+    const uint32_t bo = q < qb ? (uint32_t)(c0 + l16) * brow + (uint32_t)b_chunk<ST>(q, p.r) * 16u : kNowhere;
 #pragma unroll
     for (int n = 0; n < TN; ++n) it.bf[n] = load16(rb, bo + (uint32_t)(n * 16) * brow);
+    if constexpr (!LDS) {
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
-      it.hf[m] = load16(rh, q < chunks && id[m] == g ? (uint32_t)(pos0 + m * 16 + l16) * hrow + (uint32_t)q * 16u : kNowhere);
+      for (int m = 0; m < TM; ++m)
+        it.hf[m] = load16(rh, q < qb && id[m] == g ? (uint32_t)(pos0 + m * 16 + l16) * hrow + (uint32_t)q * 16u : kNowhere);
+    }
   };
   Item it[DEP];
 #pragma unroll
   for (int d = 0; d < DEP; ++d) next(it[d]);
+  ready();
   for (bool more = true; more;) {
 #pragma unroll
     for (int d = 0; d < DEP; ++d) {
@@ -344,19 +343,18 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
 #pragma unroll
       for (int m = 0; m < TM; ++m) {
         if (!(it[d].rows >> m & 1)) continue;
+        u32x4 hf = {0u, 0u, 0u, 0u};
+        if constexpr (LDS) {
+          const int r = lr0 + m * 16 + l16, ch = it[d].q - qa + kg;
+          if (id[m] == it[d].g && it[d].q + kg < qb) hf = *reinterpret_cast<const u32x4*>(hs + r * kLowRow + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+        } else {
+          hf = it[d].hf[m];
+        }
 #pragma unroll
-        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], it[d].hf[m], acc[m][n]);
+        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], hf, acc[m][n]);
       }
       next(it[d]);
     }
-  }
-  const bool fine = all_finite(acc);
-  if (__ballot(!fine)) {
-#pragma unroll
-    for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    add_low_apart<ST, TM, TN, WK, false>(p, id, pos0, c0, wk, lane, acc);
   }
 }
 
@@ -411,12 +409,10 @@ __device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f
 // The product with W: BM x BN outputs a workgroup, both operands staged in LDS as in
 // lin_tile_kernel, the rows of x and of the output those that the plan's order names.
 //
-// The adapters' part comes first.  Tiles of few rows (BK > 64) take it from memory while
-// the first stages are on their way (add_low).  Larger ones take it as stages before
-// those of W: for each run of rows with one adapter, 64 columns of h (rows of other
-// runs from a row of zeros) and of B_g.  A byte of either is then loaded once a
-// workgroup and in whole lines, not once a wave in halves of lines: 3584 x 1024 -> 4096 of
-// rank 64, 24 adapters, took 84 us from memory (128 x 128 tiles) and 61 so.
+// The adapters' part comes first (add_low), while the first stages are on their way.  Tiles
+// of 64 rows and more (kStaged) have their rows of h in LDS for it, 16 chunks a row in the
+// stage that the main loop fills last: a byte of h is then loaded once a workgroup, B goes
+// from memory to the waves that multiply it.
 template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU>
 __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
@@ -434,13 +430,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   constexpr int kRed = WK > 1 ? (WK - 1) * BM * BN * 4 : 0;
   constexpr int kSmem = S * kStage > kOut + kRed ? S * kStage : kOut + kRed;
   constexpr bool kStaged = CH == 8;
-  constexpr int RW = (BM + 63) / 64;  // 64-row words of a row mask
   // one LDS object: with a second one the compiler keeps them apart and waits for every
   // load to LDS in flight before an operand read
-  __shared__ __align__(16) unsigned char smem[kSmem + BM * 8 + 16];
+  __shared__ __align__(16) unsigned char smem[kSmem + BM * 8];
   int32_t* const ord = reinterpret_cast<int32_t*>(smem + kSmem);
   int32_t* const sid = ord + BM;
-  int32_t* const odd = sid + BM;  // != 0: a sum of the adapters' part is not finite
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, kg = lane >> 4;
@@ -455,7 +449,6 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     const int g = p.ids[min(row0 + i, p.M - 1)];
     sid[i] = row0 + i < p.M && (uint32_t)g < (uint32_t)p.G ? g : -1;
   }
-  if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
   int id[TM];
 #pragma unroll
@@ -478,13 +471,12 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
       load_lds16(base < BM * CH ? rx : rw, smem + st * kStage + base * 16, off[i], k * E);
     }
   };
-  // xs, ws of a stage times each other, for the 16-row products that `rows` names
   f32x4_t acc[TM][TN];
 #pragma unroll
   for (int m = 0; m < TM; ++m)
 #pragma unroll
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int st, uint32_t rows) {
+  auto multiply = [&](int st) {
     const unsigned char* xs = smem + st * kStage;
     const unsigned char* ws = xs + BM * ROW;
 #pragma unroll
@@ -502,11 +494,9 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
         wf[n] = *reinterpret_cast<const u32x4*>(ws + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
       }
 #pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        if (!(rows >> m & 1)) continue;
+      for (int m = 0; m < TM; ++m)
 #pragma unroll
         for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(wf[n], xf[m], acc[m][n]);
-      }
     }
   };
   auto wait = [&](bool last) {
@@ -520,123 +510,50 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   };
 
   const int iters = p.K / BK;
-  int st = 0;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < iters) issue(s, s * BK);
+  const int chunks = (p.r >> 2) * p.parts, pos0 = row0 + wm * TM * 16, c0 = n0 + wn * TN * 16;
   if constexpr (kStaged) {
-    // runs of rows with one adapter: masks of first and last rows, walked twice (the
-    // loads, S - 1 stages ahead, and the products)
-    uint64_t first[RW], last[RW];
-    int runs = 0;
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      const int i = w * 64 + lane;
-      const int g = i < BM ? sid[i] : -1;
-      first[w] = __ballot(g >= 0 && (i == 0 || sid[i - 1] != g));
-      last[w] = __ballot(g >= 0 && (i == BM - 1 || sid[i + 1] != g));
-      runs += __popcll(first[w]);
-    }
-    struct Walk {
-      uint64_t f[RW], l[RW];
-      int s, e, j;  // rows s .. e, stage j of the run
-    };
-    const int chunks = (p.r >> 2) * p.parts, nst = (chunks + 7) >> 3, total = runs * nst + iters;
-    auto step = [&](Walk& v) {
-      if (++v.j < nst) return;
-      v.j = 0;
-      v.s = v.e = BM;
-#pragma unroll
-      for (int w = RW - 1; w >= 0; --w) {
-        if (v.f[w]) v.s = w * 64 + __builtin_ctzll(v.f[w]);
-        if (v.l[w]) v.e = w * 64 + __builtin_ctzll(v.l[w]);
-      }
-#pragma unroll
-      for (int w = RW - 1; w >= 0; --w) {
-        if (v.s >> 6 == w) v.f[w] &= v.f[w] - 1;
-        if (v.e >> 6 == w) v.l[w] &= v.l[w] - 1;
-      }
-    };
-    Walk ld, mu;
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      ld.f[w] = mu.f[w] = first[w];
-      ld.l[w] = mu.l[w] = last[w];
-    }
-    ld.j = mu.j = nst;
-    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = (uint32_t)p.r * E;
+    constexpr int LPH = BM * kLowRow / 1024 / NW;
+    static_assert(BM * kLowRow <= kStage && BM * kLowRow % (1024 * NW) == 0, "h fits a stage");
+    unsigned char* const hs = smem + (S - 1) * kStage;
+    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts;
     const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)(p.M + 1) * hrow);
-    const uint32_t half = E == 4 ? p.r >> 2 : p.r >> 3;  // chunks of a row of B
-    auto issue_low = [&](int slot) {
-      step(ld);
-      const uint32_t b0 = (uint32_t)(ld.j * 8) % half;  // b_chunk of the stage's first chunk
-      const int g = __builtin_amdgcn_readfirstlane(sid[ld.s]);
-      const __amdgpu_buffer_rsrc_t rb = bytes_rsrc(p.b + (int64_t)g * p.N * p.r, (uint32_t)p.N * brow);
-#pragma unroll
-      for (int i = 0; i < LPS; ++i) {
-        const int base = (i * NW + wave) * 64, c = base + lane;
-        const int r = c / CH, q = ld.j * 8 + ((c ^ r) & 7);
-        uint32_t o;
-        if (base < BM * CH)
-          o = r >= ld.s && r <= ld.e && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : (uint32_t)p.M * hrow;
-        else
-          o = (uint32_t)(n0 + r - BM) * brow + (half < 8 ? (uint32_t)b_chunk<ST>(q, p.r) : b0 + ((c ^ r) & 7) - (b0 + ((c ^ r) & 7) >= half ? half : 0u)) * 16u;
-        load_lds16(base < BM * CH ? rh : rb, smem + slot * kStage + base * 16, o, 0);
-      }
-    };
-    const int nlow = runs * nst;
-    auto issue_at = [&](int slot, int it) {
-      if (it < nlow)
-        issue_low(slot);
-      else if (it < total)
-        issue(slot, (it - nlow) * BK);
-    };
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue_at(s, s);
-    for (int it = 0; it < nlow; ++it) {
-      wait(it + S - 2 >= total);
-      issue_at(st == 0 ? S - 1 : st - 1, it + S - 1);
-      step(mu);
-      uint32_t rows = 0;
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const int r = (wm * TM + m) * 16;
-        rows |= r <= mu.e && r + 15 >= mu.s ? 1u << m : 0u;
-      }
-      if (rows) multiply(st, rows);
-      st = st == S - 1 ? 0 : st + 1;
-    }
-    if (nlow) {
-      // a zero row of h times an infinity in another run's B is a NaN: then the part is
-      // made again with the adapters apart
-      const bool fine = all_finite(acc);
-      if (__ballot(!fine)) *odd = 1;
+    auto meet = [&]() {  // every wave's loads to LDS are in, its reads done
+      wait_vm<0>();
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stages stay in flight
+      __builtin_amdgcn_s_waitcnt(0xc07f);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (__builtin_amdgcn_readfirstlane(*(volatile int32_t*)odd)) {
+    };
+    for (int qa = 0; qa < chunks; qa += kLowChunks) {
+      if (qa > 0) meet();  // the chunks before are read
 #pragma unroll
-        for (int m = 0; m < TM; ++m)
-#pragma unroll
-          for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        add_low_apart<ST, TM, TN, WK, true>(p, id, row0 + wm * TM * 16, n0 + wn * TN * 16, wk, lane, acc);
+      for (int i = 0; i < LPH; ++i) {  // rows past the last, and chunks, from the row of zeros
+        const int c = (i * NW + wave) * 64 + lane, r = c / kLowChunks, pos = c % kLowChunks;
+        const int q = qa + ((pos & ~7) | ((pos ^ r) & 7));
+        const uint32_t o = row0 + r < p.M && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : (uint32_t)p.M * hrow;
+        load_lds16(rh, hs + (i * NW + wave) * 1024, o, 0);
       }
-    }
-    for (int it = nlow; it < total; ++it) {
-      wait(it + S - 2 >= total);
-      if (it + S - 1 < total) issue(st == 0 ? S - 1 : st - 1, (it - nlow + S - 1) * BK);
-      multiply(st, ~0u);
-      st = st == S - 1 ? 0 : st + 1;
+      add_low<ST, TM, TN, WK, 4, true>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, qa, min(qa + kLowChunks, chunks), meet, acc);
     }
   } else {
+    add_low<ST, TM, TN, WK, 4, false>(p, id, pos0, c0, wk, lane, nullptr, 0, 0, chunks, []() {}, acc);
+  }
+  if (__ballot(!all_finite(acc))) {
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s)
-      if (s < iters) issue(s, s * BK);
-    add_low<ST, TM, TN, WK, 4>(p, id, row0 + wm * TM * 16, n0 + wn * TN * 16, wk, lane, acc);
-    for (int it = 0; it < iters; ++it) {
-      wait(it + S - 2 >= iters);
-      if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, (it + S - 1) * BK);
-      multiply(st, ~0u);
-      st = st == S - 1 ? 0 : st + 1;
-    }
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    add_low_apart<ST, TM, TN, WK>(p, id, pos0, c0, wk, lane, acc);
+  }
+  int st = 0;
+  for (int it = 0; it < iters; ++it) {
+    wait(it + S - 2 >= iters);
+    if (it + S - 1 < iters) issue(st == 0 ? S - 1 : st - 1, (it + S - 1) * BK);
+    multiply(st);
+    st = st == S - 1 ? 0 : st + 1;
   }
   __syncthreads();
   store_out<ST, BM, BN, WM, WN, WK, TM, TN, SILU>(p, smem, acc, ord, row0, n0, wave, lane);
@@ -874,13 +791,13 @@ struct FormCost {
 };
 constexpr Form kForms[] = {{16, 16, 4, false}, {16, 32, 3, false}, {32, 32, 2, false},  {32, 64, 2, false},
                            {64, 64, 2, true},  {64, 128, 2, true}, {128, 128, 2, true}, {256, 256, 1, true}};
-constexpr FormCost kCost16[] = {{3.51f, 1.92f, 0.17f, 0.04f}, {3.59f, 2.39f, 0.15f, 0.05f}, {4.49f, 2.67f, 0.27f, 0.07f},
-                                {3.16f, 5.20f, 0.21f, 0.14f}, {3.49f, 5.02f, 0.26f, 0.42f}, {3.67f, 6.63f, 0.35f, 0.50f},
-                                {5.43f, 9.87f, 0.f, 1.12f},   {10.24f, 17.88f, 0.f, 2.12f}};
+constexpr FormCost kCost16[] = {{3.45f, 1.96f, 0.22f, 0.02f}, {3.65f, 2.43f, 0.19f, 0.04f},  {3.85f, 2.89f, 0.37f, 0.06f},
+                                {2.82f, 5.78f, 0.15f, 0.16f}, {3.72f, 4.54f, 0.38f, 0.09f},  {2.34f, 12.15f, 0.20f, 0.18f},
+                                {5.40f, 11.21f, 0.17f, 0.24f}, {6.93f, 22.57f, 0.f, 0.39f}};
 // fp32 (256 x 256 outputs of it do not fit LDS)
-constexpr FormCost kCost32[] = {{3.24f, 4.58f, 0.18f, 0.03f},  {3.57f, 5.97f, 0.17f, 0.06f},  {3.68f, 7.82f, 0.25f, 0.10f},
-                                {2.30f, 15.64f, 0.17f, 0.19f}, {4.17f, 18.60f, 0.65f, 0.53f}, {3.89f, 34.59f, 0.63f, 0.59f},
-                                {7.66f, 67.55f, 0.61f, 1.45f}};
+constexpr FormCost kCost32[] = {{3.40f, 4.35f, 0.22f, 0.03f},  {3.51f, 6.03f, 0.20f, 0.05f},  {3.57f, 7.76f, 0.28f, 0.08f},
+                                {2.26f, 15.99f, 0.13f, 0.21f}, {3.70f, 20.08f, 0.50f, 0.13f}, {1.00f, 44.28f, 0.45f, 0.27f},
+                                {5.86f, 66.81f, 0.76f, 0.32f}};
 
 // us of a launch in form f with `adapters` among the rows, or a negative number where it
 // does not fit (a stage of 128 bytes a row, 256 where the adapters are not staged)
@@ -890,7 +807,7 @@ float form_cost(const Form& f, const FormCost& c, int64_t M, int64_t N, int64_t 
   const int64_t per = (tiles + cus - 1) / cus, rounds = (per + f.occ - 1) / f.occ;
   const float k = c.s * (float)K / 1024.f;
   const float runs = fminf(fminf((float)f.bm, (float)M), 1.f + (float)(adapters - 1) * f.bm / M);
-  const int steps = f.staged ? (r * parts + 31) / 32 : (r * parts + 15) / 16;
+  const int steps = (r * parts + 15) / 16;
   return c.a + (float)(rounds - 1) * (c.a - 2.f) + (float)rounds * k + c.m * k * (float)(per - rounds) +
          c.e * runs * (float)steps * (float)per;
 }
