@@ -359,7 +359,7 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
 }
 
 // SiLU with the hardware's reciprocal (1 ulp): a full division is 11 more instructions a
-// value, 4 us of a launch of 3584 x 4096 outputs (57 values a lane-microsecond)
+// value, 4 us of a launch of 3584 x 4096 outputs
 template <int SILU>
 __device__ static inline float ad_act(float v) {
   if constexpr (SILU) return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
@@ -412,7 +412,13 @@ __device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f
 // The adapters' part comes first (add_low), while the first stages are on their way.  Tiles
 // of 64 rows and more (kStaged) have their rows of h in LDS for it, 16 chunks a row in the
 // stage that the main loop fills last: a byte of h is then loaded once a workgroup, B goes
-// from memory to the waves that multiply it.
+// from memory to the waves that multiply it.  Tiles of fewer rows read h as they read B: LDS
+// would save nothing, a wave column or two share it.
+//
+// Bound by the matrix cores and LDS reads for many rows, by the round trips of the K loop
+// for few.  bf16, without SiLU: 3584 rows 1024 -> 4096 in 38.3 us (785 TFLOP/s, without adapters),
+// 840 rows 4096 -> 1024 in 21.2 us with 12 adapters of rank 32, 61 rows with an adapter of
+// rank 16 each in 6.2 us.
 template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU>
 __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
@@ -479,24 +485,37 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   auto multiply = [&](int st) {
     const unsigned char* xs = smem + st * kStage;
     const unsigned char* ws = xs + BM * ROW;
+    u32x4 xf[KS][TM], wf[KS][TN];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int ch = (wk * KS + s) * 4 + kg;
-      u32x4 xf[TM], wf[TN];
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const int r = (wm * TM + m) * 16 + l16;
-        xf[m] = *reinterpret_cast<const u32x4*>(xs + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
-      }
 #pragma unroll
       for (int n = 0; n < TN; ++n) {
         const int r = (wn * TN + n) * 16 + l16;
-        wf[n] = *reinterpret_cast<const u32x4*>(ws + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+        wf[s][n] = *reinterpret_cast<const u32x4*>(ws + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
       }
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const int r = (wm * TM + m) * 16 + l16;
+        xf[s][m] = *reinterpret_cast<const u32x4*>(xs + r * ROW + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int m = 0; m < TM; ++m)
 #pragma unroll
-        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(wf[n], xf[m], acc[m][n]);
+        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(wf[s][n], xf[s][m], acc[m][n]);
+    // One workgroup a CU has no other to fill the matrix cores while it reads LDS: operand
+    // reads one between two matrix instructions (3584 rows 1024 -> 4096: 38.3 us, 42.4 with a
+    // step's reads before its products; 128 x 128 tiles gain nothing, 64 x 64 lose 5%).
+    if constexpr (BM == 256) {
+      __builtin_amdgcn_sched_group_barrier(0x100, TN + 2, 0);
+#pragma unroll
+      for (int i = 0; i < KS * (TM + TN) - TN - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
   };
   auto wait = [&](bool last) {
@@ -777,11 +796,11 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
 // The forms of the product and what a launch of each takes: `a` us and `s` us a 1024
 // columns for a workgroup alone on its CU, `m` of the latter for each further one beside
 // it (`occ` fit), again a - 2 for each further round, and `e` us for a step of the adapters'
-// part: a run of rows with one adapter in a tile, 16 ranks of it (from memory) or 32
-// (staged).  Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks
-// 16 and 64, from one adapter to one for every second row: the cheapest by it is the
-// fastest form or within 10%, on the mean 0.2%.  How many adapters the rows have is not
-// known on the host; the plan's tiles bound it.
+// part: a run of rows with one adapter in a tile, 16 ranks of it.
+// Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks 16
+// and 64, from one adapter to one for every second row: the cheapest by it is the fastest
+// form or within 8%, on the mean 0.1%.  How many adapters the rows have is not known on the
+// host; the plan's tiles bound it.
 struct Form {
   int bm, bn, occ;
   bool staged;
