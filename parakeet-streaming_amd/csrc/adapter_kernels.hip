@@ -5,6 +5,7 @@
 //   adapter_low_kernel   h = scale_g x A_g^T, a tile of rows of one adapter a workgroup
 //   adapter_tile_kernel  the product with W over rows in the plan's order, the
 //                        h B_g^T of the tile's adapters added to its sums
+//   adapter_few_kernel   both in one launch, for few rows with few adapters among them
 //
 // Rows are taken in the order of an adapter plan (equal adapters side by side), so 16
 // rows of a matrix instruction have few adapters: with streams of 2 frames in their
@@ -64,7 +65,7 @@ struct AdK {
   const int32_t* order;  // [M] plan: row at a position
   const int32_t* ids;    // [M] adapter at a position, -1: none
   const int4* tiles;     // {adapter, first position, rows, 0}
-  ST* h;                 // [M + 1][parts][2 r] (fp32: [M + 1][parts][r]) by position, row M zeros
+  ST* h;                 // [M][parts][2 r] (fp32: [M][parts][r]) by position
   ST* out;               // [M][N], stride out_s
   int64_t out_s;
   int32_t M, N, K, r, G;
@@ -122,12 +123,6 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
   constexpr int kRed = kLowWaves * RT * 2 * 64 * 16;
   __shared__ __align__(16) unsigned char smem[S * kStage > kRed ? S * kStage : kRed];
   static_assert(2 * RT <= kLowWaves, "a wave finishes at most one sum");
-  if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {  // the row of zeros behind the last row
-    const int n = p.r * p.parts * 4 / 16;
-    const u32x4 zero = {0u, 0u, 0u, 0u};
-    for (int i = threadIdx.x; i < n; i += 64 * kLowWaves)
-      st16(reinterpret_cast<unsigned char*>(p.h) + (int64_t)p.M * n * 16 + i * 16, zero);
-  }
   const int4 tile = p.tiles[blockIdx.x];
   if ((uint32_t)tile.x >= (uint32_t)p.G) return;  // past the last tile
   if (tile.y < 0 || tile.z <= 0 || tile.z > kLowRows || tile.y > p.M - tile.z) return;  // not a plan's
@@ -538,7 +533,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     static_assert(BM * kLowRow <= kStage && BM * kLowRow % (1024 * NW) == 0, "h fits a stage");
     unsigned char* const hs = smem + (S - 1) * kStage;
     const uint32_t hrow = (uint32_t)p.r * 4u * p.parts;
-    const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)(p.M + 1) * hrow);
+    const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
     auto meet = [&]() {  // every wave's loads to LDS are in, its reads done
       wait_vm<0>();
       asm volatile("" ::: "memory");
@@ -549,10 +544,10 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     for (int qa = 0; qa < chunks; qa += kLowChunks) {
       if (qa > 0) meet();  // the chunks before are read
 #pragma unroll
-      for (int i = 0; i < LPH; ++i) {  // rows past the last, and chunks, from the row of zeros
+      for (int i = 0; i < LPH; ++i) {
         const int c = (i * NW + wave) * 64 + lane, r = c / kLowChunks, pos = c % kLowChunks;
         const int q = qa + ((pos & ~7) | ((pos ^ r) & 7));
-        const uint32_t o = row0 + r < p.M && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : (uint32_t)p.M * hrow;
+        const uint32_t o = row0 + r < p.M && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : kNowhere;
         load_lds16(rh, hs + (i * NW + wave) * 1024, o, 0);
       }
       add_low<ST, TM, TN, WK, 4, true>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, qa, min(qa + kLowChunks, chunks), meet, acc);
@@ -799,7 +794,7 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
 // part: a run of rows with one adapter in a tile, 16 ranks of it.
 // Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks 16
 // and 64, from one adapter to one for every second row: the cheapest by it is the fastest
-// form or within 8%, on the mean 0.1%.  How many adapters the rows have is not known on the
+// form or within 12%, on the mean 0.1%.  How many adapters the rows have is not known on the
 // host; the plan's tiles bound it.
 struct Form {
   int bm, bn, occ;
@@ -810,9 +805,9 @@ struct FormCost {
 };
 constexpr Form kForms[] = {{16, 16, 4, false}, {16, 32, 3, false}, {32, 32, 2, false},  {32, 64, 2, false},
                            {64, 64, 2, true},  {64, 128, 2, true}, {128, 128, 2, true}, {256, 256, 1, true}};
-constexpr FormCost kCost16[] = {{3.45f, 1.96f, 0.22f, 0.02f}, {3.65f, 2.43f, 0.19f, 0.04f},  {3.85f, 2.89f, 0.37f, 0.06f},
-                                {2.82f, 5.78f, 0.15f, 0.16f}, {3.72f, 4.54f, 0.38f, 0.09f},  {2.34f, 12.15f, 0.20f, 0.18f},
-                                {5.40f, 11.21f, 0.17f, 0.24f}, {6.93f, 22.57f, 0.f, 0.39f}};
+constexpr FormCost kCost16[] = {{3.55f, 1.93f, 0.21f, 0.02f},  {3.65f, 2.35f, 0.19f, 0.04f},  {3.88f, 3.20f, 0.29f, 0.06f},
+                                {3.07f, 5.32f, 0.16f, 0.13f},  {3.93f, 4.65f, 0.36f, 0.09f},  {2.19f, 11.97f, 0.21f, 0.18f},
+                                {5.65f, 10.75f, 0.24f, 0.24f}, {6.91f, 13.87f, 0.f, 0.41f}};
 // fp32 (256 x 256 outputs of it do not fit LDS)
 constexpr FormCost kCost32[] = {{3.40f, 4.35f, 0.22f, 0.03f},  {3.51f, 6.03f, 0.20f, 0.05f},  {3.57f, 7.76f, 0.28f, 0.08f},
                                 {2.26f, 15.99f, 0.13f, 0.21f}, {3.70f, 20.08f, 0.50f, 0.13f}, {1.00f, 44.28f, 0.45f, 0.27f},
@@ -932,7 +927,7 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   constexpr int E = sizeof(ST);
   const int parts = k_parts(a->max_tiles, a->rank, a->k);
   if (!rows_ok(a->rows, a->x_stride, a->k, E) || !rows_ok(a->n, a->weight_stride, a->k, E) ||
-      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok((int64_t)a->rows + 1, (int64_t)a->rank * parts, (int64_t)a->rank * parts, 4) || !rows_ok(a->rank, a->k, a->k, E) ||
+      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok(a->rows, (int64_t)a->rank * parts, (int64_t)a->rank * parts, 4) || !rows_ok(a->rank, a->k, a->k, E) ||
       !rows_ok(a->n, a->rank, a->rank, E))
     return fail(PK_ERR_INVALID, "%s: row strides must be multiples of 16 bytes, at least the row, and a tensor below 2^31 bytes", what);
   AdK<ST> k{};
@@ -976,7 +971,7 @@ extern "C" int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32
   if (rows <= 0 || n <= 0 || rank <= 0 || k <= 0 || max_tiles < 0) return 0;
   const int64_t row = (int64_t)k * (dtype == PK_DTYPE_F32 ? 4 : 2);
   if (pk::few_form(rows, n, row, rank, pk::most_adapters(rows, max_tiles), pk::cu_count())) return 0;
-  return ((int64_t)rows + 1) * rank * 4 * pk::k_parts(max_tiles, rank, k);
+  return (int64_t)rows * rank * 4 * pk::k_parts(max_tiles, rank, k);
 }
 
 extern "C" int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream) {
