@@ -780,7 +780,7 @@ int pk_pool_free_list(const pk_pool* pool, int32_t* out, int32_t capacity);
  *            (pk_pool_reset_slot in turn); lengths, rows and slot_map are not read.
  * workspace: pk_page_step_workspace_bytes(batch), 16-byte aligned (NULL where that is 0).
  * Calls on one pool are ordered by the caller (one stream, or events).
- * num_pages * page_size < 2^31; num_slots <= PK_PAGE_STEP_MAX_SLOTS.
+ * num_pages * page_size < 2^31; num_slots and batch <= PK_PAGE_STEP_MAX_SLOTS.
  */
 #define PK_PAGE_STEP_MAX_SLOTS 131072
 typedef struct pk_page_step_args {
@@ -847,7 +847,7 @@ int pk_kv_append_slots(const pk_kv_append_slots_args* args, void* stream);
  *              rows of one adapter, by adapter; {-1, 0, 0, 0} past the last one.
  *              max_tiles >= pk_adapter_plan_tiles(...).
  * workspace  : pk_adapter_plan_workspace_bytes(...), 16-byte aligned (NULL where that is 0)
- * num_adapters <= PK_ADAPTER_MAX.
+ * num_adapters <= PK_ADAPTER_MAX; batch * frames and max_tiles < 2^24.
  */
 #define PK_ADAPTER_MAX 512
 #define PK_ADAPTER_MAX_RANK 128

@@ -898,7 +898,8 @@ int few_form(int64_t M, int64_t N, int64_t row_bytes, int r, int64_t adapters, i
 
 // below 2^31 bytes: 32-bit offsets, and kNowhere past them
 bool rows_ok(int64_t rows, int64_t stride, int64_t width, int bytes) {
-  return stride >= 0 && stride * bytes % 16 == 0 && (rows <= 1 || stride >= width) &&
+  if (rows > 1 && (stride < width || stride >= (int64_t{1} << 31))) return false;
+  return stride >= 0 && stride % (16 / bytes) == 0 &&
          ((rows - 1) * stride + width) * bytes < (int64_t{1} << 31);
 }
 

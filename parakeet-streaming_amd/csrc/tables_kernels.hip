@@ -120,11 +120,15 @@ __device__ static inline const uint32_t* mark_slots(const PageK& p, uint32_t* ld
   return dup;
 }
 
-// the first of equal slots has the step (rare)
+// the first of equal slots has the step (rare: a search of the streams before, 8 at a time)
 __device__ static inline bool named_before(const PageK& p, int b, int32_t slot, const uint32_t* dup) {
-  if ((uint32_t)slot < (uint32_t)p.S && (dup[slot >> 5] >> (slot & 31) & 1))
-    for (int j = 0; j < b; ++j)
-      if (p.slots[j] == slot) return true;
+  if ((uint32_t)slot >= (uint32_t)p.S || !(dup[slot >> 5] >> (slot & 31) & 1)) return false;
+  for (int j = 0; j < b; j += 8) {
+    bool hit = false;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) hit |= p.slots[min(j + u, b - 1)] == slot;
+    if (hit) return true;
+  }
   return false;
 }
 
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const PlanK 
 // Many rows: theirs and the tiles in a second launch, by all CUs (57344 rows in 512 buckets:
 // one workgroup stores 0.5 MB in 50 us).
 __global__ void __launch_bounds__(256) adapter_rows_kernel(const PlanK p) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
+  const int i = blockIdx.x * 256 + threadIdx.x;  // B T and max_tiles: below 2^24
   if (i < p.B * p.T) {
     const int s = i / p.T;
     const int2 v = p.by[s];
@@ -493,6 +497,8 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
     return fail(PK_ERR_INVALID, "%s: %d pages of %d frames are past a slot map's 2^31 frames", what, a->num_pages, a->page_size);
   if (a->num_slots > PK_PAGE_STEP_MAX_SLOTS)
     return fail(PK_ERR_UNSUPPORTED, "%s: %d slots (built: up to %d)", what, a->num_slots, PK_PAGE_STEP_MAX_SLOTS);
+  if (a->batch > PK_PAGE_STEP_MAX_SLOTS)
+    return fail(PK_ERR_UNSUPPORTED, "%s: %d streams (built: up to %d)", what, a->batch, PK_PAGE_STEP_MAX_SLOTS);
   if (a->batch == 0) return PK_OK;
   if (!a->queue || !a->head || !a->appended || !a->ring || !a->slots)
     return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
@@ -550,13 +556,15 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
 
 int adapter_plan(const pk_adapter_plan_args* a, hipStream_t s) {
   const char* what = "pk_adapter_plan";
-  if (a->batch < 0 || a->frames <= 0 || a->num_adapters <= 0 || (int64_t)a->batch * a->frames >= (int64_t{1} << 31))
-    return fail(PK_ERR_INVALID, "%s: need batch >= 0, frames and num_adapters > 0, and fewer than 2^31 rows (got %d, %d, %d)", what,
+  // a projection's rows are at least 128 bytes and its tensors below 2^31
+  if (a->batch < 0 || a->frames <= 0 || a->num_adapters <= 0 || (int64_t)a->batch * a->frames >= (int64_t{1} << 24))
+    return fail(PK_ERR_INVALID, "%s: need batch >= 0, frames and num_adapters > 0, and fewer than 2^24 rows (got %d, %d, %d)", what,
                 a->batch, a->frames, a->num_adapters);
   if (a->num_adapters > PK_ADAPTER_MAX)
     return fail(PK_ERR_UNSUPPORTED, "%s: %d adapters (built: up to %d)", what, a->num_adapters, PK_ADAPTER_MAX);
   const int64_t need = pk_adapter_plan_tiles(a->batch, a->frames, a->num_adapters);
-  if (a->max_tiles < need) return fail(PK_ERR_INVALID, "%s: %d tiles, needs %d", what, a->max_tiles, (int)need);
+  if (a->max_tiles < need || a->max_tiles >= (1 << 24))
+    return fail(PK_ERR_INVALID, "%s: %d tiles, needs %d and takes fewer than 2^24", what, a->max_tiles, (int)need);
   if (a->batch == 0) return PK_OK;
   if (!a->ids || !a->order || !a->sorted_ids || !a->tiles) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
   if (!aligned16(a->tiles)) return fail(PK_ERR_INVALID, "%s: tiles must be 16-byte aligned", what);

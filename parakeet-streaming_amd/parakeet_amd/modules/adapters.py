@@ -47,6 +47,7 @@ class EncoderAdapters:
         if not 0 < G <= _lib.ADAPTER_MAX or r % 8 or not 0 < r <= _lib.ADAPTER_MAX_RANK:
             raise ValueError(f"need 0 < num_adapters <= {_lib.ADAPTER_MAX} and a rank that is a multiple of 8, at most "
                              f"{_lib.ADAPTER_MAX_RANK}; got {num_adapters}, {rank}")
+        targets = tuple(targets)
         unknown = [t for t in targets if t not in TARGETS]
         if unknown:
             raise ValueError(f"no such projections: {unknown} (of {TARGETS})")

@@ -463,8 +463,10 @@ class EncoderStepGraph:
             raise ValueError(f"length must be a [{B}] tensor")
         if (adapters is None) != (adapter_ids is None):
             raise ValueError("adapters and adapter_ids go together")
-        if adapter_ids is not None and (tuple(adapter_ids.shape) != (B,) or adapter_ids.dtype != torch.int32 or adapter_ids.device != dev):
-            raise ValueError(f"adapter_ids must be int32 [{B}] on {dev}")
+        if adapter_ids is not None and (
+            tuple(adapter_ids.shape) != (B,) or adapter_ids.dtype != torch.int32 or adapter_ids.device != dev or not adapter_ids.is_contiguous()
+        ):
+            raise ValueError(f"adapter_ids must be contiguous int32 [{B}] on {dev}")
         self.adapters, self.adapter_ids = adapters, adapter_ids
         self.encoder = encoder
         self.state = state

@@ -1259,8 +1259,8 @@ def adapter_plan(ids: torch.Tensor, frames: int = 1, *, num_adapters: int) -> Ad
     B, T, G = ids.shape[0], int(frames), int(num_adapters)
     at, M = _i32(ids, "ids", (B,)), B * T
     dev = _require_device(ids)
-    if T <= 0 or G <= 0 or M >= 1 << 31:
-        raise ValueError(f"need frames and num_adapters > 0 and fewer than 2^31 rows, got {B} x {T}, {G}")
+    if T <= 0 or G <= 0 or M >= 1 << 24:
+        raise ValueError(f"need frames and num_adapters > 0 and fewer than 2^24 rows, got {B} x {T}, {G}")
     n = M // 32 + min(G, B)
     a = AdapterPlanArgs()
     a.device, a.batch, a.frames, a.num_adapters, a.max_tiles = _index(dev), B, T, G, n

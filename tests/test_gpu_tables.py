@@ -123,6 +123,25 @@ def test_every_slot_the_same(cuda):
     assert dev.slot_info(1)[0] == 2 and dev.free_pages() == dev.num_pages - 1
 
 
+@pytest.mark.parametrize("n", [5, 17, 63, 64, 66, 1001, 3500, 4100])
+def test_every_slot_named_twice(cuda, n):
+    """n streams, the second half naming the slots of the first in another order: the
+    second half is absent, wherever in the batch its first mention is."""
+    slots, left, chunk, P = n, 20, 7, 8
+    dev = DevicePagePool(slots, P, left, chunk, cuda)
+    model = RaggedPool(slots, P, left, chunk, np.arange(dev.num_pages))
+    rng = np.random.default_rng(n)
+    for _ in range(5):
+        once = rng.permutation(slots)[: (n + 1) // 2]
+        batch = np.concatenate([once, rng.permutation(once)])[:n].astype(np.int32)
+        lengths = rng.integers(0, chunk + 1, n)
+        rows, place = dev.advance(_up(batch, cuda), _up(lengths, cuda))
+        want_rows, want_place = model.advance(batch.tolist(), lengths.tolist())
+        np.testing.assert_array_equal(rows.cpu().numpy(), want_rows)
+        np.testing.assert_array_equal(place.cpu().numpy(), want_place)
+    _same_pool(dev, model)
+
+
 def test_positions_past_2_30(cuda):
     dev = DevicePagePool(2, 16, 70, 2, cuda)
     dev.state.appended.fill_(2**31 - 20)

@@ -9,6 +9,7 @@ import torch
 
 from oracle import paging
 from parakeet_amd import _lib, ops
+from parakeet_amd.modules import EncoderAdapters
 from parakeet_amd.pool import DevicePagePool, PagePool
 from tests._tables_model import RaggedPool, plan_model
 from tests.test_abi import _struct_fields
@@ -92,6 +93,9 @@ def test_page_step_refuses_too_many_slots_and_short_rows():
     a.num_slots, a.num_pages = _lib.PAGE_STEP_MAX_SLOTS + 1, 6 * (_lib.PAGE_STEP_MAX_SLOTS + 1)
     assert L.pk_page_step(ctypes.byref(a), None) == _lib.PK_ERR_UNSUPPORTED
     a = _page_args()
+    a.batch = _lib.PAGE_STEP_MAX_SLOTS + 1
+    assert L.pk_page_step(ctypes.byref(a), None) == _lib.PK_ERR_UNSUPPORTED and "streams" in _lib.last_error()
+    a = _page_args()
     buf = ctypes.create_string_buffer(64)  # never read: the calls are refused
     at = ctypes.addressof(buf)
     a.queue = a.head = a.appended = a.ring = a.slots = a.rows = a.slot_map = at
@@ -129,7 +133,7 @@ def test_plan_refusals():
     a.device, a.batch, a.frames, a.num_adapters, a.max_tiles = -1, 5, 2, 3, 3
     assert L.pk_adapter_plan(ctypes.byref(a), None) == _lib.PK_ERR_INVALID and "NULL" in _lib.last_error()
     for field, value, code in (("max_tiles", 2, _lib.PK_ERR_INVALID), ("frames", 0, _lib.PK_ERR_INVALID), ("num_adapters", 0, _lib.PK_ERR_INVALID),
-                               ("batch", -1, _lib.PK_ERR_INVALID), ("batch", 1 << 30, _lib.PK_ERR_INVALID),
+                               ("batch", -1, _lib.PK_ERR_INVALID), ("batch", 1 << 30, _lib.PK_ERR_INVALID), ("batch", 1 << 23, _lib.PK_ERR_INVALID), ("max_tiles", 1 << 24, _lib.PK_ERR_INVALID),
                                ("num_adapters", _lib.ADAPTER_MAX + 1, _lib.PK_ERR_UNSUPPORTED)):
         keep = getattr(a, field)
         setattr(a, field, value)
@@ -152,7 +156,7 @@ def test_adapter_linear_refusals():
     for field, value, code in (("n", 100, unsupported), ("k", 96, unsupported), ("rank", 12, unsupported), ("rank", 136, unsupported), ("rank", 0, unsupported),
                                ("num_adapters", 0, unsupported), ("num_adapters", 513, unsupported), ("activation", 2, bad), ("rows", -1, bad),
                                ("max_tiles", -1, bad), ("x", at + 8, bad), ("order", None, bad), ("x_stride", 132, bad), ("weight_stride", 64, bad),
-                               ("out_stride", 120, bad), ("out_stride", 1 << 30, bad), ("dtype", 5, bad), ("weight", None, bad)):
+                               ("out_stride", 120, bad), ("out_stride", 1 << 30, bad), ("x_stride", 1 << 62, bad), ("dtype", 5, bad), ("weight", None, bad)):
         keep = getattr(a, field)
         setattr(a, field, value)
         assert L.pk_adapter_linear(ctypes.byref(a), None) == code, (field, value)
@@ -212,3 +216,25 @@ def test_device_pool_arguments():
         with pytest.raises(ValueError, match="distinct"):
             p.advance(slots)
     assert p.free_pages() == 12 and p.free_list().tolist() == list(range(12)) and p.slot_info(1)[0] == 0
+
+
+def test_targets_may_be_an_iterator():
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.self_attn = torch.nn.Module()
+            self.self_attn.qkv = torch.nn.Linear(64, 192)
+
+    encoder = torch.nn.Module()
+    encoder.layers = torch.nn.ModuleList([Layer(), Layer()])
+    bank = EncoderAdapters(encoder, num_adapters=3, rank=8, targets=iter(["self_attn.qkv"]))
+    a, b = torch.randn(4, 64), torch.randn(192, 4)
+    bank.load(2, {"layers.1.self_attn.qkv": (a, b)}, scale=0.5)
+    kept = bank.banks[1]["self_attn.qkv"]
+    assert torch.equal(kept.a[2, :4], a) and torch.equal(kept.b[2, :, :4], b) and not kept.a[2, 4:].any() and kept.scale.tolist() == [0, 0, 0.5]
+    assert not bank.banks[0]["self_attn.qkv"].a.any()
+    for i, weights, err in ((3, {}, IndexError), (0, {"layers.2.self_attn.qkv": (a, b)}, KeyError), (0, {"layers.0.self_attn.qkv": (b, a)}, ValueError)):
+        with pytest.raises(err):
+            bank.load(i, weights)
+    bank.clear(2)
+    assert not kept.a.any() and not kept.b.any() and not kept.scale.any()
