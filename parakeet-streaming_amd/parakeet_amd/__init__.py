@@ -5,9 +5,10 @@ Drop-in host modules mirror the reference package layout:
 * ``parakeet_amd.modules.cache``      -- ``ModelCache``, ``StreamingState`` (paged)
 * ``parakeet_amd.modules.attention``  -- ``PositionalEncoding``, ``ConformerAttention``
 * ``parakeet_amd.modules.encoder``    -- ``ConformerEncoder`` (streaming state, masks, layer loop)
+* ``parakeet_amd.modules.adapters``   -- ``EncoderAdapters`` (low-rank adapters of each stream)
 * ``parakeet_amd.engine.scheduler``   -- ``Scheduler`` (slot pool + paged batches)
 
-``parakeet_amd.ops`` exposes the kernels; ``parakeet_amd.pool`` the host page pool.
+``parakeet_amd.ops`` exposes the kernels; ``parakeet_amd.pool`` the host and device page pools.
 """
 
 from . import ops, pool
