@@ -353,11 +353,13 @@ __global__ void __launch_bounds__(kPartThreads) page_back_kernel(const PageK p) 
 // counts a run of the streams (LDS), the counts are summed over waves and adapters,
 // and each wave places its run in order, 64 streams at a time, a stream's rank among
 // the equal ones of its 64 found with one ballot a bit of the number.  Streams
-// without an adapter are bucket G.
+// without an adapter are bucket G.  Bound by its chain of LDS passes and, for thousands
+// of streams, by one CU's instructions: in a graph 128 streams of 2 frames take 5.4 us, 4096 in
+// 512 buckets 9.1 (with 14 frames, two launches, 12.6), 16384 22.8.
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanTile = 32;    // rows of a tile
-constexpr int kPlanOne = 4096;   // rows of a plan in one launch
+constexpr int kPlanOne = 4096;   // rows of a plan in one launch, streams sorted in LDS
 
 struct PlanK {
   const int32_t* ids;
@@ -392,26 +394,39 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const PlanK 
   uint32_t* const hist = lds;                       // [waves][G + 1]
   uint32_t* const start = hist + kPlanWaves * G1;   // [G + 2] first stream of a bucket
   uint32_t* const tile0 = start + G1 + 1;           // [G + 1] first tile of an adapter
+  // up to kPlanOne streams: adapter + 1 and stream by position, [B], so that memory gets
+  // whole lines
+  uint32_t* const placed = tile0 + G1;
   for (int i = tid; i < kPlanWaves * G1; i += kPlanThreads) hist[i] = 0;
+  constexpr int U = 4;  // numbers a lane loads at once: 64 U streams a wave and round trip
+  auto load_ids = [&](int32_t (&id)[U], int b) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = p.ids[min(b + 64 * u, p.B - 1)];
+  };
   const int run = ((p.B + kPlanWaves - 1) / kPlanWaves + 63) & ~63;
   const int b0 = min(wave * run, p.B), b1 = min(b0 + run, p.B);
   __syncthreads();
-  for (int b = b0 + lane; b < b1; b += 64) {
-    const int32_t id = p.ids[b];
-    atomicAdd(&hist[wave * G1 + ((uint32_t)id < (uint32_t)p.G ? id : p.G)], 1u);
+  for (int b = b0 + lane; b < b1; b += 64 * U) {
+    int32_t id[U];
+    load_ids(id, b);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (b + 64 * u < b1) atomicAdd(&hist[wave * G1 + ((uint32_t)id[u] < (uint32_t)p.G ? id[u] : p.G)], 1u);
   }
   __syncthreads();
   // bucket g's streams before each wave's, and before bucket g
   uint32_t carry = 0, tcarry = 0;
   for (int g0 = 0; g0 < G1; g0 += kPlanThreads) {
     const int g = g0 + tid;
-    uint32_t c = 0;
-    if (g < G1)
-      for (int w = 0; w < kPlanWaves; ++w) {
-        const uint32_t h = hist[w * G1 + g];
-        hist[w * G1 + g] = c;
-        c += h;
-      }
+    uint32_t h[kPlanWaves], c = 0;  // every wave's at once: one LDS round trip, not 16
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) h[w] = g < G1 ? hist[w * G1 + g] : 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const uint32_t n = h[w];
+      h[w] = c;
+      c += n;
+    }
     const uint32_t tiles = g < p.G ? (c * p.T + kPlanTile - 1) / kPlanTile : 0;
     uint32_t all, tall;
     const uint32_t s = block_scan<kPlanWaves>(c, sums, all) + carry;
@@ -419,44 +434,60 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const PlanK 
     if (g < G1) {
       start[g] = s;
       tile0[g] = t;
-      for (int w = 0; w < kPlanWaves; ++w) hist[w * G1 + g] += s;
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) hist[w * G1 + g] = h[w] + s;
     }
     carry += all;
     tcarry += tall;
   }
   __syncthreads();
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int b = b0; b < b1; b += 64) {
-    const bool in = b + lane < b1;
-    const int32_t id = in ? p.ids[b + lane] : -1;
-    const bool has = (uint32_t)id < (uint32_t)p.G;
-    const int g = has ? id : p.G;
-    uint64_t same = __ballot(in);
-    for (int i = 0; i < p.bits; ++i) {
-      const uint64_t m = __ballot((g >> i) & 1);
-      same &= (g >> i) & 1 ? m : ~m;
-    }
-    uint32_t* const h = &hist[wave * G1 + g];
-    uint32_t base = 0;
-    if (in) base = *h;
-    wave_lds_sync();
-    if (in && (same >> lane) == 1) *h = base + __popcll(same);  // the last of the equal ones
-    wave_lds_sync();
-    if (in) {
-      const int32_t at = (int32_t)(base + __popcll(same & below));
-      if (p.by) {
-        p.by[at] = int2{b + lane, has ? id : -1};
-      } else {
-        for (int t = 0; t < p.T; ++t) {
-          p.order[at * p.T + t] = (b + lane) * p.T + t;
-          p.sorted[at * p.T + t] = has ? id : -1;
-        }
+  for (int b4 = b0; b4 < b1; b4 += 64 * U) {
+    int32_t ids[U];
+    load_ids(ids, b4 + lane);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = b4 + 64 * u;
+      if (b >= b1) break;
+      const bool in = b + lane < b1;
+      const int32_t id = in ? ids[u] : -1;
+      const bool has = (uint32_t)id < (uint32_t)p.G;
+      const int g = has ? id : p.G;
+      const uint64_t all = __ballot(in);
+      uint32_t lo = (uint32_t)all, up = (uint32_t)(all >> 32);
+      for (int i = p.bits; i > 0; --i) {
+        const int32_t bit = (int32_t)((uint32_t)g << (32 - i)) >> 31;  // -1 or 0
+        const uint64_t m = __ballot(bit);
+        lo &= ~((uint32_t)m ^ (uint32_t)bit);
+        up &= ~((uint32_t)(m >> 32) ^ (uint32_t)bit);
+      }
+      const uint64_t same = (uint64_t)up << 32 | lo;
+      uint32_t* const h = &hist[wave * G1 + g];
+      uint32_t base = 0;
+      if (in) base = *h;
+      wave_lds_sync();
+      if (in && (same >> lane) == 1) *h = base + __popcll(same);  // the last of the equal ones
+      wave_lds_sync();
+      if (in) {
+        const int32_t at = (int32_t)(base + __popcll(same & below));
+        if (p.B <= kPlanOne)
+          placed[at] = (uint32_t)(has ? id + 1 : 0) << 16 | (uint32_t)(b + lane);
+        else
+          p.by[at] = int2{b + lane, has ? id : -1};
       }
     }
   }
+  __syncthreads();
   if (p.by) {
+    if (p.B <= kPlanOne)
+      for (int i = tid; i < p.B; i += kPlanThreads) p.by[i] = int2{(int)(placed[i] & 0xffff), (int)(placed[i] >> 16) - 1};
     for (int i = tid; i < 2 * G1; i += kPlanThreads) p.tab[i] = i < G1 ? start[i] : tile0[i - G1];
     return;
+  }
+  for (int i = tid; i < p.B * p.T; i += kPlanThreads) {
+    const int s = i / p.T;
+    p.order[i] = (int)(placed[s] & 0xffff) * p.T + (i - s * p.T);
+    p.sorted[i] = (int)(placed[s] >> 16) - 1;
   }
   for (int t = tid; t < p.max_tiles; t += kPlanThreads) p.tiles[t] = plan_tile(p, start, tile0, t);
 }
@@ -586,7 +617,7 @@ int adapter_plan(const pk_adapter_plan_args* a, hipStream_t s) {
   }
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
-  const size_t lds = sizeof(uint32_t) * ((size_t)kPlanWaves * (k.G + 1) + 2 * (k.G + 2));
+  const size_t lds = sizeof(uint32_t) * ((size_t)kPlanWaves * (k.G + 1) + 2 * (k.G + 2) + (k.B <= kPlanOne ? k.B : 0));  // below 64 KB
   hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanThreads), lds, s, k);
   int rc = check_launch(what);
   if (rc != PK_OK || !k.by) return rc;
