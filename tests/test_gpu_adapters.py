@@ -87,6 +87,23 @@ def test_many_rows(cuda, dtype, B, T, K, N, r):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,K,N,r,G", [(256, 14, 512, 2048, 96, 24), (256, 14, 512, 1024, 128, 100), (120, 7, 2048, 512, 40, 9), (500, 1, 1024, 2048, 72, 60)])
+def test_wide_ranks_in_large_tiles(cuda, dtype, B, T, K, N, r, G):
+    """Ranks whose h takes more than one turn through LDS, or ends inside one; and with an
+    infinity in one adapter, which makes such tiles sum again, the other rows' bits."""
+    x, w, bias, ad, ids = _make(cuda, B, T, K, N, r, G, dtype, seed=r)
+    got = _run(x, w, bias, ad, ids)
+    _check(got, *_reference(x, w, bias, ad, ids, False))
+    g = int(ids[0])  # an adapter that the batch has
+    ad.b[g, N // 2, r - 1] = float("inf")
+    again, own = _run(x, w, bias, ad, ids), ids == g
+    assert not torch.isfinite(again[own][..., N // 2]).any()
+    assert torch.equal(again[~own], got[~own])
+    again[own, :, N // 2] = got[own, :, N // 2]
+    assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("how", ["none", "one", "blocks", "bad"])
 def test_mixtures(cuda, dtype, how):
     B, T, K, N, r, G = 70, 2, 128, 192, 16, 5
