@@ -47,9 +47,28 @@ struct MmaA<float> {
 // q mod r/8 of a row of B.  For ranks up to 16 both parts are one matrix instruction.
 // fp32: one part, r / 4 chunks.  Where K is split over workgroups (parts > 1) a row of h
 // is the parts' rows one after another: their sum is taken by the product with B.
+constexpr int kLowChunks = 16, kLowRow = kLowChunks * 16;  // chunks and bytes of a row of h in LDS
+
 template <typename ST>
 __device__ static inline int b_chunk(int q, int r) {
   return (int)((uint32_t)q % (uint32_t)(sizeof(ST) == 4 ? r >> 2 : r >> 3));
+}
+
+// How the product takes a row of h: `copies` of `width` chunks each multiplied with the same
+// chunks of B, `block` chunks of every copy a turn, 4 of them a step.  Staged rows (LDS)
+// read B once for the high and low parts of h and of each part of K (256 adapters of rank
+// 64: 3584 rows 1024 -> 4096 81 us so and 94 with a read each, 840 rows 60 and 78), except
+// ranks below 32, where a step of 4 chunks would be half empty; rows from memory take
+// one chunk after another.
+struct LowOrder {
+  int copies, width, block;
+  int shift;  // of a block, staged: a power of two
+};
+template <typename ST, bool LDS>
+__device__ static inline LowOrder low_order(int r, int parts) {
+  const int copies = !LDS ? 1 : sizeof(ST) == 4 ? parts : r >= 32 ? 2 * parts : 1;
+  const int width = (r >> 2) * parts / copies;
+  return LowOrder{copies, width, LDS ? kLowChunks / copies : width, 4 - (copies >> 1)};
 }
 
 template <typename ST>
@@ -213,12 +232,13 @@ __device__ static inline bool all_finite(const f32x4_t (&acc)[TM][TN]) {
 // an adapter its product is taken for all of them and kept for those, so that what a row
 // gets depends on its own adapter alone, and in the same order of sums, so that the rows
 // without them keep their bits.
-template <typename ST, int TM, int TN, int WK>
+template <typename ST, int TM, int TN, int WK, bool LDS>
 __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
                                       f32x4_t (&acc)[TM][TN]) {
   constexpr int V = Tr<ST>::VEC;
   const int l16 = lane & 15, kg = lane >> 4;
-  const int chunks = (p.r >> 2) * p.parts, hs = (sizeof(ST) == 4 ? p.r : 2 * p.r) * p.parts;
+  const int hs = (sizeof(ST) == 4 ? p.r : 2 * p.r) * p.parts;
+  const LowOrder o = low_order<ST, LDS>(p.r, p.parts);
   const u32x4 zero = {0u, 0u, 0u, 0u};
   const ST* hp[TM];
   uint64_t left[TM];
@@ -241,17 +261,21 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
     }
     if (WK > 1 && turn != wk) continue;
     const ST* const bp = p.b + ((int64_t)g * p.N + c0 + l16) * p.r;
-    auto b_of = [&](int n, int q) { return q < chunks ? ld16(bp + (int64_t)n * 16 * p.r + b_chunk<ST>(q, p.r) * V) : zero; };
+    auto b_of = [&](int n, int q, int end) { return q < end ? ld16(bp + (int64_t)n * 16 * p.r + b_chunk<ST>(q, p.r) * V) : zero; };
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       if (has[m] == 0) continue;
       f32x4_t d[TN];
 #pragma unroll
       for (int n = 0; n < TN; ++n) d[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int q = kg; q - kg < chunks; q += 4) {
-        const u32x4 hf = q < chunks ? ld16(hp[m] + q * V) : zero;
+      for (int q0 = 0; q0 < o.width; q0 += o.block) {
+        const int end = min(q0 + o.block, o.width);
+        for (int q = q0 + kg; q - kg < end; q += 4)
+          for (int c = 0; c < o.copies; ++c) {
+            const u32x4 hf = q < end ? ld16(hp[m] + (c * o.width + q) * V) : zero;
 #pragma unroll
-        for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(b_of(n, q), hf, d[n]);
+            for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(b_of(n, q, end), hf, d[n]);
+          }
       }
       if (id[m] == g) {
 #pragma unroll
@@ -262,17 +286,16 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
 }
 
 // acc[m][n] += h B^T for TM x TN products of rows pos0 + 16 m and columns c0 + 16 n, over
-// chunks qa .. qb of h, summed over the adapters among the rows (of these, part `wk` of
-// WK), each with the other adapters' rows of h read as zero.  Work items of one adapter and
-// 4 chunks a lane group, DEP items' loads on their way: a wave with few rows has up to 16
-// adapters a product, and one by one each would cost a round trip to memory (0.8 us).
+// chunks qa .. qb of the copies of h, summed over the adapters among the rows (of these,
+// part `wk` of WK), each with the other adapters' rows of h read as zero.  Work items of one
+// adapter and 4 chunks of B, DEP items' loads on their way: a wave with few rows has up to
+// 16 adapters a product, and one by one each would cost a round trip to memory (0.8 us).
 // LDS: the chunks of h are at hs, kLowRow bytes a row from local row lr0 on, once `ready` has
 // waited for them; else they are read with B's.  A zero row of h times an infinity in B is
 // a NaN in another adapter's rows: the caller makes sums that are not finite again.
-constexpr int kLowChunks = 16, kLowRow = kLowChunks * 16;
 template <typename ST, int TM, int TN, int WK, int DEP, bool LDS, typename Ready>
 __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane, const unsigned char* hs,
-                                      int lr0, int qa, int qb, Ready ready, f32x4_t (&acc)[TM][TN]) {
+                                      int lr0, const LowOrder o, int qa, int qb, Ready ready, f32x4_t (&acc)[TM][TN]) {
   constexpr uint32_t E = sizeof(ST);
   const int l16 = lane & 15, kg = lane >> 4;
   const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = p.r * E;
@@ -335,18 +358,20 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
         more = false;
         break;
       }
+      for (int c = 0; c < (LDS ? o.copies : 1); ++c) {
 #pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        if (!(it[d].rows >> m & 1)) continue;
-        u32x4 hf = {0u, 0u, 0u, 0u};
-        if constexpr (LDS) {
-          const int r = lr0 + m * 16 + l16, ch = it[d].q - qa + kg;
-          if (id[m] == it[d].g && it[d].q + kg < qb) hf = *reinterpret_cast<const u32x4*>(hs + r * kLowRow + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
-        } else {
-          hf = it[d].hf[m];
+        for (int m = 0; m < TM; ++m) {
+          if (!(it[d].rows >> m & 1)) continue;
+          u32x4 hf = {0u, 0u, 0u, 0u};
+          if constexpr (LDS) {
+            const int r = lr0 + m * 16 + l16, ch = c * o.block + it[d].q - qa + kg;
+            if (id[m] == it[d].g && it[d].q + kg < qb) hf = *reinterpret_cast<const u32x4*>(hs + r * kLowRow + ((ch & ~7) | ((ch ^ r) & 7)) * 16);
+          } else {
+            hf = it[d].hf[m];
+          }
+#pragma unroll
+          for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], hf, acc[m][n]);
         }
-#pragma unroll
-        for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], hf, acc[m][n]);
       }
       next(it[d]);
     }
@@ -410,10 +435,10 @@ __device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f
 // from memory to the waves that multiply it.  Tiles of fewer rows read h as they read B: LDS
 // would save nothing, a wave column or two share it.
 //
-// Bound by the matrix cores and LDS reads for many rows, by the round trips of the K loop
-// for few.  bf16, without SiLU: 3584 rows 1024 -> 4096 in 38.3 us (785 TFLOP/s, without adapters),
-// 840 rows 4096 -> 1024 in 21.2 us with 12 adapters of rank 32, 61 rows with an adapter of
-// rank 16 each in 6.2 us.
+// Bound by the round trips of the K loop: one stage of 64 KB a CU is on its way for the
+// largest tiles, matrix cores busy 28% of the time.  bf16: 3584 rows 1024 -> 4096 in 38.3 us
+// (785 TFLOP/s) without adapters and SiLU, 840 rows 4096 -> 1024 in 21.2 us with 12 adapters
+// of rank 32, 61 rows with an adapter of rank 16 each in 6.2 us.
 template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU>
 __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
@@ -527,7 +552,8 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
     if (s < iters) issue(s, s * BK);
-  const int chunks = (p.r >> 2) * p.parts, pos0 = row0 + wm * TM * 16, c0 = n0 + wn * TN * 16;
+  const int pos0 = row0 + wm * TM * 16, c0 = n0 + wn * TN * 16;
+  const LowOrder o = low_order<ST, kStaged>(p.r, p.parts);
   if constexpr (kStaged) {
     constexpr int LPH = BM * kLowRow / 1024 / NW;
     static_assert(BM * kLowRow <= kStage && BM * kLowRow % (1024 * NW) == 0, "h fits a stage");
@@ -541,26 +567,27 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
-    for (int qa = 0; qa < chunks; qa += kLowChunks) {
+    for (int qa = 0; qa < o.width; qa += o.block) {
       if (qa > 0) meet();  // the chunks before are read
 #pragma unroll
       for (int i = 0; i < LPH; ++i) {
         const int c = (i * NW + wave) * 64 + lane, r = c / kLowChunks, pos = c % kLowChunks;
-        const int q = qa + ((pos & ~7) | ((pos ^ r) & 7));
-        const uint32_t o = row0 + r < p.M && q < chunks ? (uint32_t)(row0 + r) * hrow + (uint32_t)q * 16u : kNowhere;
-        load_lds16(rh, hs + (i * NW + wave) * 1024, o, 0);
+        const int ch = (pos & ~7) | ((pos ^ r) & 7), copy = ch >> o.shift, q = qa + (ch & (o.block - 1));
+        const uint32_t at = (uint32_t)(row0 + r) * hrow + (uint32_t)(copy * o.width + q) * 16u;
+        load_lds16(rh, hs + (i * NW + wave) * 1024, row0 + r < p.M && q < o.width ? at : kNowhere, 0);
       }
-      add_low<ST, TM, TN, WK, 4, true>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, qa, min(qa + kLowChunks, chunks), meet, acc);
+      // 256 x 256: 3 items, with 4 the registers spill (r 16: 61 us for 54)
+      add_low<ST, TM, TN, WK, TM * TN >= 32 ? 3 : 4, true>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, o, qa, min(qa + o.block, o.width), meet, acc);
     }
   } else {
-    add_low<ST, TM, TN, WK, 4, false>(p, id, pos0, c0, wk, lane, nullptr, 0, 0, chunks, []() {}, acc);
+    add_low<ST, TM, TN, WK, 4, false>(p, id, pos0, c0, wk, lane, nullptr, 0, o, 0, o.width, []() {}, acc);
   }
   if (__ballot(!all_finite(acc))) {
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
       for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    add_low_apart<ST, TM, TN, WK>(p, id, pos0, c0, wk, lane, acc);
+    add_low_apart<ST, TM, TN, WK, kStaged>(p, id, pos0, c0, wk, lane, acc);
   }
   int st = 0;
   for (int it = 0; it < iters; ++it) {
@@ -794,7 +821,7 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
 // part: a run of rows with one adapter in a tile, 16 ranks of it.
 // Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks 16
 // and 64, from one adapter to one for every second row: the cheapest by it is the fastest
-// form or within 12%, on the mean 0.1%.  How many adapters the rows have is not known on the
+// form or within 7%, on the mean 0.2%.  How many adapters the rows have is not known on the
 // host; the plan's tiles bound it.
 struct Form {
   int bm, bn, occ;
@@ -805,13 +832,13 @@ struct FormCost {
 };
 constexpr Form kForms[] = {{16, 16, 4, false}, {16, 32, 3, false}, {32, 32, 2, false},  {32, 64, 2, false},
                            {64, 64, 2, true},  {64, 128, 2, true}, {128, 128, 2, true}, {256, 256, 1, true}};
-constexpr FormCost kCost16[] = {{3.55f, 1.93f, 0.21f, 0.02f},  {3.65f, 2.35f, 0.19f, 0.04f},  {3.88f, 3.20f, 0.29f, 0.06f},
-                                {3.07f, 5.32f, 0.16f, 0.13f},  {3.93f, 4.65f, 0.36f, 0.09f},  {2.19f, 11.97f, 0.21f, 0.18f},
-                                {5.65f, 10.75f, 0.24f, 0.24f}, {6.91f, 13.87f, 0.f, 0.41f}};
+constexpr FormCost kCost16[] = {{3.40f, 1.89f, 0.20f, 0.03f},  {3.43f, 2.33f, 0.23f, 0.05f},  {4.15f, 2.69f, 0.36f, 0.06f},
+                                {3.22f, 5.26f, 0.17f, 0.21f},  {3.78f, 4.51f, 0.44f, 0.06f},  {2.57f, 13.12f, 0.15f, 0.13f},
+                                {6.43f, 11.02f, 0.26f, 0.19f}, {9.04f, 20.58f, 0.f, 0.25f}};
 // fp32 (256 x 256 outputs of it do not fit LDS)
-constexpr FormCost kCost32[] = {{3.40f, 4.35f, 0.22f, 0.03f},  {3.51f, 6.03f, 0.20f, 0.05f},  {3.57f, 7.76f, 0.28f, 0.08f},
-                                {2.26f, 15.99f, 0.13f, 0.21f}, {3.70f, 20.08f, 0.50f, 0.13f}, {1.00f, 44.28f, 0.45f, 0.27f},
-                                {5.86f, 66.81f, 0.76f, 0.32f}};
+constexpr FormCost kCost32[] = {{3.53f, 4.16f, 0.22f, 0.03f},  {3.75f, 5.68f, 0.20f, 0.05f},  {3.61f, 7.45f, 0.28f, 0.07f},
+                                {2.56f, 15.91f, 0.22f, 0.15f}, {4.95f, 19.60f, 0.53f, 0.15f}, {1.77f, 47.99f, 0.38f, 0.25f},
+                                {7.19f, 69.32f, 0.67f, 0.33f}};
 
 // us of a launch in form f with `adapters` among the rows, or a negative number where it
 // does not fit (a stage of 128 bytes a row, 256 where the adapters are not staged)
@@ -928,8 +955,8 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   constexpr int E = sizeof(ST);
   const int parts = k_parts(a->max_tiles, a->rank, a->k);
   if (!rows_ok(a->rows, a->x_stride, a->k, E) || !rows_ok(a->n, a->weight_stride, a->k, E) ||
-      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok(a->rows, (int64_t)a->rank * parts, (int64_t)a->rank * parts, 4) || !rows_ok(a->rank, a->k, a->k, E) ||
-      !rows_ok(a->n, a->rank, a->rank, E))
+      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok(a->rows, a->rank * parts, a->rank * parts, 4) ||
+      !rows_ok(a->rank, a->k, a->k, E) || !rows_ok(a->n, a->rank, a->rank, E))
     return fail(PK_ERR_INVALID, "%s: row strides must be multiples of 16 bytes, at least the row, and a tensor below 2^31 bytes", what);
   AdK<ST> k{};
   k.x = static_cast<const ST*>(a->x);
