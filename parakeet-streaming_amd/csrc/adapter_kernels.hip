@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "pk_common.h"
 #include "pk_device.h"
@@ -41,12 +42,20 @@ struct MmaA<float> {
 };
 
 // h is kept as two storage-type parts, high + (h - high), so that the rounding of h
-// is 2^-16 (bf16) or 2^-22 (fp16) of it and not 2^-8 or 2^-11 (an h past fp16's range is
-// infinite, as it is where x A^T is a product of its own): a row of h is [high
+// is 2^-16 (bf16) or 2^-22 (fp16) of it and not 2^-8 or 2^-11: a row of h is [high
 // 0..r-1 | low 0..r-1], r / 4 chunks of 16 bytes, chunk q multiplied with chunk
 // q mod r/8 of a row of B.  For ranks up to 16 both parts are one matrix instruction.
 // fp32: one part, r / 4 chunks.  Where K is split over workgroups (parts > 1) a row of h
 // is the parts' rows one after another: their sum is taken by the product with B.
+//
+// fp16 holds 2^-24 to 65504 where h is any fp32 number, so its rows are kept in units of a
+// power of two (row_unit) that the sums are multiplied with once h B^T is taken.  A workgroup
+// of adapter_low_kernel knows its part of K and its 64 ranks only: each such piece of a row
+// has its own unit, and the product with B brings them to the row's largest (to_unit).  What
+// is below fp16's smallest step then is below 2^-36 of the row's largest entry.  The units, 4
+// floats, are a row's end, in lines that h's readers load anyway.  They cost 0.2 - 0.7 us of a
+// call (840 rows 4096 -> 1024, r 32: 26.9 us with, 26.5 without; 4000 rows 512 -> 2048 SiLU: 23.7
+// and 22.6), 4 where a row of 128 ranks has two pieces (3584 rows 1024 -> 4096: 66 and 62).
 constexpr int kLowChunks = 16, kLowRow = kLowChunks * 16;  // chunks and bytes of a row of h in LDS
 
 template <typename ST>
@@ -72,6 +81,16 @@ __device__ static inline LowOrder low_order(int r, int parts) {
 }
 
 template <typename ST>
+constexpr bool kUnits = __is_same(ST, _Float16);
+constexpr int kMaxUnits = 4;  // pieces of a row of h: 2 parts of K, 64 of 128 ranks
+
+// bytes of a row of h
+template <typename ST>
+__host__ __device__ constexpr uint32_t low_row(int r, int parts) {
+  return (uint32_t)(r * 4 * parts) + (kUnits<ST> ? 4 * kMaxUnits : 0);
+}
+
+template <typename ST>
 struct AdK {
   const ST* x;  // [M][K], stride x_s
   int64_t x_s;
@@ -84,12 +103,13 @@ struct AdK {
   const int32_t* order;  // [M] plan: row at a position
   const int32_t* ids;    // [M] adapter at a position, -1: none
   const int4* tiles;     // {adapter, first position, rows, 0}
-  ST* h;                 // [M][parts][2 r] (fp32: [M][parts][r]) by position
+  ST* h;                 // [M] rows by position: [parts][2 r], fp16 units behind; fp32 [parts][r]
   ST* out;               // [M][N], stride out_s
   int64_t out_s;
   int32_t M, N, K, r, G;
   int32_t parts, kpart;  // parts of K, columns of one (a multiple of 64)
   int32_t mtiles, xm;
+  int32_t units;  // pieces of a row of h (fp16)
 };
 
 // row at a position of the plan (positions past the last row, and entries that are no
@@ -107,11 +127,27 @@ constexpr uint32_t kNowhere = 0x80000000u;
 __device__ static inline u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
 }
+__device__ static inline u32x2 load8(const __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+}
 
-// 4 ranks of a row of h, scaled, at q (their low parts r elements on)
+// 4 fp16 entries in fp32
+__device__ static inline u32x4 wide(u32x2 v) {
+  float f[4];
+  Tr<_Float16>::two(v.x, f);
+  Tr<_Float16>::two(v.y, f + 2);
+  return Tr<float>::pack(f);
+}
+__device__ static inline u32x4 wide(u32x4 v) { return v; }
+
+// 4 ranks of a row of h, scaled (and in the row's units), at q (their low parts r elements on)
 template <typename ST>
-__device__ static inline void store_low(f32x4_t v, float sc, ST* q, int r) {
+__device__ static inline void store_low(f32x4_t v, float sc, float down, ST* q, int r) {
   float f[4] = {v.x * sc, v.y * sc, v.z * sc, v.w * sc};
+  if constexpr (kUnits<ST>) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] *= down;
+  }
   if constexpr (sizeof(ST) == 4) {
     st16(q, Tr<float>::pack(f));
   } else {
@@ -124,6 +160,56 @@ __device__ static inline void store_low(f32x4_t v, float sc, ST* q, int r) {
     *reinterpret_cast<u32x2*>(q) = pack4<ST>(f);
     *reinterpret_cast<u32x2*>(q + r) = pack4<ST>(lo);
   }
+}
+
+// the largest finite magnitude, scaled, among the ranks that the 4 lanes of a row have
+__device__ static inline float largest_of_row(f32x4_t v, float sc) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float f = fabsf(v[e] * sc);
+    m = f < __builtin_inff() ? fmaxf(m, f) : m;
+  }
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Units of a row whose largest finite magnitude is m: times `down` m is in [2^14, 2^15) (less
+// below 2^-112), `up` is its inverse; both are normal powers of two.
+struct RowUnit {
+  float down, up;
+};
+__device__ static inline RowUnit row_unit(float m) {
+  const uint32_t e = min(max(__float_as_uint(m) >> 23, 15u), 254u);
+  return RowUnit{__uint_as_float((268u - e) << 23), __uint_as_float((e - 14u) << 23)};
+}
+
+// `own` / `most`, powers of two with own <= most, as the product of two fp16 numbers (at
+// least 2^-38: entries that are below that step of a row's largest one)
+__device__ static inline uint32_t unit_ratio(float own, float most) {
+  const uint32_t d = min((__float_as_uint(most) - __float_as_uint(own)) >> 23, 38u);
+  const uint32_t d1 = min(d, 14u), d2 = d - d1;
+  return (15u - d1) << 10 | (d2 < 15u ? (15u - d2) << 10 : 1u << (24u - d2)) << 16;
+}
+
+// 8 entries of h in the row's units
+__device__ static inline u32x4 to_unit(u32x4 h, uint32_t ratio) {
+  typedef MmaL<_Float16>::H8 H8;
+  const _Float16 a = __builtin_bit_cast(_Float16, (uint16_t)ratio), b = __builtin_bit_cast(_Float16, (uint16_t)(ratio >> 16));
+  return __builtin_bit_cast(u32x4, __builtin_bit_cast(H8, h) * (H8)a * (H8)b);
+}
+
+// the piece of a row of h that chunk q of copy c is in
+__device__ static inline int piece_of(const LowOrder& o, int r, int c, int q) {
+  int part = c >> 1;  // copies: high and low of each part of K
+  if (o.copies == 1) {
+    part = q >= r >> 2 ? 1 : 0;
+    q -= part * (r >> 2);
+    if (q >= r >> 3) q -= r >> 3;
+  }
+  return part * ((r + 63) >> 6) + (q >> 3);
 }
 
 // h of a tile: its 32 rows of x and 16 RT rows of A through LDS, 512 bytes of each a
@@ -140,11 +226,13 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
   constexpr int LPS = NR * CH / 64 / kLowWaves;
   static_assert(NR * CH % (64 * kLowWaves) == 0 && BK == COLS * kLowWaves, "whole waves of chunks, a step a wave");
   constexpr int kRed = kLowWaves * RT * 2 * 64 * 16;
+  static_assert(S * kStage >= kRed + 2 * RT * 16 * 4, "a row's largest entries beside the sums");
   __shared__ __align__(16) unsigned char smem[S * kStage > kRed ? S * kStage : kRed];
   static_assert(2 * RT <= kLowWaves, "a wave finishes at most one sum");
   const int4 tile = p.tiles[blockIdx.x];
   if ((uint32_t)tile.x >= (uint32_t)p.G) return;  // past the last tile
   if (tile.y < 0 || tile.z <= 0 || tile.z > kLowRows || tile.y > p.M - tile.z) return;  // not a plan's
+  const float sc = p.scale[tile.x];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, kg = lane >> 4;
   const int r0 = blockIdx.y * RT * 16;
@@ -206,13 +294,31 @@ __global__ void __launch_bounds__(64 * kLowWaves) adapter_low_kernel(const AdK<S
 #pragma unroll
     for (int m = 0; m < 2; ++m) red[((wave * RT + j) * 2 + m) * 64 + lane] = acc[j][m];
   __syncthreads();
-  if (wave >= 2 * RT) return;
   const int row = (wave & 1) * 16 + l16, c = r0 + (wave >> 1) * 16 + kg * 4;
-  f32x4_t v = red[wave * 64 + lane];
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (wave < 2 * RT) {
+    v = red[wave * 64 + lane];
 #pragma unroll
-  for (int w = 1; w < kLowWaves; ++w) v += red[(w * RT * 2 + wave) * 64 + lane];
-  if (row >= tile.z || c >= p.r) return;  // r is a multiple of 8, c of 4
-  store_low<ST>(v, p.scale[tile.x], p.h + ((int64_t)(tile.y + row) * p.parts + blockIdx.z) * (sizeof(ST) == 4 ? p.r : 2 * p.r) + c, p.r);
+    for (int w = 1; w < kLowWaves; ++w) v += red[(w * RT * 2 + wave) * 64 + lane];
+  }
+  RowUnit u{1.f, 1.f};
+  if constexpr (kUnits<ST>) {  // ranks past the last are the last again, and no larger
+    float m = largest_of_row(v, sc);
+    if constexpr (RT > 1) {
+      float* const most = reinterpret_cast<float*>(smem + kRed);
+      if (wave < 2 * RT && kg == 0) most[wave * 16 + l16] = m;
+      __syncthreads();
+      if (wave < 2 * RT) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) m = fmaxf(m, most[(2 * j + (wave & 1)) * 16 + l16]);
+      }
+    }
+    u = row_unit(m);
+  }
+  if (wave >= 2 * RT || row >= tile.z) return;
+  ST* const hp = p.h + (tile.y + row) * (int64_t)(low_row<ST>(p.r, p.parts) / E);
+  if (kUnits<ST> && wave < 2 && kg == 0) reinterpret_cast<float*>(hp + 2 * p.r * p.parts)[blockIdx.z * gridDim.y + blockIdx.y] = u.up;
+  if (c < p.r) store_low<ST>(v, sc, u.down, hp + blockIdx.z * (E == 4 ? p.r : 2 * p.r) + c, p.r);  // r is a multiple of 8, c of 4
 }
 
 // whether every sum is finite: an infinity or NaN times zero is a NaN
@@ -232,12 +338,12 @@ __device__ static inline bool all_finite(const f32x4_t (&acc)[TM][TN]) {
 // an adapter its product is taken for all of them and kept for those, so that what a row
 // gets depends on its own adapter alone, and in the same order of sums, so that the rows
 // without them keep their bits.
-template <typename ST, int TM, int TN, int WK, bool LDS>
+template <typename ST, int TM, int TN, int WK, bool LDS, bool FIT, typename Fit>
 __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane,
-                                      f32x4_t (&acc)[TM][TN]) {
+                                            Fit fit, f32x4_t (&acc)[TM][TN]) {
   constexpr int V = Tr<ST>::VEC;
   const int l16 = lane & 15, kg = lane >> 4;
-  const int hs = (sizeof(ST) == 4 ? p.r : 2 * p.r) * p.parts;
+  const int hs = low_row<ST>(p.r, p.parts) / sizeof(ST);
   const LowOrder o = low_order<ST, LDS>(p.r, p.parts);
   const u32x4 zero = {0u, 0u, 0u, 0u};
   const ST* hp[TM];
@@ -272,7 +378,8 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
         const int end = min(q0 + o.block, o.width);
         for (int q = q0 + kg; q - kg < end; q += 4)
           for (int c = 0; c < o.copies; ++c) {
-            const u32x4 hf = q < end ? ld16(hp[m] + (c * o.width + q) * V) : zero;
+            u32x4 hf = q < end ? ld16(hp[m] + (c * o.width + q) * V) : zero;
+            if constexpr (FIT) hf = fit(m, piece_of(o, p.r, c, min(q, end - 1)), hf);
 #pragma unroll
             for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(b_of(n, q, end), hf, d[n]);
           }
@@ -291,14 +398,15 @@ __device__ static inline void add_low_apart(const AdK<ST>& p, const int (&id)[TM
 // adapter and 4 chunks of B, DEP items' loads on their way: a wave with few rows has up to
 // 16 adapters a product, and one by one each would cost a round trip to memory (0.8 us).
 // LDS: the chunks of h are at hs, kLowRow bytes a row from local row lr0 on, once `ready` has
-// waited for them; else they are read with B's.  A zero row of h times an infinity in B is
-// a NaN in another adapter's rows: the caller makes sums that are not finite again.
-template <typename ST, int TM, int TN, int WK, int DEP, bool LDS, typename Ready>
+// waited for them; else they are read with B's.  FIT: fit(m, piece, chunk) brings a chunk of h
+// to its row's units.  A zero row of h times an infinity in B is a NaN in another adapter's
+// rows: the caller makes sums that are not finite again.
+template <typename ST, int TM, int TN, int WK, int DEP, bool LDS, bool FIT, typename Ready, typename Fit>
 __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int pos0, int c0, int wk, int lane, const unsigned char* hs,
-                                      int lr0, const LowOrder o, int qa, int qb, Ready ready, f32x4_t (&acc)[TM][TN]) {
+                                      int lr0, const LowOrder o, int qa, int qb, Ready ready, Fit fit, f32x4_t (&acc)[TM][TN]) {
   constexpr uint32_t E = sizeof(ST);
   const int l16 = lane & 15, kg = lane >> 4;
-  const uint32_t hrow = (uint32_t)p.r * 4u * p.parts, brow = p.r * E;
+  const uint32_t hrow = low_row<ST>(p.r, p.parts), brow = p.r * E;
   const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
   uint64_t left[TM];
 #pragma unroll
@@ -369,6 +477,7 @@ __device__ static inline void add_low(const AdK<ST>& p, const int (&id)[TM], int
           } else {
             hf = it[d].hf[m];
           }
+          if constexpr (FIT) hf = fit(m, piece_of(o, p.r, c, min(it[d].q + kg, qb - 1)), hf);  // zeros stay zeros
 #pragma unroll
           for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(it[d].bf[n], hf, acc[m][n]);
         }
@@ -439,7 +548,9 @@ __device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f
 // largest tiles, matrix cores busy 28% of the time.  bf16: 3584 rows 1024 -> 4096 in 38.3 us
 // (785 TFLOP/s) without adapters and SiLU, 840 rows 4096 -> 1024 in 21.2 us with 12 adapters
 // of rank 32, 61 rows with an adapter of rank 16 each in 6.2 us.
-template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU>
+// FIT: rows of h in several pieces that have units (fp16).  A form of its own: 3584 rows 1024 ->
+// 4096 of rank 128 take 66 us so and 68 with a branch in the loop of h B^T.
+template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU, bool FIT>
 __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
   constexpr int NW = WM * WN * WK;
@@ -458,9 +569,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   constexpr bool kStaged = CH == 8;
   // one LDS object: with a second one the compiler keeps them apart and waits for every
   // load to LDS in flight before an operand read
-  __shared__ __align__(16) unsigned char smem[kSmem + BM * 8];
+  __shared__ __align__(16) unsigned char smem[kSmem + BM * (!kUnits<ST> || !kStaged ? 8 : FIT ? 8 + 8 * kMaxUnits : 8 + 4 * kMaxUnits)];
   int32_t* const ord = reinterpret_cast<int32_t*>(smem + kSmem);
   int32_t* const sid = ord + BM;
+  u32x4* const units = reinterpret_cast<u32x4*>(sid + BM);          // fp16, staged: the units of a row of h
+  uint32_t* const ratio = reinterpret_cast<uint32_t*>(units + BM);  // FIT: [kMaxUnits][BM] of its pieces to the largest
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, kg = lane >> 4;
@@ -469,6 +582,18 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
   xcd_tile(p.mtiles, p.xm, mt_i, nt_i);
   const int row0 = mt_i * BM, n0 = nt_i * BN;
 
+  const uint32_t hrow = low_row<ST>(p.r, p.parts);
+  const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
+  // fp16: where a row of h has its units
+  auto units_at = [&](int pos) { return pos < p.M ? (uint32_t)pos * hrow + (uint32_t)p.r * 4u * p.parts : kNowhere; };
+  auto most_of = [&](u32x4 u) {
+    float most = __uint_as_float(u[0]);
+    if constexpr (FIT) {
+#pragma unroll
+      for (int j = 1; j < kMaxUnits; ++j) most = j < p.units ? fmaxf(most, __uint_as_float(u[j])) : most;
+    }
+    return most;
+  };
   // positions past the last row read the last row, have no adapter and store nothing
   for (int i = threadIdx.x; i < BM; i += 64 * NW) {
     ord[i] = plan_row(p, row0 + i);
@@ -554,12 +679,28 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
     if (s < iters) issue(s, s * BK);
   const int pos0 = row0 + wm * TM * 16, c0 = n0 + wn * TN * 16;
   const LowOrder o = low_order<ST, kStaged>(p.r, p.parts);
+  // fp16: the sums to what they stand for (nothing is written for rows without an adapter)
+  auto in_ones = [&](auto up_of) {
+    if constexpr (kUnits<ST>) {
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const float u = up_of(m);
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] *= u;
+      }
+    }
+  };
+  auto again = [&](auto fit) {  // an infinity or NaN is among the operands
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    add_low_apart<ST, TM, TN, WK, kStaged, FIT>(p, id, pos0, c0, wk, lane, fit, acc);
+  };
   if constexpr (kStaged) {
     constexpr int LPH = BM * kLowRow / 1024 / NW;
     static_assert(BM * kLowRow <= kStage && BM * kLowRow % (1024 * NW) == 0, "h fits a stage");
     unsigned char* const hs = smem + (S - 1) * kStage;
-    const uint32_t hrow = (uint32_t)p.r * 4u * p.parts;
-    const __amdgpu_buffer_rsrc_t rh = bytes_rsrc(p.h, (uint32_t)p.M * hrow);
     auto meet = [&]() {  // every wave's loads to LDS are in, its reads done
       wait_vm<0>();
       asm volatile("" ::: "memory");
@@ -567,6 +708,28 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
+    if constexpr (kUnits<ST>) {
+      static_assert(BM <= 64 * NW, "64 rows a wave");
+      if (wave < BM / 64) load_lds16(rh, reinterpret_cast<unsigned char*>(units + wave * 64), units_at(row0 + wave * 64 + lane), 0);
+    }
+    bool first = true;
+    auto ready = [&]() {
+      meet();
+      if (FIT && first) {
+        if (threadIdx.x < BM) {
+          const u32x4 u = units[threadIdx.x];
+          const float most = most_of(u);
+#pragma unroll
+          for (int j = 0; j < kMaxUnits; ++j) ratio[j * BM + threadIdx.x] = unit_ratio(__uint_as_float(u[j]), most);
+          units[threadIdx.x][0] = __float_as_uint(most);
+        }
+        meet();
+      }
+      first = false;
+    };
+    const int row = wm * TM * 16 + l16;
+    auto fit = [&](int m, int piece, u32x4 h) { return to_unit(h, ratio[piece * BM + row + m * 16]); };
+    auto up_of = [&](int m) { return id[m] >= 0 ? __uint_as_float(units[row + m * 16][0]) : 1.f; };
     for (int qa = 0; qa < o.width; qa += o.block) {
       if (qa > 0) meet();  // the chunks before are read
 #pragma unroll
@@ -577,17 +740,27 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
         load_lds16(rh, hs + (i * NW + wave) * 1024, row0 + r < p.M && q < o.width ? at : kNowhere, 0);
       }
       // 256 x 256: 3 items, with 4 the registers spill (r 16: 61 us for 54)
-      add_low<ST, TM, TN, WK, TM * TN >= 32 ? 3 : 4, true>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, o, qa, min(qa + o.block, o.width), meet, acc);
+      constexpr int DEP = TM * TN >= 32 ? 3 : 4;
+      add_low<ST, TM, TN, WK, DEP, true, FIT>(p, id, pos0, c0, wk, lane, hs, wm * TM * 16, o, qa, min(qa + o.block, o.width), ready, fit, acc);
     }
+    if (__ballot(!all_finite(acc))) again(fit);
+    in_ones(up_of);
   } else {
-    add_low<ST, TM, TN, WK, 4, false>(p, id, pos0, c0, wk, lane, nullptr, 0, o, 0, o.width, []() {}, acc);
-  }
-  if (__ballot(!all_finite(acc))) {
+    u32x4 u[TM];
+    if constexpr (kUnits<ST>) {
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
+      for (int m = 0; m < TM; ++m) u[m] = load16(rh, units_at(pos0 + m * 16 + l16));
+    }
+    auto fit = [&](int m, int piece, u32x4 h) {
+      uint32_t own = u[m][0];
 #pragma unroll
-      for (int n = 0; n < TN; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    add_low_apart<ST, TM, TN, WK, kStaged>(p, id, pos0, c0, wk, lane, acc);
+      for (int j = 1; j < kMaxUnits; ++j) own = piece == j ? u[m][j] : own;
+      return to_unit(h, unit_ratio(__uint_as_float(own), most_of(u[m])));
+    };
+    auto up_of = [&](int m) { return id[m] >= 0 ? most_of(u[m]) : 1.f; };
+    add_low<ST, TM, TN, WK, 4, false, FIT>(p, id, pos0, c0, wk, lane, nullptr, 0, o, 0, o.width, []() {}, fit, acc);
+    if (__ballot(!all_finite(acc))) again(fit);
+    in_ones(up_of);
   }
   int st = 0;
   for (int it = 0; it < iters; ++it) {
@@ -608,6 +781,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 template <typename ST, int RW, int RT, int BN, int WN, int WK, int BKB, int S, int SILU>
 __global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST> p) {
 #pragma clang fp contract(off)
+  // fp16: h in fp32 and B widened to it for the fp32 instructions, few here; h keeps its range
+  // without units, whose maximum would be in the chain (256 rows 512 -> 2048, r 16: 7.7 us so,
+  // 8.3 with units)
+  using HT = std::conditional_t<kUnits<ST>, float, ST>;
+  using BF = std::conditional_t<kUnits<ST>, u32x2, u32x4>;
   constexpr int E = sizeof(ST), V = 16 / E, COLS = MmaA<ST>::COLS;
   constexpr int K = RW / E, BK = BKB / E, CH = BKB / 16;
   constexpr int NW = WN * WK, BM = 16, TN = BN / WN / 16;
@@ -704,7 +882,7 @@ __global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST>
         for (int j = 0; j < RT; ++j) h[j] = MmaA<ST>::step(af[u][j], x_frag(((s0 + u) * NW + wave) * 4 + kg), h[j]);
     }
     // this adapter's B for the wave's columns, on its way while the sums meet
-    u32x4 bf[RT][TN];
+    BF bf[RT][TN];
     const bool turn_mine = turn == wk;
     turn = turn == WK - 1 ? 0 : turn + 1;
     if (turn_mine) {
@@ -713,7 +891,11 @@ __global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST>
 #pragma unroll
         for (int n = 0; n < TN; ++n) {
           const uint32_t c = q * 4 + kg;  // 16 ranks a step
-          bf[q][n] = load16(rb, c < chunks ? (uint32_t)(n0 + (wn * TN + n) * 16 + l16) * arow + (uint32_t)b_chunk<ST>(c, p.r) * 16u : kNowhere);
+          const uint32_t row = (uint32_t)(n0 + (wn * TN + n) * 16 + l16) * arow;
+          if constexpr (kUnits<ST>)
+            bf[q][n] = load8(rb, c < chunks ? row + c * 8u : kNowhere);
+          else
+            bf[q][n] = load16(rb, c < chunks ? row + (uint32_t)b_chunk<ST>(c, p.r) * 16u : kNowhere);
         }
     }
 #pragma unroll
@@ -724,7 +906,7 @@ __global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST>
 #pragma unroll
       for (int w = 1; w < NW; ++w) v += red[(w * RT + wave) * 64 + lane];
       const int c = wave * 16 + kg * 4;
-      if (mine && c < p.r) store_low<ST>(v, p.scale[g], reinterpret_cast<ST*>(hs + l16 * (RT * 64)) + c, p.r);
+      if (mine && c < p.r) store_low<HT>(v, p.scale[g], 1.f, reinterpret_cast<HT*>(hs + l16 * (RT * 64)) + c, p.r);
     }
     meet();
     if (turn_mine) {
@@ -737,7 +919,7 @@ __global__ void __launch_bounds__(64 * WN * WK) adapter_few_kernel(const AdK<ST>
         u32x4 hf = {0u, 0u, 0u, 0u};
         if (mine && c < chunks) hf = *reinterpret_cast<const u32x4*>(hs + l16 * (RT * 64) + c * 16);
 #pragma unroll
-        for (int n = 0; n < TN; ++n) d[n] = MmaA<ST>::step(bf[q][n], hf, d[n]);
+        for (int n = 0; n < TN; ++n) d[n] = MmaA<HT>::step(wide(bf[q][n]), hf, d[n]);
       }
       // columns (rows of the batch) are independent: kept for the adapter's own rows
 #pragma unroll
@@ -811,7 +993,11 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
   else
     k.xm = 0;
   // BK columns of 16-bit types; of fp32 half as many, the same bytes
-  hipLaunchKernelGGL((adapter_tile_kernel<ST, BM, BN, WM, WN, WK, BK * 2 / (int)sizeof(ST), S, SILU>), grid, dim3(64 * WM * WN * WK), 0, s, k);
+  constexpr int B = BK * 2 / (int)sizeof(ST);
+  if (kUnits<ST> && k.units > 1)
+    hipLaunchKernelGGL((adapter_tile_kernel<ST, BM, BN, WM, WN, WK, B, S, SILU, kUnits<ST>>), grid, dim3(64 * WM * WN * WK), 0, s, k);
+  else
+    hipLaunchKernelGGL((adapter_tile_kernel<ST, BM, BN, WM, WN, WK, B, S, SILU, false>), grid, dim3(64 * WM * WN * WK), 0, s, k);
   return check_launch("pk_adapter_linear");
 }
 
@@ -955,7 +1141,7 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   constexpr int E = sizeof(ST);
   const int parts = k_parts(a->max_tiles, a->rank, a->k);
   if (!rows_ok(a->rows, a->x_stride, a->k, E) || !rows_ok(a->n, a->weight_stride, a->k, E) ||
-      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok(a->rows, a->rank * parts, a->rank * parts, 4) ||
+      !rows_ok(a->rows, a->out_stride, a->n, E) || !rows_ok(a->rows, low_row<ST>(a->rank, parts) / 4, low_row<ST>(a->rank, parts) / 4, 4) ||
       !rows_ok(a->rank, a->k, a->k, E) || !rows_ok(a->n, a->rank, a->rank, E))
     return fail(PK_ERR_INVALID, "%s: row strides must be multiples of 16 bytes, at least the row, and a tensor below 2^31 bytes", what);
   AdK<ST> k{};
@@ -980,6 +1166,7 @@ int adapter_typed(const pk_adapter_linear_args* a, hipStream_t s) {
   k.G = a->num_adapters;
   k.parts = parts;
   k.kpart = ((k.K / 64 + k.parts - 1) / k.parts) * 64;
+  k.units = parts * low_blocks(k.r);
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const int64_t adapters = most_adapters(k.M, a->max_tiles);
@@ -999,7 +1186,8 @@ extern "C" int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32
   if (rows <= 0 || n <= 0 || rank <= 0 || k <= 0 || max_tiles < 0) return 0;
   const int64_t row = (int64_t)k * (dtype == PK_DTYPE_F32 ? 4 : 2);
   if (pk::few_form(rows, n, row, rank, pk::most_adapters(rows, max_tiles), pk::cu_count())) return 0;
-  return (int64_t)rows * rank * 4 * pk::k_parts(max_tiles, rank, k);
+  const int parts = pk::k_parts(max_tiles, rank, k);
+  return rows * (int64_t)(dtype == PK_DTYPE_F16 ? pk::low_row<_Float16>(rank, parts) : pk::low_row<float>(rank, parts));
 }
 
 extern "C" int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream) {
