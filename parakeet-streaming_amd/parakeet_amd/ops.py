@@ -1300,9 +1300,16 @@ def adapter_linear(
     stream beside it, the output rounded once.  Two launches, or one for few rows of few
     adapters.  x [..., K], weight [N, K], bias [N] or None; N and K multiples of 64, ranks
     of 8 up to 128; ``out`` overlaps no operand.  What a row gets depends on its own
-    adapter alone.  No gradients."""
+    adapter alone.  No gradients, and no call where something else follows or rewrites
+    torch's own (forward-mode derivatives, tracing, function transforms, autocast to another
+    dtype, tensor subclasses): it would pass this one by, so it is refused."""
     A, Bm, scale, order, ids, tiles = adapters.a, adapters.b, adapters.scale, plan.order, plan.ids, plan.tiles
     dt, dev, ws, xs = x.dtype, x.device, weight.shape, x.shape
+    if (
+        _overridden(x, weight, A, Bm, scale, bias) or _forward_ad._current_level >= 0 or _tracing() or torch.is_autocast_enabled()
+        or _dispatch_modes()
+    ):
+        _refuse_transforms("adapter_linear", [t for t in (x, weight, A, Bm, scale, bias) if t is not None])
     n, k = ws if len(ws) == 2 else (0, 0)
     G, r = A.shape[:2] if A.dim() == 3 else (0, 0)
     M = x.numel() // k if k else 0
@@ -1321,12 +1328,13 @@ def adapter_linear(
         and (bias is None or (bias.shape == (n,) and bias.dtype is dt and bias.device == dev and bias.is_contiguous()))
     ):
         _refuse_adapter_linear(x, weight, bias, adapters, plan)
-    if (
+    if torch.is_grad_enabled() and (
         x.requires_grad or weight.requires_grad or A.requires_grad or Bm.requires_grad or scale.requires_grad
         or (bias is not None and bias.requires_grad)
-    ) and torch.is_grad_enabled():
+    ):
         raise RuntimeError("adapter_linear has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
-    x = _aligned_rows(x)
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        x = _aligned_rows(x)
     shape = (*xs[:-1], n)
     if out is None:
         out = x.new_empty(shape)
@@ -1352,6 +1360,32 @@ def adapter_linear(
     a.order, a.ids, a.tiles = order.data_ptr(), ids.data_ptr(), tiles.data_ptr()
     check(L.pk_adapter_linear(ctypes.byref(a), _stream(dev)), "pk_adapter_linear")
     return out
+
+
+# what each call asks, a few tenths of a microsecond together: tensor subclasses and function
+# modes, forward-mode derivatives, traces, dispatch modes
+_overridden, _forward_ad = torch.overrides.has_torch_function_variadic, torch.autograd.forward_ad
+_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+
+
+def _refuse_transforms(what: str, operands: list[torch.Tensor]) -> None:
+    """Refuses a call that something follows or rewrites which a kernel passes by."""
+    for t in operands:
+        if type(t) not in (torch.Tensor, torch.nn.Parameter):
+            raise RuntimeError(f"{what} takes plain tensors, got {type(t).__name__}")
+        if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its result would be a constant of the trace")
+    if torch._C._len_torch_dispatch_stack():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise RuntimeError(f"{what} cannot be traced: its result would be a constant of the graph")
+    dt = operands[0].dtype
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") is not dt:
+        raise RuntimeError(f"{what} keeps the dtype of its operands, {dt}: call it under torch.autocast('cuda', enabled=False), "
+                           f"or on tensors of {torch.get_autocast_dtype('cuda')}")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
