@@ -241,11 +241,25 @@ class ModelCache:
         """Opens the next step now -- the host page work for the batch and the
         upload of its rows -- instead of on the first layer update.  For callers
         that replay a recorded step, whose launches read the rows uploaded here."""
+        self._check_whole()
+        self._open_step()
+
+    def _check_whole(self) -> None:
         if self._step_open and self._seen and len(self._seen) != self.num_layers:
             raise RuntimeError(
                 f"paged cache: a new step began after layers {sorted(self._seen)} of {self.num_layers}"
             )
-        self._open_step()
+
+    @contextmanager
+    def replaying(self):
+        """Around the replay of a recorded step that opens itself
+        (:meth:`open_recorded_step`): the step before it has to be whole, and after it the
+        cache is at the end of an open step, as after an eager one."""
+        if not self.device_pages:
+            raise RuntimeError("paged cache: host pages are advanced by open_step() before a replay")
+        self._check_whole()
+        yield
+        self._step_open, self._seen = True, set(range(self.num_layers))
 
     @contextmanager
     def recording(self):

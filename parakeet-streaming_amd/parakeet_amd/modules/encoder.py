@@ -480,9 +480,8 @@ class EncoderStepGraph:
         if tuple(x.shape) != self.shape:
             raise ValueError(f"x must be {self.shape}, got {tuple(x.shape)}")
         cache = self.state.cache
-        if self.graph is None or not cache.device_pages:
-            cache.open_step()
         if self.graph is None:
+            cache.open_step()
             self.x = x.detach().clone()
             out = self._step()
             graph = torch.cuda.CUDAGraph()
@@ -495,7 +494,12 @@ class EncoderStepGraph:
         self.x.copy_(x)
         for layer in self.encoder.layers:  # the recording reads the kept position projections
             layer.self_attn.refresh_projected_pos()
-        self.graph.replay()
+        if cache.device_pages:
+            with cache.replaying():
+                self.graph.replay()
+        else:
+            cache.open_step()
+            self.graph.replay()
         return self.out
 
     def _step(self) -> Tensor:
