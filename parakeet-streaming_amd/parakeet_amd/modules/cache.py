@@ -239,8 +239,8 @@ class ModelCache:
 
     def open_step(self) -> None:
         """Opens the next step now -- the host page work for the batch and the
-        upload of its rows -- instead of on the first layer update.  For callers
-        that replay a recorded step, whose launches read the rows uploaded here."""
+        upload of its rows -- instead of on the first layer update.  A recorded step
+        is replayed inside :meth:`replaying`, which does this and closes the step."""
         self._check_whole()
         self._open_step()
 
@@ -252,20 +252,22 @@ class ModelCache:
 
     @contextmanager
     def replaying(self):
-        """Around the replay of a recorded step that opens itself
-        (:meth:`open_recorded_step`): the step before it has to be whole, and after it the
-        cache is at the end of an open step, as after an eager one."""
-        if not self.device_pages:
-            raise RuntimeError("paged cache: host pages are advanced by open_step() before a replay")
-        self._check_whole()
+        """Around the replay of a recorded step: the step before it has to be whole, host
+        pages are advanced first (:meth:`open_step`; a recording on ``device_pages`` opens
+        its own step), and after it the cache is at the end of an open step, as after an
+        eager one."""
+        if self.device_pages:
+            self._check_whole()
+        else:
+            self.open_step()
         yield
         self._step_open, self._seen = True, set(range(self.num_layers))
 
     @contextmanager
     def recording(self):
         """While recording a step (HIP graph capture), layer updates never open a
-        step: the recording must hold no host work, and each replay follows an
-        ``open_step()``."""
+        step: the recording must hold no host work, and replays run inside
+        :meth:`replaying`."""
         if self._recording:
             raise RuntimeError("paged cache: already recording")
         seen = self._seen

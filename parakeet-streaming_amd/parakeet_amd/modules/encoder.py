@@ -427,9 +427,9 @@ class EncoderStepGraph:
 
     Every launch of a step reads the same device memory each step: the page
     pools, the batch's block-table rows, the state counters, the conv state, the
-    position table and the weights; only their contents change.  A call runs
-    ``state.cache.open_step()`` (the host page work and the one upload of the
-    batch's rows), copies ``x`` into a fixed input buffer and replays.  The first
+    position table and the weights; only their contents change.  A call copies ``x``
+    into a fixed input buffer, opens the cache's step (the host page work and the one
+    upload of the batch's rows) and replays.  Replays and eager steps may alternate.  The first
     call runs the step eagerly -- its real work, which also initialises the
     libraries' handles -- and then records the step without running it.
 
@@ -494,11 +494,7 @@ class EncoderStepGraph:
         self.x.copy_(x)
         for layer in self.encoder.layers:  # the recording reads the kept position projections
             layer.self_attn.refresh_projected_pos()
-        if cache.device_pages:
-            with cache.replaying():
-                self.graph.replay()
-        else:
-            cache.open_step()
+        with cache.replaying():
             self.graph.replay()
         return self.out
 

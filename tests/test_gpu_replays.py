@@ -65,9 +65,17 @@ def test_replay_after_half_a_step(cuda, device_pages):
             graph(_x(cuda, B, 5))
 
 
-def test_replays_of_host_pages_open_their_step():
-    from parakeet_amd.modules.cache import ModelCache
-
-    cache = ModelCache(1, [8, 1], 64, 9, batch_size=1)
-    with pytest.raises(RuntimeError, match="open_step"), cache.replaying():
-        pass
+@pytest.mark.parametrize("device_pages", [False, True])
+def test_eager_steps_between_replays(cuda, device_pages):
+    B = 3
+    enc, length, (eager, mixed) = _states(cuda, B, device_pages)
+    graph = EncoderStepGraph(enc, mixed, length)
+    with torch.no_grad():
+        for step in range(9):
+            x = _x(cuda, B, step)
+            want, _ = enc(x, eager, length=length)
+            got = enc(x, mixed, length=length)[0] if step % 4 == 2 else graph(x)
+            assert torch.equal(got, want), step
+    assert eager.cache.pool.free_list().tolist() == mixed.cache.pool.free_list().tolist()
+    for slot in range(B):
+        assert eager.cache.pool.slot_info(slot)[0] == mixed.cache.pool.slot_info(slot)[0] == 9 * T
