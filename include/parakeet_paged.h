@@ -769,6 +769,7 @@ int pk_pool_free_list(const pk_pool* pool, int32_t* out, int32_t capacity);
  *   rows[b]        = {A, ring[0 .. M-1]}, A the frames before the step (as
  *                    pk_paged_layout.rows; M = (left + chunk + page_size - 2) / page_size + 1)
  *   slot_map[b][t] = page * page_size + row of the page for frame t < n_b, else -1
+ *                    (slot_map NULL: not written, for readers of the rows alone)
  * A slot out of range, or named earlier in the call, is absent: rows {0, -1 ...},
  * slot_map -1, nothing changed.
  * queue    : int32 [num_pages], a ring of free pages; head: int32 [2] = {first

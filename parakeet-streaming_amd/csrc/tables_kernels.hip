@@ -40,7 +40,7 @@ struct PageK {
   const int32_t* slots;
   const int32_t* lengths;  // or nullptr: chunk each
   int32_t* rows;
-  int32_t* slot_map;
+  int32_t* slot_map;  // or nullptr
   int64_t map_stride;
   int32_t n, S, total, M, page_shift, chunk, rows_stride;
   int32_t window;
@@ -219,7 +219,7 @@ __device__ static inline void step_scan(const PageK& p, uint32_t* lds, uint64_t*
   }
 }
 
-// Rows and slot map of a stream by a group of 32 lanes, an entry a lane: ring entry, or the page
+// Rows, and slot map where it is asked for, of a stream by a group of 32 lanes, an entry a lane: ring entry, or the page
 // from the queue's front where the entry is one that the step takes.
 __device__ static inline void step_rows(const PageK& p, int b, const StepOf s, uint32_t front, int lane) {
   const uint32_t total = (uint32_t)p.total;
@@ -236,6 +236,7 @@ __device__ static inline void step_rows(const PageK& p, int b, const StepOf s, u
     row[i] = v;
     if (i > 0 && d < taken) ring[r] = v;
   }
+  if (!p.slot_map) return;
   int32_t* const map = p.slot_map + b * p.map_stride;
   for (int t = lane; t < p.chunk; t += 32) {
     const uint32_t pos = (uint32_t)s.A + t;
@@ -534,8 +535,8 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
   if (!a->queue || !a->head || !a->appended || !a->ring || !a->slots)
     return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
   if (!a->reset) {
-    if (!a->rows || !a->slot_map) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
-    if (a->rows_stride < 1 + M || a->slot_map_stride < a->chunk)
+    if (!a->rows) return fail(PK_ERR_INVALID, "%s: a tensor pointer is NULL", what);
+    if (a->rows_stride < 1 + M || (a->slot_map && a->slot_map_stride < a->chunk))
       return fail(PK_ERR_INVALID, "%s: need rows_stride >= %d and slot_map_stride >= %d", what, 1 + M, a->chunk);
   }
   const bool two = !a->reset && a->batch > kStepOne;

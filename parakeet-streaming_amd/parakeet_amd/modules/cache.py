@@ -140,7 +140,6 @@ class ModelCache:
         self._slot_index = None if self._prefix else up(self._slots.astype(np.int64))
         self._slots_i32 = up(self._slots.copy())
         self._rows = torch.zeros((n, 1 + self.max_pages), dtype=torch.int32, device=dev)
-        self._places = torch.empty((n, self.chunk), dtype=torch.int32, device=dev) if self.device_pages else None
         self._seen: set[int] = set()
         self._step_open = False
         self._recording = False
@@ -228,7 +227,8 @@ class ModelCache:
         self._step_open = True
 
     def _advance_pages(self) -> None:
-        self.pool.advance(self._slots_i32, rows=self._rows, slot_map=self._places)
+        # whole chunks, appended through the rows: nothing reads a slot map
+        self.pool.advance(self._slots_i32, rows=self._rows, places=False)
 
     def open_recorded_step(self) -> None:
         """Inside :meth:`recording`: the opening of the step as a launch of the recording

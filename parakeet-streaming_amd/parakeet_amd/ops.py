@@ -1159,14 +1159,15 @@ def page_step(
     *,
     rows: torch.Tensor | None = None,
     slot_map: torch.Tensor | None = None,
-) -> tuple[torch.Tensor, torch.Tensor]:
+    places: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Opens one step on a device page pool: stream b appends ``lengths[b]`` frames (int32
     [B], held within 0 .. chunk; None: chunk each) to slot ``slots[b]`` (int32 [B]).
     Pages that slid out of a window go back to the queue, pages for the new frames
     come from it, streams in order, as ``PagePool.advance`` does on the host.  Returns
     (rows [B, 1 + max_pages], slot_map [B, chunk]): the block-table rows that
     :class:`PagedKV` takes, and each new frame's place (page * page_size + row, -1 past
-    a stream's frames) for :func:`kv_append_slots`.  A slot out of range or named
+    a stream's frames) for :func:`kv_append_slots`, or None without ``places``.  A slot out of range or named
     earlier in the call is absent (rows {0, -1 ...}, slot_map -1, nothing changed).
     No host work and no synchronisation: a step may be recorded in a graph."""
     a, dev, M, B = state._args(slots)
@@ -1178,12 +1179,16 @@ def page_step(
         rows = slots.new_empty((B, 1 + M))
     else:
         _require_device(slots, rows)
-    if slot_map is None:
-        slot_map = slots.new_empty((B, T))
-    else:
-        _require_device(slots, slot_map)
     a.rows, a.rows_stride = _i32(rows, "rows", (B, 1 + M)), 1 + M
-    a.slot_map, a.slot_map_stride = _i32(slot_map, "slot_map", (B, T)), T
+    if not places:
+        if slot_map is not None:
+            raise ValueError("slot_map is given for a step without places")
+    else:
+        if slot_map is None:
+            slot_map = slots.new_empty((B, T))
+        else:
+            _require_device(slots, slot_map)
+        a.slot_map, a.slot_map_stride = _i32(slot_map, "slot_map", (B, T)), T
     L = lib()
     n = L.pk_page_step_workspace_bytes(B)
     if n:

@@ -188,9 +188,9 @@ class DevicePagePool:
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
     # -- stepping
-    def advance(self, slots, lengths: torch.Tensor | None = None, rows=None, slot_map=None):
+    def advance(self, slots, lengths: torch.Tensor | None = None, rows=None, slot_map=None, places: bool = True):
         """One step for ``slots`` (in order): ``(rows, slot_map)`` of ``ops.page_step``."""
-        return ops.page_step(self.state, self.slots_tensor(slots), lengths, rows=rows, slot_map=slot_map)
+        return ops.page_step(self.state, self.slots_tensor(slots), lengths, rows=rows, slot_map=slot_map, places=places)
 
     def reset_slot(self, slot: int) -> None:
         self.reset_slots([int(slot)])
