@@ -548,7 +548,7 @@ int page_step(const pk_page_step_args* a, hipStream_t s) {
   k.appended = a->appended;
   k.ring = a->ring;
   k.slots = a->slots;
-  k.lengths = a->lengths;
+  k.lengths = a->reset ? nullptr : a->lengths;  // a reset's may be any address
   k.rows = a->rows;
   k.slot_map = a->slot_map;
   k.map_stride = a->slot_map_stride;

@@ -45,3 +45,20 @@ def test_cache_steps_write_no_places(cuda, monkeypatch):
     kv = torch.zeros(3, 5, 64, dtype=torch.float16, device=cuda)
     cache.update_attn_cache(0, kv, kv)
     assert maps == [None]
+
+
+def test_reset_reads_no_lengths(cuda):
+    """What a caller leaves in the step's other fields changes nothing in a reset."""
+    pools = [DevicePagePool(5, 8, 20, 5, cuda) for _ in range(2)]
+    batch = torch.tensor([3, 1, 4], dtype=torch.int32, device=cuda)
+    for pool in pools:
+        for _ in range(4):
+            pool.advance(batch)
+    gone = torch.tensor([4, 1], dtype=torch.int32, device=cuda)
+    pools[0].reset_slots(gone)
+    a, dev, _, _ = pools[1].state._args(gone)
+    lengths = torch.tensor([5, -7], dtype=torch.int32, device=cuda)
+    a.reset, a.lengths, a.rows_stride, a.slot_map_stride = 1, lengths.data_ptr(), -1, -1
+    _lib.check(_lib.lib().pk_page_step(ctypes.byref(a), ops._stream(dev)), "pk_page_step")
+    _same(*pools)
+    assert pools[1].slot_info(4)[0] == 0 and pools[1].slot_info(3)[0] == 20
