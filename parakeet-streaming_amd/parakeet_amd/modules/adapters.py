@@ -14,6 +14,11 @@ name theirs by number and run together:
 ``EncoderStepGraph(..., adapters=adapters, adapter_ids=ids)`` records the step; the
 streams' numbers are then read from ``ids`` at each replay.  The reference has no
 adapters.
+
+A load or clear is several launches on torch's current stream, into banks that steps read:
+it runs on the steps' stream with no step launched or replayed in between, or is ordered
+before them by events.  While steps of another thread go on, load into a number that
+no stream has, and then give it to the streams.
 """
 
 from __future__ import annotations
@@ -81,20 +86,25 @@ class EncoderAdapters:
     def load(self, i: int, weights: Mapping[str, tuple[Tensor, Tensor]], scale: float = 1.0) -> None:
         """Adapter ``i`` becomes ``weights``: {"layers.<n>.<target>": (A [r', K], B [N, r'])} with
         r' <= rank; projections that it does not name get none.  The values are copied
-        into the banks, which recorded steps read."""
-        i = self._check(i)
-        parts = []
+        into the banks, which recorded steps read, each entry written once."""
+        i, scale = self._check(i), float(scale)
+        parts = {}
         for name, (a, b) in weights.items():
             bank = self._bank(name)
             r, k, n = a.shape[0] if a.dim() == 2 else -1, bank.a.shape[2], bank.b.shape[1]
             if not 0 < r <= self.rank or tuple(a.shape) != (r, k) or tuple(b.shape) != (n, r):
                 raise ValueError(f"{name}: need A [r, {k}] and B [{n}, r] with 0 < r <= {self.rank}, got {tuple(a.shape)} and {tuple(b.shape)}")
-            parts.append((bank, a, b, r))
-        self.clear(i)
-        for bank, a, b, r in parts:
-            bank.a[i, :r].copy_(a)
-            bank.b[i, :, :r].copy_(b)
-            bank.scale[i] = float(scale)
+            parts[id(bank)] = a, b, r
+        for layer in self.banks:
+            for bank in layer.values():
+                a, b, r = parts.get(id(bank), (None, None, 0))
+                if r:
+                    bank.a[i, :r].copy_(a)
+                    bank.b[i, :, :r].copy_(b)
+                if r < self.rank:
+                    bank.a[i, r:].zero_()
+                    bank.b[i, :, r:].zero_()
+                bank.scale[i] = scale if r else 0.0
 
     @torch.no_grad()
     def clear(self, i: int) -> None:
