@@ -103,7 +103,10 @@ class Scheduler:
     # ---------------------------------------------------------- state pool
     def init_state_pool(self, encoder, device: torch.device, dtype: torch.dtype, pool_size: int, **cache_kwargs) -> None:
         """Pool of ``pool_size`` slots; ``cache_kwargs`` (page_size, num_pages,
-        page_order) go to the paged ModelCache."""
+        page_order, device_pages) go to the paged ModelCache.  Acquiring and releasing a
+        slot resets it by launches on the calling thread's current stream, which has to
+        be the steps' stream (or be ordered with it by events); with ``device_pages`` this
+        holds for every slot's pages, not the slot's alone."""
         with self._state_lock:
             self._state_encoder = encoder
             self._state_device = device

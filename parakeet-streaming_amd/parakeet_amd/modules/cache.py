@@ -68,8 +68,11 @@ class ModelCache:
     ``page_order`` (initial free-queue order, default 0..num_pages-1) and
     ``device_pages``: the page pool is kept in device memory
     (:class:`~parakeet_amd.pool.DevicePagePool`, the same rings and rows) and a step opens
-    with one launch, without host page work and upload; ``EncoderStepGraph`` then
-    records it with the step.
+    with a launch (up to 64 streams; two to 3500, four past them), without host page work and
+    upload; ``EncoderStepGraph`` then records it with the step.  The pages of all slots are then
+    handed out in stream order, without a lock: steps, replays, ``reset`` and
+    ``reset_slot``, of whichever slots and from whichever thread, run on one stream or are
+    ordered by events, or two slots could be given the same pages.
     """
 
     def __init__(

@@ -1257,8 +1257,8 @@ class AdapterPlan:
 
 def adapter_plan(ids: torch.Tensor, frames: int = 1, *, num_adapters: int) -> AdapterPlan:
     """Groups the rows of a batch [B, frames, ...] by the streams' adapters ``ids`` (int32
-    [B]; a number outside 0 .. num_adapters - 1 is no adapter).  One launch; the plan
-    serves every layer of the step."""
+    [B]; a number outside 0 .. num_adapters - 1 is no adapter).  One launch, two past 4096
+    rows; the plan serves every layer of the step."""
     if ids.dim() != 1:
         raise ValueError(f"ids must be int32 [B], got {tuple(ids.shape)}")
     B, T, G = ids.shape[0], int(frames), int(num_adapters)

@@ -5,9 +5,9 @@ Replaces the reference's slot pool / dense shift buffers
 (parakeet/engine/scheduler.py:68-104, parakeet/modules/cache.py:8-63): a slot
 owns a ring of ``max_pages`` page ids; each step frees the pages that slid out
 of its window and allocates pages for the new frames.  :class:`PagePool` does that
-on the host, a step's rows are uploaded; :class:`DevicePagePool` does it in one
-launch, so a step needs no host work and can be recorded in a graph, and its
-streams may append fewer frames than a whole chunk.
+on the host, a step's rows are uploaded; :class:`DevicePagePool` does it in launches
+(one up to 64 streams, two to 3500, four past them), so a step needs no host work and can be
+recorded in a graph, and its streams may append fewer frames than a whole chunk.
 """
 
 from __future__ import annotations
