@@ -913,6 +913,19 @@ typedef struct pk_adapter_linear_args {
 int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles);
 int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream);
 
+/* The form that pk_adapter_linear takes for these sizes on a GPU of `cus` CUs (0: the
+ * current device's): one launch for few rows with few adapters, else two, the product with
+ * the weight in tiles of tile_rows x tile_columns, x a^T in `parts` of k.  No GPU is needed;
+ * for tests and for reading profiles. */
+typedef struct pk_adapter_form {
+  int32_t launches;
+  int32_t tile_rows;
+  int32_t tile_columns;
+  int32_t parts;
+} pk_adapter_form;
+int pk_adapter_linear_form(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles, int32_t cus,
+                           pk_adapter_form* form);
+
 /* ---------------------------------------------------------------------------
  * pk_hbm_read_probe -- measurement only; it has no counterpart in the reference.
  * Reads `bytes` (a positive multiple of 16) from the device buffer `src` once,

@@ -1041,19 +1041,24 @@ float form_cost(const Form& f, const FormCost& c, int64_t M, int64_t N, int64_t 
          c.e * runs * (float)steps * (float)per;
 }
 
-template <typename ST, int SILU>
-int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
+// the cheapest form, -1: none
+int product_form(int64_t M, int64_t N, int64_t K, int elem, int r, int parts, int64_t adapters, int cus) {
   int form = -1;
   float cost = 0.f;
-  constexpr int kBuilt = sizeof(ST) == 4 ? sizeof(kCost32) / sizeof(kCost32[0]) : sizeof(kCost16) / sizeof(kCost16[0]);
-  for (int i = 0; i < kBuilt; ++i) {
-    const float c = form_cost(kForms[i], sizeof(ST) == 4 ? kCost32[i] : kCost16[i], k.M, k.N, k.K, sizeof(ST), k.r, k.parts, adapters, cus);
+  const int built = elem == 4 ? sizeof(kCost32) / sizeof(kCost32[0]) : sizeof(kCost16) / sizeof(kCost16[0]);
+  for (int i = 0; i < built; ++i) {
+    const float c = form_cost(kForms[i], elem == 4 ? kCost32[i] : kCost16[i], M, N, K, elem, r, parts, adapters, cus);
     if (c >= 0.f && (form < 0 || c < cost)) {
       form = i;
       cost = c;
     }
   }
-  switch (form) {
+  return form;
+}
+
+template <typename ST, int SILU>
+int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
+  switch (product_form(k.M, k.N, k.K, sizeof(ST), k.r, k.parts, adapters, cus)) {
     case 0: return launch_tile<ST, 16, 16, 1, 1, 4, 128, 4, SILU>(k, s);
     case 1: return launch_tile<ST, 16, 32, 1, 1, 4, 128, 4, SILU>(k, s);
     case 2: return launch_tile<ST, 32, 32, 1, 1, 4, 128, 4, SILU>(k, s);
@@ -1061,8 +1066,9 @@ int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
     case 4: return launch_tile<ST, 64, 64, 2, 2, 2, 64, 4, SILU>(k, s);
     case 5: return launch_tile<ST, 64, 128, 2, 4, 1, 64, 3, SILU>(k, s);
     case 6: return launch_tile<ST, 128, 128, 2, 2, 1, 64, 2, SILU>(k, s);
-    default:
+    case 7:
       if constexpr (sizeof(ST) == 2) return launch_tile<ST, 256, 256, 2, 4, 1, 64, 2, SILU>(k, s);
+    default:
       return fail(PK_ERR_UNSUPPORTED, "pk_adapter_linear: no form for %d -> %d", k.K, k.N);
   }
 }
@@ -1190,6 +1196,24 @@ extern "C" int64_t pk_adapter_workspace_bytes(int32_t dtype, int32_t rows, int32
   if (pk::few_form(rows, n, row, rank, pk::most_adapters(rows, max_tiles), pk::cu_count())) return 0;
   const int parts = pk::k_parts(max_tiles, rank, k);
   return rows * (int64_t)(dtype == PK_DTYPE_F16 ? pk::low_row<_Float16>(rank, parts) : pk::low_row<float>(rank, parts));
+}
+
+extern "C" int pk_adapter_linear_form(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles, int32_t cus,
+                                      pk_adapter_form* form) {
+  pk::clear_error();
+  if (!form || rows <= 0 || n <= 0 || n % 64 != 0 || k <= 0 || k % 64 != 0 || rank <= 0 || max_tiles < 0)
+    return pk::fail(PK_ERR_INVALID, "pk_adapter_linear_form: need form, rows, rank > 0, max_tiles >= 0 and widths of multiples of 64");
+  if (cus <= 0) cus = pk::cu_count();
+  const int elem = dtype == PK_DTYPE_F32 ? 4 : 2;
+  const int64_t adapters = pk::most_adapters(rows, max_tiles);
+  const int few = pk::few_form(rows, n, (int64_t)k * elem, rank, adapters, cus);
+  form->parts = few ? 1 : pk::k_parts(max_tiles, rank, k);
+  const int i = few ? -1 : pk::product_form(rows, n, k, elem, rank, form->parts, adapters, cus);
+  if (!few && i < 0) return pk::fail(PK_ERR_UNSUPPORTED, "pk_adapter_linear_form: no form for %d -> %d", k, n);
+  form->launches = few ? 1 : 2;
+  form->tile_rows = few ? 16 : pk::kForms[i].bm;
+  form->tile_columns = few ? few : pk::kForms[i].bn;
+  return PK_OK;
 }
 
 extern "C" int pk_adapter_linear(const pk_adapter_linear_args* args, void* stream) {

@@ -465,6 +465,10 @@ class AdapterLinearArgs(ctypes.Structure):
     ]
 
 
+class AdapterForm(ctypes.Structure):
+    _fields_ = [("launches", c_int32), ("tile_rows", c_int32), ("tile_columns", c_int32), ("parts", c_int32)]
+
+
 # name -> (restype, argtypes); exactly the functions include/parakeet_paged.h declares
 SIGNATURES = {
     "pk_kv_append": (c_int, [POINTER(KvAppendArgs), c_void_p]),
@@ -489,6 +493,7 @@ SIGNATURES = {
     "pk_adapter_plan_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "pk_adapter_plan": (c_int, [POINTER(AdapterPlanArgs), c_void_p]),
     "pk_adapter_workspace_bytes": (c_int64, [c_int32] * 6),
+    "pk_adapter_linear_form": (c_int, [c_int32] * 7 + [POINTER(AdapterForm)]),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
     "pk_pool_create": (
         c_int,
