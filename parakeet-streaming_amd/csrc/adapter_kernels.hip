@@ -1007,10 +1007,11 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
 // columns for a workgroup alone on its CU, `m` of the latter for each further one beside
 // it (`occ` fit), again a - 2 for each further round, and `e` us for a step of the adapters'
 // part: a run of rows with one adapter in a tile, 16 ranks of it.
-// Fitted to launches in a graph, 1 - 7600 rows (fp32 1800), K and N 512 - 4096, ranks 16
-// and 64, from one adapter to one for every second row: the cheapest by it is the fastest
-// form or within 7%, on the mean 0.2%.  How many adapters the rows have is not known on the
-// host; the plan's tiles bound it.
+// Fitted to launches in a graph, 1 - 8192 rows (fp32 1800), K and N 512 - 4096, ranks 16 to 64,
+// from one adapter to one for every second row.  Of 256 such sizes (fp32 90) the cheapest by it
+// takes 0.4% more than the fastest form on the mean and 11% at the worst in bf16, 0.3% and 8% in
+// fp16, 0.7% and 9% in fp32.  How many adapters the rows have is not known on the host; the
+// plan's tiles bound it.
 struct Form {
   int bm, bn, occ;
   bool staged;
@@ -1020,9 +1021,14 @@ struct FormCost {
 };
 constexpr Form kForms[] = {{16, 16, 4, false}, {16, 32, 3, false}, {32, 32, 2, false},  {32, 64, 2, false},
                            {64, 64, 2, true},  {64, 128, 2, true}, {128, 128, 2, true}, {256, 256, 1, true}};
-constexpr FormCost kCost16[] = {{3.40f, 1.89f, 0.20f, 0.03f},  {3.43f, 2.33f, 0.23f, 0.05f},  {4.15f, 2.69f, 0.36f, 0.06f},
-                                {3.22f, 5.26f, 0.17f, 0.21f},  {3.78f, 4.51f, 0.44f, 0.06f},  {2.57f, 13.12f, 0.15f, 0.13f},
-                                {6.43f, 11.02f, 0.26f, 0.19f}, {9.04f, 20.58f, 0.f, 0.25f}};
+constexpr FormCost kCostBf16[] = {{3.40f, 1.89f, 0.20f, 0.03f},  {3.43f, 2.33f, 0.23f, 0.05f},  {4.15f, 2.69f, 0.36f, 0.06f},
+                                  {3.22f, 5.26f, 0.17f, 0.21f},  {3.78f, 4.51f, 0.44f, 0.06f},  {2.57f, 13.12f, 0.15f, 0.13f},
+                                  {6.43f, 11.02f, 0.26f, 0.19f}, {9.04f, 20.58f, 0.f, 0.25f}};
+// (64 x 128 tiles of fp16 are compiled to a faster loop: 3584 rows 4096 -> 1024, rank 16, 52.5 us, 58.4 in
+// 128 x 128; bf16 62.8 and 58.1)
+constexpr FormCost kCostF16[] = {{3.40f, 1.89f, 0.20f, 0.03f},  {3.43f, 2.33f, 0.23f, 0.05f},  {4.15f, 2.69f, 0.36f, 0.06f},
+                                 {3.00f, 5.26f, 0.17f, 0.21f},  {3.78f, 5.14f, 0.44f, 0.06f},  {2.37f, 10.05f, 0.15f, 0.12f},
+                                 {5.88f, 11.65f, 0.26f, 0.19f}, {9.04f, 20.58f, 0.f, 0.25f}};
 // fp32 (256 x 256 outputs of it do not fit LDS)
 constexpr FormCost kCost32[] = {{3.53f, 4.16f, 0.22f, 0.03f},  {3.75f, 5.68f, 0.20f, 0.05f},  {3.61f, 7.45f, 0.28f, 0.07f},
                                 {2.56f, 15.91f, 0.22f, 0.15f}, {4.95f, 19.60f, 0.53f, 0.15f}, {1.77f, 47.99f, 0.38f, 0.25f},
@@ -1042,12 +1048,14 @@ float form_cost(const Form& f, const FormCost& c, int64_t M, int64_t N, int64_t 
 }
 
 // the cheapest form, -1: none
-int product_form(int64_t M, int64_t N, int64_t K, int elem, int r, int parts, int64_t adapters, int cus) {
+int product_form(int dtype, int64_t M, int64_t N, int64_t K, int r, int parts, int64_t adapters, int cus) {
   int form = -1;
   float cost = 0.f;
-  const int built = elem == 4 ? sizeof(kCost32) / sizeof(kCost32[0]) : sizeof(kCost16) / sizeof(kCost16[0]);
+  const FormCost* const costs = dtype == PK_DTYPE_F32 ? kCost32 : dtype == PK_DTYPE_F16 ? kCostF16 : kCostBf16;
+  const int elem = dtype == PK_DTYPE_F32 ? 4 : 2;
+  const int built = dtype == PK_DTYPE_F32 ? sizeof(kCost32) / sizeof(kCost32[0]) : sizeof(kForms) / sizeof(kForms[0]);
   for (int i = 0; i < built; ++i) {
-    const float c = form_cost(kForms[i], elem == 4 ? kCost32[i] : kCost16[i], M, N, K, elem, r, parts, adapters, cus);
+    const float c = form_cost(kForms[i], costs[i], M, N, K, elem, r, parts, adapters, cus);
     if (c >= 0.f && (form < 0 || c < cost)) {
       form = i;
       cost = c;
@@ -1058,7 +1066,8 @@ int product_form(int64_t M, int64_t N, int64_t K, int elem, int r, int parts, in
 
 template <typename ST, int SILU>
 int launch_product(const AdK<ST>& k, int64_t adapters, int cus, hipStream_t s) {
-  switch (product_form(k.M, k.N, k.K, sizeof(ST), k.r, k.parts, adapters, cus)) {
+  constexpr int dtype = sizeof(ST) == 4 ? PK_DTYPE_F32 : __is_same(ST, bf16_t) ? PK_DTYPE_BF16 : PK_DTYPE_F16;
+  switch (product_form(dtype, k.M, k.N, k.K, k.r, k.parts, adapters, cus)) {
     case 0: return launch_tile<ST, 16, 16, 1, 1, 4, 128, 4, SILU>(k, s);
     case 1: return launch_tile<ST, 16, 32, 1, 1, 4, 128, 4, SILU>(k, s);
     case 2: return launch_tile<ST, 32, 32, 1, 1, 4, 128, 4, SILU>(k, s);
@@ -1208,7 +1217,7 @@ extern "C" int pk_adapter_linear_form(int32_t dtype, int32_t rows, int32_t n, in
   const int64_t adapters = pk::most_adapters(rows, max_tiles);
   const int few = pk::few_form(rows, n, (int64_t)k * elem, rank, adapters, cus);
   form->parts = few ? 1 : pk::k_parts(max_tiles, rank, k);
-  const int i = few ? -1 : pk::product_form(rows, n, k, elem, rank, form->parts, adapters, cus);
+  const int i = few ? -1 : pk::product_form(dtype, rows, n, k, rank, form->parts, adapters, cus);
   if (!few && i < 0) return pk::fail(PK_ERR_UNSUPPORTED, "pk_adapter_linear_form: no form for %d -> %d", k, n);
   form->launches = few ? 1 : 2;
   form->tile_rows = few ? 16 : pk::kForms[i].bm;

@@ -41,7 +41,9 @@ SHAPES = {
         (321, 1, 2048, 1536, 96, 14), (22, 3, 64, 128, 8, 9), (5, 14, 64, 128, 32, 9), (12, 7, 64, 128, 72, 2), (802, 2, 256, 2560, 8, 19),
         (1608, 1, 256, 2560, 40, 7), (803, 2, 256, 2560, 128, 3), (1611, 1, 2048, 1920, 8, 78), (230, 7, 2048, 1920, 48, 9), (541, 3, 2048, 1920, 72, 7),
         (864, 3, 192, 4096, 24, 3), (1034, 2, 192, 4096, 64, 3), (2726, 1, 64, 4096, 128, 5), (1032, 2, 2048, 4096, 24, 32), (147, 14, 2048, 4096, 64, 6),
-        (286, 1, 5120, 3584, 24, 2),
+        (286, 1, 5120, 3584, 24, 2), (1231, 2, 320, 2560, 112, 4), (1834, 2, 128, 4096, 64, 3), (232, 7, 512, 2560, 56, 1), (44, 14, 128, 320, 8, 2),
+        (229, 7, 2048, 2560, 16, 12), (440, 7, 64, 4096, 112, 2), (1538, 2, 192, 4096, 24, 1), (803, 2, 2048, 2560, 40, 13), (232, 7, 2048, 2560, 96, 2),
+        (1628, 1, 512, 2560, 16, 1), (92, 7, 2048, 1536, 72, 3), (1032, 2, 128, 192, 80, 1),
     ],
     "bf16": [
         (6, 3, 512, 64, 24, 3), (17, 1, 512, 64, 8, 8), (2, 14, 1024, 64, 24, 240), (6, 3, 1024, 64, 8, 38), (19, 1, 512, 2560, 32, 3),
