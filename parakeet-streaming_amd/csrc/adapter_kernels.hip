@@ -547,9 +547,9 @@ __device__ static inline void store_out(const AdK<ST>& p, unsigned char* smem, f
 // would save nothing, a wave column or two share it.
 //
 // Bound by the round trips of the K loop: one stage of 64 KB a CU is on its way for the
-// largest tiles, matrix cores busy 28% of the time.  bf16: 3584 rows 1024 -> 4096 in 38.3 us
-// (785 TFLOP/s) without adapters and SiLU, 840 rows 4096 -> 1024 in 21.2 us with 12 adapters
-// of rank 32, 61 rows with an adapter of rank 16 each in 6.2 us.
+// largest tiles, matrix cores busy 29% of the time.  bf16: 3584 rows 1024 -> 4096 in 37.8 us
+// (795 TFLOP/s) without adapters and SiLU, 840 rows 4096 -> 1024 in 20.7 us with 12 adapters
+// of rank 32, 61 rows with an adapter of rank 16 each in 6.5 us.
 // FIT: rows of h in several pieces that have units (fp16).  A form of its own: 3584 rows 1024 ->
 // 4096 of rank 128 take 66 us so and 68 with a branch in the loop of h B^T.
 template <typename ST, int BM, int BN, int WM, int WN, int WK, int BK, int S, int SILU, bool FIT>
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) adapter_tile_kernel(const A
 #pragma unroll
         for (int n = 0; n < TN; ++n) acc[m][n] = MmaA<ST>::step(wf[s][n], xf[s][m], acc[m][n]);
     // One workgroup a CU has no other to fill the matrix cores while it reads LDS: operand
-    // reads one between two matrix instructions (3584 rows 1024 -> 4096: 38.3 us, 42.4 with a
+    // reads one between two matrix instructions (3584 rows 1024 -> 4096: 37.8 us, 42.4 with a
     // step's reads before its products; 128 x 128 tiles gain nothing, 64 x 64 lose 5%).
     if constexpr (BM == 256) {
       __builtin_amdgcn_sched_group_barrier(0x100, TN + 2, 0);
@@ -1008,10 +1008,9 @@ int launch_tile(AdK<ST> k, hipStream_t s) {
 // it (`occ` fit), again a - 2 for each further round, and `e` us for a step of the adapters'
 // part: a run of rows with one adapter in a tile, 16 ranks of it.
 // Fitted to launches in a graph, 1 - 8192 rows (fp32 1800), K and N 512 - 4096, ranks 16 to 64,
-// from one adapter to one for every second row.  Of 256 such sizes (fp32 90) the cheapest by it
-// takes 0.4% more than the fastest form on the mean and 11% at the worst in bf16, 0.3% and 8% in
-// fp16, 0.7% and 9% in fp32.  How many adapters the rows have is not known on the host; the
-// plan's tiles bound it.
+// from one adapter to one for every second row.  Over 256 such sizes of 16-bit types, and 90 of
+// fp32, the cheapest by it takes 0.3 - 0.7% more than the fastest form on the mean and 12% at the
+// worst.  How many adapters the rows have is not known on the host; the plan's tiles bound it.
 struct Form {
   int bm, bn, occ;
   bool staged;

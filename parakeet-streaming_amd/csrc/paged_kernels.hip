@@ -1739,8 +1739,8 @@ struct SlotsK {
 
 // 16 bytes of K and of V a thread, chunks of a row in neighbouring threads; `span` chunks
 // a row of the grid's x, a power of two, so that a thread finds its row without a division.
-// Bound by memory: 32768 rows x 1024 bf16, 268 MB read and written, 63 us (4.3 TB/s; a large
-// copy moves 5.1).  The pages are next read in another step, so they are stored past the
+// Bound by memory: 16384 rows x 1024 bf16, 134 MB read and written, 27 us (4.9 TB/s; a large
+// copy moves 5.1), 32768 rows 62 us (4.3).  The pages are next read in another step, so they are stored past the
 // caches, where their 64-byte rows of a block meet in the last-level one: 16384 rows 28 us
 // so, 33 with cached stores.  Four rows a wave, their loads ahead of the first store: 75 us.
 template <typename ST>
