@@ -15,7 +15,7 @@ import torch
 
 from parakeet_amd.modules.encoder import EncoderStepGraph
 
-from test_gpu_request_tables import T, _adapters, _encoder, _same
+from test_gpu_request_tables import D, T, _adapters, _encoder, _same
 
 pytestmark = pytest.mark.gpu
 
