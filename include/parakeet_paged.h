@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define PK_ABI_VERSION 11
+#define PK_ABI_VERSION 12
 
 enum pk_dtype { PK_DTYPE_F32 = 0, PK_DTYPE_F16 = 1, PK_DTYPE_BF16 = 2 };
 
@@ -872,9 +872,9 @@ int pk_adapter_plan(const pk_adapter_plan_args* args, void* stream);
  * pk_adapter_linear -- a linear layer with each row's low-rank adapter beside it:
  *   out = act(x weight^T + bias + scale[g] (x a[g]^T) b[g]^T), g the row's adapter
  * (rows without one: act(x weight^T + bias)).  fp32 accumulation, one rounding of
- * the output; h = scale[g] x a[g]^T may have any fp32 value and is kept to 2^-16 (bf16) or
- * 2^-22 (fp16, or 2^-36 of the largest entry of its row) of it between the two
- * products.  No counterpart in the reference (the projections are
+ * the output; h = scale[g] x a[g]^T may have any fp32 value and is kept to 2^-16 of it
+ * (bf16; from 2^-110 up) or 2^-22 (fp16; or 2^-36 of the largest entry of its row) between
+ * the two products.  No counterpart in the reference (the projections are
  * parakeet/modules/feedforward.py:20-26, attention.py:92,122).
  * x [rows][k], weight [n][k], out [rows][n]: row strides in elements, rows 16-byte
  * aligned; bias [n] or NULL; a [num_adapters][rank][k], b [num_adapters][n][rank]

@@ -42,7 +42,7 @@ struct MmaA<float> {
 };
 
 // h is kept as two storage-type parts, high + (h - high), so that the rounding of h
-// is 2^-16 (bf16) or 2^-22 (fp16) of it and not 2^-8 or 2^-11: a row of h is [high
+// is 2^-16 (bf16, from 2^-110 up) or 2^-22 (fp16) of it and not 2^-8 or 2^-11: a row of h is [high
 // 0..r-1 | low 0..r-1], r / 4 chunks of 16 bytes, chunk q multiplied with chunk
 // q mod r/8 of a row of B.  For ranks up to 16 both parts are one matrix instruction.
 // fp32: one part, r / 4 chunks.  Where K is split over workgroups (parts > 1) a row of h
