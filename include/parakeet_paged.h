@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define PK_ABI_VERSION 12
+#define PK_ABI_VERSION 13
 
 enum pk_dtype { PK_DTYPE_F32 = 0, PK_DTYPE_F16 = 1, PK_DTYPE_BF16 = 2 };
 
@@ -925,6 +925,215 @@ typedef struct pk_adapter_form {
 } pk_adapter_form;
 int pk_adapter_linear_form(int32_t dtype, int32_t rows, int32_t n, int32_t k, int32_t rank, int32_t max_tiles, int32_t cus,
                            pk_adapter_form* form);
+
+/* ---------------------------------------------------------------------------
+ * pk_page_fork -- streams of a device page pool (pk_page_step_args' queue, head,
+ * appended, ring) continued in other slots: slot dst[i] becomes a copy of slot src[i],
+ * pages of its own.  No counterpart in the reference.
+ * The destinations' pages go to the back of the queue, pair after pair and oldest
+ * first, then pages come from its front for what the sources hold, in the same order;
+ * frame counts and rings follow.  What the pages hold is copied by pk_kv_move_pages
+ * with the list of moves:
+ *   pairs : int32 [batch * M][2] = {page of the source, page of the destination}, one
+ *           after another, {-1, -1} past the last one
+ *   count : int32 [1] = how many
+ * A pair whose slots are out of range, whose destination is a source of the call or was
+ * named as a destination earlier in the call, is absent: nothing of it changes.
+ * left, chunk, page_size, num_pages: the pool's, as in pk_page_step; batch <= num_slots.
+ * workspace: pk_page_fork_workspace_bytes(batch, M), 16-byte aligned (NULL where that is 0).
+ * Ordered with the pool's other calls by the caller.
+ */
+typedef struct pk_page_fork_args {
+  int32_t device;
+  int32_t batch;
+  int32_t num_slots;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t left;
+  int32_t chunk;
+  int32_t* queue;
+  int32_t* head;
+  int64_t* appended;
+  int32_t* ring;
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t* pairs;
+  int32_t* count;
+  void* workspace;
+} pk_page_fork_args;
+int64_t pk_page_fork_workspace_bytes(int32_t batch, int32_t max_pages);
+int pk_page_fork(const pk_page_fork_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_page_compact -- the pages that a device pool's slots hold, N of them, become pages
+ * 0 .. N-1; the free ones, N .. num_pages-1 in this order, are the queue.  No counterpart
+ * in the reference.  Held pages from N on, in ascending order, take the places of the free
+ * ones below N, in ascending order; pairs and count list them (as pk_page_fork's; pairs
+ * int32 [capacity][2], capacity >= min(num_slots * M, num_pages / 2)) for pk_kv_move_pages.
+ * No page is source and destination.  Ring entries outside [0, num_pages) are left alone.
+ * workspace: pk_page_compact_workspace_bytes(num_slots * M, num_pages), 16-byte aligned
+ * (NULL where that is 0).
+ */
+typedef struct pk_page_compact_args {
+  int32_t device;
+  int32_t num_slots;
+  int32_t num_pages;
+  int32_t max_pages; /* M, ring entries of a slot */
+  int32_t* queue;
+  int32_t* head;
+  int32_t* ring;
+  int32_t* pairs;
+  int32_t capacity;
+  int32_t* count;
+  void* workspace;
+} pk_page_compact_args;
+int64_t pk_page_compact_workspace_bytes(int64_t ring_entries, int32_t num_pages);
+int pk_page_compact(const pk_page_compact_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_kv_move_pages -- K and V of every layer copied from page to page: the first *count
+ * pairs {from, to} of `pairs` (at most capacity); a pair with a page outside
+ * [0, num_pages) is skipped.  No page is both read and written, or written twice, in one call.
+ * pages: rows is not read.  page_size * d_model elements a multiple of 16 bytes.
+ */
+typedef struct pk_kv_move_pages_args {
+  int32_t dtype;
+  int32_t device;
+  pk_paged_layout pages;
+  const int32_t* pairs;
+  int32_t capacity;
+  const int32_t* count;
+} pk_kv_move_pages_args;
+int pk_kv_move_pages(const pk_kv_move_pages_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_qk_norm_append -- new tokens of a decoder layer: each head's query and key divided
+ * by its root mean square, rotated to its token's position, the query to `out`, key and value to
+ * their places in the pages.  No counterpart in the reference.
+ *   y = x / sqrt(mean(x^2) + eps) * weight     over the head_dim columns of a head
+ *   (y[a], y[b]) -> (y[a] cos f - y[b] sin f, y[b] cos f + y[a] sin f), f = position * inv_freq[i]
+ * for i < rotary / 2 with (a, b) = (i, i + rotary / 2), or (2 i, 2 i + 1) where `interleaved`;
+ * columns from `rotary` on are not turned.  fp32 arithmetic, one rounding; the turns of an
+ * angle in 64 bits, so that far positions keep fp32's precision.
+ * query, out: [batch][chunk][num_heads * head_dim]; key, value: [batch][chunk][d_model] with
+ * d_model a multiple of head_dim; element strides (b, t), rows 16-byte aligned with unit
+ * inner stride; out may be query.  q_weight, k_weight: [head_dim], NULL: no norm.
+ * inv_freq: double [rotary / 2].  positions: int32 [batch][chunk] (stride_b), NULL: frame t of
+ * stream b is at rows[b][0] + t.  slot_map: pk_page_step's, as pk_kv_append_slots reads it
+ * (entries below 0 or past the layer's pages: key and value are not read).
+ * head_dim 64 or 128; rotary 0 or a power of two from 16 to head_dim.
+ */
+typedef struct pk_qk_norm_append_args {
+  int32_t dtype;
+  int32_t device;
+  pk_paged_layout pages;
+  int32_t layer;
+  int32_t batch;
+  int32_t chunk;
+  int32_t num_heads;
+  int32_t head_dim;
+  int32_t rotary;
+  int32_t interleaved;
+  float eps;
+  const void* query;
+  int64_t query_stride_b;
+  int64_t query_stride_t;
+  const void* key;
+  int64_t key_stride_b;
+  int64_t key_stride_t;
+  const void* value;
+  int64_t value_stride_b;
+  int64_t value_stride_t;
+  const void* q_weight;
+  const void* k_weight;
+  const double* inv_freq;
+  const int32_t* positions;
+  int64_t positions_stride_b;
+  const int32_t* slot_map;
+  int64_t slot_map_stride_b;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_t;
+} pk_qk_norm_append_args;
+int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_chunk_attn -- attention of each stream's new tokens over its paged cache, which
+ * holds them already (pk_qk_norm_append, pk_kv_append_slots, pk_kv_append).  No counterpart in
+ * the reference, whose attention is pk_paged_relpos_attn's.
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j   over positions j in [A + i - left, A + i], j >= 0
+ * for token i < lengths[b] of stream b (held within 0 .. chunk; NULL: chunk), A = rows[b][0]; zeros for i >=
+ * lengths[b] and where no key is there (ring entries outside [0, num_pages) are not).
+ * Query head h reads key head h / (num_heads / kv_heads), kv_heads = d_model / head_dim.  fp32
+ * accumulation and softmax.  What a token gets depends on the keys and values that it sees
+ * alone, also where others are infinite or NaN.
+ * query, out: [batch][chunk][num_heads * head_dim]; element strides (b, t), rows 16-byte aligned
+ * with unit inner stride; out may be query, and overlaps nothing else.  scale: > 0 and finite.  head_dim 64 or
+ * 128.  pages.max_pages holds any window of left + chunk positions: (left + chunk + page_size - 2) /
+ * page_size + 1 <= max_pages.  lengths: int32 [batch].
+ * workspace: pk_attn_workspace_bytes(dtype, batch, chunk, num_heads, kv_heads, head_dim,
+ * left + chunk) on the call's device, 16-byte aligned (NULL where that is 0).
+ */
+typedef struct pk_chunk_attn_args {
+  int32_t dtype;
+  int32_t device;
+  pk_paged_layout pages;
+  int32_t layer;
+  int32_t batch;
+  int32_t chunk;
+  int32_t num_heads;
+  int32_t head_dim;
+  int32_t left;
+  float scale;
+  const void* query;
+  int64_t query_stride_b;
+  int64_t query_stride_t;
+  const int32_t* lengths;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_t;
+  void* workspace;
+} pk_chunk_attn_args;
+int64_t pk_attn_workspace_bytes(int32_t dtype, int32_t batch, int32_t chunk, int32_t num_heads, int32_t kv_heads,
+                                int32_t head_dim, int32_t keys);
+int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * pk_cross_attn -- attention of each stream's tokens to states of another length, as a
+ * decoder reads the encoder's:
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j   over j in [0, lengths[b])
+ * (lengths int32 [batch], held within 0 .. states; NULL: states); zeros where that is empty.  Rows of key
+ * and value from lengths[b] on are not read.  No counterpart in the reference.
+ * query, out: [batch][chunk][num_heads * head_dim]; key, value: [batch][states][kv_heads * head_dim];
+ * element strides (b, t) >= 0 (0: one stream's states for all), rows 16-byte aligned with unit inner stride; out may be
+ * query, and overlaps nothing else.  Heads, types, scale and workspace as pk_chunk_attn's, with states keys.
+ */
+typedef struct pk_cross_attn_args {
+  int32_t dtype;
+  int32_t device;
+  int32_t batch;
+  int32_t chunk;
+  int32_t states;
+  int32_t num_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  float scale;
+  const void* query;
+  int64_t query_stride_b;
+  int64_t query_stride_t;
+  const void* key;
+  int64_t key_stride_b;
+  int64_t key_stride_t;
+  const void* value;
+  int64_t value_stride_b;
+  int64_t value_stride_t;
+  const int32_t* lengths;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_t;
+  void* workspace;
+} pk_cross_attn_args;
+int pk_cross_attn(const pk_cross_attn_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
  * pk_hbm_read_probe -- measurement only; it has no counterpart in the reference.

@@ -11,6 +11,7 @@
 
 #include "pk_common.h"
 #include "pk_device.h"
+#include "pk_scan.h"
 
 namespace pk {
 
@@ -50,37 +51,6 @@ struct PageK {
   uint2* part;  // more than kStepTwo: [n] pages given back and taken
   uint2* sum;   // and of each 256 streams, then of those before them
 };
-
-// inclusive sum over the 64 lanes of a wave
-template <typename T>
-__device__ static inline T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-
-// exclusive sum over a workgroup of NW waves; `sum`: of all
-template <int NW, typename T>
-__device__ static inline T block_scan(T v, T* lds, T& sum) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const T inc = wave_scan(v);
-  if (lane == 63) lds[wave] = inc;
-  __syncthreads();
-  T before = 0;
-  sum = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const T x = lds[w];
-    if (w < wave) before += x;
-    sum += x;
-  }
-  __syncthreads();
-  return before + inc - v;
-}
 
 constexpr int kStepThreads = 1024;
 // Streams of a step in one launch (64 take 8.0 us in a graph so and 8.8 in two, 128 12 and
@@ -507,12 +477,6 @@ __global__ void __launch_bounds__(256) adapter_rows_kernel(const PlanK p) {
 }
 
 namespace {
-
-int log2_of(int32_t x) {
-  for (int s = 0; s < 31; ++s)
-    if ((int32_t{1} << s) == x) return s;
-  return -1;
-}
 
 int page_step(const pk_page_step_args* a, hipStream_t s) {
   const char* what = "pk_page_step";

@@ -9,13 +9,13 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 LIB_NAME = "libparakeet_paged.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -469,6 +469,140 @@ class AdapterForm(ctypes.Structure):
     _fields_ = [("launches", c_int32), ("tile_rows", c_int32), ("tile_columns", c_int32), ("parts", c_int32)]
 
 
+class PageForkArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", c_int32),
+        ("batch", c_int32),
+        ("num_slots", c_int32),
+        ("num_pages", c_int32),
+        ("page_size", c_int32),
+        ("left", c_int32),
+        ("chunk", c_int32),
+        ("queue", c_void_p),
+        ("head", c_void_p),
+        ("appended", c_void_p),
+        ("ring", c_void_p),
+        ("src", c_void_p),
+        ("dst", c_void_p),
+        ("pairs", c_void_p),
+        ("count", c_void_p),
+        ("workspace", c_void_p),
+    ]
+
+
+class PageCompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", c_int32),
+        ("num_slots", c_int32),
+        ("num_pages", c_int32),
+        ("max_pages", c_int32),
+        ("queue", c_void_p),
+        ("head", c_void_p),
+        ("ring", c_void_p),
+        ("pairs", c_void_p),
+        ("capacity", c_int32),
+        ("count", c_void_p),
+        ("workspace", c_void_p),
+    ]
+
+
+class KvMovePagesArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("pages", PagedLayout),
+        ("pairs", c_void_p),
+        ("capacity", c_int32),
+        ("count", c_void_p),
+    ]
+
+
+class QkNormAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("pages", PagedLayout),
+        ("layer", c_int32),
+        ("batch", c_int32),
+        ("chunk", c_int32),
+        ("num_heads", c_int32),
+        ("head_dim", c_int32),
+        ("rotary", c_int32),
+        ("interleaved", c_int32),
+        ("eps", c_float),
+        ("query", c_void_p),
+        ("query_stride_b", c_int64),
+        ("query_stride_t", c_int64),
+        ("key", c_void_p),
+        ("key_stride_b", c_int64),
+        ("key_stride_t", c_int64),
+        ("value", c_void_p),
+        ("value_stride_b", c_int64),
+        ("value_stride_t", c_int64),
+        ("q_weight", c_void_p),
+        ("k_weight", c_void_p),
+        ("inv_freq", c_void_p),
+        ("positions", c_void_p),
+        ("positions_stride_b", c_int64),
+        ("slot_map", c_void_p),
+        ("slot_map_stride_b", c_int64),
+        ("out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_t", c_int64),
+    ]
+
+
+class ChunkAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("pages", PagedLayout),
+        ("layer", c_int32),
+        ("batch", c_int32),
+        ("chunk", c_int32),
+        ("num_heads", c_int32),
+        ("head_dim", c_int32),
+        ("left", c_int32),
+        ("scale", c_float),
+        ("query", c_void_p),
+        ("query_stride_b", c_int64),
+        ("query_stride_t", c_int64),
+        ("lengths", c_void_p),
+        ("out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_t", c_int64),
+        ("workspace", c_void_p),
+    ]
+
+
+class CrossAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("device", c_int32),
+        ("batch", c_int32),
+        ("chunk", c_int32),
+        ("states", c_int32),
+        ("num_heads", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("scale", c_float),
+        ("query", c_void_p),
+        ("query_stride_b", c_int64),
+        ("query_stride_t", c_int64),
+        ("key", c_void_p),
+        ("key_stride_b", c_int64),
+        ("key_stride_t", c_int64),
+        ("value", c_void_p),
+        ("value_stride_b", c_int64),
+        ("value_stride_t", c_int64),
+        ("lengths", c_void_p),
+        ("out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_t", c_int64),
+        ("workspace", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); exactly the functions include/parakeet_paged.h declares
 SIGNATURES = {
     "pk_kv_append": (c_int, [POINTER(KvAppendArgs), c_void_p]),
@@ -495,6 +629,15 @@ SIGNATURES = {
     "pk_adapter_workspace_bytes": (c_int64, [c_int32] * 6),
     "pk_adapter_linear_form": (c_int, [c_int32] * 7 + [POINTER(AdapterForm)]),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
+    "pk_page_fork_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pk_page_fork": (c_int, [POINTER(PageForkArgs), c_void_p]),
+    "pk_page_compact_workspace_bytes": (c_int64, [c_int64, c_int32]),
+    "pk_page_compact": (c_int, [POINTER(PageCompactArgs), c_void_p]),
+    "pk_kv_move_pages": (c_int, [POINTER(KvMovePagesArgs), c_void_p]),
+    "pk_qk_norm_append": (c_int, [POINTER(QkNormAppendArgs), c_void_p]),
+    "pk_attn_workspace_bytes": (c_int64, [c_int32] * 7),
+    "pk_chunk_attn": (c_int, [POINTER(ChunkAttnArgs), c_void_p]),
+    "pk_cross_attn": (c_int, [POINTER(CrossAttnArgs), c_void_p]),
     "pk_pool_create": (
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32, POINTER(c_int32), POINTER(c_void_p)],

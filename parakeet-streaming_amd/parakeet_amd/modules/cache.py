@@ -126,6 +126,7 @@ class ModelCache:
         )
         self._base = self
         self._staging = None
+        self._moved = 0  # times that pages were moved (of the base): rows from before are stale
         self._set_slots(np.arange(batch_size, dtype=np.int32))
 
     # ------------------------------------------------------------------ views
@@ -145,6 +146,7 @@ class ModelCache:
         self._rows = torch.zeros((n, 1 + self.max_pages), dtype=torch.int32, device=dev)
         self._seen: set[int] = set()
         self._step_open = False
+        self._rows_moved = 0  # base._moved when the rows were made
         self._recording = False
 
     def _derive(self, slots: np.ndarray) -> "ModelCache":
@@ -213,10 +215,16 @@ class ModelCache:
                     f"{self.num_layers}; every layer must be updated once per step"
                 )
             self._open_step()
+        self._check_rows()
         self._seen.add(layer_idx)
+
+    def _check_rows(self) -> None:
+        if self._rows_moved != self._base._moved:
+            raise RuntimeError("paged cache: pages were moved (fork or compact) since this step was opened")
 
     def _open_step(self) -> None:
         base = self._base
+        self._rows_moved = base._moved
         if self.device_pages:
             self._advance_pages()
         elif self._rows.device.type == "cuda":
@@ -264,7 +272,7 @@ class ModelCache:
         else:
             self.open_step()
         yield
-        self._step_open, self._seen = True, set(range(self.num_layers))
+        self._step_open, self._seen, self._rows_moved = True, set(range(self.num_layers)), self._base._moved
 
     @contextmanager
     def recording(self):
@@ -342,6 +350,7 @@ class ModelCache:
         """Dense window of the last opened step (K, V) [B, L, D], for inspection."""
         if not self._step_open:
             raise RuntimeError("no step has been opened on this cache view")
+        self._check_rows()
         return ops.kv_gather(self.paged(), layer_idx, self.batch_size, self.attn_cache_len, self.chunk)
 
     # ------------------------------------------------------------------- conv
@@ -425,6 +434,38 @@ class ModelCache:
             x, branch, norm, weight, bias, dw_weight, dw_bias, self.conv_frames, layer_idx,
             None if self._prefix else self._slots_i32, pad_mask,
         )
+
+    # ------------------------------------------------------- streams and pages moved
+    def fork(self, src, dst) -> None:
+        """Rows ``dst`` continue the streams of rows ``src`` too (lists of equal length, no row in
+        both): their windows and conv states are copies from here on (``ops.page_fork``), what
+        rows ``dst`` held is gone.  Between steps, on the stream of the steps; ``device_pages`` only."""
+        s, d = self._pool_rows(src), self._pool_rows(dst)
+        moves = self.pool.fork(s, d)
+        ops.kv_move_pages(self.k_pages, self.v_pages, moves)
+        if len(d):
+            s, d = (torch.from_numpy(x.astype(np.int64)) for x in (s, d))
+            self.conv_frames[d.to(self.conv_frames.device)] = self.conv_frames[s.to(self.conv_frames.device)]
+        self._base._moved += 1
+
+    def compact(self) -> None:
+        """Moves the pages that all slots hold together, to the front of the pool (``ops.page_compact``):
+        what the streams see stays the same.  Between steps, on the stream of the steps; ``device_pages`` only."""
+        self._pool_rows([])
+        ops.kv_move_pages(self.k_pages, self.v_pages, self.pool.compact())
+        self._base._moved += 1
+
+    def _pool_rows(self, rows) -> np.ndarray:
+        """The slots of rows of this view, between two steps."""
+        if not self.device_pages:
+            raise RuntimeError("paged cache: fork and compact need device_pages")
+        if self._recording:
+            raise RuntimeError("paged cache: fork and compact are not recorded")
+        self._check_whole()
+        rows = np.asarray(rows, dtype=np.int64).reshape(-1)
+        if len(rows) and (rows.min() < 0 or rows.max() >= len(self._slots)):
+            raise ValueError(f"rows must be in [0, {len(self._slots)})")
+        return self._slots[rows]
 
     # ------------------------------------------------------------------ reset
     def reset(self) -> None:

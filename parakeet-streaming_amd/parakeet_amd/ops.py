@@ -18,15 +18,21 @@ from ._lib import (
     AdapterLinearArgs,
     AdapterPlanArgs,
     AttnArgs,
+    ChunkAttnArgs,
     ConvArgs,
+    CrossAttnArgs,
     FeArgs,
     KvAppendArgs,
     KvAppendSlotsArgs,
     KvGatherArgs,
+    KvMovePagesArgs,
     LinearArgs,
     MaskArgs,
+    PageCompactArgs,
     PagedLayout,
+    PageForkArgs,
     PageStepArgs,
+    QkNormAppendArgs,
     ResNormArgs,
     SubArgs,
     check,
@@ -1239,6 +1245,83 @@ def kv_append_slots(pages: PagedKV, layer: int, key: torch.Tensor, value: torch.
     check(lib().pk_kv_append_slots(ctypes.byref(a), _stream(dev)), "pk_kv_append_slots")
 
 
+@dataclass
+class PageMoves:
+    """Copies from page to page that a fork or a compaction asks for (:func:`kv_move_pages`):
+    ``pairs`` int32 [n, 2] = {from, to}, the first ``count`` (int32 [1]) of them."""
+
+    pairs: torch.Tensor
+    count: torch.Tensor
+
+
+def page_fork(state: PageState, src: torch.Tensor, dst: torch.Tensor) -> PageMoves:
+    """Continues the streams of slots ``src`` (int32 [n]) in slots ``dst`` (int32 [n]) too: each
+    destination gives its pages back, takes as many as its source holds, and has its frame
+    count from then on.  Returns the moves that copy what the pages hold; until
+    :func:`kv_move_pages` has run them, for every pool that these tables serve, the new
+    pages hold old frames.  A source may be forked several times.  A pair is absent (nothing
+    of it changes) where a slot is out of range or the destination is a source of the call
+    or was named before in it.  No host work and no synchronisation."""
+    n = dst.numel()
+    a, dev, M, _ = state._args(dst)
+    if n > a.num_slots:
+        raise ValueError(f"{n} pairs for {a.num_slots} slots")
+    f = PageForkArgs()
+    f.device, f.batch, f.num_slots, f.num_pages, f.page_size, f.left, f.chunk = a.device, n, a.num_slots, a.num_pages, a.page_size, a.left, a.chunk
+    f.queue, f.head, f.appended, f.ring, f.dst = a.queue, a.head, a.appended, a.ring, a.slots
+    f.src = _i32(src, "src", (n,))
+    _require_device(dst, src)
+    moves = PageMoves(dst.new_empty((n * M, 2)), dst.new_empty(1))
+    f.pairs, f.count = moves.pairs.data_ptr(), moves.count.data_ptr()
+    L = lib()
+    space = L.pk_page_fork_workspace_bytes(n, M)
+    if space:
+        space = torch.empty(space, dtype=torch.uint8, device=dev)
+        f.workspace = space.data_ptr()
+    check(L.pk_page_fork(ctypes.byref(f), _stream(dev)), "pk_page_fork")
+    return moves
+
+
+def page_compact(state: PageState) -> PageMoves:
+    """Moves the pages that the slots hold, N of them, together: they become pages 0 .. N - 1, the
+    free ones N .. num_pages - 1, queued in this order.  Held pages from N on take the free places
+    below it, both in ascending order; the returned moves copy what they hold, by
+    :func:`kv_move_pages` for every pool that these tables serve, before anything reads or appends.
+    Block-table rows of earlier steps are stale afterwards.  No host work and no synchronisation."""
+    a, dev, M, _ = state._args(state.head[:0])
+    total, S = a.num_pages, a.num_slots
+    room = min(S * M, total // 2)
+    moves = PageMoves(state.ring.new_empty((room, 2)), state.ring.new_empty(1))
+    c = PageCompactArgs()
+    c.device, c.num_slots, c.num_pages, c.max_pages, c.capacity = a.device, S, total, M, room
+    c.queue, c.head, c.ring, c.pairs, c.count = a.queue, a.head, a.ring, moves.pairs.data_ptr(), moves.count.data_ptr()
+    L = lib()
+    space = L.pk_page_compact_workspace_bytes(S * M, total)
+    if space:
+        space = torch.empty(space, dtype=torch.uint8, device=dev)
+        c.workspace = space.data_ptr()
+    check(L.pk_page_compact(ctypes.byref(c), _stream(dev)), "pk_page_compact")
+    return moves
+
+
+def kv_move_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves: PageMoves) -> None:
+    """Copies whole pages of all layers of the pools [Ly, num_pages, P, D], as ``moves`` (of
+    :func:`page_fork` or :func:`page_compact`) says; pairs of pages out of range are skipped.  No
+    page is both read and written, or written twice, in one call."""
+    pairs, count = moves.pairs, moves.count
+    n = pairs.shape[0] if pairs.dim() == 2 else -1
+    a = KvMovePagesArgs()
+    a.pairs, a.count, a.capacity = _i32(pairs, "moves.pairs", (n, 2)), _i32(count, "moves.count", (1,)), n
+    dev = _require_device(k_pool, v_pool, pairs, count)
+    if k_pool.shape != v_pool.shape or k_pool.dim() != 4 or k_pool.dtype != v_pool.dtype or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("k_pool and v_pool must be matching contiguous [Ly, num_pages, P, D] tensors")
+    a.dtype, a.device = dtype_code(k_pool.dtype), _index(dev)
+    L = a.pages
+    L.k_pool, L.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
+    L.num_layers, L.num_pages, L.page_size, L.d_model = k_pool.shape
+    check(lib().pk_kv_move_pages(ctypes.byref(a), _stream(dev)), "pk_kv_move_pages")
+
+
 # ---------------------------------------------------------------------------
 # low-rank adapters
 
@@ -1424,3 +1507,260 @@ def _refuse_adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     _i32(plan.ids, "plan.ids", (M,))
     _i32(plan.tiles, "plan.tiles", (plan.tiles.shape[0] if plan.tiles.dim() else 0, 4))
     raise ValueError(f"adapter_linear does not take x {tuple(x.shape)}, weight {tuple(weight.shape)} with strides {weight.stride()}")
+
+
+# ---------------------------------------------------------------------------
+# a text decoder's attention
+
+
+def _plain_call(what: str, tensors: list[torch.Tensor]) -> None:
+    """Refuses calls that something follows or rewrites, and such that need a gradient."""
+    if _overridden(*tensors) or _forward_ad._current_level >= 0 or _tracing() or torch.is_autocast_enabled() or _dispatch_modes():
+        _refuse_transforms(what, tensors)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
+
+
+def _head_rows(name: str, t: torch.Tensor, B: int, T: int, dtype: torch.dtype, heads: int | None = None) -> None:
+    """t is [B, T, whole heads] of dtype with 16-byte aligned rows."""
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != T or (heads is not None and t.shape[2] != heads):
+        raise ValueError(f"{name}: expected shape {(B, T, 'D' if heads is None else heads)}, got {tuple(t.shape)}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: dtype {t.dtype} != {dtype}")
+    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or (t.stride(0) | t.stride(1)) * t.element_size() % 16):
+        raise ValueError(f"{name}: rows must be contiguous and 16-byte aligned, got strides {t.stride()}")
+
+
+def _head_dim(query: torch.Tensor, num_heads: int) -> int:
+    """Columns of a head of query [B, T, num_heads * head_dim]."""
+    H = int(num_heads)
+    if query.dim() != 3 or H <= 0 or query.shape[2] % H:
+        raise ValueError(f"query must be [B, T, {H} heads], got {tuple(query.shape)}")
+    hd = query.shape[2] // H
+    if hd not in (64, 128):
+        raise NotImplementedError(f"built for heads of 64 and 128 columns, got {hd}")
+    return hd
+
+
+def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """:func:`_overlap`, but not for rows that are different columns of the same wider rows (the
+    query, key and value of one projection)."""
+    if not _overlap(a, b):
+        return False
+    if a.dim() == b.dim() == 3 and a.stride() == b.stride() and a.element_size() == b.element_size():
+        width = a.stride(1)
+        if width > 0 and (a.stride(0) % width == 0 or a.shape[0] == b.shape[0] == 1):
+            apart = b.data_ptr() - a.data_ptr()
+            at, rest = apart // a.element_size() % width, apart % a.element_size()
+            if rest == 0 and a.shape[2] <= at and at + b.shape[2] <= width:
+                return False
+    return True
+
+
+def _head_out(out: torch.Tensor | None, query: torch.Tensor, dev: torch.device, operands) -> torch.Tensor:
+    """The output [B, T, D] of a call: a new tensor, or ``out``, which may be query and meets nothing else."""
+    B, T, D = query.shape
+    if out is None:
+        return torch.empty((B, T, D), dtype=query.dtype, device=dev)
+    _head_rows("out", out, B, T, query.dtype, D)
+    if out.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} and {out.device}")
+    if (out.stride(1) < D and T > 1) or (B > 1 and out.stride(0) < D):
+        raise ValueError(f"out: rows overlap, strides {out.stride()}")
+    same = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+    if any(_rows_meet(out, t) for t in operands) or (not same and _rows_meet(out, query)):
+        raise ValueError("out must not overlap an operand, unless it is query itself")
+    return out
+
+
+def qk_norm_append(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    pages: PagedKV,
+    layer: int,
+    slot_map: torch.Tensor,
+    *,
+    num_heads: int,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    inv_freq: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """New tokens of a decoder layer, in one launch: every head's query and key divided by its
+    root mean square and multiplied with ``q_weight`` / ``k_weight`` [head_dim] (None: no norm),
+    rotated to its token's position, keys and values written to the places in ``layer``'s
+    pages that ``slot_map`` (int32 [B, T], :func:`page_step`'s) names.  Returns the queries
+    [B, T, num_heads * head_dim]; ``out`` may be ``query``.
+
+    query [B, T, num_heads * head_dim], key/value [B, T, D] with D the pages' columns, whole heads
+    (views of one projection are fine); heads of 64 or 128 columns.  ``inv_freq``: float64
+    [rotary / 2], the angle that a position adds to a pair of columns (None: no rotation;
+    rotary a power of two from 16 to head_dim, columns past it are not turned); pairs are (i, i +
+    rotary / 2), or (2 i, 2 i + 1) where ``interleaved``.  ``positions``: int32 [B, T]; None: token t of stream b is
+    at ``pages.rows[b, 0] + t``.  The turns of an angle are made in 64 bits.  No gradients."""
+    operands = [t for t in (query, key, value, q_weight, k_weight, inv_freq) if t is not None]
+    _plain_call("qk_norm_append", operands)
+    hd, kp, dt = _head_dim(query, num_heads), pages.k_pool, query.dtype
+    B, T, _ = query.shape
+    D = kp.shape[-1]
+    if D % hd:
+        raise ValueError(f"pages of {D} columns are not whole heads of {hd}")
+    if kp.dtype is not dt:
+        raise TypeError(f"pages dtype {kp.dtype} != {dt}")
+    _head_rows("query", query, B, T, dt)
+    _head_rows("key", key, B, T, dt, D)
+    _head_rows("value", value, B, T, dt, D)
+    dev = _require_device(query, key, value, kp, pages.v_pool, pages.rows, slot_map)
+    a = QkNormAppendArgs()
+    a.pages = pages.layout()
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if w.shape != (hd,) or w.dtype is not dt or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
+                raise ValueError(f"{name} must be contiguous, 16-byte aligned [{hd}] of {dt} on {dev}, got {tuple(w.shape)} {w.dtype}")
+            setattr(a, name, w.data_ptr())
+    if inv_freq is not None:
+        n = 2 * inv_freq.numel()
+        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != dev:
+            raise ValueError(f"inv_freq must be contiguous float64 [rotary / 2] on {dev}, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+        if n < 16 or n > hd or n & (n - 1):
+            raise NotImplementedError(f"built for rotations of 16 to {hd} columns, a power of two, got {n}")
+        a.rotary, a.inv_freq = n, inv_freq.data_ptr()
+        if positions is None and pages.rows.shape[0] < B:
+            raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
+    for name, t in (("slot_map", slot_map), ("positions", positions)):
+        if t is not None:
+            if t.dtype is not _INT32 or t.shape != (B, T) or (t.numel() and t.stride(1) != 1) or t.device != dev:
+                raise ValueError(f"{name} must be int32 {[B, T]} with unit inner stride on {dev}, got {tuple(t.shape)} {t.dtype}")
+    if not eps >= 0 or eps == math.inf:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    out = _head_out(out, query, dev, [key, value, kp, pages.v_pool])
+    if B == 0 or T == 0:
+        return out
+    a.dtype, a.device, a.layer, a.batch, a.chunk, a.num_heads, a.head_dim = dtype_code(dt), _index(dev), int(layer), B, T, int(num_heads), hd
+    a.interleaved, a.eps = int(bool(interleaved)), float(eps)
+    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    a.query_stride_b, a.query_stride_t, _ = query.stride()
+    a.key_stride_b, a.key_stride_t, _ = key.stride()
+    a.value_stride_b, a.value_stride_t, _ = value.stride()
+    a.out_stride_b, a.out_stride_t, _ = out.stride()
+    a.slot_map, a.slot_map_stride_b = slot_map.data_ptr(), slot_map.stride(0)
+    if positions is not None:
+        a.positions, a.positions_stride_b = positions.data_ptr(), positions.stride(0)
+    check(lib().pk_qk_norm_append(ctypes.byref(a), _stream(dev)), "pk_qk_norm_append")
+    return out
+
+
+def _attend(a, query: torch.Tensor, out: torch.Tensor, B: int, T: int, H: int, Hkv: int, hd: int, keys: int, scale: float | None,
+            lengths: torch.Tensor | None, dev: torch.device):
+    """What both attentions put into their arguments; returns the workspace, to be kept until the launch."""
+    if H % Hkv:
+        raise ValueError(f"{H} query heads are not whole groups over {Hkv} key heads")
+    if scale is None:
+        scale = hd**-0.5
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be > 0 and finite, got {scale}")
+    if lengths is not None:
+        a.lengths = _i32(lengths, "lengths", (B,))
+        _require_device(query, lengths)
+    a.dtype, a.device, a.batch, a.chunk, a.num_heads, a.head_dim, a.scale = dtype_code(query.dtype), _index(dev), B, T, H, hd, scale
+    a.query, a.out = query.data_ptr(), out.data_ptr()
+    a.query_stride_b, a.query_stride_t, _ = query.stride()
+    a.out_stride_b, a.out_stride_t, _ = out.stride()
+    n = lib().pk_attn_workspace_bytes(a.dtype, B, T, H, Hkv, hd, keys)
+    if n:
+        space = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace = space.data_ptr()
+        return space
+    return None
+
+
+def chunk_attn(
+    query: torch.Tensor,
+    pages: PagedKV,
+    layer: int,
+    *,
+    num_heads: int,
+    lengths: torch.Tensor | None = None,
+    left: int | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each stream's new tokens over its paged cache, which holds them already
+    (:func:`qk_norm_append` or :func:`kv_append_slots` of this step): token i of stream b, at position
+    ``rows[b, 0] + i``, sees itself and the ``left`` positions before it (None: the most that
+    the ring holds for any alignment).  query [B, T, num_heads * head_dim], heads of 64 or 128 columns; the
+    pages' D columns are D / head_dim key heads, each read by num_heads * head_dim / D query heads.
+    ``lengths``: int32 [B], new tokens of each stream (held within 0 .. T; None: T).  Returns [B, T,
+    num_heads * head_dim]: zeros past a stream's tokens and where no key is there; ``out`` may be ``query``.  ``scale``: None is
+    head_dim ** -0.5.  fp32 accumulation and softmax.  What a token gets depends on the keys and values that
+    it sees alone.  No gradients."""
+    _plain_call("chunk_attn", [query])
+    hd, kp, dt = _head_dim(query, num_heads), pages.k_pool, query.dtype
+    B, T, _ = query.shape
+    a = ChunkAttnArgs()
+    a.pages = pages.layout()
+    P, D = kp.shape[2:]
+    if D % hd or D == 0:
+        raise ValueError(f"pages of {D} columns are not whole heads of {hd}")
+    if kp.dtype is not dt:
+        raise TypeError(f"pages dtype {kp.dtype} != {dt}")
+    _head_rows("query", query, B, T, dt)
+    dev = _require_device(query, kp, pages.v_pool, pages.rows)
+    if pages.rows.shape[0] < B:
+        raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
+    most = (pages.max_pages - 1) * P + 1 - T
+    left = most if left is None else int(left)
+    if not 0 <= left <= most:
+        raise ValueError(f"{pages.max_pages} ring entries of {P} frames hold {most} positions before {T} new ones at any alignment, left is {left}")
+    out = _head_out(out, query, dev, [kp, pages.v_pool, pages.rows] + ([lengths] if lengths is not None else []))
+    space = _attend(a, query, out, B, T, int(num_heads), D // hd, hd, left + T, scale, lengths, dev)  # noqa: F841
+    if B == 0 or T == 0:
+        return out
+    a.layer, a.left = int(layer), left
+    check(lib().pk_chunk_attn(ctypes.byref(a), _stream(dev)), "pk_chunk_attn")
+    return out
+
+
+def cross_attn(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    *,
+    num_heads: int,
+    lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each stream's tokens to states of another length, as a decoder reads the
+    encoder's: query [B, T, num_heads * head_dim], key/value [B, S, D] of the states (views of one projection,
+    or expanded over the batch, are fine), D / head_dim key heads each read by num_heads * head_dim / D query heads.
+    ``lengths``: int32 [B], states of each stream (held within 0 .. S; None: S); those past it are not read.
+    Several texts of one stream are rows of its T.  Returns [B, T, num_heads * head_dim], zeros where there is no state; ``out`` may be
+    ``query``.  Heads of 64 or 128 columns, ``scale`` None is head_dim ** -0.5, fp32 accumulation and
+    softmax.  No gradients."""
+    _plain_call("cross_attn", [query, key, value])
+    hd, dt = _head_dim(query, num_heads), query.dtype
+    dtype_code(dt)
+    B, T, _ = query.shape
+    S, D = key.shape[1:] if key.dim() == 3 else (0, 0)
+    if D % hd or D == 0:
+        raise ValueError(f"key must be [{B}, S, whole heads of {hd}], got {tuple(key.shape)}")
+    _head_rows("query", query, B, T, dt)
+    _head_rows("key", key, B, S, dt)
+    _head_rows("value", value, B, S, dt, D)
+    dev = _require_device(query, key, value)
+    out = _head_out(out, query, dev, [key, value] + ([lengths] if lengths is not None else []))
+    a = CrossAttnArgs()
+    space = _attend(a, query, out, B, T, int(num_heads), D // hd, hd, S, scale, lengths, dev)  # noqa: F841
+    if B == 0 or T == 0:
+        return out
+    a.states, a.kv_heads = S, D // hd
+    a.key, a.value = key.data_ptr(), value.data_ptr()
+    a.key_stride_b, a.key_stride_t, _ = key.stride()
+    a.value_stride_b, a.value_stride_t, _ = value.stride()
+    check(lib().pk_cross_attn(ctypes.byref(a), _stream(dev)), "pk_cross_attn")
+    return out

@@ -183,7 +183,10 @@ class DevicePagePool:
         s = np.ascontiguousarray(np.asarray(slots, dtype=np.int32).reshape(-1))
         if len(np.unique(s)) != len(s) or (len(s) and (s.min() < 0 or s.max() >= self.num_slots)):
             raise ValueError(f"slots must be distinct and in [0, {self.num_slots})")
-        t = torch.from_numpy(s)
+        return self._upload(s)
+
+    def _upload(self, a: np.ndarray) -> torch.Tensor:
+        t = torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32))
         # from pinned memory, without waiting (torch keeps it until the copy has run)
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
@@ -201,6 +204,24 @@ class DevicePagePool:
 
     def reset_all(self) -> None:
         ops.page_reset(self.state, torch.arange(self.num_slots, dtype=torch.int32, device=self.device))
+
+    # -- streams and pages moved
+    def fork(self, src, dst) -> ops.PageMoves:
+        """Slots ``dst`` continue the streams of slots ``src`` (``ops.page_fork``); the moves
+        that ``ops.kv_move_pages`` copies, for each pool of pages, are returned."""
+        s, d = (x if isinstance(x, torch.Tensor) and x.device.type == "cuda" else np.asarray(x, dtype=np.int64).reshape(-1) for x in (src, dst))
+        if isinstance(s, np.ndarray) and isinstance(d, np.ndarray):
+            if len(s) != len(d) or set(s.tolist()) & set(d.tolist()):
+                raise ValueError("a fork needs as many sources as destinations, none of them both")
+        if isinstance(s, np.ndarray):
+            if len(s) and (s.min() < 0 or s.max() >= self.num_slots):
+                raise ValueError(f"slots must be in [0, {self.num_slots})")
+            s = self._upload(s)  # a source may be named twice
+        return ops.page_fork(self.state, s, self.slots_tensor(d))
+
+    def compact(self) -> ops.PageMoves:
+        """The held pages become the pool's first ones (``ops.page_compact``)."""
+        return ops.page_compact(self.state)
 
     # -- inspection
     def free_pages(self) -> int:
