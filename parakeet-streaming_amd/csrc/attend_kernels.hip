@@ -9,6 +9,7 @@
 #include "pk_common.h"
 #include "pk_device.h"
 #include "pk_scan.h"
+#include "pk_tile.h"
 
 namespace pk {
 
@@ -153,6 +154,10 @@ struct AttendK {
   const int32_t* lengths;
   int32_t B, T, Hq, Hkv, G, left, states;
   float scale;  // times log2(e)
+  int32_t R;                 // rows of a key head: T * G
+  int32_t row_tiles, splits;  // workgroups along the rows, and along the keys
+  float* part;   // splits > 1: [B * Hkv * R][splits][HD] sums over a split's keys
+  float2* ml;    // and [B * Hkv * R][splits] their {maximum in log2 units, sum of weights}
 };
 
 constexpr float kNone = -__builtin_inff();
@@ -199,10 +204,11 @@ __device__ static inline int64_t key_at(const AttendK<ST>& p, int b, int hd_byte
 }
 
 // One row by one wave, without the matrix cores: 64 keys at a time, a key a lane for the
-// scores, columns over the lanes for the sums. q: the row, in fp32, in LDS. Gives the
+// scores, columns over the lanes for the sums. q: the row, in fp32, in LDS. Keys first ..
+// first + n - 1 (counted: positions run up to 2^31 - 1). Gives the
 // maximum (log2 units), the sum, and the sums of columns lane + 64 c.
 template <typename ST, int HD, bool PAGED>
-__device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, const float* q, int first, int last, float& m, float& l,
+__device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, const float* q, int first, int n, float& m, float& l,
                                          float (&acc)[HD / 64]) {
   constexpr int VEC = Tr<ST>::VEC, CB = 64 / (int)sizeof(ST), E = (int)sizeof(ST);
   const int lane = threadIdx.x & 63;
@@ -211,7 +217,6 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
   l = 0.f;
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) acc[c] = 0.f;
-  const int n = last - first + 1;  // at most 2^30: positions run up to 2^31 - 1, so numbers from `first` on are counted
   for (int d0 = 0; d0 < n; d0 += 64) {
     const int64_t at = d0 + lane < n ? key_at<ST, PAGED>(p, b, HD * E, h, first + d0 + lane, false) : -1;
     float s = kNone;
@@ -250,23 +255,442 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
   }
 }
 
-template <typename ST, int HD, bool PAGED>
-__global__ void __launch_bounds__(256) attend_rows_kernel(const AttendK<ST> p) {
-  __shared__ float qs[4][HD];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= (int64_t)p.B * p.T * p.Hq) return;
-  const int h = (int)(row % p.Hq), i = (int)(row / p.Hq % p.T), b = (int)(row / p.Hq / p.T);
-  const ST* const q = p.q + b * p.q_sb + i * p.q_st + (int64_t)h * HD;
-  for (int c = lane; c < HD; c += 64) qs[wave][c] = from_st(q[c]);
-  wave_lds_sync();
-  const StreamOf s = stream_of<ST, PAGED>(p, b);
-  float m = kNone, l = 0.f, acc[HD / 64];
-  const int2 seen = seen_by<ST, PAGED>(p, s, i);
-  attend_row<ST, HD, PAGED>(p, b, h / p.G, qs[wave], i < s.n ? seen.x : 0, i < s.n ? seen.y : -1, m, l, acc);
-  ST* const o = p.out + b * p.o_sb + i * p.o_st + (int64_t)h * HD;
+// ---- few rows
+
+// matrix products of 64 bytes of columns (a column block): D[a's row][b's row] += a . b, where
+// lane (r = lane & 15, g = lane >> 4) holds bytes 16 g .. 16 g + 15 of row r of each, and gets D of
+// rows 4 g .. 4 g + 3 of a with row r of b. fp32: element e of a lane is column 4 g + e, so
+// step e multiplies columns e, 4 + e, 8 + e and 12 + e.
+template <typename ST>
+__device__ static inline f32x4_t mma_block(const u32x4 a, const u32x4 b, f32x4_t c) {
+  if constexpr (sizeof(ST) == 2) {
+    return MmaL<ST>::k32(a, b, c);
+  } else {
 #pragma unroll
-  for (int c = 0; c < HD / 64; ++c) o[lane + 64 * c] = to_st<ST>(l == 0.f ? 0.f : acc[c] / l);
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// largest of the four lanes l & 15, l & 15 + 16, ...
+__device__ static inline float max_of_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ static inline float sum_of_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// what a workgroup works on
+struct ItemOf {
+  int32_t b, hk, row0, split;
+  bool live;
+};
+
+// Workgroup -> (stream and key head and split, row tile): workgroups go to the XCDs in turn, and
+// the row tiles of the same keys to the same one, whose L2 then has them.
+template <typename ST>
+__device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows) {
+  const uint32_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
+  const uint32_t tile = y % (uint32_t)p.row_tiles, u = y / (uint32_t)p.row_tiles * 8 + x;
+  const uint32_t unit = u / (uint32_t)p.splits;
+  ItemOf it;
+  it.split = (int32_t)(u - unit * (uint32_t)p.splits);
+  it.b = (int32_t)(unit / (uint32_t)p.Hkv);
+  it.hk = (int32_t)(unit - (uint32_t)it.b * (uint32_t)p.Hkv);
+  it.row0 = (int32_t)tile * rows;
+  it.live = it.b < p.B;
+  return it;
+}
+
+// Keys of a row tile, in tiles of KT: number d of a key counts from k0 (a multiple of KT, so that
+// a tile meets few pages); some row sees keys lo .. hi. The split has tiles t0 .. t1 - 1.
+struct KeysOf {
+  int32_t k0, lo, hi, t0, t1;
+};
+
+template <typename ST, bool PAGED, int KT>
+__device__ static inline KeysOf keys_of(const AttendK<ST>& p, const StreamOf& s, int row0, int rows, int split) {
+  const int i0 = row0 / p.G, i1 = min((min(row0 + rows, p.R) - 1) / p.G, s.n - 1);
+  KeysOf k{0, 0, -1, 0, 0};
+  if (i1 < i0) return k;
+  const int first = seen_by<ST, PAGED>(p, s, i0).x, last = seen_by<ST, PAGED>(p, s, i1).y;
+  if (last < first) return k;
+  k.k0 = first & ~(KT - 1);
+  k.lo = first - k.k0;
+  k.hi = last - k.k0;
+  // at least a tile a wave, so that short streams of a long batch leave splits empty
+  const int tiles = k.hi / KT + 1, per = max((tiles + p.splits - 1) / p.splits, 4);
+  k.t0 = min(split * per, tiles);
+  k.t1 = min(k.t0 + per, tiles);
+  return k;
+}
+
+// The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled alike),
+// the quotient, or the split's part. WAVES parts of [rows][HD + 4] floats at `sums`.
+template <typename ST, int HD, bool PAGED, int ROWS, int WAVES>
+__device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, int KT, const float* sums,
+                                         const float2* ml, uint32_t* bad, float* qs) {
+  constexpr int VEC = 8, PER = HD / VEC, STRIDE = HD + 4, N = (ROWS * PER + 255) / 256;
+  const bool check = PAGED && p.T > 1;
+  if (check) {
+    for (int i = threadIdx.x; i < (ROWS + 31) / 32; i += 256) bad[i] = 0;
+    __syncthreads();
+  }
+  float o[N][VEC], m[N], l[N];
+#pragma unroll
+  for (int y = 0; y < N; ++y) {
+    const int x = y * 256 + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC;
+    if (r >= ROWS) continue;
+    m[y] = kNone;
+    l[y] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      m[y] = fmaxf(m[y], ml[w * ROWS + r].x);
+      l[y] += ml[w * ROWS + r].y;
+    }
+    float t = l[y];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      o[y][e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) o[y][e] += sums[(w * ROWS + r) * STRIDE + c + e];
+      t = fmaf(o[y][e], 0.f, t);
+    }
+    if (check && it.row0 + r < p.R && !(fabsf(t) < __builtin_inff())) atomicOr(&bad[r >> 5], 1u << (r & 31));
+  }
+  if (check) __syncthreads();
+#pragma unroll
+  for (int y = 0; y < N; ++y) {
+    const int x = y * 256 + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC, row = it.row0 + r;
+    if (r >= ROWS || row >= p.R) continue;
+    if (check && (bad[r >> 5] >> (r & 31) & 1)) continue;
+    const int i = row / p.G, h = it.hk * p.G + row - i * p.G;
+    if (p.splits > 1) {
+      const int64_t at = (((int64_t)it.b * p.Hkv + it.hk) * p.R + row) * p.splits + it.split;
+      float* const to = p.part + at * HD + c;
+      *reinterpret_cast<f32x4_t*>(to) = f32x4_t{o[y][0], o[y][1], o[y][2], o[y][3]};
+      *reinterpret_cast<f32x4_t*>(to + 4) = f32x4_t{o[y][4], o[y][5], o[y][6], o[y][7]};
+      if (c == 0) p.ml[at] = float2{m[y], l[y]};
+    } else {
+      const float inv = l[y] == 0.f ? 0.f : 1.f / l[y];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[y][e] *= inv;
+      ST* const to = p.out + it.b * p.o_sb + i * p.o_st + (int64_t)h * HD + c;
+      st16(to, Tr<ST>::pack(o[y]));
+      if constexpr (sizeof(ST) == 4) st16(to + 4, Tr<ST>::pack(o[y] + 4));
+    }
+  }
+  if (!check) return;
+  // A row that is not finite may have met, as 0 times it, a value that it does not see: it is
+  // made again from the keys that it sees, one by one (rare). It is not written yet: out may be
+  // the query that is read again.
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int r = wave; r < ROWS; r += 4) {
+    if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
+    const int row = it.row0 + r, i = row / p.G, h = it.hk * p.G + row % p.G;
+    const ST* const q = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)h * HD;
+    for (int c = lane; c < HD; c += 64) qs[wave * HD + c] = from_st(q[c]);
+    wave_lds_sync();
+    const int2 seen = seen_by<ST, PAGED>(p, s, i);
+    const int first = max(seen.x, keys.k0 + keys.t0 * KT), n = min(seen.y - keys.k0, keys.t1 * KT - 1) - (first - keys.k0) + 1;
+    float m, l, acc[HD / 64];
+    attend_row<ST, HD, PAGED>(p, it.b, it.hk, qs + wave * HD, first, n, m, l, acc);
+    const int64_t at = (((int64_t)it.b * p.Hkv + it.hk) * p.R + row) * p.splits + it.split;
+    ST* const to = p.out + it.b * p.o_sb + i * p.o_st + (int64_t)h * HD;
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) {
+      if (p.splits > 1)
+        p.part[at * HD + lane + 64 * c] = acc[c];
+      else
+        to[lane + 64 * c] = to_st<ST>(l == 0.f ? 0.f : acc[c] / l);
+    }
+    if (p.splits > 1 && lane == 0) p.ml[at] = float2{m, l};
+    wave_lds_sync();
+  }
+}
+
+// Up to 16 RT rows of a key head a workgroup; its 4 waves take tiles of KT keys in turn. Bound by the
+// reads of K and V, once, so a wave keeps a tile of both on its way: K's registers are
+// asked for again when the scores are made, V's when they are staged, the page numbers a tile ahead.
+// Products are taken transposed, keys (then columns of V) as rows: a lane has one query, 4 keys a
+// register group, so maxima and sums are in the lane but for 4 lanes, and the weights are the next
+// product's operand where they are. 16-bit types: two tiles of 16 keys make one step of 32, in
+// the order that the registers have; V comes back transposed from LDS; weights go into the
+// product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them.
+template <typename ST, int HD, bool PAGED, int RT>
+__global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p) {
+  constexpr int E = (int)sizeof(ST), ROWS = 16 * RT, SUB = E == 2 ? 2 : 1, KT = 16 * SUB, NB = HD * E / 64, NT = HD / 16;
+  constexpr int VROW = HD * E + 16;  // bytes of a staged row of V: 16 more spread the rows over the banks
+  constexpr int STRIDE = HD + 4;
+  constexpr int kStage = 4 * KT * VROW, kSums = 4 * ROWS * STRIDE * 4;
+  __shared__ __align__(16) unsigned char smem[kStage > kSums ? kStage : kSums];
+  __shared__ float2 ml[4 * ROWS];
+  __shared__ uint32_t bad[(ROWS + 31) / 32];
+  __shared__ float qs[PAGED ? 4 * HD : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const ItemOf it = item_of(p, ROWS);
+  if (!it.live) return;
+  const StreamOf s = stream_of<ST, PAGED>(p, it.b);
+  const KeysOf keys = keys_of<ST, PAGED, KT>(p, s, it.row0, ROWS, it.split);
+
+  // the rows: their queries and what they see
+  u32x4 q[RT][NB];
+  int lo[RT], hi[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = it.row0 + 16 * t + r16, i = min(row, p.R - 1) / p.G, gq = min(row, p.R - 1) - i * p.G;
+    const ST* const from = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)(it.hk * p.G + gq) * HD + g * (16 / E);
+#pragma unroll
+    for (int c = 0; c < NB; ++c) q[t][c] = ld16(from + c * (64 / E));
+    const bool live = row < p.R && i < s.n;
+    const int2 seen = seen_by<ST, PAGED>(p, s, i);
+    lo[t] = live ? seen.x - keys.k0 : 0;
+    hi[t] = live ? seen.y - keys.k0 : -1;
+  }
+  f32x4_t o[RT][NT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m[t] = kNone;
+    l[t] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[t][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (keys.t0 < keys.t1) {
+    const int64_t step = PAGED ? (int64_t)64 << p.page_shift : 64;
+    const unsigned char *kb, *vb;
+    if constexpr (PAGED) {
+      const int64_t head = ((int64_t)it.hk * (HD * E) << p.page_shift) + g * 16;
+      kb = p.k + head;
+      vb = p.v + head;
+    } else {
+      kb = p.k + it.b * p.k_sb + (int64_t)it.hk * (HD * E) + g * 16;
+      vb = p.v + it.b * p.v_sb + (int64_t)it.hk * (HD * E) + g * 16;
+    }
+    const int32_t* const ring = PAGED ? p.rows + it.b * p.rows_stride + 1 : nullptr;
+    // page of key lane % KT of tile t, -1 where no row of the workgroup sees it or it is not there
+    auto page_of = [&](int t) {
+      if constexpr (PAGED) {
+        const int d = t * KT + (lane & (KT - 1));
+        int page = -1;
+        if (t < keys.t1 && d >= keys.lo && d <= keys.hi) page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
+        return page;
+      } else {
+        return 0;
+      }
+    };
+    int64_t ko[SUB], vo[SUB];
+    bool ok[SUB];
+    auto places = [&](int t, int page) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int d = t * KT + 16 * u + r16;
+        if constexpr (PAGED) {
+          const int mine = __shfl(page, 16 * u + r16);
+          ok[u] = (uint32_t)mine < (uint32_t)p.num_pages;
+          ko[u] = vo[u] = ok[u] ? mine * p.page_bytes + ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6) : 0;
+        } else {
+          ok[u] = t < keys.t1 && d <= keys.hi;
+          ko[u] = ok[u] ? d * p.k_st : 0;  // row 0 is there; what it holds is not used
+          vo[u] = ok[u] ? d * p.v_st : 0;
+        }
+      }
+    };
+    u32x4 kr[SUB][NB], vr[SUB][NB];
+    auto ask = [&](u32x4 (&x)[SUB][NB], const unsigned char* base, const int64_t (&at)[SUB]) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int c = 0; c < NB; ++c) x[u][c] = *reinterpret_cast<const u32x4*>(base + at[u] + c * step);
+    };
+    unsigned char* const stage = smem + wave * (KT * VROW);
+    int t = keys.t0 + wave;
+    places(t, page_of(t));
+    ask(kr, kb, ko);
+    ask(vr, vb, vo);
+    int next = page_of(t + 4);
+    for (; t < keys.t1; t += 4) {
+      bool now[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) now[u] = ok[u];
+      f32x4_t x[RT][SUB];
+#pragma unroll
+      for (int a = 0; a < RT; ++a)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          x[a][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NB; ++c) x[a][u] = mma_block<ST>(kr[u][c], q[a][c], x[a][u]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      places(t + 4, next);
+      next = page_of(t + 8);
+      ask(kr, kb, ko);
+      __builtin_amdgcn_sched_barrier(0);
+      // weights: key d = t KT + 16 u + 4 g + e of query r16
+      uint64_t there[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) there[u] = __ballot(now[u]);  // bit r16: key 16 u + r16
+      bool whole = true;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) whole &= there[u] == ~0ull;
+      u32x4 w[RT], wl[RT];
+#pragma unroll
+      for (int a = 0; a < RT; ++a) {
+        float e[SUB][4], top = kNone;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int in = 4 * g + k, d = t * KT + 16 * u + in;
+            const bool sees = d >= lo[a] && d <= hi[a] && (there[u] >> in & 1);
+            e[u][k] = sees ? x[a][u][k] * p.scale : kNone;
+            top = fmaxf(top, e[u][k]);
+          }
+        top = fmaxf(m[a], max_of_groups(top));
+        const float base = top == kNone ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[a] - base);
+        m[a] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            e[u][k] = __builtin_amdgcn_exp2f(e[u][k] - base);
+            sum += e[u][k];
+          }
+        l[a] = fmaf(l[a], keep, sum);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[a][n] *= keep;
+        if constexpr (E == 2) {
+          float low[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) low[k] = e[k >> 2][k & 3] - round_to<ST>(e[k >> 2][k & 3]);
+          w[a] = Tr<ST>::pack(&e[0][0]);
+          wl[a] = Tr<ST>::pack(low);
+        } else {
+          w[a] = Tr<ST>::pack(&e[0][0]);
+        }
+      }
+      // V: a key that is not there gives zeros, since 0 times what memory holds might not be
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          u32x4 v = vr[u][c];
+          if (!whole && !now[u]) v = u32x4{0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4*>(stage + (16 * u + r16) * VROW + c * 64 + g * 16) = v;
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      ask(vr, vb, vo);
+      __builtin_amdgcn_sched_barrier(0);
+      wave_lds_sync();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (E == 2) {
+          typedef short i16x4 __attribute__((ext_vector_type(4)));
+          i16x4 v[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            unsigned char* src = stage + (16 * u + 4 * g + (r16 >> 2)) * VROW + (n * 16 + 4 * (r16 & 3)) * 2;
+            v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)src);
+          }
+          const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
+          const u32x4 vt = u32x4{v0.x, v0.y, v1.x, v1.y};
+#pragma unroll
+          for (int a = 0; a < RT; ++a) {
+            o[a][n] = MmaL<ST>::k32(vt, w[a], o[a][n]);
+            o[a][n] = MmaL<ST>::k32(vt, wl[a], o[a][n]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float v = *reinterpret_cast<const float*>(stage + (4 * g + k) * VROW + (n * 16 + r16) * 4);
+#pragma unroll
+            for (int a = 0; a < RT; ++a) o[a][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, __uint_as_float(w[a][k]), o[a][n], 0, 0, 0);
+          }
+        }
+      }
+      wave_lds_sync();  // the next tile overwrites the staged rows
+    }
+  }
+
+  // the waves' parts meet: scaled to the largest maximum, side by side in LDS
+#pragma unroll
+  for (int a = 0; a < RT; ++a) {
+    l[a] = sum_of_groups(l[a]);
+    if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
+  }
+  __syncthreads();  // and every wave is done with its staged rows
+  float* const sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int a = 0; a < RT; ++a) {
+    float top = kNone;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * ROWS + 16 * a + r16].x);
+    const float f = __builtin_amdgcn_exp2f(m[a] - (top == kNone ? 0.f : top));
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = o[a][n] * f;
+    l[a] *= f;
+    m[a] = top;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int a = 0; a < RT; ++a)
+    if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
+  __syncthreads();
+  attend_end<ST, HD, PAGED, ROWS, 4>(p, it, s, keys, KT, sums, ml, bad, qs);
+}
+
+// The splits of a row meet: weights by their maxima, sums over them. A workgroup a row.
+constexpr int kMaxSplits = 256;
+template <typename ST, int HD>
+__global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
+  constexpr int LANES = HD / 4, SIDE = 256 / LANES;  // lanes a split's row, splits at once
+  __shared__ float weight[kMaxSplits];
+  __shared__ float red[4], total[4];
+  __shared__ f32x4_t sums[256];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t x = blockIdx.x, unit = x / (uint32_t)p.R, row = x - unit * (uint32_t)p.R;
+  const int b = (int)(unit / (uint32_t)p.Hkv), hk = (int)(unit - (uint32_t)b * p.Hkv), i = (int)(row / (uint32_t)p.G), gq = (int)(row - (uint32_t)i * p.G);
+  const float2 v = tid < p.splits ? p.ml[(int64_t)x * p.splits + tid] : float2{kNone, 0.f};
+  float top = v.x;
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float w = __builtin_amdgcn_exp2f(v.x - (top == kNone ? 0.f : top));
+  weight[tid] = v.y == 0.f ? 0.f : w;  // a split without keys for the row is not read
+  const float l = group_sum<64>(v.y == 0.f ? 0.f : v.y * w);
+  if (lane == 0) total[wave] = l;
+  __syncthreads();
+  const int c = (tid & (LANES - 1)) * 4;
+  f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float* const from = p.part + (int64_t)x * p.splits * HD + c;
+#pragma unroll 4
+  for (int sp = tid / LANES; sp < p.splits; sp += SIDE) {
+    const float ws = weight[sp];
+    if (ws != 0.f) acc += *reinterpret_cast<const f32x4_t*>(from + (int64_t)sp * HD) * ws;
+  }
+  sums[tid] = acc;
+  __syncthreads();
+  if (tid >= LANES) return;
+#pragma unroll
+  for (int k = 1; k < SIDE; ++k) acc += sums[tid + k * LANES];
+  const float sum = (total[0] + total[1]) + (total[2] + total[3]), inv = sum == 0.f ? 0.f : 1.f / sum;
+  ST* const to = p.out + b * p.o_sb + i * p.o_st + (int64_t)(hk * p.G + gq) * HD + c;
+  float f[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+  if constexpr (sizeof(ST) == 4)
+    st16(to, Tr<ST>::pack(f));
+  else
+    *reinterpret_cast<u32x2*>(to) = pack4<ST>(f);
 }
 
 namespace {
@@ -371,15 +795,59 @@ int attend_ok(const char* what, int batch, int chunk, int heads, int kv_heads, i
   return PK_OK;
 }
 
-template <typename ST, bool PAGED>
-int attend_launch(const char* what, const AttendK<ST>& p, int head_dim, hipStream_t s) {
-  const int64_t rows = (int64_t)p.B * p.T * p.Hq;
-  const dim3 grid((unsigned)((rows + 3) / 4));
-  if (head_dim == 64)
-    hipLaunchKernelGGL((attend_rows_kernel<ST, 64, PAGED>), grid, dim3(256), 0, s, p);
+// How a call is cut: rows of a workgroup, workgroups along the rows and along the keys.
+struct AttendCut {
+  int rows, row_tiles, splits;
+  int64_t groups;  // workgroups
+};
+
+AttendCut attend_cut(int batch, int chunk, int heads, int kv_heads, int keys) {
+  AttendCut c;
+  const int64_t R = (int64_t)chunk * (heads / kv_heads), units = (int64_t)batch * kv_heads;
+  c.rows = R <= 16 ? 16 : 32;
+  c.row_tiles = (int)((R + c.rows - 1) / c.rows);
+  const int64_t whole = units * c.row_tiles, want = (512 + whole - 1) / whole, most = (keys + 511) / 512;
+  int64_t n = want < most ? want : most;
+  n = n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
+  c.splits = (int)n;
+  c.groups = (units * n + 7) / 8 * 8 * c.row_tiles;
+  return c;
+}
+
+int64_t attend_space(int64_t rows, int splits, int head_dim) { return splits > 1 ? rows * splits * (4 * head_dim + 8) : 0; }
+
+template <typename ST, int HD, bool PAGED>
+int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hipStream_t s) {
+  const dim3 grid((unsigned)c.groups), block(256);
+  if (c.rows == 16)
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((attend_rows_kernel<ST, 128, PAGED>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 2>), grid, block, 0, s, p);
+  int rc = check_launch(what);
+  if (rc != PK_OK || p.splits == 1) return rc;
+  hipLaunchKernelGGL((attend_join_kernel<ST, HD>), dim3((unsigned)((int64_t)p.B * p.Hkv * p.R)), block, 0, s, p);
   return check_launch(what);
+}
+
+// Both attentions, from the cut on.
+template <typename ST, bool PAGED>
+int attend(const char* what, AttendK<ST>& p, int head_dim, int keys, void* workspace, int device, hipStream_t s) {
+  p.G = p.Hq / p.Hkv;
+  p.R = p.T * p.G;
+  const AttendCut c = attend_cut(p.B, p.T, p.Hq, p.Hkv, keys);
+  p.row_tiles = c.row_tiles;
+  p.splits = c.splits;
+  const int64_t rows = (int64_t)p.B * p.T * p.Hq;
+  // a grid has fewer than 2^32 threads
+  if (c.groups >= (1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);
+  if (c.splits > 1) {
+    if (!workspace || !aligned16(workspace)) return fail(PK_ERR_INVALID, "%s: workspace must be non-NULL and 16-byte aligned", what);
+    p.part = static_cast<float*>(workspace);
+    p.ml = reinterpret_cast<float2*>(p.part + rows * c.splits * head_dim);
+  }
+  DeviceGuard dg(device);
+  if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, device);
+  return head_dim == 64 ? attend_launch<ST, 64, PAGED>(what, p, c, s) : attend_launch<ST, 128, PAGED>(what, p, c, s);
 }
 
 template <typename ST>
@@ -418,12 +886,9 @@ int chunk_attn(const pk_chunk_attn_args* a, hipStream_t s) {
   p.T = a->chunk;
   p.Hq = a->num_heads;
   p.Hkv = L.d_model / a->head_dim;
-  p.G = p.Hq / p.Hkv;
   p.left = a->left;
   p.scale = a->scale * 1.44269504088896341f;
-  DeviceGuard dg(a->device);
-  if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
-  return attend_launch<ST, true>(what, p, a->head_dim, s);
+  return attend<ST, true>(what, p, a->head_dim, a->left + a->chunk, a->workspace, a->device, s);
 }
 
 template <typename ST>
@@ -458,12 +923,9 @@ int cross_attn(const pk_cross_attn_args* a, hipStream_t s) {
   p.T = a->chunk;
   p.Hq = a->num_heads;
   p.Hkv = a->kv_heads;
-  p.G = p.Hq / p.Hkv;
   p.states = a->states;
   p.scale = a->scale * 1.44269504088896341f;
-  DeviceGuard dg(a->device);
-  if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
-  return attend_launch<ST, false>(what, p, a->head_dim, s);
+  return attend<ST, false>(what, p, a->head_dim, a->states, a->workspace, a->device, s);
 }
 
 }  // namespace
@@ -485,7 +947,11 @@ extern "C" {
 
 int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream) { PK_BY_DTYPE("pk_qk_norm_append", norm_append) }
 
-int64_t pk_attn_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+int64_t pk_attn_workspace_bytes(int32_t dtype, int32_t batch, int32_t chunk, int32_t num_heads, int32_t kv_heads, int32_t head_dim, int32_t keys) {
+  if (batch <= 0 || chunk <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 || head_dim <= 0 || keys < 0) return 0;
+  (void)dtype;
+  return pk::attend_space((int64_t)batch * chunk * num_heads, pk::attend_cut(batch, chunk, num_heads, kv_heads, keys).splits, head_dim);
+}
 
 int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream) { PK_BY_DTYPE("pk_chunk_attn", chunk_attn) }
 
