@@ -333,19 +333,19 @@ __device__ static inline KeysOf keys_of(const AttendK<ST>& p, const StreamOf& s,
 
 // The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled alike),
 // the quotient, or the split's part. WAVES parts of [rows][HD + 4] floats at `sums`.
-template <typename ST, int HD, bool PAGED, int ROWS, int WAVES>
+template <typename ST, int HD, bool PAGED, int ROWS, int WAVES, int THREADS>
 __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, int KT, const float* sums,
                                          const float2* ml, uint32_t* bad, float* qs) {
-  constexpr int VEC = 8, PER = HD / VEC, STRIDE = HD + 4, N = (ROWS * PER + 255) / 256;
+  constexpr int VEC = 8, PER = HD / VEC, STRIDE = HD + 4, N = (ROWS * PER + THREADS - 1) / THREADS;
   const bool check = PAGED && p.T > 1;
   if (check) {
-    for (int i = threadIdx.x; i < (ROWS + 31) / 32; i += 256) bad[i] = 0;
+    for (int i = threadIdx.x; i < (ROWS + 31) / 32; i += THREADS) bad[i] = 0;
     __syncthreads();
   }
   float o[N][VEC], m[N], l[N];
 #pragma unroll
   for (int y = 0; y < N; ++y) {
-    const int x = y * 256 + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC;
+    const int x = y * THREADS + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC;
     if (r >= ROWS) continue;
     m[y] = kNone;
     l[y] = 0.f;
@@ -367,7 +367,7 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
   if (check) __syncthreads();
 #pragma unroll
   for (int y = 0; y < N; ++y) {
-    const int x = y * 256 + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC, row = it.row0 + r;
+    const int x = y * THREADS + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC, row = it.row0 + r;
     if (r >= ROWS || row >= p.R) continue;
     if (check && (bad[r >> 5] >> (r & 31) & 1)) continue;
     const int i = row / p.G, h = it.hk * p.G + row - i * p.G;
@@ -391,7 +391,7 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
   // made again from the keys that it sees, one by one (rare). It is not written yet: out may be
   // the query that is read again.
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int r = wave; r < ROWS; r += 4) {
+  for (int r = wave; r < ROWS; r += THREADS / 64) {
     if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
     const int row = it.row0 + r, i = row / p.G, h = it.hk * p.G + row % p.G;
     const ST* const q = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)h * HD;
@@ -646,7 +646,258 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
   for (int a = 0; a < RT; ++a)
     if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, 4>(p, it, s, keys, KT, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, 4, 256>(p, it, s, keys, KT, sums, ml, bad, qs);
+}
+
+// ---- many rows
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+// D[a's row][b's row] += a . b over 16 columns: lane (r = lane & 31, h = lane >> 5) holds columns 8 h .. 8 h + 7
+// of row r of each, and gets D of rows 8 j + 4 h + e of a (register 4 j + e) with row r of b.
+template <typename ST>
+__device__ static inline f32x16_t mma32(const u32x4 a, const u32x4 b, const f32x16_t c) {
+  typedef typename MmaL<ST>::H8 H8;
+  if constexpr (__is_same(ST, bf16_t))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
+}
+
+// Where the 16-byte pieces of a row of a staged tile lie: piece c of row r at c ^ mix(r). A product's
+// operand reads one piece of 32 rows, the transposed read of V 64 bytes of 8 rows: either then
+// meets all banks alike.
+template <int HD>
+__device__ static inline int mix(int r) {
+  if constexpr (HD == 128) return (r & 3) << 2 | (r >> 2 & 3);
+  return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+}
+
+constexpr uint32_t kNowhere = 0xffffffffu;  // past any resource: reads zeros
+
+// A buffer resource as four words: rows of `stride` bytes (0: bytes) from base, `records` of them.
+__device__ static inline u32x4 resource_words(const void* base, uint32_t stride, uint32_t records) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  return u32x4{(uint32_t)at, ((uint32_t)(at >> 32) & 0xffffu) | (stride << 16), records, 0x00020000u};  // word 3 as bytes_rsrc's
+}
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0, which nothing else here uses, is written
+// 16 bytes a lane, from byte `off` of row `row`, to lds + 16 lane (lds wave-uniform). Written as assembly
+// because the compiler waits for every load to LDS that it knows of before any read of LDS,
+// which would end the overlap with the tile that is worked on; it names no register as output,
+// and wait_vm counts it. s_nop: the cycles that m0, and words that vector code may have made, need.
+__device__ static inline void stage_row(const u32x4 r, const unsigned char* lds, uint32_t row, uint32_t off) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 idxen offen lds" ::"s"(at), "v"(u32x2{row, off}), "s"(r) : "memory", "m0");
+}
+__device__ static inline void stage_bytes(const u32x4 r, const unsigned char* lds, uint32_t off) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// 128 rows of a key head a workgroup, 32 a wave; KG groups of 4 waves take tiles of 64 keys in turn.
+// A group stages its tile of K and V in LDS, a tile ahead, straight from memory. As in
+// attend_few_kernel products are transposed, so that a lane has one query; the weights are rounded once to
+// the type for the second product (half a step of it relative to each).
+template <typename ST, int HD, bool PAGED, int KG>
+__global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<ST> p) {
+  constexpr int ROWS = 128, KT = 64, C = HD / 8, RB = HD * 2, NB = HD / 32, NK = HD / 16, RPI = 64 / C, LOADS = 16 / RPI;
+  constexpr int kTile = KT * RB, kBuf = 2 * kTile;  // K and V of a tile
+  constexpr int STRIDE = HD + 4, kSums = KG * ROWS * STRIDE * 4;
+  constexpr int kStage = KG * 2 * kBuf;
+  __shared__ __align__(16) unsigned char smem[kStage > kSums ? kStage : kSums];
+  __shared__ float2 ml[KG * ROWS];
+  __shared__ uint32_t bad[(ROWS + 31) / 32];
+  __shared__ float qs[PAGED ? 4 * KG * HD : 1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, wv = wave & 3, kg = wave >> 2;
+  const ItemOf it = item_of(p, ROWS);
+  if (!it.live) return;
+  const StreamOf s = stream_of<ST, PAGED>(p, it.b);
+  const KeysOf keys = keys_of<ST, PAGED, KT>(p, s, it.row0, ROWS, it.split);
+
+  const int row = it.row0 + 32 * wv + r32;
+  u32x4 q[NK];
+  int lo, hi;
+  {
+    const int rr = min(row, p.R - 1), i = rr / p.G;
+    const ST* const from = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)(it.hk * p.G + rr - i * p.G) * HD + h * 8;
+#pragma unroll
+    for (int c = 0; c < NK; ++c) q[c] = ld16(from + c * 16);
+    const bool live = row < p.R && i < s.n;
+    const int2 seen = seen_by<ST, PAGED>(p, s, i);
+    lo = live ? seen.x - keys.k0 : 0;
+    hi = live ? seen.y - keys.k0 : -1;
+  }
+  // what all rows of the wave see, and what some do
+  int all_lo = lo, all_hi = hi, some_lo = hi < 0 ? 0x7fffffff : lo, some_hi = hi;
+  for (int d = 1; d < 32; d <<= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, d));
+    all_hi = min(all_hi, __shfl_xor(all_hi, d));
+    some_lo = min(some_lo, __shfl_xor(some_lo, d));
+    some_hi = max(some_hi, __shfl_xor(some_hi, d));
+  }
+  f32x16_t o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[n][e] = 0.f;
+  float m = kNone, l = 0.f;
+
+  if (keys.t0 < keys.t1) {
+    // What is read, by an index that the hardware checks: pages as rows of 64 bytes, a tile of states by the byte;
+    // kNowhere gives zeros, so that 0 times what memory holds for a key that is not there is 0.
+    u32x4 kb, vb;
+    const uint32_t page_rows = (uint32_t)(p.page_bytes >> 6);  // rows of 64 bytes of a page
+    if constexpr (PAGED) {
+      const uint32_t head = (uint32_t)it.hk * NB << p.page_shift, rows = (uint32_t)p.num_pages * page_rows - head;
+      kb = resource_words(p.k + ((int64_t)head << 6), 64, rows);
+      vb = resource_words(p.v + ((int64_t)head << 6), 64, rows);
+    }
+    const int32_t* const ring = PAGED ? p.rows + it.b * p.rows_stride + 1 : nullptr;
+    // a wave stages rows 16 wv .. 16 wv + 15 of its group's tiles; the page of row lane % 16
+    auto page_of = [&](int t) {
+      if constexpr (PAGED) {
+        const int d = t * KT + 16 * wv + (lane & 15);
+        int page = -1;
+        if (t < keys.t1 && d >= keys.lo && d <= keys.hi) page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
+        return page;
+      } else {
+        return 0;
+      }
+    };
+    unsigned char* const group = smem + kg * 2 * kBuf;
+    auto ask = [&](int t, int page, int buf) {
+      unsigned char* const at = group + buf * kBuf + 16 * wv * RB;
+      if constexpr (!PAGED) {
+        kb = resource_words(p.k + it.b * p.k_sb + (int64_t)it.hk * RB + (int64_t)t * KT * p.k_st, 0, (uint32_t)(KT * p.k_st));
+        vb = resource_words(p.v + it.b * p.v_sb + (int64_t)it.hk * RB + (int64_t)t * KT * p.v_st, 0, (uint32_t)(KT * p.v_st));
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = i * RPI + lane / C, rt = 16 * wv + x, d = t * KT + rt, c = (lane & (C - 1)) ^ mix<HD>(rt);
+        if constexpr (PAGED) {
+          const uint32_t mine = (uint32_t)__shfl(page, x);
+          const uint32_t in = ((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u);
+          const uint32_t row = mine < (uint32_t)p.num_pages ? mine * page_rows + ((uint32_t)(c >> 2) << p.page_shift) + in : kNowhere;
+          stage_row(kb, at + i * 1024, row, (c & 3) * 16);
+          stage_row(vb, at + kTile + i * 1024, row, (c & 3) * 16);
+        } else {
+          const bool ok = t < keys.t1 && d <= keys.hi;
+          stage_bytes(kb, at + i * 1024, ok ? (uint32_t)rt * (uint32_t)p.k_st + c * 16 : kNowhere);
+          stage_bytes(vb, at + kTile + i * 1024, ok ? (uint32_t)rt * (uint32_t)p.v_st + c * 16 : kNowhere);
+        }
+      }
+    };
+    // operand addresses in a tile
+    const int kx = mix<HD>(r32);
+    int va[2];
+    const int l16 = lane & 15, dg = lane >> 4 & 1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) va[u] = 8 * u + 4 * h + (l16 >> 2);
+    int t = keys.t0 + kg, buf = 0;
+    ask(t, page_of(t), 0);
+    int next = page_of(t + KG);
+    const int turns = (keys.t1 - keys.t0 + KG - 1) / KG;
+    for (int turn = 0; turn < turns; ++turn, t += KG, buf ^= 1) {
+      wait_vm<0>();
+      __syncthreads();  // the tile is there, and every wave is done with the one before
+      ask(t + KG, next, buf ^ 1);
+      next = page_of(t + 2 * KG);
+      const int d0 = t * KT;
+      if (t >= keys.t1 || d0 > some_hi || d0 + KT - 1 < some_lo) continue;  // wave-uniform
+      const unsigned char* const kt = group + buf * kBuf;
+      const unsigned char* const vt = kt + kTile;
+      f32x16_t x[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+          x[u] = mma32<ST>(*reinterpret_cast<const u32x4*>(kt + (32 * u + r32) * RB + (((2 * c + h) ^ kx) * 16)), q[c], x[u]);
+      }
+      if (d0 < all_lo || d0 + KT - 1 > all_hi) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int d = d0 + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (d < lo || d > hi) x[u][e] = kNone;
+          }
+      }
+      float top = kNone;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
+      {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * p.scale;
+      }
+      if (__any(top > m)) {
+        top = fmaxf(top, m);
+        const float keep = top == kNone ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n] *= keep;
+      }
+      const float base = m == kNone ? 0.f : m;
+      u32x4 w[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float e[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          e[k] = __builtin_amdgcn_exp2f(fmaf(x[u][k], p.scale, -base));
+          l += e[k];
+        }
+        w[2 * u] = Tr<ST>::pack(e);
+        w[2 * u + 1] = Tr<ST>::pack(e + 8);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          i16x4_t v[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int c = (4 * n + 2 * dg + (l16 >> 1 & 1)) ^ mix<HD>(va[u]);
+            const unsigned char* src = vt + (16 * k + va[u]) * RB + c * 16 + (l16 & 1) * 8;
+            v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)src);
+          }
+          const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
+          o[n] = mma32<ST>(u32x4{v0.x, v0.y, v1.x, v1.y}, w[k], o[n]);
+        }
+    }
+    wait_vm<0>();  // what was asked for behind the last tile
+  }
+
+  {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{m, l};
+  __syncthreads();  // and every wave is done with the tiles
+  float* const sums = reinterpret_cast<float*>(smem);
+  float top = kNone;
+#pragma unroll
+  for (int k = 0; k < KG; ++k) top = fmaxf(top, ml[k * ROWS + 32 * wv + r32].x);
+  const float f = __builtin_amdgcn_exp2f(m - (top == kNone ? 0.f : top));
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t v = f32x4_t{o[n][4 * j], o[n][4 * j + 1], o[n][4 * j + 2], o[n][4 * j + 3]};
+      *reinterpret_cast<f32x4_t*>(sums + (kg * ROWS + 32 * wv + r32) * STRIDE + 32 * n + 8 * j + 4 * h) = v * f;
+    }
+  __syncthreads();
+  if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{top, l * f};
+  __syncthreads();
+  attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG>(p, it, s, keys, KT, sums, ml, bad, qs);
 }
 
 // The splits of a row meet: weights by their maxima, sums over them. A workgroup a row.
@@ -715,6 +966,9 @@ int pool_ok(const char* what, const pk_paged_layout& L, int layer, int head_dim)
     return fail(PK_ERR_INVALID, "%s: need 0 < num_pages * page_size < 2^31", what);
   if (L.d_model <= 0 || L.d_model % head_dim != 0)
     return fail(PK_ERR_INVALID, "%s: pages of %d columns are not whole heads of %d", what, L.d_model, head_dim);
+  // rows of 64 bytes of a layer have 32-bit numbers
+  if ((int64_t)L.num_pages * L.page_size * (L.d_model / 16) >= (int64_t{1} << 32))
+    return fail(PK_ERR_INVALID, "%s: %d pages of %d x %d are past a layer's 2^32 column blocks", what, L.num_pages, L.page_size, L.d_model);
   return PK_OK;
 }
 
@@ -797,14 +1051,15 @@ int attend_ok(const char* what, int batch, int chunk, int heads, int kv_heads, i
 
 // How a call is cut: rows of a workgroup, workgroups along the rows and along the keys.
 struct AttendCut {
-  int rows, row_tiles, splits;
+  int rows, key_groups, row_tiles, splits;
   int64_t groups;  // workgroups
 };
 
-AttendCut attend_cut(int batch, int chunk, int heads, int kv_heads, int keys) {
+AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, int keys) {
   AttendCut c;
   const int64_t R = (int64_t)chunk * (heads / kv_heads), units = (int64_t)batch * kv_heads;
-  c.rows = R <= 16 ? 16 : 32;
+  c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 ? 32 : 128;
+  c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
   const int64_t whole = units * c.row_tiles, want = (512 + whole - 1) / whole, most = (keys + 511) / 512;
   int64_t n = want < most ? want : most;
@@ -821,7 +1076,14 @@ int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hi
   const dim3 grid((unsigned)c.groups), block(256);
   if (c.rows == 16)
     hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
-  else
+  else if constexpr (sizeof(ST) == 2) {
+    if (c.rows == 32)
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 2>), grid, block, 0, s, p);
+    else if (c.key_groups == 1)
+      hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 2>), grid, dim3(512), 0, s, p);
+  } else
     hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 2>), grid, block, 0, s, p);
   int rc = check_launch(what);
   if (rc != PK_OK || p.splits == 1) return rc;
@@ -831,10 +1093,10 @@ int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hi
 
 // Both attentions, from the cut on.
 template <typename ST, bool PAGED>
-int attend(const char* what, AttendK<ST>& p, int head_dim, int keys, void* workspace, int device, hipStream_t s) {
+int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, void* workspace, int device, hipStream_t s) {
   p.G = p.Hq / p.Hkv;
   p.R = p.T * p.G;
-  const AttendCut c = attend_cut(p.B, p.T, p.Hq, p.Hkv, keys);
+  const AttendCut c = attend_cut(dtype, p.B, p.T, p.Hq, p.Hkv, keys);
   p.row_tiles = c.row_tiles;
   p.splits = c.splits;
   const int64_t rows = (int64_t)p.B * p.T * p.Hq;
@@ -888,7 +1150,7 @@ int chunk_attn(const pk_chunk_attn_args* a, hipStream_t s) {
   p.Hkv = L.d_model / a->head_dim;
   p.left = a->left;
   p.scale = a->scale * 1.44269504088896341f;
-  return attend<ST, true>(what, p, a->head_dim, a->left + a->chunk, a->workspace, a->device, s);
+  return attend<ST, true>(what, p, a->dtype, a->head_dim, a->left + a->chunk, a->workspace, a->device, s);
 }
 
 template <typename ST>
@@ -903,6 +1165,8 @@ int cross_attn(const pk_cross_attn_args* a, hipStream_t s) {
   if (a->states > 0) {
     if ((rc = rows_ok<ST>(what, "key", a->key, a->key_stride_b, a->key_stride_t)) != PK_OK) return rc;
     if ((rc = rows_ok<ST>(what, "value", a->value, a->value_stride_b, a->value_stride_t)) != PK_OK) return rc;
+    // a tile of 64 states is addressed with 32 bits
+    if (a->key_stride_t >= (1 << 23) || a->value_stride_t >= (1 << 23)) return fail(PK_ERR_UNSUPPORTED, "%s: rows of 2^23 elements or more", what);
   }
   AttendK<ST> p{};
   constexpr int64_t E = sizeof(ST);
@@ -925,7 +1189,7 @@ int cross_attn(const pk_cross_attn_args* a, hipStream_t s) {
   p.Hkv = a->kv_heads;
   p.states = a->states;
   p.scale = a->scale * 1.44269504088896341f;
-  return attend<ST, false>(what, p, a->head_dim, a->states, a->workspace, a->device, s);
+  return attend<ST, false>(what, p, a->dtype, a->head_dim, a->states, a->workspace, a->device, s);
 }
 
 }  // namespace
@@ -949,8 +1213,7 @@ int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream) { PK_BY_
 
 int64_t pk_attn_workspace_bytes(int32_t dtype, int32_t batch, int32_t chunk, int32_t num_heads, int32_t kv_heads, int32_t head_dim, int32_t keys) {
   if (batch <= 0 || chunk <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 || head_dim <= 0 || keys < 0) return 0;
-  (void)dtype;
-  return pk::attend_space((int64_t)batch * chunk * num_heads, pk::attend_cut(batch, chunk, num_heads, kv_heads, keys).splits, head_dim);
+  return pk::attend_space((int64_t)batch * chunk * num_heads, pk::attend_cut(dtype, batch, chunk, num_heads, kv_heads, keys).splits, head_dim);
 }
 
 int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream) { PK_BY_DTYPE("pk_chunk_attn", chunk_attn) }
