@@ -674,6 +674,7 @@ __device__ static inline int mix(int r) {
   return (r >> 1 & 1) << 2 | (r >> 2 & 3);
 }
 
+constexpr float kSlack = 6.f;
 constexpr uint32_t kNowhere = 0xffffffffu;  // past any resource: reads zeros
 
 // A buffer resource as four words: rows of `stride` bytes (0: bytes) from base, `records` of them.
@@ -804,21 +805,26 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     for (int turn = 0; turn < turns; ++turn, t += KG, buf ^= 1) {
       wait_vm<0>();
       __syncthreads();  // the tile is there, and every wave is done with the one before
-      ask(t + KG, next, buf ^ 1);
-      next = page_of(t + 2 * KG);
       const int d0 = t * KT;
-      if (t >= keys.t1 || d0 > some_hi || d0 + KT - 1 < some_lo) continue;  // wave-uniform
+      const bool idle = t >= keys.t1 || d0 > some_hi || d0 + KT - 1 < some_lo;  // wave-uniform
       const unsigned char* const kt = group + buf * kBuf;
       const unsigned char* const vt = kt + kTile;
       f32x16_t x[2];
+      if (!idle) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
+          for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NK; ++c)
-          x[u] = mma32<ST>(*reinterpret_cast<const u32x4*>(kt + (32 * u + r32) * RB + (((2 * c + h) ^ kx) * 16)), q[c], x[u]);
+          for (int c = 0; c < NK; ++c)
+            x[u] = mma32<ST>(*reinterpret_cast<const u32x4*>(kt + (32 * u + r32) * RB + (((2 * c + h) ^ kx) * 16)), q[c], x[u]);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      ask(t + KG, next, buf ^ 1);  // its addresses are made while the products run
+      next = page_of(t + 2 * KG);
+      __builtin_amdgcn_sched_barrier(0);
+      if (idle) continue;
       if (d0 < all_lo || d0 + KT - 1 > all_hi) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -837,7 +843,9 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
         top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * p.scale;
       }
-      if (__any(top > m)) {
+      // the weights' base follows the maximum in steps of 2^kSlack or more: sums are rescaled in the
+      // first tile and hardly ever again, and weights up to 2^kSlack round as well as those up to 1
+      if (__any(top > m + kSlack)) {
         top = fmaxf(top, m);
         const float keep = top == kNone ? 1.f : __builtin_amdgcn_exp2f(m - top);
         m = top;
