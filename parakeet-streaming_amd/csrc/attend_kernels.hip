@@ -740,6 +740,10 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     some_lo = min(some_lo, __shfl_xor(some_lo, d));
     some_hi = max(some_hi, __shfl_xor(some_hi, d));
   }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  some_lo = __builtin_amdgcn_readfirstlane(some_lo);
+  some_hi = __builtin_amdgcn_readfirstlane(some_hi);
   f32x16_t o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -770,25 +774,23 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
       }
     };
     unsigned char* const group = smem + kg * 2 * kBuf;
-    auto ask = [&](int t, int page, int buf) {
-      unsigned char* const at = group + buf * kBuf + 16 * wv * RB;
-      if constexpr (!PAGED) {
-        kb = resource_words(p.k + it.b * p.k_sb + (int64_t)it.hk * RB + (int64_t)t * KT * p.k_st, 0, (uint32_t)(KT * p.k_st));
-        vb = resource_words(p.v + it.b * p.v_sb + (int64_t)it.hk * RB + (int64_t)t * KT * p.v_st, 0, (uint32_t)(KT * p.v_st));
-      }
+    // a tile of K or V to the group's buffer
+    auto ask = [&](bool v, int t, int page, int buf) {
+      unsigned char* const at = group + buf * kBuf + (v ? kTile : 0) + 16 * wv * RB;
+      u32x4 from = v ? vb : kb;
+      const int64_t st = v ? p.v_st : p.k_st;
+      if constexpr (!PAGED) from = resource_words((v ? p.v : p.k) + it.b * (v ? p.v_sb : p.k_sb) + (int64_t)it.hk * RB + (int64_t)t * KT * st, 0, (uint32_t)(KT * st));
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int x = i * RPI + lane / C, rt = 16 * wv + x, d = t * KT + rt, c = (lane & (C - 1)) ^ mix<HD>(rt);
         if constexpr (PAGED) {
           const uint32_t mine = (uint32_t)__shfl(page, x);
           const uint32_t in = ((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u);
-          const uint32_t row = mine < (uint32_t)p.num_pages ? mine * page_rows + ((uint32_t)(c >> 2) << p.page_shift) + in : kNowhere;
-          stage_row(kb, at + i * 1024, row, (c & 3) * 16);
-          stage_row(vb, at + kTile + i * 1024, row, (c & 3) * 16);
+          const uint32_t row = mine * page_rows + ((uint32_t)(c >> 2) << p.page_shift) + in;
+          stage_row(from, at + i * 1024, mine < (uint32_t)p.num_pages ? row : kNowhere, (c & 3) * 16);
         } else {
           const bool ok = t < keys.t1 && d <= keys.hi;
-          stage_bytes(kb, at + i * 1024, ok ? (uint32_t)rt * (uint32_t)p.k_st + c * 16 : kNowhere);
-          stage_bytes(vb, at + kTile + i * 1024, ok ? (uint32_t)rt * (uint32_t)p.v_st + c * 16 : kNowhere);
+          stage_bytes(from, at + i * 1024, ok ? (uint32_t)rt * (uint32_t)st + c * 16 : kNowhere);
         }
       }
     };
@@ -798,40 +800,73 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const int l16 = lane & 15, dg = lane >> 4 & 1;
 #pragma unroll
     for (int u = 0; u < 2; ++u) va[u] = 8 * u + 4 * h + (l16 >> 2);
-    int t = keys.t0 + kg, buf = 0;
-    ask(t, page_of(t), 0);
-    int next = page_of(t + KG);
-    const int turns = (keys.t1 - keys.t0 + KG - 1) / KG;
-    for (int turn = 0; turn < turns; ++turn, t += KG, buf ^= 1) {
-      wait_vm<0>();
-      __syncthreads();  // the tile is there, and every wave is done with the one before
-      const int d0 = t * KT;
-      const bool idle = t >= keys.t1 || d0 > some_hi || d0 + KT - 1 < some_lo;  // wave-uniform
-      const unsigned char* const kt = group + buf * kBuf;
-      const unsigned char* const vt = kt + kTile;
-      f32x16_t x[2];
-      if (!idle) {
+    // Scores of tile t from K in buffer b, and the tile before's weights with V in the other one: all matrix
+    // products of a turn, one after the other.
+    u32x4 w[4];
+    f32x16_t x[2];
+    bool weighed = false;  // w holds the weights of the tile before (wave-uniform)
+    auto scores = [&](int b) {
+      const unsigned char* const kt = group + b * kBuf + r32 * RB;
+      u32x4 k[2][4];  // operands of 4 products, asked for 4 ahead
+      auto load = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
-#pragma unroll
-          for (int c = 0; c < NK; ++c)
-            x[u] = mma32<ST>(*reinterpret_cast<const u32x4*>(kt + (32 * u + r32) * RB + (((2 * c + h) ^ kx) * 16)), q[c], x[u]);
+        for (int y = 0; y < 4; ++y) {
+          const int c = 2 * i + (y >> 1);
+          k[i & 1][y] = *reinterpret_cast<const u32x4*>(kt + 32 * RB * (y & 1) + (((2 * c + h) ^ kx) * 16));
         }
+      };
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
+      load(0);
+#pragma unroll
+      for (int i = 0; i < NK / 2; ++i) {
+        if (i + 1 < NK / 2) load(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y & 1] = mma32<ST>(k[i & 1][y], q[2 * i + (y >> 1)], x[y & 1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      ask(t + KG, next, buf ^ 1);  // its addresses are made while the products run
-      next = page_of(t + 2 * KG);
-      __builtin_amdgcn_sched_barrier(0);
-      if (idle) continue;
+    };
+    auto sums_of = [&](int b) {
+      const unsigned char* const vt = group + b * kBuf + kTile;
+      u32x4 v[2][NB];
+      auto load = [&](int k) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          u32x2 part[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int c = (4 * n + 2 * dg + (l16 >> 1 & 1)) ^ mix<HD>(va[u]);
+            const unsigned char* src = vt + (16 * k + va[u]) * RB + c * 16 + (l16 & 1) * 8;
+            part[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)src));
+          }
+          v[k & 1][n] = u32x4{part[0].x, part[0].y, part[1].x, part[1].y};
+        }
+      };
+      load(0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k < 3) load(k + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n] = mma32<ST>(v[k & 1][n], w[k], o[n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto weights = [&](int d0) {
       if (d0 < all_lo || d0 + KT - 1 > all_hi) {
+        const uint32_t from = (uint32_t)(d0 + 4 * h - lo), span = (uint32_t)(hi - lo);  // no keys: hi - lo is -1
+        const bool none = hi < lo;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int d = d0 + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (d < lo || d > hi) x[u][e] = kNone;
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (none || from + (32 * u + 8 * j + e) > span) x[u][4 * j + e] = kNone;
+            __builtin_amdgcn_sched_barrier(0);  // few conditions at a time in scalar registers
           }
       }
       float top = kNone;
@@ -854,33 +889,49 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
         for (int n = 0; n < NB; ++n) o[n] *= keep;
       }
       const float base = m == kNone ? 0.f : m;
-      u32x4 w[4];
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float e[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           e[k] = __builtin_amdgcn_exp2f(fmaf(x[u][k], p.scale, -base));
-          l += e[k];
+          part[k & 3] += e[k];
         }
         w[2 * u] = Tr<ST>::pack(e);
         w[2 * u + 1] = Tr<ST>::pack(e + 8);
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          i16x4_t v[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int c = (4 * n + 2 * dg + (l16 >> 1 & 1)) ^ mix<HD>(va[u]);
-            const unsigned char* src = vt + (16 * k + va[u]) * RB + c * 16 + (l16 & 1) * 8;
-            v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)src);
-          }
-          const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
-          o[n] = mma32<ST>(u32x4{v0.x, v0.y, v1.x, v1.y}, w[k], o[n]);
-        }
+      l += (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    auto meet = [&]() {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    // The two groups take turns at the matrix cores: while one multiplies, the other makes weights. A group's
+    // turn: its tile of K and the tile before of V are there; ask for the next ones; multiply | weigh.
+    int t = keys.t0 + kg, buf = 0;
+    int page = page_of(t), next = page_of(t + KG);
+    ask(false, t, page, 0);
+    const int turns = (keys.t1 - keys.t0 + KG - 1) / KG;
+    if (kg == 1) meet();
+    for (int turn = 0; turn <= turns; ++turn, t += KG, buf ^= 1) {
+      wait_vm<0>();
+      meet();
+      ask(true, t, page, buf);  // behind the last tile zeros, so that no branch holds up the counts of loads
+      ask(false, t + KG, next, buf ^ 1);
+      page = next;
+      next = page_of(t + 2 * KG);
+      const bool idle = t >= keys.t1 || t * KT > some_hi || t * KT + KT - 1 < some_lo;  // wave-uniform
+      __builtin_amdgcn_s_setprio(1);
+      if (weighed) sums_of(buf ^ 1);
+      if (!idle) scores(buf);
+      __builtin_amdgcn_s_setprio(0);
+      meet();
+      weighed = !idle;
+      if (!idle) weights(t * KT);
     }
+    if (KG == 2 && kg == 0) meet();
     wait_vm<0>();  // what was asked for behind the last tile
   }
 
@@ -1069,7 +1120,9 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
   c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 ? 32 : 128;
   c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
-  const int64_t whole = units * c.row_tiles, want = (512 + whole - 1) / whole, most = (keys + 511) / 512;
+  // keys are split over workgroups where the rows leave CUs without one: 256 CUs hold one of attend_many_kernel's
+  // workgroups each, and two or more of attend_few_kernel's
+  const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512, want = (full * 3 / 4 + whole - 1) / whole, most = (keys + 511) / 512;
   int64_t n = want < most ? want : most;
   n = n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
   c.splits = (int)n;
