@@ -677,22 +677,18 @@ __device__ static inline int mix(int r) {
 constexpr float kSlack = 6.f;
 constexpr uint32_t kNowhere = 0xffffffffu;  // past any resource: reads zeros
 
-// A buffer resource as four words: rows of `stride` bytes (0: bytes) from base, `records` of them.
-__device__ static inline u32x4 resource_words(const void* base, uint32_t stride, uint32_t records) {
+// A buffer resource as four words: `records` bytes from base.
+__device__ static inline u32x4 resource_words(const void* base, uint32_t records) {
   const uint64_t at = reinterpret_cast<uint64_t>(base);
-  return u32x4{(uint32_t)at, ((uint32_t)(at >> 32) & 0xffffu) | (stride << 16), records, 0x00020000u};  // word 3 as bytes_rsrc's
+  return u32x4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, records, 0x00020000u};  // word 3 as bytes_rsrc's
 }
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0, which nothing else here uses, is written
-// 16 bytes a lane, from byte `off` of row `row`, to lds + 16 lane (lds wave-uniform). Written as assembly
+// 16 bytes a lane, from byte `off`, to lds + 16 lane (lds wave-uniform). Written as assembly
 // because the compiler waits for every load to LDS that it knows of before any read of LDS,
 // which would end the overlap with the tile that is worked on; it names no register as output,
 // and wait_vm counts it. s_nop: the cycles that m0, and words that vector code may have made, need.
-__device__ static inline void stage_row(const u32x4 r, const unsigned char* lds, uint32_t row, uint32_t off) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 idxen offen lds" ::"s"(at), "v"(u32x2{row, off}), "s"(r) : "memory", "m0");
-}
 __device__ static inline void stage_bytes(const u32x4 r, const unsigned char* lds, uint32_t off) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory", "m0");
@@ -752,45 +748,58 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
   float m = kNone, l = 0.f;
 
   if (keys.t0 < keys.t1) {
-    // What is read, by an index that the hardware checks: pages as rows of 64 bytes, a tile of states by the byte;
-    // kNowhere gives zeros, so that 0 times what memory holds for a key that is not there is 0.
-    u32x4 kb, vb;
-    const uint32_t page_rows = (uint32_t)(p.page_bytes >> 6);  // rows of 64 bytes of a page
-    if constexpr (PAGED) {
-      const uint32_t head = (uint32_t)it.hk * NB << p.page_shift, rows = (uint32_t)p.num_pages * page_rows - head;
-      kb = resource_words(p.k + ((int64_t)head << 6), 64, rows);
-      vb = resource_words(p.v + ((int64_t)head << 6), 64, rows);
-    }
+    // What is read goes by offsets that the hardware checks: kNowhere gives zeros, so that 0 times what memory
+    // holds for a key that is not there is 0.
     const int32_t* const ring = PAGED ? p.rows + it.b * p.rows_stride + 1 : nullptr;
-    // a wave stages rows 16 wv .. 16 wv + 15 of its group's tiles; the page of row lane % 16
+    // A wave stages rows 16 wv .. 16 wv + 15 of its group's tiles: of one page, since pages have 16 frames or
+    // more here and k0 is a multiple of KT, so that a load needs no arithmetic but its page's address.
     auto page_of = [&](int t) {
       if constexpr (PAGED) {
-        const int d = t * KT + 16 * wv + (lane & 15);
+        const int d = t * KT + 16 * wv;
         int page = -1;
-        if (t < keys.t1 && d >= keys.lo && d <= keys.hi) page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
+        if (t < keys.t1 && d + 15 >= keys.lo && d <= keys.hi)
+          page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
         return page;
       } else {
         return 0;
       }
     };
     unsigned char* const group = smem + kg * 2 * kBuf;
+    // a lane's byte in the wave's 16 rows, of each load
+    uint32_t koff[LOADS], voff[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * RPI + lane / C, c = (lane & (C - 1)) ^ mix<HD>(x);
+      koff[i] = PAGED ? (((uint32_t)(c >> 2) << p.page_shift) + x) * 64 + (c & 3) * 16 : (uint32_t)x * (uint32_t)p.k_st + c * 16;
+      voff[i] = PAGED ? koff[i] : (uint32_t)x * (uint32_t)p.v_st + c * 16;
+    }
     // a tile of K or V to the group's buffer
     auto ask = [&](bool v, int t, int page, int buf) {
       unsigned char* const at = group + buf * kBuf + (v ? kTile : 0) + 16 * wv * RB;
-      u32x4 from = v ? vb : kb;
-      const int64_t st = v ? p.v_st : p.k_st;
-      if constexpr (!PAGED) from = resource_words((v ? p.v : p.k) + it.b * (v ? p.v_sb : p.k_sb) + (int64_t)it.hk * RB + (int64_t)t * KT * st, 0, (uint32_t)(KT * st));
+      const int d = t * KT + 16 * wv;
+      const unsigned char* base = v ? p.v : p.k;
+      bool there = t < keys.t1;
+      uint32_t records;
+      if constexpr (PAGED) {
+        const uint32_t mine = (uint32_t)__builtin_amdgcn_readfirstlane(page);
+        there = mine < (uint32_t)p.num_pages;
+        base += (int64_t)(there ? mine : 0) * p.page_bytes + ((int64_t)it.hk * NB << (p.page_shift + 6)) +
+                ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6);
+        records = 0x7fffffffu;  // offsets are within the page, below 2^31
+      } else {
+        const int64_t st = v ? p.v_st : p.k_st;
+        base += it.b * (v ? p.v_sb : p.k_sb) + (int64_t)it.hk * RB + (int64_t)(there ? d : 0) * st;
+        records = (uint32_t)(16 * st);
+      }
+      const u32x4 from = resource_words(base, records);
+      if (there && d >= keys.lo && d + 15 <= keys.hi) {  // wave-uniform
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int x = i * RPI + lane / C, rt = 16 * wv + x, d = t * KT + rt, c = (lane & (C - 1)) ^ mix<HD>(rt);
-        if constexpr (PAGED) {
-          const uint32_t mine = (uint32_t)__shfl(page, x);
-          const uint32_t in = ((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u);
-          const uint32_t row = mine * page_rows + ((uint32_t)(c >> 2) << p.page_shift) + in;
-          stage_row(from, at + i * 1024, mine < (uint32_t)p.num_pages ? row : kNowhere, (c & 3) * 16);
-        } else {
-          const bool ok = t < keys.t1 && d <= keys.hi;
-          stage_bytes(from, at + i * 1024, ok ? (uint32_t)rt * (uint32_t)st + c * 16 : kNowhere);
+        for (int i = 0; i < LOADS; ++i) stage_bytes(from, at + i * 1024, v ? voff[i] : koff[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int x = d + i * RPI + lane / C;
+          stage_bytes(from, at + i * 1024, there && x >= keys.lo && x <= keys.hi ? v ? voff[i] : koff[i] : kNowhere);
         }
       }
     };
@@ -1114,10 +1123,10 @@ struct AttendCut {
   int64_t groups;  // workgroups
 };
 
-AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, int keys) {
+AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, int keys, bool narrow) {
   AttendCut c;
   const int64_t R = (int64_t)chunk * (heads / kv_heads), units = (int64_t)batch * kv_heads;
-  c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 ? 32 : 128;
+  c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 || narrow ? 32 : 128;
   c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
   // keys are split over workgroups where the rows leave CUs without one: 256 CUs hold one of attend_many_kernel's
@@ -1157,7 +1166,7 @@ template <typename ST, bool PAGED>
 int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, void* workspace, int device, hipStream_t s) {
   p.G = p.Hq / p.Hkv;
   p.R = p.T * p.G;
-  const AttendCut c = attend_cut(dtype, p.B, p.T, p.Hq, p.Hkv, keys);
+  const AttendCut c = attend_cut(dtype, p.B, p.T, p.Hq, p.Hkv, keys, PAGED && p.page_shift < 4);
   p.row_tiles = c.row_tiles;
   p.splits = c.splits;
   const int64_t rows = (int64_t)p.B * p.T * p.Hq;
@@ -1183,6 +1192,7 @@ int chunk_attn(const pk_chunk_attn_args* a, hipStream_t s) {
   if (a->left < 0 || L.max_pages <= 0 || L.rows_stride < 1 + L.max_pages || ((int64_t)a->left + a->chunk + L.page_size - 2) / L.page_size + 1 > L.max_pages)
     return fail(PK_ERR_INVALID, "%s: %d ring entries of %d frames do not hold any window of %d + %d (rows_stride %d)", what, L.max_pages, L.page_size,
                 a->left, a->chunk, L.rows_stride);
+  if (L.page_size > (1 << 20)) return fail(PK_ERR_UNSUPPORTED, "%s: pages of %d frames (built: up to 2^20)", what, L.page_size);
   if ((int64_t)a->left + a->chunk > (1 << 30)) return fail(PK_ERR_INVALID, "%s: a window of more than 2^30 positions", what);
   if (a->batch == 0 || a->chunk == 0) return PK_OK;
   if (!L.rows) return fail(PK_ERR_INVALID, "%s: rows is NULL", what);
@@ -1274,7 +1284,9 @@ int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream) { PK_BY_
 
 int64_t pk_attn_workspace_bytes(int32_t dtype, int32_t batch, int32_t chunk, int32_t num_heads, int32_t kv_heads, int32_t head_dim, int32_t keys) {
   if (batch <= 0 || chunk <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 || head_dim <= 0 || keys < 0) return 0;
-  return pk::attend_space((int64_t)batch * chunk * num_heads, pk::attend_cut(dtype, batch, chunk, num_heads, kv_heads, keys).splits, head_dim);
+  // for pages of any size
+  const int a = pk::attend_cut(dtype, batch, chunk, num_heads, kv_heads, keys, false).splits, b = pk::attend_cut(dtype, batch, chunk, num_heads, kv_heads, keys, true).splits;
+  return pk::attend_space((int64_t)batch * chunk * num_heads, a > b ? a : b, head_dim);
 }
 
 int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream) { PK_BY_DTYPE("pk_chunk_attn", chunk_attn) }
