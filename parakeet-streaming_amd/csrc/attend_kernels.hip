@@ -5,6 +5,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "pk_common.h"
 #include "pk_device.h"
@@ -675,7 +676,7 @@ __device__ static inline int mix(int r) {
 }
 
 constexpr float kSlack = 6.f;
-constexpr uint32_t kNowhere = 0xffffffffu;  // past any resource: reads zeros
+constexpr uint32_t kNowhere = 0xc0000000u;  // past any resource, also with an instruction's offset: reads zeros
 
 // A buffer resource as four words: `records` bytes from base.
 __device__ static inline u32x4 resource_words(const void* base, uint32_t records) {
@@ -685,13 +686,24 @@ __device__ static inline u32x4 resource_words(const void* base, uint32_t records
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0, which nothing else here uses, is written
-// 16 bytes a lane, from byte `off`, to lds + 16 lane (lds wave-uniform). Written as assembly
-// because the compiler waits for every load to LDS that it knows of before any read of LDS,
-// which would end the overlap with the tile that is worked on; it names no register as output,
-// and wait_vm counts it. s_nop: the cycles that m0, and words that vector code may have made, need.
-__device__ static inline void stage_bytes(const u32x4 r, const unsigned char* lds, uint32_t off) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory", "m0");
+// N loads of 16 bytes a lane: from byte off[i] + 1024 i to lds + 1024 i + 16 lane (lds wave-uniform; an
+// instruction's offset counts on both sides). Written as assembly because the compiler waits for every
+// load to LDS that it knows of before any read of LDS, which would end the overlap with the tile that
+// is worked on; it names no register as output, and wait_vm counts it. s_nop: the cycles that m0, and
+// words that vector code may have made, need.
+template <int N>
+__device__ static inline void stage_bytes(const u32x4 r, uint32_t lds, const uint32_t (&off)[N]) {
+  static_assert(N == 2 || N == 4, "16 rows of 128 or 256 bytes");
+  if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\tbuffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds" ::"s"(lds),
+                 "v"(off[0]), "v"(off[1]), "s"(r)
+                 : "memory", "m0");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\tbuffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\tbuffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds" ::"s"(lds),
+        "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(r)
+        : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -753,54 +765,60 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const int32_t* const ring = PAGED ? p.rows + it.b * p.rows_stride + 1 : nullptr;
     // A wave stages rows 16 wv .. 16 wv + 15 of its group's tiles: of one page, since pages have 16 frames or
     // more here and k0 is a multiple of KT, so that a load needs no arithmetic but its page's address.
+    // Page of tile t's rows, for tiles in ascending order (the ring entry goes along, so that there is a division
+    // only where it wraps). A scalar load: the counts of vector loads are those of the tiles alone.
+    uint32_t at_page = 0, at_entry = 0;
     auto page_of = [&](int t) {
       if constexpr (PAGED) {
         const int d = t * KT + 16 * wv;
-        int page = -1;
-        if (t < keys.t1 && d + 15 >= keys.lo && d <= keys.hi)
-          page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
-        return page;
+        if (t >= keys.t1 || d + 15 < keys.lo || d > keys.hi) return -1;
+        const uint32_t page = ((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift;
+        at_entry += page - at_page;
+        at_page = page;
+        if (at_entry >= (uint32_t)p.max_pages) at_entry %= (uint32_t)p.max_pages;
+        return (int)reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(ring))[at_entry];
       } else {
         return 0;
       }
     };
     unsigned char* const group = smem + kg * 2 * kBuf;
-    // a lane's byte in the wave's 16 rows, of each load
+    const uint32_t group_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)group) + 16 * wv * RB;
+    // a lane's byte in the wave's 16 rows, of each load (sources start kBack early, for the instructions' offsets)
+    constexpr uint32_t kBack = 1024 * (LOADS - 1);
     uint32_t koff[LOADS], voff[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int x = i * RPI + lane / C, c = (lane & (C - 1)) ^ mix<HD>(x);
-      koff[i] = PAGED ? (((uint32_t)(c >> 2) << p.page_shift) + x) * 64 + (c & 3) * 16 : (uint32_t)x * (uint32_t)p.k_st + c * 16;
-      voff[i] = PAGED ? koff[i] : (uint32_t)x * (uint32_t)p.v_st + c * 16;
+      koff[i] = kBack - 1024 * i + (PAGED ? (((uint32_t)(c >> 2) << p.page_shift) + x) * 64 + (c & 3) * 16 : (uint32_t)x * (uint32_t)p.k_st + c * 16);
+      voff[i] = PAGED ? koff[i] : kBack - 1024 * i + (uint32_t)x * (uint32_t)p.v_st + c * 16;
     }
-    // a tile of K or V to the group's buffer
-    auto ask = [&](bool v, int t, int page, int buf) {
-      unsigned char* const at = group + buf * kBuf + (v ? kTile : 0) + 16 * wv * RB;
+    const unsigned char* const kb = p.k - kBack + (PAGED ? (int64_t)it.hk * NB << (p.page_shift + 6) : it.b * p.k_sb + (int64_t)it.hk * RB);
+    const unsigned char* const vb = p.v - kBack + (PAGED ? (int64_t)it.hk * NB << (p.page_shift + 6) : it.b * p.v_sb + (int64_t)it.hk * RB);
+    // where the wave's rows of tile t are: bytes from the base of pages, or the first of the states; -1: nowhere
+    auto place_of = [&](int t, int page) -> int64_t {
       const int d = t * KT + 16 * wv;
-      const unsigned char* base = v ? p.v : p.k;
-      bool there = t < keys.t1;
-      uint32_t records;
       if constexpr (PAGED) {
-        const uint32_t mine = (uint32_t)__builtin_amdgcn_readfirstlane(page);
-        there = mine < (uint32_t)p.num_pages;
-        base += (int64_t)(there ? mine : 0) * p.page_bytes + ((int64_t)it.hk * NB << (p.page_shift + 6)) +
-                ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6);
-        records = 0x7fffffffu;  // offsets are within the page, below 2^31
+        if ((uint32_t)page >= (uint32_t)p.num_pages) return -1;
+        return page * p.page_bytes + ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6);
       } else {
-        const int64_t st = v ? p.v_st : p.k_st;
-        base += it.b * (v ? p.v_sb : p.k_sb) + (int64_t)it.hk * RB + (int64_t)(there ? d : 0) * st;
-        records = (uint32_t)(16 * st);
+        return t < keys.t1 ? d : -1;
       }
-      const u32x4 from = resource_words(base, records);
-      if (there && d >= keys.lo && d + 15 <= keys.hi) {  // wave-uniform
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) stage_bytes(from, at + i * 1024, v ? voff[i] : koff[i]);
+    };
+    auto ask = [&](bool v, int t, int64_t place, int buf) {
+      const int d = t * KT + 16 * wv;
+      const int64_t st = v ? p.v_st : p.k_st;
+      const u32x4 from = resource_words((v ? vb : kb) + (PAGED ? max(place, (int64_t)0) : max(place, (int64_t)0) * st), PAGED ? 0x7fffffffu : (uint32_t)(15 * st) + RB + kBack);
+      const uint32_t to = group_at + buf * kBuf + (v ? kTile : 0);
+      if (place >= 0 && d >= keys.lo && d + 15 <= keys.hi) {  // wave-uniform
+        stage_bytes<LOADS>(from, to, v ? voff : koff);
       } else {
+        uint32_t off[LOADS];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
           const int x = d + i * RPI + lane / C;
-          stage_bytes(from, at + i * 1024, there && x >= keys.lo && x <= keys.hi ? v ? voff[i] : koff[i] : kNowhere);
+          off[i] = place >= 0 && x >= keys.lo && x <= keys.hi ? (v ? voff[i] : koff[i]) : kNowhere;
         }
+        stage_bytes<LOADS>(from, to, off);
       }
     };
     // operand addresses in a tile
@@ -809,8 +827,8 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const int l16 = lane & 15, dg = lane >> 4 & 1;
 #pragma unroll
     for (int u = 0; u < 2; ++u) va[u] = 8 * u + 4 * h + (l16 >> 2);
-    // Scores of tile t from K in buffer b, and the tile before's weights with V in the other one: all matrix
-    // products of a turn, one after the other.
+    // Scores of a tile from K in buffer b, and the tile before's weights with V in buffer b: a turn's matrix
+    // products.
     u32x4 w[4];
     f32x16_t x[2];
     bool weighed = false;  // w holds the weights of the tile before (wave-uniform)
@@ -917,28 +935,41 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
-    // The two groups take turns at the matrix cores: while one multiplies, the other makes weights. A group's
-    // turn: its tile of K and the tile before of V are there; ask for the next ones; multiply | weigh.
-    int t = keys.t0 + kg, buf = 0;
-    int page = page_of(t), next = page_of(t + KG);
-    ask(false, t, page, 0);
+    // The two groups take turns at the matrix cores: while one multiplies, the other makes weights. A turn of a
+    // group: multiply (tile `turn`'s K, the tile before's V) | ask for the tile after next's K and the next one's V,
+    // whose buffers are free now, and weigh. So what a turn multiplies was asked for in the turn before
+    // the last, and only those loads are waited for. Behind the last tile zeros are asked for.
+    auto tile = [&](int turn) { return keys.t0 + kg + turn * KG; };
     const int turns = (keys.t1 - keys.t0 + KG - 1) / KG;
+    int64_t at = place_of(tile(0), page_of(tile(0)));
+    ask(false, tile(0), at, 0);
+    ask(true, tile(0), at, 0);
+    at = place_of(tile(1), page_of(tile(1)));  // of the tile whose V is asked for next
+    ask(false, tile(1), at, 1);
+    int page = page_of(tile(2));
     if (kg == 1) meet();
-    for (int turn = 0; turn <= turns; ++turn, t += KG, buf ^= 1) {
-      wait_vm<0>();
+    wait_vm<0>();
+    auto turn_of = [&](int turn, auto parity) {
+      constexpr int b = decltype(parity)::value;
+      wait_vm<2 * LOADS>();
       meet();
-      ask(true, t, page, buf);  // behind the last tile zeros, so that no branch holds up the counts of loads
-      ask(false, t + KG, next, buf ^ 1);
-      page = next;
-      next = page_of(t + 2 * KG);
+      const int t = tile(turn);
       const bool idle = t >= keys.t1 || t * KT > some_hi || t * KT + KT - 1 < some_lo;  // wave-uniform
       __builtin_amdgcn_s_setprio(1);
-      if (weighed) sums_of(buf ^ 1);
-      if (!idle) scores(buf);
+      if (weighed) sums_of(b ^ 1);
+      if (!idle) scores(b);
       __builtin_amdgcn_s_setprio(0);
       meet();
+      ask(true, tile(turn + 1), at, b ^ 1);
+      at = place_of(tile(turn + 2), page);
+      ask(false, tile(turn + 2), at, b);
+      page = page_of(tile(turn + 3));
       weighed = !idle;
       if (!idle) weights(t * KT);
+    };
+    for (int turn = 0; turn <= turns; turn += 2) {
+      turn_of(turn, std::integral_constant<int, 0>());
+      turn_of(turn + 1, std::integral_constant<int, 1>());  // one past the last may be empty
     }
     if (KG == 2 && kg == 0) meet();
     wait_vm<0>();  // what was asked for behind the last tile
