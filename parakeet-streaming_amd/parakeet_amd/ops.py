@@ -8,6 +8,7 @@ here computes on the CPU: without the library or a HIP device the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -1513,18 +1514,27 @@ def _refuse_adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
 # a text decoder's attention
 
 
-def _plain_call(what: str, tensors: list[torch.Tensor]) -> None:
-    """Refuses calls that something follows or rewrites, and such that need a gradient."""
+def _follows(*tensors: torch.Tensor) -> bool:
+    """Whether something may follow or rewrite a call on these tensors, or needs its gradient."""
     if _overridden(*tensors) or _forward_ad._current_level >= 0 or _tracing() or torch.is_autocast_enabled() or _dispatch_modes():
-        _refuse_transforms(what, tensors)
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return False
+
+
+def _refuse_followed(what: str, tensors: list[torch.Tensor]) -> None:
+    _refuse_transforms(what, tensors)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
 
 
-def _head_rows(name: str, t: torch.Tensor, B: int, T: int, dtype: torch.dtype, heads: int | None = None) -> None:
-    """t is [B, T, whole heads] of dtype with 16-byte aligned rows."""
-    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != T or (heads is not None and t.shape[2] != heads):
-        raise ValueError(f"{name}: expected shape {(B, T, 'D' if heads is None else heads)}, got {tuple(t.shape)}")
+def _head_rows(name: str, t: torch.Tensor, B: int, T: int, dtype: torch.dtype, columns: int | None = None) -> None:
+    """Says what is wrong with t as [B, T, whole heads] of dtype with 16-byte aligned rows."""
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != T or (columns is not None and t.shape[2] != columns):
+        raise ValueError(f"{name}: expected shape {(B, T, 'D' if columns is None else columns)}, got {tuple(t.shape)}")
     if t.dtype is not dtype:
         raise TypeError(f"{name}: dtype {t.dtype} != {dtype}")
     if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or (t.stride(0) | t.stride(1)) * t.element_size() % 16):
@@ -1539,7 +1549,26 @@ def _head_dim(query: torch.Tensor, num_heads: int) -> int:
     hd = query.shape[2] // H
     if hd not in (64, 128):
         raise NotImplementedError(f"built for heads of 64 and 128 columns, got {hd}")
+    dtype_code(query.dtype)
     return hd
+
+
+def _refuse_pages(pages: PagedKV, dtype: torch.dtype, hd: int) -> None:
+    kp = pages.k_pool
+    pages.layout()
+    if kp.shape[3] % hd or kp.shape[3] == 0:
+        raise ValueError(f"pages of {kp.shape[3]} columns are not whole heads of {hd}")
+    if kp.dtype is not dtype:
+        raise TypeError(f"pages dtype {kp.dtype} != {dtype}")
+
+
+_ELEMENT = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_space(*sizes: int) -> int:
+    """Workspace bytes of an attention, of its sizes alone."""
+    return lib().pk_attn_workspace_bytes(*sizes)
 
 
 def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1603,79 +1632,76 @@ def qk_norm_append(
     rotary / 2), or (2 i, 2 i + 1) where ``interleaved``.  ``positions``: int32 [B, T]; None: token t of stream b is
     at ``pages.rows[b, 0] + t``.  The turns of an angle are made in 64 bits.  No gradients."""
     operands = [t for t in (query, key, value, q_weight, k_weight, inv_freq) if t is not None]
-    _plain_call("qk_norm_append", operands)
-    hd, kp, dt = _head_dim(query, num_heads), pages.k_pool, query.dtype
-    B, T, _ = query.shape
-    D = kp.shape[-1]
-    if D % hd:
-        raise ValueError(f"pages of {D} columns are not whole heads of {hd}")
-    if kp.dtype is not dt:
-        raise TypeError(f"pages dtype {kp.dtype} != {dt}")
-    _head_rows("query", query, B, T, dt)
-    _head_rows("key", key, B, T, dt, D)
-    _head_rows("value", value, B, T, dt, D)
-    dev = _require_device(query, key, value, kp, pages.v_pool, pages.rows, slot_map)
-    a = QkNormAppendArgs()
-    a.pages = pages.layout()
+    if _follows(*operands):
+        _refuse_followed("qk_norm_append", operands)
+    kp, vp, rows, dt, at, shape = pages.k_pool, pages.v_pool, pages.rows, query.dtype, query.get_device(), query.shape
+    H, E, M = int(num_heads), _ELEMENT.get(dt, 0), pages.max_pages
+    B, T, W = shape if len(shape) == 3 else (0, 0, 0)
+    Ly, N, P, D = kp.shape if kp.dim() == 4 else (0, 0, 0, 0)
+    hd = W // H if H > 0 else 0
+    n = 2 * inv_freq.numel() if inv_freq is not None else 0
+    qp, kyp, vlp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    if not (
+        query.is_cuda and (hd == 64 or hd == 128) and W == H * hd and E and D and D % hd == 0
+        and key.shape == (B, T, D) and value.shape == (B, T, D) and slot_map.shape == (B, T) and vp.shape == kp.shape
+        and key.dtype is dt and value.dtype is dt and kp.dtype is dt and vp.dtype is dt and slot_map.dtype is _INT32 and rows.dtype is _INT32
+        and key.get_device() == at and value.get_device() == at and kp.get_device() == at and vp.get_device() == at and rows.get_device() == at and slot_map.get_device() == at
+        and kp.is_contiguous() and vp.is_contiguous() and rows.dim() == 2 and rows.shape[1] >= 1 + M
+        and (rows.shape[0] >= B or n == 0 or positions is not None) and (n == 0 or (16 <= n <= hd and n & (n - 1) == 0))
+        and 0 <= eps < math.inf
+    ):
+        _refuse_norm_append(query, key, value, pages, slot_map, H, q_weight, k_weight, inv_freq, positions, eps)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            if w.shape != (hd,) or w.dtype is not dt or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
-                raise ValueError(f"{name} must be contiguous, 16-byte aligned [{hd}] of {dt} on {dev}, got {tuple(w.shape)} {w.dtype}")
-            setattr(a, name, w.data_ptr())
-    if inv_freq is not None:
-        n = 2 * inv_freq.numel()
-        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != dev:
-            raise ValueError(f"inv_freq must be contiguous float64 [rotary / 2] on {dev}, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
-        if n < 16 or n > hd or n & (n - 1):
-            raise NotImplementedError(f"built for rotations of 16 to {hd} columns, a power of two, got {n}")
-        a.rotary, a.inv_freq = n, inv_freq.data_ptr()
-        if positions is None and pages.rows.shape[0] < B:
-            raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
-    for name, t in (("slot_map", slot_map), ("positions", positions)):
-        if t is not None:
-            if t.dtype is not _INT32 or t.shape != (B, T) or (t.numel() and t.stride(1) != 1) or t.device != dev:
-                raise ValueError(f"{name} must be int32 {[B, T]} with unit inner stride on {dev}, got {tuple(t.shape)} {t.dtype}")
-    if not eps >= 0 or eps == math.inf:
-        raise ValueError(f"eps must be >= 0, got {eps}")
-    out = _head_out(out, query, dev, [key, value, kp, pages.v_pool])
+        if w is not None and (w.shape != (hd,) or w.dtype is not dt or w.get_device() != at or w.data_ptr() % 16 or not w.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous, 16-byte aligned [{hd}] of {dt} on {query.device}, got {tuple(w.shape)} {w.dtype}")
+    if n and (inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or inv_freq.get_device() != at or not inv_freq.is_contiguous()):
+        raise ValueError(f"inv_freq must be contiguous float64 [rotary / 2] on {query.device}, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    if positions is not None and (positions.shape != (B, T) or positions.dtype is not _INT32 or positions.get_device() != at):
+        raise ValueError(f"positions must be int32 {[B, T]} on {query.device}, got {tuple(positions.shape)} {positions.dtype}")
+    if out is None:
+        out = torch.empty_like(query)
+    else:
+        out = _head_out(out, query, query.device, [key, value, kp, vp])
     if B == 0 or T == 0:
         return out
-    a.dtype, a.device, a.layer, a.batch, a.chunk, a.num_heads, a.head_dim = dtype_code(dt), _index(dev), int(layer), B, T, int(num_heads), hd
-    a.interleaved, a.eps = int(bool(interleaved)), float(eps)
-    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
-    a.query_stride_b, a.query_stride_t, _ = query.stride()
-    a.key_stride_b, a.key_stride_t, _ = key.stride()
-    a.value_stride_b, a.value_stride_t, _ = value.stride()
-    a.out_stride_b, a.out_stride_t, _ = out.stride()
-    a.slot_map, a.slot_map_stride_b = slot_map.data_ptr(), slot_map.stride(0)
-    if positions is not None:
-        a.positions, a.positions_stride_b = positions.data_ptr(), positions.stride(0)
-    check(lib().pk_qk_norm_append(ctypes.byref(a), _stream(dev)), "pk_qk_norm_append")
+    (qb, qt, qu), (kb, kt, ku), (vb, vt, vu), (ob, ot, _), (mb, mu) = query.stride(), key.stride(), value.stride(), out.stride(), slot_map.stride()
+    rb, ru = rows.stride()
+    if (
+        qu != 1 or ku != 1 or vu != 1 or ((qp | kyp | vlp) & 15) or ((qb | qt | kb | kt | vb | vt) * E & 15) or (mu != 1 and T > 1) or (ru != 1 and n)
+        or (positions is not None and positions.stride(1) != 1 and T > 1)
+    ):
+        _refuse_norm_append(query, key, value, pages, slot_map, H, q_weight, k_weight, inv_freq, positions, eps)
+    stream = torch._C._cuda_getCurrentRawStream(at)
+    a = QkNormAppendArgs(
+        _DTYPES[dt], at, PagedLayout(kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M), layer, B, T, H, hd, n, 1 if interleaved else 0, eps,
+        qp, qb, qt, kyp, kb, kt, vlp, vb, vt, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+        inv_freq.data_ptr() if n else None, None if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
+        slot_map.data_ptr(), mb, out.data_ptr(), ob, ot,
+    )
+    check(lib().pk_qk_norm_append(ctypes.byref(a), stream), "pk_qk_norm_append")
     return out
 
 
-def _attend(a, query: torch.Tensor, out: torch.Tensor, B: int, T: int, H: int, Hkv: int, hd: int, keys: int, scale: float | None,
-            lengths: torch.Tensor | None, dev: torch.device):
-    """What both attentions put into their arguments; returns the workspace, to be kept until the launch."""
-    if H % Hkv:
-        raise ValueError(f"{H} query heads are not whole groups over {Hkv} key heads")
-    if scale is None:
-        scale = hd**-0.5
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale must be > 0 and finite, got {scale}")
-    if lengths is not None:
-        a.lengths = _i32(lengths, "lengths", (B,))
-        _require_device(query, lengths)
-    a.dtype, a.device, a.batch, a.chunk, a.num_heads, a.head_dim, a.scale = dtype_code(query.dtype), _index(dev), B, T, H, hd, scale
-    a.query, a.out = query.data_ptr(), out.data_ptr()
-    a.query_stride_b, a.query_stride_t, _ = query.stride()
-    a.out_stride_b, a.out_stride_t, _ = out.stride()
-    n = lib().pk_attn_workspace_bytes(a.dtype, B, T, H, Hkv, hd, keys)
-    if n:
-        space = torch.empty(n, dtype=torch.uint8, device=dev)
-        a.workspace = space.data_ptr()
-        return space
-    return None
+def _refuse_norm_append(query, key, value, pages, slot_map, H, q_weight, k_weight, inv_freq, positions, eps) -> None:
+    """Says what :func:`qk_norm_append` does not take of a call."""
+    hd, dt = _head_dim(query, H), query.dtype
+    B, T, _ = query.shape
+    _refuse_pages(pages, dt, hd)
+    D = pages.k_pool.shape[3]
+    _head_rows("query", query, B, T, dt)
+    _head_rows("key", key, B, T, dt, D)
+    _head_rows("value", value, B, T, dt, D)
+    dev = _require_device(query, key, value, pages.k_pool, pages.v_pool, pages.rows, slot_map)
+    if inv_freq is not None:
+        n = 2 * inv_freq.numel()
+        if n < 16 or n > hd or n & (n - 1):
+            raise NotImplementedError(f"built for rotations of 16 to {hd} columns, a power of two, got {n}")
+        if positions is None and pages.rows.shape[0] < B:
+            raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
+    for name, t in (("slot_map", slot_map), ("positions", positions)):
+        if t is not None and (t.dtype is not _INT32 or t.shape != (B, T) or (t.numel() and t.stride(1) != 1)):
+            raise ValueError(f"{name} must be int32 {[B, T]} with unit inner stride on {dev}, got {tuple(t.shape)} {t.dtype}")
+    raise ValueError(f"qk_norm_append does not take query {tuple(query.shape)} with eps {eps}")
 
 
 def chunk_attn(
@@ -1698,31 +1724,72 @@ def chunk_attn(
     num_heads * head_dim]: zeros past a stream's tokens and where no key is there; ``out`` may be ``query``.  ``scale``: None is
     head_dim ** -0.5.  fp32 accumulation and softmax.  What a token gets depends on the keys and values that
     it sees alone.  No gradients."""
-    _plain_call("chunk_attn", [query])
-    hd, kp, dt = _head_dim(query, num_heads), pages.k_pool, query.dtype
-    B, T, _ = query.shape
-    a = ChunkAttnArgs()
-    a.pages = pages.layout()
-    P, D = kp.shape[2:]
-    if D % hd or D == 0:
-        raise ValueError(f"pages of {D} columns are not whole heads of {hd}")
-    if kp.dtype is not dt:
-        raise TypeError(f"pages dtype {kp.dtype} != {dt}")
-    _head_rows("query", query, B, T, dt)
-    dev = _require_device(query, kp, pages.v_pool, pages.rows)
-    if pages.rows.shape[0] < B:
-        raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
-    most = (pages.max_pages - 1) * P + 1 - T
-    left = most if left is None else int(left)
-    if not 0 <= left <= most:
-        raise ValueError(f"{pages.max_pages} ring entries of {P} frames hold {most} positions before {T} new ones at any alignment, left is {left}")
-    out = _head_out(out, query, dev, [kp, pages.v_pool, pages.rows] + ([lengths] if lengths is not None else []))
-    space = _attend(a, query, out, B, T, int(num_heads), D // hd, hd, left + T, scale, lengths, dev)  # noqa: F841
+    if _follows(query):
+        _refuse_followed("chunk_attn", [query])
+    kp, vp, rows, dt, at, shape = pages.k_pool, pages.v_pool, pages.rows, query.dtype, query.get_device(), query.shape
+    H, E, M = int(num_heads), _ELEMENT.get(dt, 0), pages.max_pages
+    B, T, W = shape if len(shape) == 3 else (0, 0, 0)
+    Ly, N, P, D = kp.shape if kp.dim() == 4 else (0, 0, 0, 0)
+    hd = W // H if H > 0 else 0
+    most = (M - 1) * P + 1 - T
+    if left is None:
+        left = most
+    if scale is None:
+        scale = hd**-0.5 if hd else 1.0
+    qp = query.data_ptr()
+    if not (
+        query.is_cuda and (hd == 64 or hd == 128) and W == H * hd and E and D and D % hd == 0 and H * hd % D == 0
+        and vp.shape == kp.shape and rows.dim() == 2 and rows.shape[0] >= B and rows.shape[1] >= 1 + M
+        and kp.dtype is dt and vp.dtype is dt and rows.dtype is _INT32
+        and kp.get_device() == at and vp.get_device() == at and rows.get_device() == at and kp.is_contiguous() and vp.is_contiguous()
+        and 0 <= left <= most and 0 < scale < math.inf
+        and (lengths is None or (lengths.shape == (B,) and lengths.dtype is _INT32 and lengths.get_device() == at and lengths.is_contiguous()))
+    ):
+        _refuse_chunk_attn(query, pages, H, lengths, left, most, scale)
+    if out is None:
+        out = torch.empty_like(query)
+    else:
+        out = _head_out(out, query, query.device, [kp, vp, rows] + ([lengths] if lengths is not None else []))
     if B == 0 or T == 0:
         return out
-    a.layer, a.left = int(layer), left
-    check(lib().pk_chunk_attn(ctypes.byref(a), _stream(dev)), "pk_chunk_attn")
+    (qb, qt, qu), (ob, ot, _), (rb, ru) = query.stride(), out.stride(), rows.stride()
+    if qu != 1 or qp & 15 or (qb | qt) * E & 15 or ru != 1:
+        _refuse_chunk_attn(query, pages, H, lengths, left, most, scale)
+    code, stream = _DTYPES[dt], torch._C._cuda_getCurrentRawStream(at)
+    n = _attn_space(code, B, T, H, D // hd, hd, left + T)
+    space = torch.empty(n, dtype=torch.uint8, device=query.device) if n else None
+    a = ChunkAttnArgs(
+        code, at, PagedLayout(kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M), layer, B, T, H, hd, left, scale, qp, qb, qt,
+        None if lengths is None else lengths.data_ptr(), out.data_ptr(), ob, ot, None if space is None else space.data_ptr(),
+    )
+    check(lib().pk_chunk_attn(ctypes.byref(a), stream), "pk_chunk_attn")
     return out
+
+
+def _refuse_chunk_attn(query, pages, H, lengths, left, most, scale) -> None:
+    """Says what :func:`chunk_attn` does not take of a call."""
+    hd, dt = _head_dim(query, H), query.dtype
+    B, T, _ = query.shape
+    _refuse_pages(pages, dt, hd)
+    _head_rows("query", query, B, T, dt)
+    _require_device(query, pages.k_pool, pages.v_pool, pages.rows)
+    if pages.rows.shape[0] < B:
+        raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
+    if not 0 <= left <= most:
+        raise ValueError(f"{pages.max_pages} ring entries of {pages.k_pool.shape[2]} frames hold {most} positions before {T} new ones at any "
+                         f"alignment, left is {left}")
+    _refuse_attention(query, H, pages.k_pool.shape[3] // hd, lengths, scale)
+
+
+def _refuse_attention(query, H, kv_heads, lengths, scale) -> None:
+    if H % kv_heads:
+        raise ValueError(f"{H} query heads are not whole groups over {kv_heads} key heads")
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be > 0 and finite, got {scale}")
+    if lengths is not None:
+        _i32(lengths, "lengths", (query.shape[0],))
+        _require_device(query, lengths)
+    raise ValueError(f"attention does not take query {tuple(query.shape)} with strides {query.stride()}")
 
 
 def cross_attn(
@@ -1742,9 +1809,46 @@ def cross_attn(
     Several texts of one stream are rows of its T.  Returns [B, T, num_heads * head_dim], zeros where there is no state; ``out`` may be
     ``query``.  Heads of 64 or 128 columns, ``scale`` None is head_dim ** -0.5, fp32 accumulation and
     softmax.  No gradients."""
-    _plain_call("cross_attn", [query, key, value])
-    hd, dt = _head_dim(query, num_heads), query.dtype
-    dtype_code(dt)
+    if _follows(query, key, value):
+        _refuse_followed("cross_attn", [query, key, value])
+    dt, at, shape, kshape = query.dtype, query.get_device(), query.shape, key.shape
+    H, E = int(num_heads), _ELEMENT.get(dt, 0)
+    B, T, W = shape if len(shape) == 3 else (0, 0, 0)
+    _, S, D = kshape if len(kshape) == 3 else (0, 0, 0)
+    hd = W // H if H > 0 else 0
+    if scale is None:
+        scale = hd**-0.5 if hd else 1.0
+    qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    if not (
+        query.is_cuda and (hd == 64 or hd == 128) and W == H * hd and E and D and D % hd == 0 and H * hd % D == 0
+        and kshape[0] == B and value.shape == kshape and key.dtype is dt and value.dtype is dt and key.get_device() == at and value.get_device() == at
+        and 0 < scale < math.inf
+        and (lengths is None or (lengths.shape == (B,) and lengths.dtype is _INT32 and lengths.get_device() == at and lengths.is_contiguous()))
+    ):
+        _refuse_cross_attn(query, key, value, H, lengths, scale)
+    if out is None:
+        out = torch.empty_like(query)
+    else:
+        out = _head_out(out, query, query.device, [key, value] + ([lengths] if lengths is not None else []))
+    if B == 0 or T == 0:
+        return out
+    (qb, qt, qu), (kb, kt, ku), (vb, vt, vu), (ob, ot, _) = query.stride(), key.stride(), value.stride(), out.stride()
+    if qu != 1 or qp & 15 or (qb | qt) * E & 15 or (S and (ku != 1 or vu != 1 or (kp | vp) & 15 or (kb | kt | vb | vt) * E & 15)):
+        _refuse_cross_attn(query, key, value, H, lengths, scale)
+    code, stream = _DTYPES[dt], torch._C._cuda_getCurrentRawStream(at)
+    n = _attn_space(code, B, T, H, D // hd, hd, S)
+    space = torch.empty(n, dtype=torch.uint8, device=query.device) if n else None
+    a = CrossAttnArgs(
+        code, at, B, T, S, H, D // hd, hd, scale, qp, qb, qt, kp, kb, kt, vp, vb, vt, None if lengths is None else lengths.data_ptr(),
+        out.data_ptr(), ob, ot, None if space is None else space.data_ptr(),
+    )
+    check(lib().pk_cross_attn(ctypes.byref(a), stream), "pk_cross_attn")
+    return out
+
+
+def _refuse_cross_attn(query, key, value, H, lengths, scale) -> None:
+    """Says what :func:`cross_attn` does not take of a call."""
+    hd, dt = _head_dim(query, H), query.dtype
     B, T, _ = query.shape
     S, D = key.shape[1:] if key.dim() == 3 else (0, 0)
     if D % hd or D == 0:
@@ -1752,15 +1856,5 @@ def cross_attn(
     _head_rows("query", query, B, T, dt)
     _head_rows("key", key, B, S, dt)
     _head_rows("value", value, B, S, dt, D)
-    dev = _require_device(query, key, value)
-    out = _head_out(out, query, dev, [key, value] + ([lengths] if lengths is not None else []))
-    a = CrossAttnArgs()
-    space = _attend(a, query, out, B, T, int(num_heads), D // hd, hd, S, scale, lengths, dev)  # noqa: F841
-    if B == 0 or T == 0:
-        return out
-    a.states, a.kv_heads = S, D // hd
-    a.key, a.value = key.data_ptr(), value.data_ptr()
-    a.key_stride_b, a.key_stride_t, _ = key.stride()
-    a.value_stride_b, a.value_stride_t, _ = value.stride()
-    check(lib().pk_cross_attn(ctypes.byref(a), _stream(dev)), "pk_cross_attn")
-    return out
+    _require_device(query, key, value)
+    _refuse_attention(query, H, D // hd, lengths, scale)
