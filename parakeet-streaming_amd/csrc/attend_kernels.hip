@@ -424,8 +424,12 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 // product's operand where they are. 16-bit types: two tiles of 16 keys make one step of 32, in
 // the order that the registers have; V comes back transposed from LDS; weights go into the
 // product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them.
-template <typename ST, int HD, bool PAGED, int RT>
+// Where keys are: a tensor of states; pages of 16 frames and more, so that 16 keys from a multiple of 16 on are of
+// one page, whose number is a scalar; smaller pages, looked up key by key.
+enum Source { kStates, kPages, kSmallPages };
+template <typename ST, int HD, Source SRC, int RT>
 __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p) {
+  constexpr bool PAGED = SRC != kStates;
   constexpr int E = (int)sizeof(ST), ROWS = 16 * RT, SUB = E == 2 ? 2 : 1, KT = 16 * SUB, NB = HD * E / 64, NT = HD / 16;
   constexpr int VROW = HD * E + 16;  // bytes of a staged row of V: 16 more spread the rows over the banks
   constexpr int STRIDE = HD + 4;
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
   __shared__ float2 ml[4 * ROWS];
   __shared__ uint32_t bad[(ROWS + 31) / 32];
   __shared__ float qs[PAGED ? 4 * HD : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const ItemOf it = item_of(p, ROWS);
   if (!it.live) return;
   const StreamOf s = stream_of<ST, PAGED>(p, it.b);
@@ -466,57 +470,77 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 
   if (keys.t0 < keys.t1) {
     const int64_t step = PAGED ? (int64_t)64 << p.page_shift : 64;
-    const unsigned char *kb, *vb;
-    if constexpr (PAGED) {
-      const int64_t head = ((int64_t)it.hk * (HD * E) << p.page_shift) + g * 16;
-      kb = p.k + head;
-      vb = p.v + head;
-    } else {
-      kb = p.k + it.b * p.k_sb + (int64_t)it.hk * (HD * E) + g * 16;
-      vb = p.v + it.b * p.v_sb + (int64_t)it.hk * (HD * E) + g * 16;
-    }
+    const unsigned char* const kb = p.k + (PAGED ? (int64_t)it.hk * (HD * E) << p.page_shift : it.b * p.k_sb + (int64_t)it.hk * (HD * E));
+    const unsigned char* const vb = p.v + (PAGED ? (int64_t)it.hk * (HD * E) << p.page_shift : it.b * p.v_sb + (int64_t)it.hk * (HD * E));
     const int32_t* const ring = PAGED ? p.rows + it.b * p.rows_stride + 1 : nullptr;
-    // page of key lane % KT of tile t, -1 where no row of the workgroup sees it or it is not there
-    auto page_of = [&](int t) {
-      if constexpr (PAGED) {
-        const int d = t * KT + (lane & (KT - 1));
-        int page = -1;
-        if (t < keys.t1 && d >= keys.lo && d <= keys.hi) page = ring[(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift) % (uint32_t)p.max_pages];
-        return page;
-      } else {
-        return 0;
-      }
+    // The page numbers of tile t: of its 16 keys u, or of key lane % KT; -1 where no row of the workgroup
+    // sees any. Read without a branch, so that the loads that go on are counted exactly.
+    struct Pages {
+      int32_t of[SUB];
     };
-    int64_t ko[SUB], vo[SUB];
+    auto pages_of = [&](int t) {
+      Pages x{};
+      if constexpr (SRC == kPages) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          const int d = t * KT + 16 * u;
+          const bool in = t < keys.t1 && d + 15 >= keys.lo && d <= keys.hi;
+          const uint32_t entry = (((uint32_t)keys.k0 + (uint32_t)(in ? d : keys.lo)) >> p.page_shift) % (uint32_t)p.max_pages;
+          const int32_t page = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(ring))[__builtin_amdgcn_readfirstlane(entry)];
+          x.of[u] = in ? page : -1;
+        }
+      } else if constexpr (SRC == kSmallPages) {
+        const int d = t * KT + (lane & (KT - 1));
+        const bool in = t < keys.t1 && d >= keys.lo && d <= keys.hi;
+        const int32_t page = ring[(((uint32_t)keys.k0 + (uint32_t)(in ? d : keys.lo)) >> p.page_shift) % (uint32_t)p.max_pages];
+        x.of[0] = in ? page : -1;
+      }
+      return x;
+    };
+    // Of 16 keys u of a tile: a place that all lanes share, a lane's bytes from there, and whether its key is there
+    // (what memory holds for one that is not is not used).
+    int64_t ks[SUB], vs[SUB];
+    uint32_t kl[SUB], vl[SUB];
     bool ok[SUB];
-    auto places = [&](int t, int page) {
+    auto places = [&](int t, const Pages& pages) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        const int d = t * KT + 16 * u + r16;
-        if constexpr (PAGED) {
-          const int mine = __shfl(page, 16 * u + r16);
-          ok[u] = (uint32_t)mine < (uint32_t)p.num_pages;
-          ko[u] = vo[u] = ok[u] ? mine * p.page_bytes + ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6) : 0;
+        const int d0 = t * KT + 16 * u, d = d0 + r16;
+        ok[u] = t < keys.t1 && d >= keys.lo && d <= keys.hi;
+        if constexpr (SRC == kStates) {
+          const int at = min(d0, keys.hi), more = min(r16, keys.hi - at);  // rows past the last are not touched
+          ks[u] = at * p.k_st;
+          vs[u] = at * p.v_st;
+          kl[u] = (uint32_t)more * (uint32_t)p.k_st + g * 16;
+          vl[u] = (uint32_t)more * (uint32_t)p.v_st + g * 16;
+        } else if constexpr (SRC == kPages) {
+          const bool there = (uint32_t)pages.of[u] < (uint32_t)p.num_pages;
+          ok[u] = ok[u] && there;
+          ks[u] = vs[u] = (there ? pages.of[u] : 0) * p.page_bytes + ((((uint32_t)keys.k0 + (uint32_t)d0) & ((1u << p.page_shift) - 1u)) << 6);
+          kl[u] = vl[u] = r16 * 64 + g * 16;
         } else {
-          ok[u] = t < keys.t1 && d <= keys.hi;
-          ko[u] = ok[u] ? d * p.k_st : 0;  // row 0 is there; what it holds is not used
-          vo[u] = ok[u] ? d * p.v_st : 0;
+          const int32_t mine = __shfl(pages.of[0], 16 * u + r16);
+          ok[u] = (uint32_t)mine < (uint32_t)p.num_pages;
+          ks[u] = vs[u] = ok[u] ? mine * p.page_bytes + ((((uint32_t)keys.k0 + (uint32_t)d) & ((1u << p.page_shift) - 1u)) << 6) : 0;
+          kl[u] = vl[u] = g * 16;
         }
       }
     };
     u32x4 kr[SUB][NB], vr[SUB][NB];
-    auto ask = [&](u32x4 (&x)[SUB][NB], const unsigned char* base, const int64_t (&at)[SUB]) {
+    auto ask = [&](u32x4 (&x)[SUB][NB], const unsigned char* base, const int64_t (&at)[SUB], const uint32_t (&off)[SUB]) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int c = 0; c < NB; ++c) x[u][c] = *reinterpret_cast<const u32x4*>(base + at[u] + c * step);
+        for (int c = 0; c < NB; ++c) x[u][c] = *reinterpret_cast<const u32x4*>(base + at[u] + c * step + off[u]);
     };
     unsigned char* const stage = smem + wave * (KT * VROW);
     int t = keys.t0 + wave;
-    places(t, page_of(t));
-    ask(kr, kb, ko);
-    ask(vr, vb, vo);
-    int next = page_of(t + 4);
+    places(t, pages_of(t));
+    Pages next = pages_of(t + 4);  // ahead of the loads, as in the loop: waiting for it is no wait for them
+    __builtin_amdgcn_sched_barrier(0);
+    ask(kr, kb, ks, kl);
+    __builtin_amdgcn_sched_barrier(0);
+    ask(vr, vb, vs, vl);
     for (; t < keys.t1; t += 4) {
       bool now[SUB];
 #pragma unroll
@@ -532,8 +556,9 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
         }
       __builtin_amdgcn_sched_barrier(0);
       places(t + 4, next);
-      next = page_of(t + 8);
-      ask(kr, kb, ko);
+      next = pages_of(t + 8);
+      __builtin_amdgcn_sched_barrier(0);
+      ask(kr, kb, ks, kl);
       __builtin_amdgcn_sched_barrier(0);
       // weights: key d = t KT + 16 u + 4 g + e of query r16
       uint64_t there[SUB];
@@ -589,7 +614,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
           *reinterpret_cast<u32x4*>(stage + (16 * u + r16) * VROW + c * 64 + g * 16) = v;
         }
       __builtin_amdgcn_sched_barrier(0);
-      ask(vr, vb, vo);
+      ask(vr, vb, vs, vl);
       __builtin_amdgcn_sched_barrier(0);
       wave_lds_sync();
 #pragma unroll
@@ -1175,17 +1200,23 @@ int64_t attend_space(int64_t rows, int splits, int head_dim) { return splits > 1
 template <typename ST, int HD, bool PAGED>
 int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hipStream_t s) {
   const dim3 grid((unsigned)c.groups), block(256);
-  if (c.rows == 16)
-    hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
+  constexpr Source SRC = PAGED ? kPages : kStates;
+  if (PAGED && p.page_shift < 4) {
+    if (c.rows == 16)
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1>), grid, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2>), grid, block, 0, s, p);
+  } else if (c.rows == 16)
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1>), grid, block, 0, s, p);
   else if constexpr (sizeof(ST) == 2) {
     if (c.rows == 32)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 2>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2>), grid, block, 0, s, p);
     else if (c.key_groups == 1)
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
     else
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 2>), grid, dim3(512), 0, s, p);
   } else
-    hipLaunchKernelGGL((attend_few_kernel<ST, HD, PAGED, 2>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2>), grid, block, 0, s, p);
   int rc = check_launch(what);
   if (rc != PK_OK || p.splits == 1) return rc;
   hipLaunchKernelGGL((attend_join_kernel<ST, HD>), dim3((unsigned)((int64_t)p.B * p.Hkv * p.R)), block, 0, s, p);
