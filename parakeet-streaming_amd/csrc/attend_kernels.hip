@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -426,8 +427,10 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 // product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them.
 // Where keys are: a tensor of states; pages of 16 frames and more, so that 16 keys from a multiple of 16 on are of
 // one page, whose number is a scalar; smaller pages, looked up key by key.
+// Pages that one row tile reads are read past the caches (128 streams of up to 4096: 119 us cached, 107 so); rows of states
+// are not, since a load has half of a 128-byte line of each (60 x 4 rows over up to 1500: 43 us, 63 past the caches).
 enum Source { kStates, kPages, kSmallPages };
-template <typename ST, int HD, Source SRC, int RT>
+template <typename ST, int HD, Source SRC, int RT, bool STREAM>
 __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p) {
   constexpr bool PAGED = SRC != kStates;
   constexpr int E = (int)sizeof(ST), ROWS = 16 * RT, SUB = E == 2 ? 2 : 1, KT = 16 * SUB, NB = HD * E / 64, NT = HD / 16;
@@ -446,18 +449,28 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 
   // the rows: their queries and what they see
   u32x4 q[RT][NB];
-  int lo[RT], hi[RT];
+  int lo[RT], hi[RT], all_lo = 0, all_hi = 0x7fffffff;
+  bool live[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int row = it.row0 + 16 * t + r16, i = min(row, p.R - 1) / p.G, gq = min(row, p.R - 1) - i * p.G;
     const ST* const from = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)(it.hk * p.G + gq) * HD + g * (16 / E);
 #pragma unroll
     for (int c = 0; c < NB; ++c) q[t][c] = ld16(from + c * (64 / E));
-    const bool live = row < p.R && i < s.n;
-    const int2 seen = seen_by<ST, PAGED>(p, s, i);
-    lo[t] = live ? seen.x - keys.k0 : 0;
-    hi[t] = live ? seen.y - keys.k0 : -1;
+    // a row past the stream's tokens sees what its last token sees, and gives nothing in the end
+    live[t] = i < s.n;
+    const int2 seen = seen_by<ST, PAGED>(p, s, min(i, s.n - 1));
+    lo[t] = seen.x - keys.k0;
+    hi[t] = seen.y - keys.k0;
+    all_lo = max(all_lo, lo[t]);
+    all_hi = min(all_hi, hi[t]);
   }
+  for (int d = 1; d < 16; d <<= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, d));
+    all_hi = min(all_hi, __shfl_xor(all_hi, d));
+  }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   f32x4_t o[RT][NT];
   float m[RT], l[RT];
 #pragma unroll
@@ -531,7 +544,10 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int c = 0; c < NB; ++c) x[u][c] = *reinterpret_cast<const u32x4*>(base + at[u] + c * step + off[u]);
+        for (int c = 0; c < NB; ++c) {
+          const u32x4* const from = reinterpret_cast<const u32x4*>(base + at[u] + c * step + off[u]);
+          x[u][c] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
     };
     unsigned char* const stage = smem + wave * (KT * VROW);
     int t = keys.t0 + wave;
@@ -561,26 +577,29 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
       ask(kr, kb, ks, kl);
       __builtin_amdgcn_sched_barrier(0);
       // weights: key d = t KT + 16 u + 4 g + e of query r16
-      uint64_t there[SUB];
+      bool whole = t * KT >= all_lo && t * KT + KT - 1 <= all_hi;  // all rows see all keys (wave-uniform)
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) there[u] = __ballot(now[u]);  // bit r16: key 16 u + r16
-      bool whole = true;
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) whole &= there[u] == ~0ull;
+      for (int u = 0; u < SUB; ++u) whole = whole && __ballot(now[u]) == ~0ull;
       u32x4 w[RT], wl[RT];
 #pragma unroll
       for (int a = 0; a < RT; ++a) {
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) {
+            const uint64_t there = __ballot(now[u]);  // bit r16: key 16 u + r16
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int in = 4 * g + k, d = t * KT + 16 * u + in;
+              if (!(d >= lo[a] && d <= hi[a] && (there >> in & 1))) x[a][u][k] = kNone;
+            }
+          }
+        }
         float e[SUB][4], top = kNone;
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int in = 4 * g + k, d = t * KT + 16 * u + in;
-            const bool sees = d >= lo[a] && d <= hi[a] && (there[u] >> in & 1);
-            e[u][k] = sees ? x[a][u][k] * p.scale : kNone;
-            top = fmaxf(top, e[u][k]);
-          }
-        top = fmaxf(m[a], max_of_groups(top));
+          for (int k = 0; k < 4; ++k) top = fmaxf(top, x[a][u][k]);
+        top = fmaxf(m[a], max_of_groups(top) * p.scale);
         const float base = top == kNone ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[a] - base);
         m[a] = top;
         float sum = 0.f;
@@ -588,7 +607,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            e[u][k] = __builtin_amdgcn_exp2f(e[u][k] - base);
+            e[u][k] = __builtin_amdgcn_exp2f(fmaf(x[a][u][k], p.scale, -base));
             sum += e[u][k];
           }
         l[a] = fmaf(l[a], keep, sum);
@@ -651,6 +670,10 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
     l[a] = sum_of_groups(l[a]);
+    if (!live[a]) {
+      m[a] = kNone;
+      l[a] = 0.f;
+    }
     if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
   }
   __syncthreads();  // and every wave is done with its staged rows
@@ -663,7 +686,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
     const float f = __builtin_amdgcn_exp2f(m[a] - (top == kNone ? 0.f : top));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = o[a][n] * f;
+      *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = live[a] ? o[a][n] * f : f32x4_t{0.f, 0.f, 0.f, 0.f};
     l[a] *= f;
     m[a] = top;
   }
@@ -1185,11 +1208,13 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
   c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 || narrow ? 32 : 128;
   c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
-  // keys are split over workgroups where the rows leave CUs without one: 256 CUs hold one of attend_many_kernel's
-  // workgroups each, and two or more of attend_few_kernel's
-  const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512, want = (full * 3 / 4 + whole - 1) / whole, most = (keys + 511) / 512;
-  int64_t n = want < most ? want : most;
-  n = n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
+  // keys are split over workgroups where the rows leave CUs without one (256 CUs hold one of attend_many_kernel's
+  // workgroups each, and two of attend_few_kernel's), and long ones so that streams of different lengths fill them
+  // alike; a part has 512 keys or 1024 at least, since parts are joined in a launch of 4 us
+  const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512;
+  auto parts = [&](int64_t groups, int least) { return std::min((groups + whole - 1) / whole, (int64_t)keys / least); };
+  int64_t n = std::max(parts(full * 3 / 4, 512), c.rows == 128 ? 0 : parts(2048, 1024));
+  n = std::min(std::max(n, (int64_t)1), (int64_t)kMaxSplits);
   c.splits = (int)n;
   c.groups = (units * n + 7) / 8 * 8 * c.row_tiles;
   return c;
@@ -1203,20 +1228,22 @@ int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hi
   constexpr Source SRC = PAGED ? kPages : kStates;
   if (PAGED && p.page_shift < 4) {
     if (c.rows == 16)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1, false>), grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2>), grid, block, 0, s, p);
-  } else if (c.rows == 16)
-    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1>), grid, block, 0, s, p);
-  else if constexpr (sizeof(ST) == 2) {
-    if (c.rows == 32)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2>), grid, block, 0, s, p);
-    else if (c.key_groups == 1)
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2, false>), grid, block, 0, s, p);
+  } else if (c.rows == 16) {
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, PAGED>), grid, block, 0, s, p);
+  } else if (c.rows == 32) {
+    if (PAGED && c.row_tiles == 1)
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, PAGED>), grid, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, false>), grid, block, 0, s, p);
+  } else if constexpr (sizeof(ST) == 2) {
+    if (c.key_groups == 1)
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
     else
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 2>), grid, dim3(512), 0, s, p);
-  } else
-    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2>), grid, block, 0, s, p);
+  }
   int rc = check_launch(what);
   if (rc != PK_OK || p.splits == 1) return rc;
   hipLaunchKernelGGL((attend_join_kernel<ST, HD>), dim3((unsigned)((int64_t)p.B * p.Hkv * p.R)), block, 0, s, p);
