@@ -53,86 +53,112 @@ __device__ static inline float2 turn_of(int32_t pos, double inv) {
   return float2{c, s};
 }
 
-template <typename ST, int HD, int TOK>
-__global__ void __launch_bounds__(256) qk_norm_append_kernel(const NormK<ST> p) {
-  constexpr int VEC = Tr<ST>::VEC, LPH = HD / VEC, CB = 64 / (int)sizeof(ST);
-  __shared__ float2 cs[TOK][HD / 2];
-  const int heads = p.Hq + 2 * p.Hkv, per = heads * LPH, half = p.rotary >> 1;
-  const int64_t total = (int64_t)p.B * p.T, first = (int64_t)blockIdx.x * TOK;
-  for (int i = threadIdx.x; i < TOK * half; i += 256) {
-    const int t = i / half, f = i - t * half;
-    const int64_t row = first + t;
-    if (row < total) {
-      const int b = (int)(row / p.T), at = (int)(row - (int64_t)b * p.T);
-      const int32_t pos = p.pos ? p.pos[b * p.pos_sb + at] : p.rows[b * p.rows_stride] + at;
-      cs[t][f] = turn_of(pos, p.inv[f]);
+// x of lane ^ span within a head's lanes, span a power of two below them (wave-uniform)
+__device__ static inline float of_partner(float x, int span) {
+  switch (span) {
+    case 1: return dpp_f<0xB1>(x);                   // quad_perm [1, 0, 3, 2]
+    case 2: return dpp_f<0x4E>(x);                   // quad_perm [2, 3, 0, 1]
+    case 4: return dpp_f<0x1B>(dpp_f<0x141>(x));     // row_half_mirror: lane ^ 7, quad_perm [3, 2, 1, 0]: lane ^ 3
+    case 8: return dpp_f<0x128>(x);                  // row_ror 8
+    default: {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      return __uint_as_float(threadIdx.x & 16 ? r[0] : r[1]);
     }
   }
+}
+
+// A wave takes the 64 / LPH heads of an item at once (q's, k's and v's in a row, so that an item is 1 KB), TOK tokens'
+// items over the workgroup's waves; U items' loads are on their way together. 16 K tokens of 16 + 2 + 2
+// heads of 128 in bf16 move 144 MB.
+template <typename ST, int HD, int TOK, int U>
+__global__ void __launch_bounds__(256) qk_norm_append_kernel(const NormK<ST> p) {
+  constexpr int VEC = Tr<ST>::VEC, LPH = HD / VEC, CB = 64 / (int)sizeof(ST), HPI = 64 / LPH;
+  __shared__ float2 cs[TOK][HD / 2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int heads = p.Hq + 2 * p.Hkv, per = (heads + HPI - 1) / HPI, half = p.rotary >> 1;
+  const uint32_t total = (uint32_t)p.B * (uint32_t)p.T, first = blockIdx.x * (uint32_t)TOK;  // below 2^31
+  const int tokens = (int)min((uint32_t)TOK, total - first), items = tokens * per;
+  const int c = (lane & (LPH - 1)) * VEC;
+
+  u32x4 raw[U];
+  ST* to[U];
+  // asks for item `item`: its token's row, and where it goes (nullptr: nowhere)
+  auto ask = [&](int u, int item) {
+    to[u] = nullptr;
+    if (item >= items) return;
+    const int t = item / per, head = (item - t * per) * HPI + lane / LPH;
+    const uint32_t row = first + t, b = row / (uint32_t)p.T, at = row - b * (uint32_t)p.T;
+    const uint32_t place = (uint32_t)p.map[b * p.map_sb + at];
+    const ST* from = nullptr;
+    if (head < p.Hq) {
+      const int col = head * HD + c;
+      from = p.q + b * p.q_sb + at * p.q_st + col;
+      to[u] = p.out + b * p.o_sb + at * p.o_st + col;
+    } else if (head < heads && place < p.places) {
+      const bool key = head < p.Hq + p.Hkv;
+      const int col = (head - p.Hq - (key ? 0 : p.Hkv)) * HD + c, rest = (int)place & ((1 << p.page_shift) - 1);
+      from = key ? p.k + b * p.k_sb + at * p.k_st + col : p.v + b * p.v_sb + at * p.v_st + col;
+      to[u] = (key ? p.kp : p.vp) + (int64_t)(place >> p.page_shift) * (((int64_t)p.Hkv * HD) << p.page_shift) +
+              ((int64_t)(col / CB) * CB << p.page_shift) + (int64_t)rest * CB + col % CB;
+    }
+    raw[u] = to[u] ? ld16(from) : u32x4{0u, 0u, 0u, 0u};
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) ask(u, wave + 4 * u);
+  float qg[VEC], kg[VEC];
+  if (p.qw) Tr<ST>::unpack(ld16(p.qw + c), qg);
+  if (p.kw) Tr<ST>::unpack(ld16(p.kw + c), kg);
+  for (int i = threadIdx.x; i < tokens * half; i += 256) {
+    const int t = i / half, f = i - t * half;
+    const uint32_t row = first + t, b = row / (uint32_t)p.T, at = row - b * (uint32_t)p.T;
+    cs[t][f] = turn_of(p.pos ? p.pos[b * p.pos_sb + at] : p.rows[b * p.rows_stride] + (int32_t)at, p.inv[f]);
+  }
   __syncthreads();
-  // columns of a token in order: the heads of q, k and v
-  const int all = TOK * per;
-  for (int i0 = 0; i0 < all; i0 += 256) {
-    const int i = min(i0 + (int)threadIdx.x, all - 1);  // every lane takes part in the sums
-    const int t = i / per, j = i - t * per, head = j / LPH, c = (j - head * LPH) * VEC;
-    const int64_t row = first + t;
-    bool live = i0 + (int)threadIdx.x < all && row < total;
-    const int b = live ? (int)(row / p.T) : 0, at = live ? (int)(row - (int64_t)b * p.T) : 0;
-    const int which = head < p.Hq ? 0 : head < p.Hq + p.Hkv ? 1 : 2;
-    const int h = which == 0 ? head : which == 1 ? head - p.Hq : head - p.Hq - p.Hkv;
-    ST* to = nullptr;
-    if (which == 0) {
-      to = p.out + b * p.o_sb + at * p.o_st + (int64_t)h * HD + c;
-    } else if (live) {
-      const uint32_t place = (uint32_t)p.map[b * p.map_sb + at];
-      live = place < p.places;
-      const int col = h * HD + c, mask = (1 << p.page_shift) - 1;
-      const int64_t e = (int64_t)(place >> p.page_shift) * (((int64_t)p.Hkv * HD) << p.page_shift) +
-                        (int64_t)(col / CB) * (CB << p.page_shift) + (int64_t)(place & mask) * CB + col % CB;
-      to = (which == 1 ? p.kp : p.vp) + e;
-    }
-    const ST* const from = which == 0   ? p.q + b * p.q_sb + at * p.q_st + (int64_t)h * HD + c
-                           : which == 1 ? p.k + b * p.k_sb + at * p.k_st + (int64_t)h * HD + c
-                                        : p.v + b * p.v_sb + at * p.v_st + (int64_t)h * HD + c;
-    u32x4 raw = u32x4{0u, 0u, 0u, 0u};
-    if (live) raw = ld16(from);
-    float x[VEC];
-    Tr<ST>::unpack(raw, x);
-    const ST* const w = which == 0 ? p.qw : p.kw;
-    float ss = 0.f;
+  const int span = half / VEC;  // lanes between the columns of a pair
+  for (int i0 = wave; i0 < items; i0 += 4 * U) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) ss = fmaf(x[e], x[e], ss);
-    ss = group_sum<LPH>(ss);
-    if (w && which < 2) {
-      const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
-      float g[VEC];
-      Tr<ST>::unpack(ld16(w + c), g);
+    for (int u = 0; u < U; ++u) {
+      const int item = i0 + 4 * u;
+      if (item >= items) break;  // wave-uniform
+      const int t = item / per, head = (item - t * per) * HPI + lane / LPH;
+      const bool key = head >= p.Hq, turned = head < p.Hq + p.Hkv && c < p.rotary;
+      float x[VEC];
+      Tr<ST>::unpack(raw[u], x);
+      float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[e] = x[e] * r * g[e];
-    }
-    if (p.interleaved) {
-      if (which < 2 && c < p.rotary) {
+      for (int e = 0; e < VEC; ++e) ss = fmaf(x[e], x[e], ss);
+      ss = group_sum<LPH>(ss);
+      if (key ? p.kw != nullptr : p.qw != nullptr) {
+        const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
 #pragma unroll
-        for (int e = 0; e < VEC; e += 2) {
-          const float2 f = cs[t][(c + e) >> 1];
-          const float a = x[e], z = x[e + 1];
-          x[e] = a * f.x - z * f.y;
-          x[e + 1] = z * f.x + a * f.y;
+        for (int e = 0; e < VEC; ++e) x[e] = x[e] * r * (key ? kg[e] : qg[e]);
+      }
+      if (half > 0) {
+        if (p.interleaved) {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 f = cs[t][min((c + e) >> 1, half - 1)];
+            const float a = x[e], z = x[e + 1];
+            if (turned) {
+              x[e] = a * f.x - z * f.y;
+              x[e + 1] = z * f.x + a * f.y;
+            }
+          }
+        } else {
+          const bool upper = c >= half;
+          const float2* const f0 = &cs[t][c < p.rotary ? (upper ? c - half : c) : 0];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float other = of_partner(x[e], span);
+            const float2 f = f0[e];
+            if (turned) x[e] = fmaf(other, upper ? f.y : -f.y, x[e] * f.x);
+          }
         }
       }
-    } else if (half > 0) {
-      const int span = half / VEC;  // lanes, a power of two
-      const bool turned = which < 2 && c < p.rotary, upper = c >= half;
-      const int f0 = upper ? c - half : c;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float other = __shfl_xor(x[e], span);
-        if (turned) {
-          const float2 f = cs[t][f0 + e];
-          x[e] = upper ? x[e] * f.x + other * f.y : x[e] * f.x - other * f.y;
-        }
-      }
+      if (to[u]) st16(to[u], head < p.Hq + p.Hkv ? Tr<ST>::pack(x) : raw[u]);
     }
-    if (live) st16(to, which == 2 ? raw : Tr<ST>::pack(x));
+#pragma unroll
+    for (int u = 0; u < U; ++u) ask(u, i0 + 4 * (U + u));
   }
 }
 
@@ -430,17 +456,17 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 // Pages that one row tile reads are read past the caches (128 streams of up to 4096: 119 us cached, 107 so); rows of states
 // are not, since a load has half of a 128-byte line of each (60 x 4 rows over up to 1500: 43 us, 63 past the caches).
 enum Source { kStates, kPages, kSmallPages };
-template <typename ST, int HD, Source SRC, int RT, bool STREAM>
-__global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p) {
+template <typename ST, int HD, Source SRC, int RT, int NW, bool STREAM>
+__global__ void __launch_bounds__(64 * NW, 2) attend_few_kernel(const AttendK<ST> p) {
   constexpr bool PAGED = SRC != kStates;
   constexpr int E = (int)sizeof(ST), ROWS = 16 * RT, SUB = E == 2 ? 2 : 1, KT = 16 * SUB, NB = HD * E / 64, NT = HD / 16;
   constexpr int VROW = HD * E + 16;  // bytes of a staged row of V: 16 more spread the rows over the banks
   constexpr int STRIDE = HD + 4;
-  constexpr int kStage = 4 * KT * VROW, kSums = 4 * ROWS * STRIDE * 4;
+  constexpr int kStage = NW * KT * VROW, kSums = NW * ROWS * STRIDE * 4;
   __shared__ __align__(16) unsigned char smem[kStage > kSums ? kStage : kSums];
-  __shared__ float2 ml[4 * ROWS];
+  __shared__ float2 ml[NW * ROWS];
   __shared__ uint32_t bad[(ROWS + 31) / 32];
-  __shared__ float qs[PAGED ? 4 * HD : 1];
+  __shared__ float qs[PAGED ? NW * HD : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const ItemOf it = item_of(p, ROWS);
   if (!it.live) return;
@@ -552,12 +578,12 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
     unsigned char* const stage = smem + wave * (KT * VROW);
     int t = keys.t0 + wave;
     places(t, pages_of(t));
-    Pages next = pages_of(t + 4);  // ahead of the loads, as in the loop: waiting for it is no wait for them
+    Pages next = pages_of(t + NW);  // ahead of the loads, as in the loop: waiting for it is no wait for them
     __builtin_amdgcn_sched_barrier(0);
     ask(kr, kb, ks, kl);
     __builtin_amdgcn_sched_barrier(0);
     ask(vr, vb, vs, vl);
-    for (; t < keys.t1; t += 4) {
+    for (; t < keys.t1; t += NW) {
       bool now[SUB];
 #pragma unroll
       for (int u = 0; u < SUB; ++u) now[u] = ok[u];
@@ -571,8 +597,8 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
           for (int c = 0; c < NB; ++c) x[a][u] = mma_block<ST>(kr[u][c], q[a][c], x[a][u]);
         }
       __builtin_amdgcn_sched_barrier(0);
-      places(t + 4, next);
-      next = pages_of(t + 8);
+      places(t + NW, next);
+      next = pages_of(t + 2 * NW);
       __builtin_amdgcn_sched_barrier(0);
       ask(kr, kb, ks, kl);
       __builtin_amdgcn_sched_barrier(0);
@@ -682,7 +708,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
   for (int a = 0; a < RT; ++a) {
     float top = kNone;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * ROWS + 16 * a + r16].x);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * ROWS + 16 * a + r16].x);
     const float f = __builtin_amdgcn_exp2f(m[a] - (top == kNone ? 0.f : top));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -695,7 +721,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
   for (int a = 0; a < RT; ++a)
     if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, 4, 256>(p, it, s, keys, KT, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW>(p, it, s, keys, KT, sums, ml, bad, qs);
 }
 
 // ---- many rows
@@ -1051,7 +1077,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
 constexpr int kMaxSplits = 256;
 template <typename ST, int HD>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
-  constexpr int LANES = HD / 4, SIDE = 256 / LANES;  // lanes a split's row, splits at once
+  constexpr int LANES = HD / 4, SIDE = 256 / LANES, AHEAD = 8;  // lanes a split's row, splits at once, turns on their way
   __shared__ float weight[kMaxSplits];
   __shared__ float red[4], total[4];
   __shared__ f32x4_t sums[256];
@@ -1059,24 +1085,30 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
   const uint32_t x = blockIdx.x, unit = x / (uint32_t)p.R, row = x - unit * (uint32_t)p.R;
   const int b = (int)(unit / (uint32_t)p.Hkv), hk = (int)(unit - (uint32_t)b * p.Hkv), i = (int)(row / (uint32_t)p.G), gq = (int)(row - (uint32_t)i * p.G);
   const float2 v = tid < p.splits ? p.ml[(int64_t)x * p.splits + tid] : float2{kNone, 0.f};
+  // the parts are on their way while their weights are made; one without keys for the row holds zeros
+  const int c = (tid & (LANES - 1)) * 4;
+  const float* const from = p.part + (int64_t)x * p.splits * HD + c;
+  f32x4_t ahead[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) ahead[u] = *reinterpret_cast<const f32x4_t*>(from + (int64_t)min(tid / LANES + u * SIDE, p.splits - 1) * HD);
   float top = v.x;
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) red[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float w = __builtin_amdgcn_exp2f(v.x - (top == kNone ? 0.f : top));
-  weight[tid] = v.y == 0.f ? 0.f : w;  // a split without keys for the row is not read
+  weight[tid] = v.y == 0.f ? 0.f : w;
   const float l = group_sum<64>(v.y == 0.f ? 0.f : v.y * w);
   if (lane == 0) total[wave] = l;
   __syncthreads();
-  const int c = (tid & (LANES - 1)) * 4;
   f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const float* const from = p.part + (int64_t)x * p.splits * HD + c;
-#pragma unroll 4
-  for (int sp = tid / LANES; sp < p.splits; sp += SIDE) {
-    const float ws = weight[sp];
-    if (ws != 0.f) acc += *reinterpret_cast<const f32x4_t*>(from + (int64_t)sp * HD) * ws;
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) {
+    const float ws = weight[tid / LANES + u * SIDE];  // 0 past the splits
+    acc += ws == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : ahead[u] * ws;
   }
+#pragma unroll 4
+  for (int sp = tid / LANES + AHEAD * SIDE; sp < p.splits; sp += SIDE) acc += *reinterpret_cast<const f32x4_t*>(from + (int64_t)sp * HD) * weight[sp];
   sums[tid] = acc;
   __syncthreads();
   if (tid >= LANES) return;
@@ -1177,11 +1209,21 @@ int norm_append(const pk_qk_norm_append_args* a, hipStream_t s) {
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const int64_t total = (int64_t)p.B * p.T;
-  const dim3 grid((unsigned)total);
-  if (a->head_dim == 64)
-    hipLaunchKernelGGL((qk_norm_append_kernel<ST, 64, 1>), grid, dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((qk_norm_append_kernel<ST, 128, 1>), grid, dim3(256), 0, s, p);
+  // few tokens: one a workgroup, for the shortest chain; many: 4, whose loads go together
+  const int tok = total <= 1024 ? 1 : 4;
+  const dim3 grid((unsigned)((total + tok - 1) / tok));
+  if ((int64_t)grid.x >= (1 << 24)) return fail(PK_ERR_UNSUPPORTED, "%s: %lld tokens in one call (built: up to 2^26)", what, (long long)total);
+  if (tok == 1) {
+    if (a->head_dim == 64)
+      hipLaunchKernelGGL((qk_norm_append_kernel<ST, 64, 1, 2>), grid, dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL((qk_norm_append_kernel<ST, 128, 1, 2>), grid, dim3(256), 0, s, p);
+  } else {
+    if (a->head_dim == 64)
+      hipLaunchKernelGGL((qk_norm_append_kernel<ST, 64, 4, 4>), grid, dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL((qk_norm_append_kernel<ST, 128, 4, 4>), grid, dim3(256), 0, s, p);
+  }
   return check_launch(what);
 }
 
@@ -1213,7 +1255,7 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
   // alike; a part has 512 keys or 1024 at least, since parts are joined in a launch of 4 us
   const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512;
   auto parts = [&](int64_t groups, int least) { return std::min((groups + whole - 1) / whole, (int64_t)keys / least); };
-  int64_t n = std::max(parts(full * 3 / 4, 512), c.rows == 128 ? 0 : parts(2048, 1024));
+  int64_t n = std::max(parts(full * 3 / 4, 512), c.rows == 128 ? 0 : parts(1024, 1024));
   n = std::min(std::max(n, (int64_t)1), (int64_t)kMaxSplits);
   c.splits = (int)n;
   c.groups = (units * n + 7) / 8 * 8 * c.row_tiles;
@@ -1223,21 +1265,26 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
 int64_t attend_space(int64_t rows, int splits, int head_dim) { return splits > 1 ? rows * splits * (4 * head_dim + 8) : 0; }
 
 template <typename ST, int HD, bool PAGED>
-int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hipStream_t s) {
+int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, int keys, hipStream_t s) {
   const dim3 grid((unsigned)c.groups), block(256);
   constexpr Source SRC = PAGED ? kPages : kStates;
   if (PAGED && p.page_shift < 4) {
     if (c.rows == 16)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1, 4, false>), grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2, 4, false>), grid, block, 0, s, p);
   } else if (c.rows == 16) {
-    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, PAGED>), grid, block, 0, s, p);
+    // waves of a workgroup: 8 for long parts of pages (128 streams of up to 4096: 105 us with 4, 99 with 8), 4 for
+    // others (5 tokens over 516: 13.7 and 14.7; 60 x 4 rows over up to 1500 states: 43 and 46)
+    if (PAGED && keys / p.splits >= 1024)
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, PAGED ? 8 : 4, PAGED>), grid, dim3(512), 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, 4, PAGED>), grid, block, 0, s, p);
   } else if (c.rows == 32) {
     if (PAGED && c.row_tiles == 1)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, PAGED>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, 4, PAGED>), grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, 4, false>), grid, block, 0, s, p);
   } else if constexpr (sizeof(ST) == 2) {
     if (c.key_groups == 1)
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
@@ -1268,7 +1315,7 @@ int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, 
   }
   DeviceGuard dg(device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, device);
-  return head_dim == 64 ? attend_launch<ST, 64, PAGED>(what, p, c, s) : attend_launch<ST, 128, PAGED>(what, p, c, s);
+  return head_dim == 64 ? attend_launch<ST, 64, PAGED>(what, p, c, keys, s) : attend_launch<ST, 128, PAGED>(what, p, c, keys, s);
 }
 
 template <typename ST>
