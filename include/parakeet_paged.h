@@ -1070,7 +1070,7 @@ int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream);
  * query, out: [batch][chunk][num_heads * head_dim]; element strides (b, t), rows 16-byte aligned
  * with unit inner stride; out may be query, and overlaps nothing else.  scale: > 0 and finite.  head_dim 64 or
  * 128.  pages.max_pages holds any window of left + chunk positions: (left + chunk + page_size - 2) /
- * page_size + 1 <= max_pages.  lengths: int32 [batch].
+ * page_size + 1 <= max_pages; pages of up to 2^20 frames.  lengths: int32 [batch].
  * workspace: pk_attn_workspace_bytes(dtype, batch, chunk, num_heads, kv_heads, head_dim,
  * left + chunk) on the call's device, 16-byte aligned (NULL where that is 0).
  */
@@ -1105,8 +1105,9 @@ int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream);
  * (lengths int32 [batch], held within 0 .. states; NULL: states); zeros where that is empty.  Rows of key
  * and value from lengths[b] on are not read.  No counterpart in the reference.
  * query, out: [batch][chunk][num_heads * head_dim]; key, value: [batch][states][kv_heads * head_dim];
- * element strides (b, t) >= 0 (0: one stream's states for all), rows 16-byte aligned with unit inner stride; out may be
- * query, and overlaps nothing else.  Heads, types, scale and workspace as pk_chunk_attn's, with states keys.
+ * element strides (b, t) >= 0 (0: one stream's states for all; key's and value's t below 2^23), rows 16-byte aligned with
+ * unit inner stride; out may be query, and overlaps nothing else.  Heads, types, scale and workspace as
+ * pk_chunk_attn's, with states keys.
  */
 typedef struct pk_cross_attn_args {
   int32_t dtype;

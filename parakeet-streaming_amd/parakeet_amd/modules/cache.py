@@ -444,8 +444,8 @@ class ModelCache:
         moves = self.pool.fork(s, d)
         ops.kv_move_pages(self.k_pages, self.v_pages, moves)
         if len(d):
-            s, d = (torch.from_numpy(x.astype(np.int64)) for x in (s, d))
-            self.conv_frames[d.to(self.conv_frames.device)] = self.conv_frames[s.to(self.conv_frames.device)]
+            s, d = (self.pool._upload(x).long() for x in (s, d))
+            self.conv_frames[d] = self.conv_frames[s]
         self._base._moved += 1
 
     def compact(self) -> None:

@@ -92,7 +92,7 @@ def test_heads_and_tokens(cuda, dtype, hd, heads, kv_heads, B, T):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("hd,rotary", [(64, 16), (64, 32), (128, 16), (128, 64), (128, 128), (64, 0)])
+@pytest.mark.parametrize("hd,rotary", [(64, 16), (64, 32), (128, 16), (128, 32), (128, 64), (128, 128), (64, 0)])
 def test_rotations(cuda, dtype, interleaved, hd, rotary):
     _run(cuda, dtype, hd, 4, 2, 3, 9, rotary=rotary, interleaved=interleaved)
     _run(cuda, dtype, hd, 4, 2, 3, 9, rotary=rotary, interleaved=interleaved, norm=False, given=True)
