@@ -379,8 +379,9 @@ __device__ static inline KeysOf keys_of(const AttendK<ST>& p, const StreamOf& s,
   return k;
 }
 
-// The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled alike),
-// the quotient, or the split's part. WAVES parts of [rows][HD + 4] floats at `sums`.
+// The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled to their largest
+// maximum; ml: each part's own maximum and sum of weights), the quotient, or the split's part.
+// WAVES parts of [rows][HD + 4] floats at `sums`.
 template <typename ST, int HD, bool PAGED, int ROWS, int WAVES, int THREADS>
 __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, int KT, const float* sums,
                                          const float2* ml, uint32_t* bad, float* qs) {
@@ -398,10 +399,10 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
     m[y] = kNone;
     l[y] = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      m[y] = fmaxf(m[y], ml[w * ROWS + r].x);
-      l[y] += ml[w * ROWS + r].y;
-    }
+    for (int w = 0; w < WAVES; ++w) m[y] = fmaxf(m[y], ml[w * ROWS + r].x);
+    const float base = m[y] == kNone ? 0.f : m[y];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) l[y] = fmaf(ml[w * ROWS + r].y, __builtin_amdgcn_exp2f(ml[w * ROWS + r].x - base), l[y]);
     float t = l[y];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -733,13 +734,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attend_few_kernel(const AttendK<ST
 #pragma unroll
     for (int n = 0; n < NT; ++n)
       *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = live[a] ? o[a][n] * f : f32x4_t{0.f, 0.f, 0.f, 0.f};
-    l[a] *= f;
-    m[a] = top;
   }
-  __syncthreads();
-#pragma unroll
-  for (int a = 0; a < RT; ++a)
-    if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
   __syncthreads();
   attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW>(p, it, s, keys, KT, sums, ml, bad, qs);
 }
@@ -1087,8 +1082,6 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
       const f32x4_t v = f32x4_t{o[n][4 * j], o[n][4 * j + 1], o[n][4 * j + 2], o[n][4 * j + 3]};
       *reinterpret_cast<f32x4_t*>(sums + (kg * ROWS + 32 * wv + r32) * STRIDE + 32 * n + 8 * j + 4 * h) = v * f;
     }
-  __syncthreads();
-  if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{top, l * f};
   __syncthreads();
   attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG>(p, it, s, keys, KT, sums, ml, bad, qs);
 }
