@@ -447,7 +447,9 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
     for (int c = lane; c < HD; c += 64) qs[wave * HD + c] = from_st(q[c]);
     wave_lds_sync();
     const int2 seen = seen_by<ST, PAGED>(p, s, i);
-    const int first = max(seen.x, keys.k0 + keys.t0 * KT), n = min(seen.y - keys.k0, keys.t1 * KT - 1) - (first - keys.k0) + 1;
+    const int first = max(seen.x, keys.k0 + keys.t0 * KT);
+    // a token past the stream's sees nothing
+    const int n = i < s.n ? min(seen.y - keys.k0, keys.t1 * KT - 1) - (first - keys.k0) + 1 : 0;
     float m, l, acc[HD / 64];
     attend_row<ST, HD, PAGED>(p, it.b, it.hk, qs + wave * HD, first, n, m, l, acc);
     const int64_t at = (((int64_t)it.b * p.Hkv + it.hk) * p.R + row) * p.splits + it.split;

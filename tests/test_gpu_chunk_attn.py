@@ -157,6 +157,22 @@ def test_what_is_not_seen_is_not_felt(cuda, dtype, bad, T):
     assert not torch.isfinite(again[0, sees]).any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hd,heads,T,n", [(64, 2, 4, 2), (64, 2, 70, 41), (128, 3, 50, 20), (128, 4, 40, 33)])
+def test_tokens_past_a_stream_feel_nothing(cuda, dtype, hd, heads, T, n):
+    """A value that is not finite, of a position that a stream's last tokens see: the tokens past them
+    are zeros all the same."""
+    A, left, P = 40, 200, 16
+    at = A + n - 1
+    out, q, pages = _chunk(cuda, dtype, hd, heads, 1, P, T, left, [A], [n])
+    rows, M = pages.rows.cpu().numpy(), pages.max_pages
+    ops.page_blocks(pages.v_pool)[1, int(rows[0, 1 + at // P % M]), :, at % P] = float("inf")
+    again = ops.chunk_attn(q.to(cuda), pages, 1, num_heads=heads, left=left, lengths=torch.tensor([n], dtype=torch.int32, device=cuda))
+    assert (again[0, n:] == 0).all()
+    assert not torch.isfinite(again[0, n - 1]).any()
+    assert torch.allclose(again[0, : n - 1].double(), out[0, : n - 1].double(), rtol=4 * torch.finfo(dtype).eps, atol=4 * torch.finfo(dtype).eps)
+
+
 def test_layouts(cuda):
     """A query that is a view of a wider projection, rows of a wider block table, an output that is a
     view, the query itself as output: the same bits as the plain call."""
@@ -176,6 +192,36 @@ def test_layouts(cuda):
     assert call(own, out=own) is own and torch.equal(own, out)
     assert torch.equal(ops.chunk_attn(q.to(cuda)[:, :0], there, 1, num_heads=4), out[:, :0])
     assert ops.chunk_attn(q.to(cuda)[:0], there, 1, num_heads=4).shape == (0, 5, 512)
+
+
+def test_a_query_of_all_streams(cuda):
+    """One row of queries for all streams and all tokens (strides of 0): the bits of its copies."""
+    _, _, pages = _chunk(cuda, BF16, 64, 4, 2, 16, 3, 100, [80, 3], [3, 3], whole=True)
+    q = torch.randn(1, 1, 256, device=cuda).to(BF16)
+    many = q.expand(2, 3, -1)
+    got = ops.chunk_attn(many, pages, 1, num_heads=4, left=100)
+    assert torch.equal(got, ops.chunk_attn(many.contiguous(), pages, 1, num_heads=4, left=100)) and torch.isfinite(got).all()
+    kv = torch.randn(2, 70, 256, device=cuda).to(BF16)
+    assert torch.equal(ops.cross_attn(many, kv, kv, num_heads=4), ops.cross_attn(many.contiguous(), kv, kv, num_heads=4))
+
+
+def test_two_streams_at_once(cuda):
+    """Split calls that run at the same time on two streams keep apart: the bits of one after another."""
+    _, q, pages = _chunk(cuda, BF16, 128, 8, 2, 16, 1, 9000, [8999, 700, 5000], [1, 1, 1])
+    q = [x.to(cuda) for x in (q, -q, q * 0.5, q * 0.25)]
+    kv = torch.randn(3, 4000, 512, device=cuda).to(BF16)
+    k, v = kv[..., :256], kv[..., 256:]
+    calls = [lambda x: ops.chunk_attn(x, pages, 1, num_heads=8, left=9000), lambda x: ops.cross_attn(x, k, v, num_heads=8)]
+    want = [call(x) for x in q for call in calls]
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for x in q:
+        for call, stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                got.append(call(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_another_stream_and_repeats(cuda):
@@ -233,6 +279,21 @@ def test_states_shared_and_long(cuda, dtype):
     _cross(cuda, dtype, 64, 2, 1, 3, 700, [700, 650, 3], expand=True)
     _cross(cuda, dtype, 128, 2, 2, 1, 6001, [6001], scale=0.3)
     _cross(cuda, dtype, 64, 4, 4, 150, 333, [333, 7])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [1, 20, 140])
+def test_a_state_for_all(cuda, dtype, T):
+    """States that are one row (a stride of 0 along them): the mean of equal values is the value, up to
+    the weights' and the quotient's roundings."""
+    g = torch.Generator().manual_seed(3)
+    q, kv = torch.randn(2, T, 128, generator=g).to(dtype), torch.randn(2, 1, 256, generator=g).to(dtype)
+    k, v = (x.expand(-1, 90, -1) for x in (kv.to(cuda)[..., :128], kv.to(cuda)[..., 128:]))
+    out = ops.cross_attn(q.to(cuda), k, v, num_heads=2, lengths=torch.tensor([90, 33], dtype=torch.int32, device=cuda))
+    want = kv[..., 128:].double().expand(-1, T, -1)
+    # output and weights each rounded once to the type; 2^-20: fp32 sums of 90 weights, exp2 and the quotient
+    tol = (3 * torch.finfo(dtype).eps / 2 + 2.0**-20) * want.abs() + (2.0**-25 if dtype is F16 else 0)
+    _check(out, want, tol, "one state")
 
 
 def test_no_states(cuda):

@@ -226,3 +226,36 @@ def test_encoder_streams_forked_and_compacted(cuda):
                     t[3] = 0
             cache.compact()
             assert sorted(cache.pool.free_list().tolist()) == cache.pool.free_list().tolist()
+
+
+def test_rows_of_a_view_are_forked(cuda):
+    """A view's rows name its own slots; a view whose step was open before the fork says so."""
+    Ly, D, S = 2, 64, 5
+    cache = ModelCache(Ly, (40, 1), D, 9, batch_size=S, device=cuda, dtype=torch.float16, device_pages=True)
+    other = cache.batch([0, 2])
+    g = torch.Generator(device=cuda).manual_seed(1)
+
+    def step(view, n):
+        return [view.update_attn_cache(layer, *(torch.randn(n, 2, D, generator=g, device=cuda).half() for _ in range(2))) for layer in range(Ly)]
+
+    for _ in range(30):
+        held = step(cache, S)
+    cache.conv_frames.normal_(generator=g)
+    view = cache.batch([3, 1, 4])
+    step(other, 2)
+    before = cache.conv_frames.clone()
+    view.fork([0], [2])  # slot 3 into slot 4
+    assert torch.equal(cache.conv_frames[4], before[3]) and torch.equal(cache.conv_frames[:4], before[:4])
+    with pytest.raises(RuntimeError, match="moved"):
+        other.window(0)
+    after = step(cache, S)
+    for old, new in zip(held, after):
+        for a, b in zip(old, new):
+            assert torch.equal(b[4, :-2], a[3, 2:]) and torch.equal(b[1, :-2], a[1, 2:]) and torch.equal(b[3, :-2], a[3, 2:])
+    with pytest.raises(ValueError, match="rows"):
+        view.fork([3], [0])
+    with pytest.raises(ValueError, match="both"):
+        view.fork([0, 1], [1, 2])
+    with pytest.raises(ValueError, match="distinct"):
+        view.fork([0, 0], [1, 1])
+    assert torch.equal(cache.conv_frames[4], before[3])  # refused calls change nothing
