@@ -1586,11 +1586,13 @@ def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-def _head_out(out: torch.Tensor | None, query: torch.Tensor, dev: torch.device, operands) -> torch.Tensor:
+def _head_out(what: str, out: torch.Tensor | None, query: torch.Tensor, dev: torch.device, operands) -> torch.Tensor:
     """The output [B, T, D] of a call: a new tensor, or ``out``, which may be query and meets nothing else."""
     B, T, D = query.shape
     if out is None:
         return torch.empty((B, T, D), dtype=query.dtype, device=dev)
+    if _follows(out):
+        _refuse_followed(what, [out])
     _head_rows("out", out, B, T, query.dtype, D)
     if out.device != dev:
         raise ValueError(f"tensors on different devices: {dev} and {out.device}")
@@ -1661,7 +1663,7 @@ def qk_norm_append(
     if out is None:
         out = torch.empty_like(query)
     else:
-        out = _head_out(out, query, query.device, [key, value, kp, vp])
+        out = _head_out("qk_norm_append", out, query, query.device, [key, value, kp, vp, rows, slot_map] + [t for t in (q_weight, k_weight, inv_freq, positions) if t is not None])
     if B == 0 or T == 0:
         return out
     (qb, qt, qu), (kb, kt, ku), (vb, vt, vu), (ob, ot, _), (mb, mu) = query.stride(), key.stride(), value.stride(), out.stride(), slot_map.stride()
@@ -1749,7 +1751,7 @@ def chunk_attn(
     if out is None:
         out = torch.empty_like(query)
     else:
-        out = _head_out(out, query, query.device, [kp, vp, rows] + ([lengths] if lengths is not None else []))
+        out = _head_out("chunk_attn", out, query, query.device, [kp, vp, rows] + ([lengths] if lengths is not None else []))
     if B == 0 or T == 0:
         return out
     (qb, qt, qu), (ob, ot, _), (rb, ru) = query.stride(), out.stride(), rows.stride()
@@ -1829,7 +1831,7 @@ def cross_attn(
     if out is None:
         out = torch.empty_like(query)
     else:
-        out = _head_out(out, query, query.device, [key, value] + ([lengths] if lengths is not None else []))
+        out = _head_out("cross_attn", out, query, query.device, [key, value] + ([lengths] if lengths is not None else []))
     if B == 0 or T == 0:
         return out
     (qb, qt, qu), (kb, kt, ku), (vb, vt, vu), (ob, ot, _) = query.stride(), key.stride(), value.stride(), out.stride()

@@ -334,3 +334,21 @@ def test_outputs_that_meet_operands_are_refused(cuda):
         ops.chunk_attn(q[:, :1], pages, 0, num_heads=2, out=pages.v_pool.view(1, 8, 128)[:, 3:4])
     with pytest.raises(ValueError, match="overlap"):
         ops.cross_attn(q.expand(2, -1, -1), kv.expand(2, -1, -1), kv.expand(2, -1, -1), num_heads=2, out=q.expand(2, -1, -1))
+
+
+def test_outputs_that_something_follows_are_refused(cuda):
+    q, kv = torch.randn(1, 2, 64, device=cuda), torch.randn(1, 9, 64, device=cuda)
+    pool = torch.zeros(1, 1, 16, 64, device=cuda)
+    pages = ops.PagedKV(pool, pool.clone(), torch.zeros(1, 3, dtype=torch.int32, device=cuda), 2)
+    slots = torch.zeros(1, 2, dtype=torch.int32, device=cuda)
+    weight = torch.ones(64, device=cuda)
+    calls = [lambda out: ops.cross_attn(q, kv, kv, num_heads=1, out=out), lambda out: ops.chunk_attn(q, pages, 0, num_heads=1, left=4, out=out),
+             lambda out: ops.qk_norm_append(q, kv[:, :2], kv[:, 2:4], pages, 0, slots, num_heads=1, q_weight=weight, out=out)]
+    for call in calls:
+        leaf = torch.zeros_like(q, requires_grad=True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(leaf)
+        with torch.no_grad():
+            assert call(leaf) is leaf
+    with pytest.raises(ValueError, match="overlap"):
+        ops.qk_norm_append(q[:, :1], kv[:, :1], kv[:, 1:2], pages, 0, slots[:, :1], num_heads=1, q_weight=weight, out=weight.view(1, 1, 64))
