@@ -1324,8 +1324,8 @@ int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, 
   p.row_tiles = c.row_tiles;
   p.splits = c.splits;
   const int64_t rows = (int64_t)p.B * p.T * p.Hq;
-  // a grid has fewer than 2^32 threads
-  if (c.groups >= (1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);
+  // a grid has fewer than 2^32 threads, of up to 512 a workgroup of 16 rows
+  if (c.groups >= (c.rows == 16 ? 1 << 23 : 1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);
   if (c.splits > 1) {
     if (!workspace || !aligned16(workspace)) return fail(PK_ERR_INVALID, "%s: workspace must be non-NULL and 16-byte aligned", what);
     p.part = static_cast<float*>(workspace);

@@ -459,7 +459,7 @@ class ModelCache:
         """The slots of rows of this view, between two steps."""
         if not self.device_pages:
             raise RuntimeError("paged cache: fork and compact need device_pages")
-        if self._recording:
+        if self._recording or (self.k_pages.is_cuda and torch.cuda.is_current_stream_capturing()):
             raise RuntimeError("paged cache: fork and compact are not recorded")
         self._check_whole()
         rows = np.asarray(rows, dtype=np.int64).reshape(-1)

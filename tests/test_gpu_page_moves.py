@@ -259,3 +259,18 @@ def test_rows_of_a_view_are_forked(cuda):
     with pytest.raises(ValueError, match="distinct"):
         view.fork([0, 0], [1, 1])
     assert torch.equal(cache.conv_frames[4], before[3])  # refused calls change nothing
+
+
+def test_moves_of_a_cache_are_not_recorded(cuda):
+    """A cache counts its moves on the host: neither a fork nor a compaction goes into a graph."""
+    cache = ModelCache(1, (20, 1), 64, 9, batch_size=3, device=cuda, dtype=torch.float16, device_pages=True)
+    x = torch.randn(3, 2, 64, device=cuda).half()
+    cache.update_attn_cache(0, x, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x + 1  # a graph holds something
+        for call in (lambda: cache.fork([0], [1]), cache.compact):
+            with pytest.raises(RuntimeError, match="not recorded"):
+                call()
+    cache.window(0)  # not stale
