@@ -65,8 +65,9 @@ __device__ static inline float of_partner(float x) {
 }
 
 // A wave takes the 64 / LPH heads of an item at once (q's, k's and v's in a row, so that an item is 1 KB), TOK tokens'
-// items over the workgroup's waves; U items' loads are on their way together. 16 K tokens of 16 + 2 + 2
-// heads of 128 in bf16 move 144 MB.
+// items over the workgroup's waves; U items' loads are on their way together. 15.6 K tokens of 16 + 2 + 2
+// heads of 128 in bf16, half of them with a place, 144 MB read and written: 28.6 us, 5.0 TB/s (a large copy: 5.2). Of so many tokens the
+// caches keep nothing, so their stores go past them: 33.6 us through them; loads past them as well 33.7.
 template <typename ST, int HD, int TOK, int U>
 __global__ void __launch_bounds__(256) qk_norm_append_kernel(const NormK<ST> p) {
   constexpr int VEC = Tr<ST>::VEC, LPH = HD / VEC, CB = 64 / (int)sizeof(ST), HPI = 64 / LPH;
@@ -165,7 +166,12 @@ __global__ void __launch_bounds__(256) qk_norm_append_kernel(const NormK<ST> p) 
       else
         turn(x, f, turned, integral_constant<int, 1>());
     }
-    if (to[u]) st16(to[u], value ? raw[u] : Tr<ST>::pack(x));
+    const u32x4 made = value ? raw[u] : Tr<ST>::pack(x);
+    if (!to[u]) return;
+    if constexpr (TOK == 8)
+      __builtin_nontemporal_store(made, reinterpret_cast<u32x4*>(to[u]));
+    else
+      st16(to[u], made);
   };
   for (int i0 = wave; i0 < items; i0 += 4 * U) {
 #pragma unroll
@@ -1225,7 +1231,7 @@ int norm_append(const pk_qk_norm_append_args* a, hipStream_t s) {
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const int64_t total = (int64_t)p.B * p.T;
   // few tokens: one a workgroup, for the shortest chain; many: 4 or 8, whose loads go together (15.6 K tokens of 20 heads
-  // of 128 in bf16, 144 MB: 32.5 us with 4, 30.7 with 8)
+  // of 128 in bf16, stored through the caches: 32.5 us with 4, 30.7 with 8)
   const int tok = total <= 1024 ? 1 : total <= 8192 ? 4 : 8;
   const dim3 grid((unsigned)((total + tok - 1) / tok));
   if ((int64_t)grid.x >= (1 << 24)) return fail(PK_ERR_UNSUPPORTED, "%s: %lld tokens in one call (built: fewer than 2^27)", what, (long long)total);
