@@ -1094,7 +1094,55 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
   attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG>(p, it, s, keys, KT, sums, ml, bad, qs);
 }
 
-// The splits of a row meet: weights by their maxima, sums over them. A workgroup a row.
+// where a row of a join goes
+template <typename ST>
+__device__ static inline ST* joined_at(const AttendK<ST>& p, uint32_t x, int head_dim) {
+  const uint32_t unit = x / (uint32_t)p.R, row = x - unit * (uint32_t)p.R;
+  const uint32_t b = unit / (uint32_t)p.Hkv, hk = unit - b * (uint32_t)p.Hkv, i = row / (uint32_t)p.G, gq = row - i * (uint32_t)p.G;
+  return p.out + b * p.o_sb + i * p.o_st + (int64_t)(hk * p.G + gq) * head_dim;
+}
+template <typename ST>
+__device__ static inline void put4(ST* to, f32x4_t v) {
+  float f[4] = {v[0], v[1], v[2], v[3]};
+  if constexpr (sizeof(ST) == 4)
+    st16(to, Tr<ST>::pack(f));
+  else
+    *reinterpret_cast<u32x2*>(to) = pack4<ST>(f);
+}
+
+// The splits of a row meet: weights by their maxima, sums over them. Few splits: HD / 4 lanes a row, a lane
+// with the splits' four columns at once.
+constexpr int kFewSplits = 8;
+template <typename ST, int HD>
+__global__ void __launch_bounds__(256) attend_join_few_kernel(const AttendK<ST> p, uint32_t rows) {
+  constexpr int LANES = HD / 4;
+  const uint32_t x = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (x >= rows) return;
+  const int c = (threadIdx.x & (LANES - 1)) * 4;
+  float2 v[kFewSplits];
+  f32x4_t part[kFewSplits];
+#pragma unroll
+  for (int u = 0; u < kFewSplits; ++u) {
+    const int64_t at = (int64_t)x * p.splits + min(u, p.splits - 1);
+    v[u] = p.ml[at];
+    part[u] = *reinterpret_cast<const f32x4_t*>(p.part + at * HD + c);
+  }
+  float top = kNone, l = 0.f;
+#pragma unroll
+  for (int u = 0; u < kFewSplits; ++u) top = fmaxf(top, v[u].x);
+  if (top == kNone) top = 0.f;
+  f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < kFewSplits; ++u) {
+    if (u >= p.splits || v[u].y == 0.f) continue;
+    const float w = __builtin_amdgcn_exp2f(v[u].x - top);
+    l = fmaf(v[u].y, w, l);
+    acc += part[u] * w;
+  }
+  put4(joined_at(p, x, HD) + c, acc * (l == 0.f ? 0.f : 1.f / l));
+}
+
+// More: a workgroup a row.
 constexpr int kMaxSplits = 256;
 template <typename ST, int HD>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
@@ -1103,8 +1151,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
   __shared__ float red[4], total[4];
   __shared__ f32x4_t sums[256];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t x = blockIdx.x, unit = x / (uint32_t)p.R, row = x - unit * (uint32_t)p.R;
-  const int b = (int)(unit / (uint32_t)p.Hkv), hk = (int)(unit - (uint32_t)b * p.Hkv), i = (int)(row / (uint32_t)p.G), gq = (int)(row - (uint32_t)i * p.G);
+  const uint32_t x = blockIdx.x;
   const float2 v = tid < p.splits ? p.ml[(int64_t)x * p.splits + tid] : float2{kNone, 0.f};
   // the parts are on their way while their weights are made; one without keys for the row holds zeros
   const int c = (tid & (LANES - 1)) * 4;
@@ -1136,12 +1183,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
 #pragma unroll
   for (int k = 1; k < SIDE; ++k) acc += sums[tid + k * LANES];
   const float sum = (total[0] + total[1]) + (total[2] + total[3]), inv = sum == 0.f ? 0.f : 1.f / sum;
-  ST* const to = p.out + b * p.o_sb + i * p.o_st + (int64_t)(hk * p.G + gq) * HD + c;
-  float f[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
-  if constexpr (sizeof(ST) == 4)
-    st16(to, Tr<ST>::pack(f));
-  else
-    *reinterpret_cast<u32x2*>(to) = pack4<ST>(f);
+  put4(joined_at(p, x, HD) + c, acc * inv);
 }
 
 namespace {
@@ -1317,7 +1359,11 @@ int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, in
   }
   int rc = check_launch(what);
   if (rc != PK_OK || p.splits == 1) return rc;
-  hipLaunchKernelGGL((attend_join_kernel<ST, HD>), dim3((unsigned)((int64_t)p.B * p.Hkv * p.R)), block, 0, s, p);
+  const uint32_t rows = (uint32_t)p.B * p.Hkv * p.R;
+  if (p.splits <= kFewSplits)
+    hipLaunchKernelGGL((attend_join_few_kernel<ST, HD>), dim3((rows + 1024 / HD - 1) / (1024 / HD)), block, 0, s, p, rows);
+  else
+    hipLaunchKernelGGL((attend_join_kernel<ST, HD>), dim3(rows), block, 0, s, p);
   return check_launch(what);
 }
 
