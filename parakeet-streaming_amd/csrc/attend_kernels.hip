@@ -210,9 +210,13 @@ struct AttendK {
   float scale;  // times log2(e)
   int32_t R;                 // rows of a key head: T * G
   int32_t row_tiles, splits;  // workgroups along the rows, and along the keys
+  int32_t order, key_bits;    // Order; bits of the most keys
   float* part;   // splits > 1: [B * Hkv * R][splits][HD] sums over a split's keys
   float2* ml;    // and [B * Hkv * R][splits] their {maximum in log2 units, sum of weights}
 };
+
+// Streams in the order of the batch; the longest first, 64 at a time; so, but every second one from the end
+enum Order { kAsTheyAre, kLongFirst, kFolded };
 
 constexpr float kNone = -__builtin_inff();
 
@@ -347,9 +351,13 @@ struct ItemOf {
 };
 
 // Workgroup -> (stream and key head and split, row tile): workgroups go to the XCDs in turn, and
-// the row tiles of the same keys to the same one, whose L2 then has them.
-template <typename ST>
-__device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows) {
+// the row tiles of the same keys to the same one, whose L2 then has them. Streams of different lengths: the
+// longest first, so that the last workgroups to end are short ones; where all are on the GPU at once,
+// and none waits for another, every second one in the other order, so that a CU has a long and a short one
+// (60 x 4 rows over up to 1500 states: 54.7 us as they are, 43.9 folded; 8 x 197 rows in fp32 over up to
+// 751: 31.8 and 25.1).
+template <typename ST, bool PAGED>
+__device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows, StreamOf& s) {
   const uint32_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
   const uint32_t tile = y % (uint32_t)p.row_tiles, u = y / (uint32_t)p.row_tiles * 8 + x;
   const uint32_t unit = u / (uint32_t)p.splits;
@@ -359,6 +367,30 @@ __device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows) {
   it.hk = (int32_t)(unit - (uint32_t)it.b * (uint32_t)p.Hkv);
   it.row0 = (int32_t)tile * rows;
   it.live = it.b < p.B;
+  if (!it.live) return it;
+  if (p.order == kAsTheyAre) {
+    s = stream_of<ST, PAGED>(p, it.b);
+    return it;
+  }
+  // the stream that has `want` longer ones before it, of the 64 around b; by the six highest bits of the keys that it has
+  const int lane = threadIdx.x & 63, b0 = it.b & ~63, n = min(64, p.B - b0);
+  const StreamOf mine = stream_of<ST, PAGED>(p, b0 + min(lane, n - 1));
+  const uint32_t keys = (uint32_t)(PAGED ? (mine.n > 0 ? min(mine.A, p.left) + mine.n : 0) : mine.end);
+  int want = it.b - b0;
+  if (p.order == kFolded && (p.B > 64 ? b0 >> 6 & 1 : want >= (n + 1) >> 1)) want = p.B > 64 ? n - 1 - want : n - 1 - (want - ((n + 1) >> 1));
+  uint64_t left = n == 64 ? ~0ull : (1ull << n) - 1;
+  for (int bit = p.key_bits - 1, last = max(p.key_bits - 6, 0); bit >= last; --bit) {
+    const uint64_t longer = __ballot(keys >> bit & 1) & left;
+    const int c = __popcll(longer);
+    left = want < c ? longer : left & ~longer;
+    want -= want < c ? 0 : c;
+  }
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
+  const int at = __builtin_ctzll(__ballot((left >> lane & 1) && before == want));
+  it.b = b0 + at;
+  s.A = __builtin_amdgcn_readlane(mine.A, at);
+  s.n = __builtin_amdgcn_readlane(mine.n, at);
+  s.end = __builtin_amdgcn_readlane(mine.end, at);
   return it;
 }
 
@@ -497,9 +529,9 @@ __global__ void __launch_bounds__(64 * NW, 2) attend_few_kernel(const AttendK<ST
   __shared__ uint32_t bad[(ROWS + 31) / 32];
   __shared__ float qs[PAGED ? NW * HD : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const ItemOf it = item_of(p, ROWS);
+  StreamOf s;
+  const ItemOf it = item_of<ST, PAGED>(p, ROWS, s);
   if (!it.live) return;
-  const StreamOf s = stream_of<ST, PAGED>(p, it.b);
   const KeysOf keys = keys_of<ST, PAGED, KT>(p, s, it.row0, ROWS, it.split);
 
   // the rows: their queries and what they see
@@ -819,9 +851,9 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
   __shared__ uint32_t bad[(ROWS + 31) / 32];
   __shared__ float qs[PAGED ? 4 * KG * HD : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, wv = wave & 3, kg = wave >> 2;
-  const ItemOf it = item_of(p, ROWS);
+  StreamOf s;
+  const ItemOf it = item_of<ST, PAGED>(p, ROWS, s);
   if (!it.live) return;
-  const StreamOf s = stream_of<ST, PAGED>(p, it.b);
   const KeysOf keys = keys_of<ST, PAGED, KT>(p, s, it.row0, ROWS, it.split);
 
   const int row = it.row0 + 32 * wv + r32;
@@ -1375,6 +1407,12 @@ int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, 
   const AttendCut c = attend_cut(dtype, p.B, p.T, p.Hq, p.Hkv, keys, PAGED && p.page_shift < 4);
   p.row_tiles = c.row_tiles;
   p.splits = c.splits;
+  // workgroups that have a CU each need no order; two of those of 256 threads are on a CU at once. Few keys do not
+  // differ by what finding it costs (5 tokens of 60 streams over up to 516: 15.8 us as they are, 16.5 in order; one
+  // of 60 over up to 2001: 31.2 and 26.4)
+  const bool ragged = p.B > 1 && (PAGED || p.lengths) && keys >= (PAGED ? 1024 : 256);
+  p.order = !ragged || c.groups <= 256 ? kAsTheyAre : c.groups <= 512 && c.key_groups == 1 ? kFolded : kLongFirst;
+  p.key_bits = 32 - __builtin_clz((unsigned)keys | 1);
   const int64_t rows = (int64_t)p.B * p.T * p.Hq;
   // a grid has fewer than 2^32 threads, of up to 512 a workgroup of 16 rows
   if (c.groups >= (c.rows == 16 ? 1 << 23 : 1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);

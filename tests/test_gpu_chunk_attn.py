@@ -103,6 +103,14 @@ def test_long_cache(cuda, dtype):
     _chunk(cuda, dtype, 128, 8, 1, 16, 3, 9000, [8990], [3])
 
 
+@pytest.mark.parametrize("dtype,n,heads,kv_heads,T", [(BF16, 70, 8, 4, 1), (F16, 70, 2, 2, 2), (BF16, 17, 8, 8, 1), (F32, 64, 5, 5, 1), (F16, 66, 4, 4, 33)])
+def test_many_streams_over_caches_of_any_lengths(cuda, dtype, n, heads, kv_heads, T):
+    rng = np.random.default_rng(n)
+    A, new = rng.integers(0, 2500, n), rng.integers(0, T + 1, n)
+    A[1], A[2], new[2], new[3] = 0, A[4], T, 0
+    _chunk(cuda, dtype, 64, heads, kv_heads, 16, T, 1100, A.tolist(), new.tolist())
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("T", [1, 6, 40])
 def test_far_positions(cuda, dtype, T):
@@ -294,6 +302,16 @@ def test_a_state_for_all(cuda, dtype, T):
     # output and weights each rounded once to the type; 2^-20: fp32 sums of 90 weights, exp2 and the quotient
     tol = (3 * torch.finfo(dtype).eps / 2 + 2.0**-20) * want.abs() + (2.0**-25 if dtype is F16 else 0)
     _check(out, want, tol, "one state")
+
+
+@pytest.mark.parametrize("dtype,n,heads,kv_heads,T", [(F16, 40, 8, 8, 4), (BF16, 64, 8, 8, 1), (F16, 130, 4, 2, 3), (BF16, 70, 8, 8, 2), (F32, 45, 7, 7, 9),
+                                                      (BF16, 20, 4, 4, 600), (F16, 30, 4, 4, 700), (F32, 9, 4, 4, 300)])
+def test_many_streams_of_any_lengths(cuda, dtype, n, heads, kv_heads, T):
+    """Batches whose workgroups are more than the CUs: each stream is answered once, in whatever order they are taken."""
+    rng, S = np.random.default_rng(n), 270
+    lens = rng.integers(0, S + 1, n).tolist()
+    lens[1], lens[2], lens[3], lens[n - 1], lens[n - 2] = 0, S, S, 1, lens[4]
+    _cross(cuda, dtype, 64, heads, kv_heads, T, S, lens)
 
 
 def test_no_states(cuda):
