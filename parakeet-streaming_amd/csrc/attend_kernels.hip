@@ -215,7 +215,7 @@ struct AttendK {
   float2* ml;    // and [B * Hkv * R][splits] their {maximum in log2 units, sum of weights}
 };
 
-// Streams in the order of the batch; the longest first, 64 at a time; so, but every second one from the end
+// Streams in the order of the batch; the longest first, 256 at a time; so, but every second one from the end
 enum Order { kAsTheyAre, kLongFirst, kFolded };
 
 constexpr float kNone = -__builtin_inff();
@@ -354,8 +354,8 @@ struct ItemOf {
 // the row tiles of the same keys to the same one, whose L2 then has them. Streams of different lengths: the
 // longest first, so that the last workgroups to end are short ones; where all are on the GPU at once,
 // and none waits for another, every second one in the other order, so that a CU has a long and a short one
-// (60 x 4 rows over up to 1500 states: 54.7 us as they are, 43.9 folded; 8 x 197 rows in fp32 over up to
-// 751: 31.8 and 25.1).
+// (60 x 4 rows over up to 1500 states: 54.7 us as they are, 43.3 folded; 8 x 197 rows in fp32 over up to
+// 751: 31.8 and 25.4; 100 streams of 8 heads of 64 over up to 3000 tokens, longest first: 62.0 and 57.3).
 template <typename ST, bool PAGED>
 __device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows, StreamOf& s) {
   const uint32_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
@@ -372,25 +372,57 @@ __device__ static inline ItemOf item_of(const AttendK<ST>& p, int rows, StreamOf
     s = stream_of<ST, PAGED>(p, it.b);
     return it;
   }
-  // the stream that has `want` longer ones before it, of the 64 around b; by the six highest bits of the keys that it has
-  const int lane = threadIdx.x & 63, b0 = it.b & ~63, n = min(64, p.B - b0);
-  const StreamOf mine = stream_of<ST, PAGED>(p, b0 + min(lane, n - 1));
-  const uint32_t keys = (uint32_t)(PAGED ? (mine.n > 0 ? min(mine.A, p.left) + mine.n : 0) : mine.end);
+  // the stream that has `want` longer ones before it, of the 256 around b, four a lane; by the six highest bits of the
+  // keys that it has
+  constexpr int N = 4;
+  const int lane = threadIdx.x & 63, b0 = it.b & -(64 * N), n = min(64 * N, p.B - b0);
+  StreamOf mine[N];
+  uint32_t keys[N];
+  uint64_t left[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    keys[j] = 0;
+    left[j] = 0;
+    if (64 * j >= n) continue;
+    mine[j] = stream_of<ST, PAGED>(p, b0 + min(64 * j + lane, n - 1));
+    keys[j] = (uint32_t)(PAGED ? (mine[j].n > 0 ? min(mine[j].A, p.left) + mine[j].n : 0) : mine[j].end);
+    left[j] = n >= 64 * (j + 1) ? ~0ull : (1ull << (n - 64 * j)) - 1;
+  }
   int want = it.b - b0;
-  if (p.order == kFolded && (p.B > 64 ? b0 >> 6 & 1 : want >= (n + 1) >> 1)) want = p.B > 64 ? n - 1 - want : n - 1 - (want - ((n + 1) >> 1));
-  uint64_t left = n == 64 ? ~0ull : (1ull << n) - 1;
+  if (p.order == kFolded) {  // the second half of the 256, or of the batch's, from the end
+    const bool one = p.B <= 64 * N;
+    const int half = one ? (n + 1) >> 1 : 0;
+    if (one ? want >= half : 2 * (b0 / (64 * N)) >= (p.B + 64 * N - 1) / (64 * N)) want = n - 1 - (want - half);
+  }
   for (int bit = p.key_bits - 1, last = max(p.key_bits - 6, 0); bit >= last; --bit) {
-    const uint64_t longer = __ballot(keys >> bit & 1) & left;
-    const int c = __popcll(longer);
-    left = want < c ? longer : left & ~longer;
+    uint64_t longer[N];
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (64 * j >= n) continue;
+      longer[j] = __ballot(keys[j] >> bit & 1) & left[j];
+      c += __popcll(longer[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (64 * j < n) left[j] = want < c ? longer[j] : left[j] & ~longer[j];
     want -= want < c ? 0 : c;
   }
-  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
-  const int at = __builtin_ctzll(__ballot((left >> lane & 1) && before == want));
-  it.b = b0 + at;
-  s.A = __builtin_amdgcn_readlane(mine.A, at);
-  s.n = __builtin_amdgcn_readlane(mine.n, at);
-  s.end = __builtin_amdgcn_readlane(mine.end, at);
+  // of those that are left, the want-th
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (64 * j >= n) continue;
+    const int c = __popcll(left[j]);
+    if (want >= 0 && want < c) {
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left[j], 0));
+      const int at = __builtin_ctzll(__ballot((left[j] >> lane & 1) && before == want));
+      it.b = b0 + 64 * j + at;
+      s.A = __builtin_amdgcn_readlane(mine[j].A, at);
+      s.n = __builtin_amdgcn_readlane(mine[j].n, at);
+      s.end = __builtin_amdgcn_readlane(mine[j].end, at);
+    }
+    want -= c;
+  }
   return it;
 }
 
@@ -514,12 +546,13 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 // product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them.
 // Where keys are: a tensor of states; pages of 16 frames and more, so that 16 keys from a multiple of 16 on are of
 // one page, whose number is a scalar; smaller pages, looked up key by key.
-// Pages that one row tile reads are read past the caches (128 streams of up to 4096: 119 us cached, 107 so); rows of states
+// Pages that one row tile reads are read past the caches (128 streams of up to 4096, before they were put in order: 119 us cached, 107 so); rows of states
 // are not, since a load has half of a 128-byte line of each (60 x 4 rows over up to 1500: 43 us, 63 past the caches).
 enum Source { kStates, kPages, kSmallPages };
-template <typename ST, int HD, Source SRC, int RT, int NW, bool STREAM>
-__global__ void __launch_bounds__(64 * NW, 2) attend_few_kernel(const AttendK<ST> p) {
+template <typename ST, int HD, Source SRC, int RT, bool STREAM>
+__global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p) {
   constexpr bool PAGED = SRC != kStates;
+  constexpr int NW = 4;
   constexpr int E = (int)sizeof(ST), ROWS = 16 * RT, SUB = E == 2 ? 2 : 1, KT = 16 * SUB, NB = HD * E / 64, NT = HD / 16;
   constexpr int VROW = HD * E + 16;  // bytes of a staged row of V: 16 more spread the rows over the banks
   constexpr int STRIDE = HD + 4;
@@ -1349,11 +1382,11 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
   c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
   // keys are split over workgroups where the rows leave CUs without one (256 CUs hold one of attend_many_kernel's
-  // workgroups each, and two of attend_few_kernel's), and long ones so that streams of different lengths fill them
-  // alike; a part has 512 keys or 1024 at least, since parts are joined in a launch of 4 us
+  // workgroups each, and two of attend_few_kernel's); a part has 512 keys at least, since parts are joined in a launch
+  // of 4 us. Streams of different lengths are left whole and put in order (128 over up to 4096: 88 us whole,
+  // 97 in two parts)
   const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512;
-  auto parts = [&](int64_t groups, int least) { return std::min((groups + whole - 1) / whole, (int64_t)keys / least); };
-  int64_t n = std::max(parts(full * 3 / 4, 512), c.rows == 128 ? 0 : parts(1024, 1024));
+  int64_t n = std::min((full * 3 / 4 + whole - 1) / whole, (int64_t)keys / 512);
   n = std::min(std::max(n, (int64_t)1), (int64_t)kMaxSplits);
   c.splits = (int)n;
   c.groups = (units * n + 7) / 8 * 8 * c.row_tiles;
@@ -1368,21 +1401,16 @@ int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, in
   constexpr Source SRC = PAGED ? kPages : kStates;
   if (PAGED && p.page_shift < 4) {
     if (c.rows == 16)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1, 4, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 1, false>), grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2, 4, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, kSmallPages, 2, false>), grid, block, 0, s, p);
   } else if (c.rows == 16) {
-    // waves of a workgroup: 8 for long parts of pages (128 streams of up to 4096: 105 us with 4, 99 with 8), 4 for
-    // others (5 tokens over 516: 13.7 and 14.7; 60 x 4 rows over up to 1500 states: 43 and 46)
-    if (PAGED && keys / p.splits >= 1024)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, PAGED ? 8 : 4, PAGED>), grid, dim3(512), 0, s, p);
-    else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, 4, PAGED>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 1, PAGED>), grid, block, 0, s, p);
   } else if (c.rows == 32) {
     if (PAGED && c.row_tiles == 1)
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, 4, PAGED>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, PAGED>), grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, 4, false>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attend_few_kernel<ST, HD, SRC, 2, false>), grid, block, 0, s, p);
   } else if constexpr (sizeof(ST) == 2) {
     if (c.key_groups == 1)
       hipLaunchKernelGGL((attend_many_kernel<ST, HD, PAGED, 1>), grid, block, 0, s, p);
@@ -1409,13 +1437,13 @@ int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, 
   p.splits = c.splits;
   // workgroups that have a CU each need no order; two of those of 256 threads are on a CU at once. Few keys do not
   // differ by what finding it costs (5 tokens of 60 streams over up to 516: 15.8 us as they are, 16.5 in order; one
-  // of 60 over up to 2001: 31.2 and 26.4)
-  const bool ragged = p.B > 1 && (PAGED || p.lengths) && keys >= (PAGED ? 1024 : 256);
+  // of 60 over up to 2001: 31.2 and 26.3; 240 x 4 rows over up to 375 states: 48.0 and 52.7)
+  const bool ragged = p.B > 1 && (PAGED || p.lengths) && keys >= (PAGED ? 1024 : 512);
   p.order = !ragged || c.groups <= 256 ? kAsTheyAre : c.groups <= 512 && c.key_groups == 1 ? kFolded : kLongFirst;
   p.key_bits = 32 - __builtin_clz((unsigned)keys | 1);
   const int64_t rows = (int64_t)p.B * p.T * p.Hq;
-  // a grid has fewer than 2^32 threads, of up to 512 a workgroup of 16 rows
-  if (c.groups >= (c.rows == 16 ? 1 << 23 : 1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);
+  // a grid has fewer than 2^32 threads
+  if (c.groups >= (1 << 24) || (c.splits > 1 && rows >= (1 << 24))) return fail(PK_ERR_UNSUPPORTED, "%s: %lld rows in one call", what, (long long)rows);
   if (c.splits > 1) {
     if (!workspace || !aligned16(workspace)) return fail(PK_ERR_INVALID, "%s: workspace must be non-NULL and 16-byte aligned", what);
     p.part = static_cast<float*>(workspace);
