@@ -128,7 +128,7 @@ __device__ static inline void fork_entry(const ForkK& p, const ForkOf& f, uint32
   if (j == 0) p.appended[f.dst] = p.appended[f.src];
 }
 
-// A few pairs in one launch: bound by its chain of round trips.
+// A few pairs in one launch: bound by its chain of round trips (4 pairs of 32 slots: 4.3 us, 48 of 230: 4.7).
 constexpr int kForkOne = 256, kForkOneEntries = 8192;  // pairs, and their ring entries
 __global__ void __launch_bounds__(kForkThreads) page_fork_kernel(const ForkK p) {
   extern __shared__ uint32_t lds[];
@@ -227,7 +227,7 @@ __device__ static inline void compact_entry(const CompactK& p, const uint32_t* b
   if (page >= N && page < (uint32_t)p.total) p.ring[i] = p.pairs[held_below(bits, before, page) - held_below(bits, before, N)].y;
 }
 
-// Small pools in one launch, bits in LDS.
+// Small pools in one launch, bits in LDS (230 slots of 7 entries: 4.7 us).
 constexpr int kCompactOne = 32768;  // pages
 __global__ void __launch_bounds__(kCompactThreads) page_compact_kernel(const CompactK p) {
   __shared__ uint32_t bits[kCompactOne / 32], before[kCompactOne / 32 + 1], sums[kCompactThreads / 64];
