@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -38,6 +39,7 @@ from ._lib import (
     SubArgs,
     check,
     lib,
+    packer,
 )
 
 _DTYPES = {
@@ -1562,6 +1564,7 @@ def _refuse_pages(pages: PagedKV, dtype: torch.dtype, hd: int) -> None:
         raise TypeError(f"pages dtype {kp.dtype} != {dtype}")
 
 
+_pack_norm_append, _pack_chunk_attn, _pack_cross_attn = packer(QkNormAppendArgs), packer(ChunkAttnArgs), packer(CrossAttnArgs)
 _ELEMENT = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
 
@@ -1674,13 +1677,13 @@ def qk_norm_append(
     ):
         _refuse_norm_append(query, key, value, pages, slot_map, H, q_weight, k_weight, inv_freq, positions, eps)
     stream = torch._C._cuda_getCurrentRawStream(at)
-    a = QkNormAppendArgs(
-        _DTYPES[dt], at, PagedLayout(kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M), layer, B, T, H, hd, n, 1 if interleaved else 0, eps,
-        qp, qb, qt, kyp, kb, kt, vlp, vb, vt, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-        inv_freq.data_ptr() if n else None, None if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
+    a = _pack_norm_append(
+        _DTYPES[dt], at, kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M, operator.index(layer), B, T, H, hd, n, 1 if interleaved else 0, eps,
+        qp, qb, qt, kyp, kb, kt, vlp, vb, vt, 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        inv_freq.data_ptr() if n else 0, 0 if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
         slot_map.data_ptr(), mb, out.data_ptr(), ob, ot,
     )
-    check(lib().pk_qk_norm_append(ctypes.byref(a), stream), "pk_qk_norm_append")
+    check(lib().pk_qk_norm_append(a, stream), "pk_qk_norm_append")
     return out
 
 
@@ -1760,11 +1763,11 @@ def chunk_attn(
     code, stream = _DTYPES[dt], torch._C._cuda_getCurrentRawStream(at)
     n = _attn_space(code, B, T, H, D // hd, hd, left + T)
     space = torch.empty(n, dtype=torch.uint8, device=query.device) if n else None
-    a = ChunkAttnArgs(
-        code, at, PagedLayout(kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M), layer, B, T, H, hd, left, scale, qp, qb, qt,
-        None if lengths is None else lengths.data_ptr(), out.data_ptr(), ob, ot, None if space is None else space.data_ptr(),
+    a = _pack_chunk_attn(
+        code, at, kp.data_ptr(), vp.data_ptr(), Ly, N, P, D, rows.data_ptr(), rb, M, operator.index(layer), B, T, H, hd, operator.index(left), scale, qp, qb, qt,
+        0 if lengths is None else lengths.data_ptr(), out.data_ptr(), ob, ot, 0 if space is None else space.data_ptr(),
     )
-    check(lib().pk_chunk_attn(ctypes.byref(a), stream), "pk_chunk_attn")
+    check(lib().pk_chunk_attn(a, stream), "pk_chunk_attn")
     return out
 
 
@@ -1840,11 +1843,11 @@ def cross_attn(
     code, stream = _DTYPES[dt], torch._C._cuda_getCurrentRawStream(at)
     n = _attn_space(code, B, T, H, D // hd, hd, S)
     space = torch.empty(n, dtype=torch.uint8, device=query.device) if n else None
-    a = CrossAttnArgs(
-        code, at, B, T, S, H, D // hd, hd, scale, qp, qb, qt, kp, kb, kt, vp, vb, vt, None if lengths is None else lengths.data_ptr(),
-        out.data_ptr(), ob, ot, None if space is None else space.data_ptr(),
+    a = _pack_cross_attn(
+        code, at, B, T, S, H, D // hd, hd, scale, qp, qb, qt, kp, kb, kt, vp, vb, vt, 0 if lengths is None else lengths.data_ptr(),
+        out.data_ptr(), ob, ot, 0 if space is None else space.data_ptr(),
     )
-    check(lib().pk_cross_attn(ctypes.byref(a), stream), "pk_cross_attn")
+    check(lib().pk_cross_attn(a, stream), "pk_cross_attn")
     return out
 
 

@@ -340,3 +340,25 @@ def test_pool_places_are_the_blocks():
     kp, _, k, _ = fill_pages(rows, 4, 2, 96, [3], [6], torch.float16, torch.Generator().manual_seed(0))
     assert torch.equal(kp.view(-1)[pool_places(kp)[1, 1, 3]], k[0][0]) and torch.isnan(kp.view(-1)[pool_places(kp)[1, 1, 2]]).all()
     assert torch.equal(kp.view(-1)[pool_places(kp)[1, 0, 1]], k[0][2])
+
+
+@pytest.mark.parametrize("args", [_lib.QkNormAppendArgs, _lib.ChunkAttnArgs, _lib.CrossAttnArgs])
+def test_packed_arguments_are_the_structure(args):
+    """The bytes that a packer makes are the structure's, field by field; values out of a field's range are refused."""
+    kinds = [kind for _, kind in _lib._layout(args)]
+    values = [{"f": 0.5 + i, "Q": 2**63 + i}.get(kind, 100 + i) for i, kind in enumerate(kinds)]
+    data = _lib.packer(args)(*values)
+    a = args.from_buffer_copy(data)
+    assert len(data) == ctypes.sizeof(args)
+
+    def flat(s):
+        for name, kind in s._fields_:
+            x = getattr(s, name)
+            yield from flat(x) if isinstance(x, ctypes.Structure) else (x,)
+
+    assert list(flat(a)) == values
+    for i, kind in enumerate(kinds):
+        bad = list(values)
+        bad[i] = 1e39 if kind == "f" else 2**64
+        with pytest.raises(ValueError, match=args.__name__):
+            _lib.packer(args)(*bad)
