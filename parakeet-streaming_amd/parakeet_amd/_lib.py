@@ -662,10 +662,10 @@ SIGNATURES = {
     "pk_adapter_linear_form": (c_int, [c_int32] * 7 + [POINTER(AdapterForm)]),
     "pk_adapter_linear": (c_int, [POINTER(AdapterLinearArgs), c_void_p]),
     "pk_page_fork_workspace_bytes": (c_int64, [c_int32, c_int32]),
-    "pk_page_fork": (c_int, [POINTER(PageForkArgs), c_void_p]),
+    "pk_page_fork": (c_int, [c_void_p, c_void_p]),  # PageForkArgs, or the bytes of one
     "pk_page_compact_workspace_bytes": (c_int64, [c_int64, c_int32]),
     "pk_page_compact": (c_int, [POINTER(PageCompactArgs), c_void_p]),
-    "pk_kv_move_pages": (c_int, [POINTER(KvMovePagesArgs), c_void_p]),
+    "pk_kv_move_pages": (c_int, [c_void_p, c_void_p]),  # KvMovePagesArgs, or the bytes of one
     "pk_qk_norm_append": (c_int, [c_void_p, c_void_p]),  # QkNormAppendArgs, or the bytes of one
     "pk_attn_workspace_bytes": (c_int64, [c_int32] * 7),
     "pk_chunk_attn": (c_int, [c_void_p, c_void_p]),  # ChunkAttnArgs, or the bytes of one

@@ -1248,6 +1248,9 @@ def kv_append_slots(pages: PagedKV, layer: int, key: torch.Tensor, value: torch.
     check(lib().pk_kv_append_slots(ctypes.byref(a), _stream(dev)), "pk_kv_append_slots")
 
 
+_pack_page_fork, _pack_move_pages = packer(PageForkArgs), packer(KvMovePagesArgs)
+
+
 @dataclass
 class PageMoves:
     """Copies from page to page that a fork or a compaction asks for (:func:`kv_move_pages`):
@@ -1265,23 +1268,21 @@ def page_fork(state: PageState, src: torch.Tensor, dst: torch.Tensor) -> PageMov
     pages hold old frames.  A source may be forked several times.  A pair is absent (nothing
     of it changes) where a slot is out of range or the destination is a source of the call
     or was named before in it.  No host work and no synchronisation."""
-    n = dst.numel()
-    a, dev, M, _ = state._args(dst)
-    if n > a.num_slots:
-        raise ValueError(f"{n} pairs for {a.num_slots} slots")
-    f = PageForkArgs()
-    f.device, f.batch, f.num_slots, f.num_pages, f.page_size, f.left, f.chunk = a.device, n, a.num_slots, a.num_pages, a.page_size, a.left, a.chunk
-    f.queue, f.head, f.appended, f.ring, f.dst = a.queue, a.head, a.appended, a.ring, a.slots
-    f.src = _i32(src, "src", (n,))
+    a, dev, M, n = state._args(dst)
+    S = a.num_slots
+    if n > S:
+        raise ValueError(f"{n} pairs for {S} slots")
+    src_at = _i32(src, "src", (n,))
     _require_device(dst, src)
     moves = PageMoves(dst.new_empty((n * M, 2)), dst.new_empty(1))
-    f.pairs, f.count = moves.pairs.data_ptr(), moves.count.data_ptr()
     L = lib()
     space = L.pk_page_fork_workspace_bytes(n, M)
-    if space:
-        space = torch.empty(space, dtype=torch.uint8, device=dev)
-        f.workspace = space.data_ptr()
-    check(L.pk_page_fork(ctypes.byref(f), _stream(dev)), "pk_page_fork")
+    space = torch.empty(space, dtype=torch.uint8, device=dev) if space else None
+    f = _pack_page_fork(
+        a.device, n, S, a.num_pages, state.page_size, state.left, state.chunk, a.queue, a.head, a.appended, a.ring, src_at, a.slots or 0,
+        moves.pairs.data_ptr(), moves.count.data_ptr(), 0 if space is None else space.data_ptr(),
+    )
+    check(L.pk_page_fork(f, _stream(dev)), "pk_page_fork")
     return moves
 
 
@@ -1313,16 +1314,13 @@ def kv_move_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves: PageMoves) 
     page is both read and written, or written twice, in one call."""
     pairs, count = moves.pairs, moves.count
     n = pairs.shape[0] if pairs.dim() == 2 else -1
-    a = KvMovePagesArgs()
-    a.pairs, a.count, a.capacity = _i32(pairs, "moves.pairs", (n, 2)), _i32(count, "moves.count", (1,)), n
+    pairs_at, count_at = _i32(pairs, "moves.pairs", (n, 2)), _i32(count, "moves.count", (1,))
     dev = _require_device(k_pool, v_pool, pairs, count)
-    if k_pool.shape != v_pool.shape or k_pool.dim() != 4 or k_pool.dtype != v_pool.dtype or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+    shape, dt = k_pool.shape, k_pool.dtype
+    if len(shape) != 4 or v_pool.shape != shape or v_pool.dtype is not dt or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("k_pool and v_pool must be matching contiguous [Ly, num_pages, P, D] tensors")
-    a.dtype, a.device = dtype_code(k_pool.dtype), _index(dev)
-    L = a.pages
-    L.k_pool, L.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
-    L.num_layers, L.num_pages, L.page_size, L.d_model = k_pool.shape
-    check(lib().pk_kv_move_pages(ctypes.byref(a), _stream(dev)), "pk_kv_move_pages")
+    a = _pack_move_pages(dtype_code(dt), _index(dev), k_pool.data_ptr(), v_pool.data_ptr(), *shape, 0, 0, 0, pairs_at, n, count_at)
+    check(lib().pk_kv_move_pages(a, _stream(dev)), "pk_kv_move_pages")
 
 
 # ---------------------------------------------------------------------------

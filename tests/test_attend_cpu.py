@@ -342,7 +342,7 @@ def test_pool_places_are_the_blocks():
     assert torch.equal(kp.view(-1)[pool_places(kp)[1, 0, 1]], k[0][2])
 
 
-@pytest.mark.parametrize("args", [_lib.QkNormAppendArgs, _lib.ChunkAttnArgs, _lib.CrossAttnArgs])
+@pytest.mark.parametrize("args", [_lib.QkNormAppendArgs, _lib.ChunkAttnArgs, _lib.CrossAttnArgs, _lib.PageForkArgs, _lib.KvMovePagesArgs])
 def test_packed_arguments_are_the_structure(args):
     """The bytes that a packer makes are the structure's, field by field; values out of a field's range are refused."""
     kinds = [kind for _, kind in _lib._layout(args)]
