@@ -1389,8 +1389,9 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);
   // keys are split over workgroups where the rows leave CUs without one (256 CUs hold one of attend_many_kernel's
   // workgroups each, and two of attend_few_kernel's); a part has 512 keys at least, since parts are joined in a launch
-  // of 4 us. Streams of different lengths are left whole and put in order (128 over up to 4096: 88 us whole,
-  // 97 in two parts)
+  // of 4 us. So 384 workgroups or more are left whole (128 streams over up to 4096, 512 of them: 88 us whole,
+  // 97 in two parts), fewer are not (36 x 4 rows over up to 1500 states, 288: 41.1 us whole, 36.3 in two; 61 streams over up to
+  // 4000, 244: 46.3 in two, 50.9 in three)
   const int64_t whole = units * c.row_tiles, full = c.rows == 128 ? 256 : 512;
   int64_t n = std::min((full * 3 / 4 + whole - 1) / whole, (int64_t)keys / 512);
   n = std::min(std::max(n, (int64_t)1), (int64_t)kMaxSplits);
@@ -1402,7 +1403,7 @@ AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, i
 int64_t attend_space(int64_t rows, int splits, int head_dim) { return splits > 1 ? rows * splits * (4 * head_dim + 8) : 0; }
 
 template <typename ST, int HD, bool PAGED>
-int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, int keys, hipStream_t s) {
+int attend_launch(const char* what, const AttendK<ST>& p, const AttendCut& c, hipStream_t s) {
   const dim3 grid((unsigned)c.groups), block(256);
   constexpr Source SRC = PAGED ? kPages : kStates;
   if (PAGED && p.page_shift < 4) {
@@ -1457,7 +1458,7 @@ int attend(const char* what, AttendK<ST>& p, int dtype, int head_dim, int keys, 
   }
   DeviceGuard dg(device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, device);
-  return head_dim == 64 ? attend_launch<ST, 64, PAGED>(what, p, c, keys, s) : attend_launch<ST, 128, PAGED>(what, p, c, keys, s);
+  return head_dim == 64 ? attend_launch<ST, 64, PAGED>(what, p, c, s) : attend_launch<ST, 128, PAGED>(what, p, c, s);
 }
 
 template <typename ST>
