@@ -292,7 +292,7 @@ class ModelCache:
 
     def paged(self) -> ops.PagedKV:
         """Device view (pools + this batch's rows) for the kernels."""
-        return ops.PagedKV(self.k_pages, self.v_pages, self._rows, self.max_pages)
+        return ops.PagedKV(self.k_pages, self.v_pages, self._rows, self.max_pages, self.left_attn)
 
     def _check_chunk(self, key: Tensor, value: Tensor) -> None:
         B, T = key.shape[:2]

@@ -114,12 +114,14 @@ class PagedKV:
     """Device view of a batch's pages: pools of Ly x num_pages pages of P frames
     x D columns (tensors [Ly, num_pages, P, D] whose pages are stored as 64-byte
     column blocks, see page_blocks) and the per-stream rows {A, ring[max_pages]}
-    (int32 [B, 1 + max_pages])."""
+    (int32 [B, 1 + max_pages]). ``left``: the window of the page pool that the rows come
+    from, which :func:`chunk_attn` takes unless it is given one."""
 
     k_pool: torch.Tensor
     v_pool: torch.Tensor
     rows: torch.Tensor
     max_pages: int
+    left: int | None = None
 
     def layout(self) -> PagedLayout:
         kp, vp, rows = self.k_pool, self.v_pool, self.rows
@@ -1720,9 +1722,9 @@ def chunk_attn(
 ) -> torch.Tensor:
     """Attention of each stream's new tokens over its paged cache, which holds them already
     (:func:`qk_norm_append` or :func:`kv_append_slots` of this step): token i of stream b, at position
-    ``rows[b, 0] + i``, sees itself and the ``left`` positions before it (None: the most that
-    the ring holds for any alignment).  query [B, T, num_heads * head_dim], heads of 64 or 128 columns; the
-    pages' D columns are D / head_dim key heads, each read by num_heads * head_dim / D query heads.
+    ``rows[b, 0] + i``, sees itself and the ``left`` positions before it (None: ``pages.left``, the
+    pool's window; what a pool's ring holds beyond it changes with the place in a page).  query
+    [B, T, num_heads * head_dim], heads of 64 or 128 columns; the pages' D columns are D / head_dim key heads, each read by num_heads * head_dim / D query heads.
     ``lengths``: int32 [B], new tokens of each stream (held within 0 .. T; None: T).  Returns [B, T,
     num_heads * head_dim]: zeros past a stream's tokens and where no key is there; ``out`` may be ``query``.  ``scale``: None is
     head_dim ** -0.5.  fp32 accumulation and softmax.  What a token gets depends on the keys and values that
@@ -1736,7 +1738,9 @@ def chunk_attn(
     hd = W // H if H > 0 else 0
     most = (M - 1) * P + 1 - T
     if left is None:
-        left = most
+        left = pages.left
+        if left is None and (most <= 0 or not B or not T):
+            left = min(most, 0)  # no other window fits the ring, or nothing looks through it
     if scale is None:
         scale = hd**-0.5 if hd else 1.0
     qp = query.data_ptr()
@@ -1745,7 +1749,7 @@ def chunk_attn(
         and vp.shape == kp.shape and rows.dim() == 2 and rows.shape[0] >= B and rows.shape[1] >= 1 + M
         and kp.dtype is dt and vp.dtype is dt and rows.dtype is _INT32
         and kp.get_device() == at and vp.get_device() == at and rows.get_device() == at and kp.is_contiguous() and vp.is_contiguous()
-        and 0 <= left <= most and 0 < scale < math.inf
+        and left is not None and 0 <= left <= most and 0 < scale < math.inf
         and (lengths is None or (lengths.shape == (B,) and lengths.dtype is _INT32 and lengths.get_device() == at and lengths.is_contiguous()))
     ):
         _refuse_chunk_attn(query, pages, H, lengths, left, most, scale)
@@ -1778,6 +1782,8 @@ def _refuse_chunk_attn(query, pages, H, lengths, left, most, scale) -> None:
     _require_device(query, pages.k_pool, pages.v_pool, pages.rows)
     if pages.rows.shape[0] < B:
         raise ValueError(f"rows covers {pages.rows.shape[0]} streams, batch is {B}")
+    if left is None:
+        raise ValueError("left: the positions that a token sees before it; give it, or the window of the rows' pool as PagedKV's left")
     if not 0 <= left <= most:
         raise ValueError(f"{pages.max_pages} ring entries of {pages.k_pool.shape[2]} frames hold {most} positions before {T} new ones at any "
                          f"alignment, left is {left}")

@@ -103,7 +103,7 @@ class AttentionStep:
         D = sh.d_model
         x = self.qkv[layer]
         q, k, v = x.chunk(3, dim=-1)
-        pages = ops.PagedKV(self.k_pages, self.v_pages, self.rows, self.pool.max_pages)
+        pages = ops.PagedKV(self.k_pages, self.v_pages, self.rows, self.pool.max_pages, self.shape.left)
         a = AttnArgs()
         a.dtype = ops.dtype_code(sh.dtype)
         a.device = self.device.index if self.device.index is not None else torch.cuda.current_device()
