@@ -220,6 +220,12 @@ enum Order { kAsTheyAre, kLongFirst, kFolded };
 
 constexpr float kNone = -__builtin_inff();
 
+// Weights are 2^(score - m), m following the maximum. fp16 loses bits of those below 2^-14 and all of those below
+// 2^-25, and a long tail of them can be a good part of the sum; it ends at 2^16 only, so there m stays below the maximum, by
+// what keeps the largest weights at 2^kTop. The quotient cancels it.
+template <typename ST>
+constexpr float kTop = __is_same(ST, _Float16) ? 15.f : 0.f;
+
 // what a workgroup needs of a stream
 struct StreamOf {
   int32_t A;     // position of token 0 (pages)
@@ -544,7 +550,8 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 // register group, so maxima and sums are in the lane but for 4 lanes, and the weights are the next
 // product's operand where they are. 16-bit types: two tiles of 16 keys make one step of 32, in
 // the order that the registers have; V comes back transposed from LDS; weights go into the
-// product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them.
+// product as a high and a low 16-bit part, which costs nothing here and keeps 2^-16 or better of them (fp16: of those from
+// 2^-24 of the largest on; the low part ends at 2^-40 of it).
 // Where keys are: a tensor of states; pages of 16 frames and more, so that 16 keys from a multiple of 16 on are of
 // one page, whose number is a scalar; smaller pages, looked up key by key.
 // Pages that one row tile reads are read past the caches (128 streams of up to 4096, before they were put in order: 119 us cached, 107 so); rows of states
@@ -720,7 +727,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = fmaxf(top, x[a][u][k]);
-        top = fmaxf(m[a], max_of_groups(top) * p.scale);
+        top = fmaxf(m[a], fmaf(max_of_groups(top), p.scale, -kTop<ST>));
         const float base = top == kNone ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[a] - base);
         m[a] = top;
         float sum = 0.f;
@@ -839,6 +846,8 @@ __device__ static inline int mix(int r) {
 }
 
 constexpr float kSlack = 6.f;
+template <typename ST>
+constexpr float kLift = kTop<ST> > 0.f ? kTop<ST> - kSlack : 0.f;
 constexpr uint32_t kNowhere = 0xc0000000u;  // past any resource, also with an instruction's offset: reads zeros
 
 // A buffer resource as four words: `records` bytes from base.
@@ -873,8 +882,8 @@ __device__ static inline void stage_bytes(const u32x4 r, uint32_t lds, const uin
 // 128 rows of a key head a workgroup, 32 a wave; KG groups of 4 waves take tiles of 64 keys in turn.
 // A group stages its tile of K and V in LDS, a tile ahead, straight from memory. As in
 // attend_few_kernel products are transposed, so that a lane has one query; the weights are rounded once to
-// the type for the second product (half a step of it relative to each). Bound by the matrix cores and by the exp2
-// and conversions of the weights, which the other group's products hide where there are two: 4 x 512 tokens of 16 heads
+// the type for the second product (half a step of it relative to each; fp16: those below 2^-23 of the largest to 2^-34
+// of it). Bound by the matrix cores and by the exp2 and conversions of the weights, which the other group's products hide where there are two: 4 x 512 tokens of 16 heads
 // over 4 of 128 behind 3500 earlier ones, 58.7 GFLOP, 66 us (890 TFLOP/s); with one tile of registers between
 // the products 119, staged straight to LDS 113, two groups in turn 81, a wave's loads from one page 73. One group is enough
 // where there are 512 workgroups, two of which are on a CU.
@@ -1103,10 +1112,10 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
         for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
       {
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * p.scale;
+        top = fmaf(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), p.scale, -kLift<ST>);
       }
-      // the weights' base follows the maximum in steps of 2^kSlack or more: sums are rescaled in the
-      // first tile and hardly ever again, and weights up to 2^kSlack round as well as those up to 1
+      // the weights' base follows the maximum less kLift in steps of 2^kSlack or more: sums are rescaled in the
+      // first tile and hardly ever again, and weights up to 2^(kLift + kSlack) round as well as those up to 1
       if (__any(top > m + kSlack)) {
         top = fmaxf(top, m);
         const float keep = top == kNone ? 1.f : __builtin_amdgcn_exp2f(m - top);

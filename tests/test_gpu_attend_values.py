@@ -1,0 +1,67 @@
+"""Attention over scores at the ends of a type's range: one key far above a long tail of others."""
+
+import math
+
+import pytest
+import torch
+
+from parakeet_amd import ops
+from tests._attend_model import HALF, pool_places
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _paged(cuda, k, v, P, T):
+    """One stream's keys and values [L, D], the last T of them a step's, on pages in reverse order."""
+    L, D = k.shape
+    n = (L + P - 1) // P
+    pools = []
+    for x in (k, v):
+        pool = torch.full((1, n, P, D), float("nan"), dtype=x.dtype)
+        pos = torch.arange(L)
+        pool.view(-1)[pool_places(pool)[0, n - 1 - pos // P, pos % P]] = x
+        pools.append(pool.to(cuda))
+    rows = torch.tensor([[L - T] + list(range(n - 1, -1, -1)) + [-1] * (T // P + 2)], dtype=torch.int32, device=cuda)
+    return ops.PagedKV(*pools, rows, rows.shape[1] - 1)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bits", [16.25, 20.5, 25.25])
+@pytest.mark.parametrize("top", [0, 7777, 19999])
+@pytest.mark.parametrize("T", [1, 40])
+def test_a_long_tail(cuda, dtype, bits, top, T):
+    """20,000 keys whose weights are 2^-bits of one key's, which is first, last or between, and whose value is 0:
+    the output is the tail's mass times its values, for texts over states and tokens over pages.
+
+    How far a kernel may be, with u half a step of the type and p the tail's mass (n 2^-bits / (1 + n 2^-bits)):
+    the output's rounding, a weight's before the product with its value and its sum's, u each; fp32 sums over n
+    keys in tiles of 16: 2^-24 a tile; a score of `bits` and its product with log2 e, each rounded, exp2 and the quotient: 2^-18."""
+    n, hd, heads = 20000, 64, 2
+    g = torch.Generator().manual_seed(top)
+    # the key's score: q . k = (bits / log2 e) in its first column, in fp32; 16-bit types: the nearest they have
+    high = torch.tensor(bits / math.log2(math.e)).to(dtype)
+    weight = 2.0 ** (-float(high) * math.log2(math.e))
+    q = torch.zeros(1, T, heads * hd).to(dtype)
+    q[..., ::hd] = 1
+    k = torch.zeros(n, heads * hd).to(dtype)
+    k[top, ::hd] = high
+    v = (torch.rand(n, heads * hd, generator=g) + 0.5).to(dtype)
+    v[top] = 0
+    u, total = HALF[dtype], 1 + (n - 1) * weight
+    want = weight * v.double().sum(0) / total
+    tol = (3 * u + 2.0**-18 + n / 16 * 2.0**-24) * want
+    print(f"[tail] {dtype} bits {bits} top {top} T {T}", flush=True)
+    kd, vd = (x[None].to(cuda) for x in (k, v))
+    out = ops.cross_attn(q.to(cuda), kd, vd, num_heads=heads, scale=1.0).double().cpu()
+    far = ((out - want).abs() / tol).max()
+    assert far <= 1, f"states: {far:.2f} times the tolerance"
+    # tokens: all see the first n keys; the last of T tokens see T - 1 more of the tail
+    more = T - 1
+    kp, vp = torch.cat([k, torch.zeros(more, heads * hd).to(dtype)]), torch.cat([v, torch.ones(more, heads * hd).to(dtype)])
+    out = ops.chunk_attn(q.to(cuda), _paged(cuda, kp, vp, 64, T), 0, num_heads=heads, scale=1.0, left=n + T).double().cpu()[0]
+    i = torch.arange(T)[:, None]
+    want = weight * (v.double().sum(0) + i) / (1 + (n - 1 + i) * weight)
+    far = ((out - want).abs() / ((3 * u + 2.0**-18 + n / 16 * 2.0**-24) * want)).max()
+    assert far <= 1, f"tokens: {far:.2f} times the tolerance"
