@@ -1063,7 +1063,8 @@ int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream);
  * the reference, whose attention is pk_paged_relpos_attn's.
  *   out_i = sum_j softmax_j(scale q_i . k_j) v_j   over positions j in [A + i - left, A + i], j >= 0
  * for token i < lengths[b] of stream b (held within 0 .. chunk; NULL: chunk), A = rows[b][0]; zeros for i >=
- * lengths[b] and where no key is there (ring entries outside [0, num_pages) are not).
+ * lengths[b] and where no key is there (ring entries outside [0, num_pages) are not); NaN, as the softmax is, where
+ * all scores are -inf.
  * Query head h reads key head h / (num_heads / kv_heads), kv_heads = d_model / head_dim.  fp32
  * accumulation and softmax.  What a token gets depends on the keys and values that it sees
  * alone, also where others are infinite or NaN.
@@ -1102,7 +1103,7 @@ int pk_chunk_attn(const pk_chunk_attn_args* args, void* stream);
  * pk_cross_attn -- attention of each stream's tokens to states of another length, as a
  * decoder reads the encoder's:
  *   out_i = sum_j softmax_j(scale q_i . k_j) v_j   over j in [0, lengths[b])
- * (lengths int32 [batch], held within 0 .. states; NULL: states); zeros where that is empty.  Rows of key
+ * (lengths int32 [batch], held within 0 .. states; NULL: states); zeros where that is empty, NaN where all scores are -inf.  Rows of key
  * and value from lengths[b] on are not read.  No counterpart in the reference.
  * query, out: [batch][chunk][num_heads * head_dim]; key, value: [batch][states][kv_heads * head_dim];
  * element strides (b, t) >= 0 (0: one stream's states for all; key's and value's t below 2^23), rows 16-byte aligned with

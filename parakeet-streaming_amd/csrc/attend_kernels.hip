@@ -218,7 +218,11 @@ struct AttendK {
 // Streams in the order of the batch; the longest first, 256 at a time; so, but every second one from the end
 enum Order { kAsTheyAre, kLongFirst, kFolded };
 
-constexpr float kNone = -__builtin_inff();
+// A row's maximum before it has met a key; and of one that has met keys whose scores were all -inf, since a softmax
+// of them is NaN where one of no keys is zeros here.
+constexpr float kNone = -__builtin_inff(), kLeast = -__FLT_MAX__;
+// 1 / l, of a row of sum l and maximum m
+__device__ static inline float quotient(float m, float l) { return l != 0.f ? 1.f / l : m == kNone ? 0.f : __builtin_nanf(""); }
 
 // Weights are 2^(score - m), m following the maximum. fp16 loses bits of those below 2^-14 and all of those below
 // 2^-25, and a long tail of them can be a good part of the sum; it ends at 2^16 only, so there m stays below the maximum, by
@@ -279,10 +283,12 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
   const int64_t step = PAGED ? (int64_t)64 << p.page_shift : 64;
   m = kNone;
   l = 0.f;
+  bool met = false;
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) acc[c] = 0.f;
   for (int d0 = 0; d0 < n; d0 += 64) {
     const int64_t at = d0 + lane < n ? key_at<ST, PAGED>(p, b, HD * E, h, first + d0 + lane, false) : -1;
+    met = met || __any(at >= 0);
     float s = kNone;
     if (at >= 0) {
       float d = 0.f;
@@ -317,6 +323,7 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
       }
     }
   }
+  if (met) m = fmaxf(m, kLeast);
 }
 
 // ---- few rows
@@ -455,6 +462,29 @@ __device__ static inline KeysOf keys_of(const AttendK<ST>& p, const StreamOf& s,
   return k;
 }
 
+// Whether a row that sees keys lo .. hi and whose maximum is none all the same has met a key, in tiles that its wave takes
+// (every N-th of the split's, from number `first` on): its scores were -inf then. Rare, so looked up when the tiles are done.
+template <typename ST, bool PAGED, int KT, int N>
+__device__ static inline bool has_met(const AttendK<ST>& p, int b, const KeysOf& keys, int first, int lo, int hi, float m) {
+  const int a = max(lo / KT, keys.t0), last = min(hi / KT, keys.t1 - 1);
+  const bool met = m == kNone && lo <= hi && a + ((first - (a - keys.t0)) & (N - 1)) <= last;
+  if constexpr (!PAGED) return met;
+  if (!__any(met)) return false;
+  // of the pages that the split meets, whether there is one with a key of the row
+  const int32_t* const ring = p.rows + b * p.rows_stride + 1;
+  const int from = max(lo, keys.t0 * KT), to = min(hi, keys.t1 * KT - 1);
+  auto page_of = [&](int d) { return (int)(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift); };
+  const int page0 = page_of(max(keys.lo, keys.t0 * KT)), pages = page_of(min(keys.hi, keys.t1 * KT - 1)) - page0 + 1;
+  uint64_t any = 0;
+  for (int i0 = 0; i0 < pages; i0 += 64) {
+    const int i = min(i0 + (int)(threadIdx.x & 63), pages - 1);
+    const uint64_t there = __ballot((uint32_t)ring[(uint32_t)(page0 + i) % (uint32_t)p.max_pages] < (uint32_t)p.num_pages);
+    const int x = max(page_of(from) - page0 - i0, 0), y = min(page_of(to) - page0 - i0, 63);
+    any |= x <= y ? there >> x & (~0ull >> (63 - (y - x))) : 0ull;
+  }
+  return met && any != 0;
+}
+
 // The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled to their largest
 // maximum; ml: each part's own maximum and sum of weights), the quotient, or the split's part.
 // WAVES parts of [rows][HD + 4] floats at `sums`.
@@ -503,7 +533,7 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
       *reinterpret_cast<f32x4_t*>(to + 4) = f32x4_t{o[y][4], o[y][5], o[y][6], o[y][7]};
       if (c == 0) p.ml[at] = float2{m[y], l[y]};
     } else {
-      const float inv = l[y] == 0.f ? 0.f : 1.f / l[y];
+      const float inv = quotient(m[y], l[y]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[y][e] *= inv;
       ST* const to = p.out + it.b * p.o_sb + i * p.o_st + (int64_t)h * HD + c;
@@ -528,6 +558,7 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
     const int n = i < s.n ? min(seen.y - keys.k0, keys.t1 * KT - 1) - (first - keys.k0) + 1 : 0;
     float m, l, acc[HD / 64];
     attend_row<ST, HD, PAGED>(p, it.b, it.hk, qs + wave * HD, first, n, m, l, acc);
+    const float inv = quotient(m, l);
     const int64_t at = (((int64_t)it.b * p.Hkv + it.hk) * p.R + row) * p.splits + it.split;
     ST* const to = p.out + it.b * p.o_sb + i * p.o_st + (int64_t)h * HD;
 #pragma unroll
@@ -535,7 +566,7 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
       if (p.splits > 1)
         p.part[at * HD + lane + 64 * c] = acc[c];
       else
-        to[lane + 64 * c] = to_st<ST>(l == 0.f ? 0.f : acc[c] / l);
+        to[lane + 64 * c] = to_st<ST>(l != 0.f ? acc[c] / l : inv);
     }
     if (p.splits > 1 && lane == 0) p.ml[at] = float2{m, l};
     wave_lds_sync();
@@ -798,6 +829,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
     l[a] = sum_of_groups(l[a]);
+    if (has_met<ST, PAGED, KT, NW>(p, it.b, keys, wave, lo[a], live[a] ? hi[a] : -1, m[a])) m[a] = kLeast;
     if (!live[a]) {
       m[a] = kNone;
       l[a] = 0.f;
@@ -1189,6 +1221,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
+  if (has_met<ST, PAGED, KT, KG>(p, it.b, keys, kg, lo, hi, m)) m = kLeast;
   if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{m, l};
   __syncthreads();  // and every wave is done with the tiles
   float* const sums = reinterpret_cast<float*>(smem);
@@ -1244,7 +1277,6 @@ __global__ void __launch_bounds__(256) attend_join_few_kernel(const AttendK<ST> 
   float top = kNone, l = 0.f;
 #pragma unroll
   for (int u = 0; u < kFewSplits; ++u) top = fmaxf(top, v[u].x);
-  if (top == kNone) top = 0.f;
   f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < kFewSplits; ++u) {
@@ -1253,7 +1285,7 @@ __global__ void __launch_bounds__(256) attend_join_few_kernel(const AttendK<ST> 
     l = fmaf(v[u].y, w, l);
     acc += part[u] * w;
   }
-  put4(joined_at(p, x, HD) + c, acc * (l == 0.f ? 0.f : 1.f / l));
+  put4(joined_at(p, x, HD) + c, acc * quotient(top, l));
 }
 
 // More: a workgroup a row (16 rows of 120 parts: 4.0 us).
@@ -1296,7 +1328,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK<ST> p) {
   if (tid >= LANES) return;
 #pragma unroll
   for (int k = 1; k < SIDE; ++k) acc += sums[tid + k * LANES];
-  const float sum = (total[0] + total[1]) + (total[2] + total[3]), inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float sum = (total[0] + total[1]) + (total[2] + total[3]), inv = quotient(top, sum);
   put4(joined_at(p, x, HD) + c, acc * inv);
 }
 

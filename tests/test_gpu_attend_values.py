@@ -1,4 +1,4 @@
-"""Attention over scores at the ends of a type's range: one key far above a long tail of others."""
+"""Attention over scores at the ends of a type's range: one key far above a long tail of others, scores of -inf."""
 
 import math
 
@@ -65,3 +65,47 @@ def test_a_long_tail(cuda, dtype, bits, top, T):
     want = weight * (v.double().sum(0) + i) / (1 + (n - 1 + i) * weight)
     far = ((out - want).abs() / ((3 * u + 2.0**-18 + n / 16 * 2.0**-24) * want)).max()
     assert far <= 1, f"tokens: {far:.2f} times the tolerance"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [1, 50, 3000])
+@pytest.mark.parametrize("T", [1, 20, 50])
+def test_scores_of_minus_infinity(cuda, dtype, n, T):
+    """Rows all of whose scores are -inf are NaN, as a softmax of them is; one finite score has the whole weight,
+    wherever it is. Where no key is there, zeros stay zeros."""
+    hd, heads = 64, 2
+    q = torch.zeros(1, T, heads * hd).to(dtype)
+    q[..., ::hd] = 1
+    L = n + T - 1
+    g = torch.Generator().manual_seed(n)
+    v = torch.randn(L, heads * hd, generator=g).to(dtype)
+    k = torch.zeros(L, heads * hd).to(dtype)
+    k[:, ::hd] = -math.inf
+    qd = q.to(cuda)
+    lengths = torch.tensor([T - T // 3], dtype=torch.int32, device=cuda)
+
+    def both(k, away=False):
+        pages = _paged(cuda, k, v, 16, T)
+        if away:
+            pages.rows[0, 1:] = -1
+        yield ops.chunk_attn(qd, pages, 0, num_heads=heads, lengths=lengths, left=L).cpu()[0]
+        if not away:
+            yield ops.cross_attn(qd, k[None].to(cuda), v[None].to(cuda), num_heads=heads).cpu()[0]
+
+    m = T - T // 3
+    print(f"[-inf] {dtype} n {n} T {T}", flush=True)
+    tokens, texts = both(k)
+    assert torch.isnan(tokens[:m]).all() and (tokens[m:] == 0).all() and torch.isnan(texts).all()
+    (tokens,) = both(k, away=True)
+    assert (tokens == 0).all()
+    for at in {0, n // 2, n - 1}:
+        one = k.clone()
+        one[at] = 0
+        tokens, texts = both(one)
+        assert torch.equal(tokens[:m], v[at].expand(m, -1)) and (tokens[m:] == 0).all()
+        assert torch.equal(texts, v[at].expand(T, -1))
+    # a value that most tokens do not see is not finite: those rows are made again
+    if T > 1:
+        v[-1] = math.inf
+        tokens, _ = both(k)
+        assert torch.isnan(tokens[:m]).all() and (tokens[m:] == 0).all()
