@@ -127,6 +127,8 @@ class ModelCache:
         self._base = self
         self._staging = None
         self._moved = 0  # times that pages were moved (of the base): rows from before are stale
+        # of the base, slots whose frames of an opened step are not all written (device pages)
+        self._unwritten = np.zeros(batch_size, dtype=bool)
         self._set_slots(np.arange(batch_size, dtype=np.int32))
 
     # ------------------------------------------------------------------ views
@@ -217,6 +219,8 @@ class ModelCache:
             self._open_step()
         self._check_rows()
         self._seen.add(layer_idx)
+        if self.device_pages and len(self._seen) == self.num_layers:
+            self._base._unwritten[self._slots] = False
 
     def _check_rows(self) -> None:
         if self._rows_moved != self._base._moved:
@@ -227,6 +231,7 @@ class ModelCache:
         self._rows_moved = base._moved
         if self.device_pages:
             self._advance_pages()
+            base._unwritten[self._slots] = True
         elif self._rows.device.type == "cuda":
             if base._staging is None:
                 base._staging = _RowStaging(max(1, base.pool.num_slots), 1 + self.max_pages)
@@ -273,6 +278,7 @@ class ModelCache:
             self.open_step()
         yield
         self._step_open, self._seen, self._rows_moved = True, set(range(self.num_layers)), self._base._moved
+        self._base._unwritten[self._slots] = False
 
     @contextmanager
     def recording(self):
@@ -439,7 +445,8 @@ class ModelCache:
     def fork(self, src, dst) -> None:
         """Rows ``dst`` continue the streams of rows ``src`` too (lists of equal length, no row in
         both): their windows and conv states are copies from here on (``ops.page_fork``), what
-        rows ``dst`` held is gone.  Between steps, on the stream of the steps; ``device_pages`` only."""
+        rows ``dst`` held is gone.  Between steps (of every view: a step that is given up is ended by resetting its
+        rows), on the stream of the steps; ``device_pages`` only."""
         s, d = self._pool_rows(src), self._pool_rows(dst)
         moves = self.pool.fork(s, d)
         ops.kv_move_pages(self.k_pages, self.v_pages, moves)
@@ -450,7 +457,7 @@ class ModelCache:
 
     def compact(self) -> None:
         """Moves the pages that all slots hold together, to the front of the pool (``ops.page_compact``):
-        what the streams see stays the same.  Between steps, on the stream of the steps; ``device_pages`` only."""
+        what the streams see stays the same.  When and where as :meth:`fork`."""
         self._pool_rows([])
         ops.kv_move_pages(self.k_pages, self.v_pages, self.pool.compact())
         self._base._moved += 1
@@ -461,7 +468,11 @@ class ModelCache:
             raise RuntimeError("paged cache: fork and compact need device_pages")
         if self._recording or (self.k_pages.is_cuda and torch.cuda.is_current_stream_capturing()):
             raise RuntimeError("paged cache: fork and compact are not recorded")
-        self._check_whole()
+        if self._base._unwritten.any():
+            raise RuntimeError(
+                f"paged cache: a step was opened for slots {np.flatnonzero(self._base._unwritten).tolist()} whose layers "
+                "are not all updated; pages move between steps"
+            )
         rows = np.asarray(rows, dtype=np.int64).reshape(-1)
         if len(rows) and (rows.min() < 0 or rows.max() >= len(self._slots)):
             raise ValueError(f"rows must be in [0, {len(self._slots)})")
@@ -472,6 +483,7 @@ class ModelCache:
         """All slots empty (parakeet/modules/cache.py:55-58)."""
         self.pool.reset_all()
         self.conv_frames.zero_()
+        self._base._unwritten[:] = False
         self._step_open = False
         self._seen = set()
 
@@ -480,6 +492,7 @@ class ModelCache:
         as zeros again (parakeet/modules/cache.py:60-63)."""
         pool_slot = int(self._slots[slot])
         self.pool.reset_slot(pool_slot)
+        self._base._unwritten[pool_slot] = False
         self.conv_frames[pool_slot].zero_()
 
 
