@@ -297,7 +297,9 @@ class ModelCache:
             self._seen = seen
 
     def paged(self) -> ops.PagedKV:
-        """Device view (pools + this batch's rows) for the kernels."""
+        """Device view (pools + this batch's rows) for the kernels; what it gives out is stale once pages move."""
+        if self._step_open and not self._recording:
+            self._check_rows()
         return ops.PagedKV(self.k_pages, self.v_pages, self._rows, self.max_pages, self.left_attn)
 
     def _check_chunk(self, key: Tensor, value: Tensor) -> None:

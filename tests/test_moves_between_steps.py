@@ -98,3 +98,22 @@ def test_a_replayed_step(cache):
     with cache.replaying():
         pass
     _allowed(cache)
+
+
+def test_stale_rows_are_not_given_out(cache):
+    """`paged()` of a step from before the pages moved; of one that follows, and of a view without a step, as ever."""
+    view, fresh = cache.batch([0, 2]), cache.batch([1])
+    _layers(cache)
+    _layers(view)
+    cache.paged(), view.paged()
+    cache._base._moved += 1  # as a fork or a compaction does
+    for c in (cache, view):
+        with pytest.raises(RuntimeError, match="moved"):
+            c.paged()
+    assert isinstance(fresh.paged(), ops.PagedKV)
+    with cache.recording():
+        cache.paged()
+    cache.open_step()
+    assert cache.paged().rows is cache._rows and cache.paged().left == 70
+    with pytest.raises(RuntimeError, match="moved"):
+        view.paged()
