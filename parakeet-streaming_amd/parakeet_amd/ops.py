@@ -1314,6 +1314,9 @@ def kv_move_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves: PageMoves) 
     """Copies whole pages of all layers of the pools [Ly, num_pages, P, D], as ``moves`` (of
     :func:`page_fork` or :func:`page_compact`) says; pairs of pages out of range are skipped.  No
     page is both read and written, or written twice, in one call."""
+    if _follows(k_pool, v_pool):
+        with torch.autocast("cuda", enabled=False):  # which changes no copy
+            _refuse_followed("kv_move_pages", [k_pool, v_pool])
     pairs, count = moves.pairs, moves.count
     n = pairs.shape[0] if pairs.dim() == 2 else -1
     pairs_at, count_at = _i32(pairs, "moves.pairs", (n, 2)), _i32(count, "moves.count", (1,))
@@ -1636,7 +1639,7 @@ def qk_norm_append(
     rotary a power of two from 16 to head_dim, columns past it are not turned); pairs are (i, i +
     rotary / 2), or (2 i, 2 i + 1) where ``interleaved``.  ``positions``: int32 [B, T]; None: token t of stream b is
     at ``pages.rows[b, 0] + t``.  The turns of an angle are made in 64 bits.  No gradients."""
-    operands = [t for t in (query, key, value, q_weight, k_weight, inv_freq) if t is not None]
+    operands = [t for t in (query, key, value, pages.k_pool, pages.v_pool, q_weight, k_weight, inv_freq) if t is not None]
     if _follows(*operands):
         _refuse_followed("qk_norm_append", operands)
     kp, vp, rows, dt, at, shape = pages.k_pool, pages.v_pool, pages.rows, query.dtype, query.get_device(), query.shape
@@ -1729,8 +1732,8 @@ def chunk_attn(
     num_heads * head_dim]: zeros past a stream's tokens and where no key is there; ``out`` may be ``query``.  ``scale``: None is
     head_dim ** -0.5.  fp32 accumulation and softmax.  What a token gets depends on the keys and values that
     it sees alone.  No gradients."""
-    if _follows(query):
-        _refuse_followed("chunk_attn", [query])
+    if _follows(query, pages.k_pool, pages.v_pool):
+        _refuse_followed("chunk_attn", [query, pages.k_pool, pages.v_pool])
     kp, vp, rows, dt, at, shape = pages.k_pool, pages.v_pool, pages.rows, query.dtype, query.get_device(), query.shape
     H, E, M = int(num_heads), _ELEMENT.get(dt, 0), pages.max_pages
     B, T, W = shape if len(shape) == 3 else (0, 0, 0)

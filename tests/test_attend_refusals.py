@@ -1,0 +1,45 @@
+"""What a text decoder's calls refuse, on the CPU: pools that something follows, outputs whose rows meet, scales past
+fp32, slots past 32 bits."""
+
+import ctypes
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from parakeet_amd import _lib, ops
+from parakeet_amd.pool import DevicePagePool
+
+
+class _Marked(torch.Tensor):
+    pass
+
+
+def _pool_calls():
+    z = lambda *s: torch.zeros(s)  # noqa: E731
+    rows, slots = torch.zeros(2, 7, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32)
+    moves = ops.PageMoves(torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    return {
+        "qk_norm_append": lambda k, v: ops.qk_norm_append(z(2, 3, 256), z(2, 3, 128), z(2, 3, 128), ops.PagedKV(k, v, rows, 6), 0, slots, num_heads=4),
+        "chunk_attn": lambda k, v: ops.chunk_attn(z(2, 3, 256), ops.PagedKV(k, v, rows, 6), 0, num_heads=4, left=9),
+        "kv_move_pages": lambda k, v: ops.kv_move_pages(k, v, moves),
+    }
+
+
+@pytest.mark.parametrize("name", ["qk_norm_append", "chunk_attn", "kv_move_pages"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_pools_that_something_follows(name, which):
+    call = _pool_calls()[name]
+    pools = [torch.zeros(1, 8, 16, 128) for _ in range(2)]
+    other = lambda t: [t if i == which else p for i, p in enumerate(pools)]  # noqa: E731
+    leaf = torch.zeros(1, 8, 16, 128, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        call(*other(leaf))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="HIP device"):
+        call(*other(leaf))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        call(*other(forward_ad.make_dual(leaf.detach(), torch.ones_like(leaf))))
+    with pytest.raises(RuntimeError, match="plain tensors"):
+        call(*other(leaf.detach().as_subclass(_Marked)))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        call(*pools)
