@@ -1592,6 +1592,19 @@ def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
+def _rows_cross(B: int, T: int, sb: int, st: int, D: int) -> bool:
+    """Whether two of the rows of D elements at b sb + t st meet."""
+    if (T > 1 and st < D) or (B > 1 and sb < D):
+        return True
+    if B <= 1 or T <= 1 or sb >= (T - 1) * st + D or st >= (B - 1) * sb + D:
+        return False
+    for b in range(1, B):  # neither kind of row is within the other's steps (rare)
+        t = b * sb // st
+        if any(0 < u < T and abs(b * sb - u * st) < D for u in (t, t + 1)):
+            return True
+    return False
+
+
 def _head_out(what: str, out: torch.Tensor | None, query: torch.Tensor, dev: torch.device, operands) -> torch.Tensor:
     """The output [B, T, D] of a call: a new tensor, or ``out``, which may be query and meets nothing else."""
     B, T, D = query.shape
@@ -1602,7 +1615,7 @@ def _head_out(what: str, out: torch.Tensor | None, query: torch.Tensor, dev: tor
     _head_rows("out", out, B, T, query.dtype, D)
     if out.device != dev:
         raise ValueError(f"tensors on different devices: {dev} and {out.device}")
-    if (out.stride(1) < D and T > 1) or (B > 1 and out.stride(0) < D):
+    if _rows_cross(B, T, out.stride(0), out.stride(1), D):
         raise ValueError(f"out: rows overlap, strides {out.stride()}")
     same = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
     if any(_rows_meet(out, t) for t in operands) or (not same and _rows_meet(out, query)):

@@ -43,3 +43,36 @@ def test_pools_that_something_follows(name, which):
         call(*other(leaf.detach().as_subclass(_Marked)))
     with pytest.raises(RuntimeError, match="HIP device"):
         call(*pools)
+
+
+# strides of out [3, 2, 64] and whether rows of it meet
+@pytest.mark.parametrize("strides,meet", [
+    ((128, 64, 1), False), ((64, 192, 1), False), ((64, 64, 1), True), ((64, 128, 1), True), ((128, 128, 1), True), ((192, 64, 1), False),
+    ((128, 320, 1), False), ((64, 136, 1), True), ((128, 192, 1), False), ((72, 64, 1), True), ((256, 72, 1), False),
+])
+def test_outputs_whose_rows_meet(strides, meet):
+    cells = torch.zeros(3, 2, 64)
+    idx = torch.arange(3)[:, None, None] * strides[0] + torch.arange(2)[None, :, None] * strides[1] + torch.arange(64)
+    assert (idx.unique().numel() < cells.numel()) == meet
+    out = torch.zeros(2000).as_strided((3, 2, 64), strides)
+    call = lambda: ops._head_out("chunk_attn", out, torch.zeros(3, 2, 64), out.device, [])  # noqa: E731
+    if meet:
+        with pytest.raises(ValueError, match="rows overlap"):
+            call()
+    else:
+        assert call() is out
+
+
+def test_outputs_of_many_rows():
+    """Neither stride is a multiple of the other's rows: still told apart."""
+    query = torch.zeros(5, 7, 64)
+    for sb in range(64, 1200, 64):
+        for st in range(64, 1200, 64):
+            out = torch.zeros(20000).as_strided((5, 7, 64), (sb, st, 1))
+            at = (torch.arange(5)[:, None] * sb + torch.arange(7) * st).flatten()
+            meet = at.unique().numel() < 35
+            try:
+                ops._head_out("cross_attn", out, query, out.device, [])
+                assert not meet, (sb, st)
+            except ValueError:
+                assert meet, (sb, st)
