@@ -1069,7 +1069,7 @@ int pk_qk_norm_append(const pk_qk_norm_append_args* args, void* stream);
  * accumulation and softmax.  What a token gets depends on the keys and values that it sees
  * alone, also where others are infinite or NaN.
  * query, out: [batch][chunk][num_heads * head_dim]; element strides (b, t), rows 16-byte aligned
- * with unit inner stride; out may be query, and overlaps nothing else.  scale: > 0 and finite.  head_dim 64 or
+ * with unit inner stride; out may be query, and overlaps nothing else.  scale: > 0, below 2^127.4.  head_dim 64 or
  * 128.  pages.max_pages holds any window of left + chunk positions: (left + chunk + page_size - 2) /
  * page_size + 1 <= max_pages; pages of up to 2^20 frames.  lengths: int32 [batch].
  * workspace: pk_attn_workspace_bytes(dtype, batch, chunk, num_heads, kv_heads, head_dim,

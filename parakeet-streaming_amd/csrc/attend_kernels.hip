@@ -1439,6 +1439,8 @@ int norm_append(const pk_qk_norm_append_args* a, hipStream_t s) {
   return check_launch(what);
 }
 
+constexpr float kLog2E = 1.44269504088896341f;
+
 // What both attentions ask of a call.
 int attend_ok(const char* what, int batch, int chunk, int heads, int kv_heads, int head_dim, float scale) {
   if (head_dim != 64 && head_dim != 128) return fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (built: 64, 128)", what, head_dim);
@@ -1446,7 +1448,7 @@ int attend_ok(const char* what, int batch, int chunk, int heads, int kv_heads, i
     return fail(PK_ERR_INVALID, "%s: need batch and chunk >= 0 and whole groups of query heads (got %d, %d, %d over %d)", what, batch, chunk, heads,
                 kv_heads);
   if ((int64_t)batch * chunk * heads >= (int64_t{1} << 31)) return fail(PK_ERR_INVALID, "%s: 2^31 rows or more", what);
-  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(PK_ERR_INVALID, "%s: scale must be > 0 and finite", what);
+  if (!(scale > 0.f) || !std::isfinite(scale * kLog2E)) return fail(PK_ERR_INVALID, "%s: scale must be > 0 and finite, times log2(e) too", what);
   return PK_OK;
 }
 
@@ -1574,7 +1576,7 @@ int chunk_attn(const pk_chunk_attn_args* a, hipStream_t s) {
   p.Hq = a->num_heads;
   p.Hkv = L.d_model / a->head_dim;
   p.left = a->left;
-  p.scale = a->scale * 1.44269504088896341f;
+  p.scale = a->scale * kLog2E;
   return attend<ST, true>(what, p, a->dtype, a->head_dim, a->left + a->chunk, a->workspace, a->device, s);
 }
 
@@ -1613,7 +1615,7 @@ int cross_attn(const pk_cross_attn_args* a, hipStream_t s) {
   p.Hq = a->num_heads;
   p.Hkv = a->kv_heads;
   p.states = a->states;
-  p.scale = a->scale * 1.44269504088896341f;
+  p.scale = a->scale * kLog2E;
   return attend<ST, false>(what, p, a->dtype, a->head_dim, a->states, a->workspace, a->device, s);
 }
 

@@ -1,5 +1,5 @@
 """What a text decoder's calls refuse, on the CPU: pools that something follows, outputs whose rows meet, scales past
-fp32, slots past 32 bits."""
+fp32."""
 
 import ctypes
 
@@ -8,7 +8,6 @@ import torch
 from torch.autograd import forward_ad
 
 from parakeet_amd import _lib, ops
-from parakeet_amd.pool import DevicePagePool
 
 
 class _Marked(torch.Tensor):
@@ -76,3 +75,22 @@ def test_outputs_of_many_rows():
                 assert not meet, (sb, st)
             except ValueError:
                 assert meet, (sb, st)
+
+
+@pytest.mark.parametrize("name,make", [("pk_chunk_attn", _lib.ChunkAttnArgs), ("pk_cross_attn", _lib.CrossAttnArgs)])
+@pytest.mark.parametrize("scale,ok", [(2.0e38, True), (2.4e38, False), (3.4e38, False), (1e-45, True)])
+def test_scales_at_the_ends_of_fp32(name, make, scale, ok):
+    """Scores are counted in powers of two: the scale times log2 e has to be finite, too. An empty batch asks no more."""
+    memory = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(memory) + 15 & ~15
+    a = make()
+    a.device, a.batch, a.chunk, a.num_heads, a.head_dim, a.scale = -1, 0, 1, 1, 64, scale
+    if make is _lib.ChunkAttnArgs:
+        L = a.pages
+        L.k_pool = L.v_pool = L.rows = at
+        L.num_layers, L.num_pages, L.page_size, L.d_model, L.rows_stride, L.max_pages = 1, 1, 16, 64, 2, 1
+    else:
+        a.kv_heads, a.states = 1, 1
+    rc = getattr(_lib.lib(), name)(ctypes.byref(a), None)
+    assert rc == (_lib.PK_OK if ok else _lib.PK_ERR_INVALID), _lib.last_error()
+    assert ok or "scale" in _lib.last_error()
