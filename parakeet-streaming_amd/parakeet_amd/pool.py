@@ -180,7 +180,7 @@ class DevicePagePool:
         tensor is taken as it is (``ops.page_step`` leaves its bad entries out)."""
         if isinstance(slots, torch.Tensor) and slots.device.type == "cuda":
             return slots
-        s = np.ascontiguousarray(np.asarray(slots, dtype=np.int32).reshape(-1))
+        s = np.asarray(slots, dtype=np.int64).reshape(-1)
         if len(np.unique(s)) != len(s) or (len(s) and (s.min() < 0 or s.max() >= self.num_slots)):
             raise ValueError(f"slots must be distinct and in [0, {self.num_slots})")
         return self._upload(s)

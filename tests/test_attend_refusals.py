@@ -1,5 +1,5 @@
 """What a text decoder's calls refuse, on the CPU: pools that something follows, outputs whose rows meet, scales past
-fp32."""
+fp32, slots past 32 bits."""
 
 import ctypes
 
@@ -8,6 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from parakeet_amd import _lib, ops
+from parakeet_amd.pool import DevicePagePool
 
 
 class _Marked(torch.Tensor):
@@ -94,3 +95,10 @@ def test_scales_at_the_ends_of_fp32(name, make, scale, ok):
     rc = getattr(_lib.lib(), name)(ctypes.byref(a), None)
     assert rc == (_lib.PK_OK if ok else _lib.PK_ERR_INVALID), _lib.last_error()
     assert ok or "scale" in _lib.last_error()
+
+
+
+@pytest.mark.parametrize("src,dst", [([0], [2**32 + 1]), ([0], [-(2**32) + 1]), ([2**32], [1])])
+def test_slots_past_32_bits(src, dst):
+    with pytest.raises(ValueError, match="slots must be"):
+        DevicePagePool(4, 16, 70, 2, "cpu").fork(src, dst)
