@@ -97,7 +97,6 @@ def test_scales_at_the_ends_of_fp32(name, make, scale, ok):
     assert ok or "scale" in _lib.last_error()
 
 
-
 @pytest.mark.parametrize("src,dst", [([0], [2**32 + 1]), ([0], [-(2**32) + 1]), ([2**32], [1])])
 def test_slots_past_32_bits(src, dst):
     with pytest.raises(ValueError, match="slots must be"):
