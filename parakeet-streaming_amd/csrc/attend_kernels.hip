@@ -462,17 +462,16 @@ __device__ static inline KeysOf keys_of(const AttendK<ST>& p, const StreamOf& s,
   return k;
 }
 
-// Whether a row that sees keys lo .. hi and whose maximum is none all the same has met a key, in tiles that its wave takes
-// (every N-th of the split's, from number `first` on): its scores were -inf then. Rare, so looked up when the tiles are done.
-template <typename ST, bool PAGED, int KT, int N>
-__device__ static inline bool has_met(const AttendK<ST>& p, int b, const KeysOf& keys, int first, int lo, int hi, float m) {
-  const int a = max(lo / KT, keys.t0), last = min(hi / KT, keys.t1 - 1);
-  const bool met = m == kNone && lo <= hi && a + ((first - (a - keys.t0)) & (N - 1)) <= last;
+// Whether a row that sees keys lo .. hi and whose maximum is none all the same has met a key in its split: the scores were
+// -inf then. Rare, so it is looked up when all is done.
+template <typename ST, bool PAGED, int KT>
+__device__ static inline bool has_met(const AttendK<ST>& p, int b, const KeysOf& keys, int lo, int hi, bool none) {
+  const int from = max(lo, keys.t0 * KT), to = min(hi, keys.t1 * KT - 1);
+  const bool met = none && from <= to;
   if constexpr (!PAGED) return met;
   if (!__any(met)) return false;
   // of the pages that the split meets, whether there is one with a key of the row
   const int32_t* const ring = p.rows + b * p.rows_stride + 1;
-  const int from = max(lo, keys.t0 * KT), to = min(hi, keys.t1 * KT - 1);
   auto page_of = [&](int d) { return (int)(((uint32_t)keys.k0 + (uint32_t)d) >> p.page_shift); };
   const int page0 = page_of(max(keys.lo, keys.t0 * KT)), pages = page_of(min(keys.hi, keys.t1 * KT - 1)) - page0 + 1;
   uint64_t any = 0;
@@ -488,10 +487,11 @@ __device__ static inline bool has_met(const AttendK<ST>& p, int b, const KeysOf&
 // The end of a workgroup's rows: sums over the waves' parts of the keys (in LDS, scaled to their largest
 // maximum; ml: each part's own maximum and sum of weights), the quotient, or the split's part.
 // WAVES parts of [rows][HD + 4] floats at `sums`.
-template <typename ST, int HD, bool PAGED, int ROWS, int WAVES, int THREADS>
-__device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, int KT, const float* sums,
+template <typename ST, int HD, bool PAGED, int ROWS, int WAVES, int THREADS, int KT>
+__device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, const float* sums,
                                          const float2* ml, uint32_t* bad, float* qs) {
   constexpr int VEC = 8, PER = HD / VEC, STRIDE = HD + 4, N = (ROWS * PER + THREADS - 1) / THREADS;
+  static_assert(ROWS * PER % 64 == 0, "a wave has rows in all lanes or in none");
   const bool check = PAGED && p.T > 1;
   if (check) {
     for (int i = threadIdx.x; i < (ROWS + 31) / 32; i += THREADS) bad[i] = 0;
@@ -507,6 +507,12 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) m[y] = fmaxf(m[y], ml[w * ROWS + r].x);
     const float base = m[y] == kNone ? 0.f : m[y];
+    if (__builtin_expect(keys.t0 < keys.t1 && __any(m[y] == kNone && it.row0 + r < p.R), 0)) {
+      const int i = min(it.row0 + r, p.R - 1) / p.G;
+      const int2 seen = seen_by<ST, PAGED>(p, s, i);
+      const bool none = m[y] == kNone && it.row0 + r < p.R && i < s.n;
+      if (has_met<ST, PAGED, KT>(p, it.b, keys, seen.x - keys.k0, seen.y - keys.k0, none)) m[y] = kLeast;
+    }
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) l[y] = fmaf(ml[w * ROWS + r].y, __builtin_amdgcn_exp2f(ml[w * ROWS + r].x - base), l[y]);
     float t = l[y];
@@ -829,7 +835,6 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
     l[a] = sum_of_groups(l[a]);
-    if (has_met<ST, PAGED, KT, NW>(p, it.b, keys, wave, lo[a], live[a] ? hi[a] : -1, m[a])) m[a] = kLeast;
     if (!live[a]) {
       m[a] = kNone;
       l[a] = 0.f;
@@ -849,7 +854,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
       *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = live[a] ? o[a][n] * f : f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW>(p, it, s, keys, KT, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW, KT>(p, it, s, keys, sums, ml, bad, qs);
 }
 
 // ---- many rows
@@ -1031,20 +1036,26 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     };
     // Pages of the split's keys that are not there (rare): the hardware's zeros would weigh as scores of 0, so their
     // 16 keys are taken out of each tile, by the ring again. Whether there are any is found while the first tiles are on
-    // their way; where there are none, that is all it costs (the prompts above: 69.4 us without it, 69.6 with).
+    // their way, by entries that are asked for before them, and sends each tile by way of the masks then: without absent pages
+    // the prompts above take 65.3 us, 65.0 without all of this (a loop that looks here, 65.7; a test of its own in each turn, 65.9).
+    constexpr int LOOK = PAGED ? 4 : 1;
+    int32_t look[LOOK];
+    const int page0 = PAGED ? (int)(((uint32_t)keys.k0 + (uint32_t)max(keys.lo, keys.t0 * KT)) >> p.page_shift) : 0;
+    const int pages = PAGED ? (int)(((uint32_t)keys.k0 + (uint32_t)min(keys.hi, keys.t1 * KT - 1)) >> p.page_shift) - page0 + 1 : 0;
+    auto entry_of = [&](int i) { return (uint32_t)(page0 + min(i, pages - 1)) % (uint32_t)p.max_pages; };
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int u = 0; u < LOOK; ++u) look[u] = ring[entry_of(64 * u + lane)];
+    }
     bool holes = false;  // wave-uniform
     auto find_holes = [&]() {
       if constexpr (PAGED) {
-        const uint32_t page0 = ((uint32_t)keys.k0 + (uint32_t)max(keys.lo, keys.t0 * KT)) >> p.page_shift;
-        const uint32_t n = (((uint32_t)keys.k0 + (uint32_t)min(keys.hi, keys.t1 * KT - 1)) >> p.page_shift) - page0 + 1;
-        uint32_t entry = (page0 + lane) % (uint32_t)p.max_pages;
         bool away = false;
-        for (uint32_t i = lane; i < n; i += 64) {
-          away = away || (uint32_t)ring[entry] >= (uint32_t)p.num_pages;
-          entry += 64;
-          if (entry >= (uint32_t)p.max_pages) entry %= (uint32_t)p.max_pages;
-        }
+#pragma unroll
+        for (int u = 0; u < LOOK; ++u) away |= (uint32_t)look[u] >= (uint32_t)p.num_pages;
+        for (int i = 64 * LOOK + lane; i < pages; i += 64) away |= (uint32_t)ring[entry_of(i)] >= (uint32_t)p.num_pages;
         holes = __any(away);
+        if (holes) all_hi = -1;  // each tile goes where keys are taken out
       }
     };
     // whether keys d .. d + 15 (wave-uniform, d a multiple of 16) have a page; those that nobody sees have one
@@ -1128,13 +1139,13 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
               if (none || from + (32 * u + 8 * j + e) > span) x[u][4 * j + e] = kNone;
             __builtin_amdgcn_sched_barrier(0);  // few conditions at a time in scalar registers
           }
-      }
-      if (holes) {  // keys 16 y .. 16 y + 15 of the tile are registers 8 (y & 1) .. 8 (y & 1) + 7 of x[y / 2]
+        if (holes) {  // keys 16 y .. 16 y + 15 of the tile are registers 8 (y & 1) .. 8 (y & 1) + 7 of x[y / 2]
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          if (there(d0 + 16 * y)) continue;
+          for (int y = 0; y < 4; ++y) {
+            if (there(d0 + 16 * y)) continue;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[y >> 1][8 * (y & 1) + e] = kNone;
+            for (int e = 0; e < 8; ++e) x[y >> 1][8 * (y & 1) + e] = kNone;
+          }
         }
       }
       float top = kNone;
@@ -1188,9 +1199,9 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     at = place_of(tile(1), page_of(tile(1)));  // of the tile whose V is asked for next
     ask(false, tile(1), at, 1);
     int page = page_of(tile(2));
-    find_holes();
     if (kg == 1) meet();
     wait_vm<0>();
+    find_holes();
     auto turn_of = [&](int turn, auto parity) {
       constexpr int b = decltype(parity)::value;
       wait_vm<2 * LOADS>();
@@ -1221,7 +1232,6 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  if (has_met<ST, PAGED, KT, KG>(p, it.b, keys, kg, lo, hi, m)) m = kLeast;
   if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{m, l};
   __syncthreads();  // and every wave is done with the tiles
   float* const sums = reinterpret_cast<float*>(smem);
@@ -1237,7 +1247,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
       *reinterpret_cast<f32x4_t*>(sums + (kg * ROWS + 32 * wv + r32) * STRIDE + 32 * n + 8 * j + 4 * h) = v * f;
     }
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG>(p, it, s, keys, KT, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG, KT>(p, it, s, keys, sums, ml, bad, qs);
 }
 
 // where a row of a join goes
