@@ -920,8 +920,10 @@ __device__ static inline void stage_bytes(const u32x4 r, uint32_t lds, const uin
 // A group stages its tile of K and V in LDS, a tile ahead, straight from memory. As in
 // attend_few_kernel products are transposed, so that a lane has one query; the weights are rounded once to
 // the type for the second product (half a step of it relative to each; fp16: those below 2^-23 of the largest to 2^-34
-// of it). Bound by the matrix cores and by the exp2 and conversions of the weights, which the other group's products hide where there are two: 4 x 512 tokens of 16 heads
-// over 4 of 128 behind 3500 earlier ones, 58.7 GFLOP, 66 us (890 TFLOP/s); with one tile of registers between
+// of it; a low part as attend_few_kernel's would be half as many matrix instructions again, and there are no registers
+// for it). 4 x 512 tokens of 16 heads over 4 of 128 behind 3500 earlier ones, 58.7 GFLOP: 66 us (890 TFLOP/s). Bound by no
+// one thing: of 68.4 us, 61.6 are left without the weights (exp2, conversions), 63.1 without the operands' reads from LDS, 53.7
+// without both, where a large product's rate is 41.5; the other group's products hide a part of each. With one tile of registers between
 // the products 119, staged straight to LDS 113, two groups in turn 81, a wave's loads from one page 73. One group is enough
 // where there are 512 workgroups, two of which are on a CU.
 template <typename ST, int HD, bool PAGED, int KG>
@@ -1428,8 +1430,9 @@ int norm_append(const pk_qk_norm_append_args* a, hipStream_t s) {
   DeviceGuard dg(a->device);
   if (!dg.ok) return fail(PK_ERR_HIP, "%s: cannot select device %d", what, a->device);
   const int64_t total = (int64_t)p.B * p.T;
-  // few tokens: one a workgroup, for the shortest chain; many: 4 or 8, whose loads go together (15.6 K tokens of 20 heads
-  // of 128 in bf16, stored through the caches: 32.5 us with 4, 30.7 with 8)
+  // few tokens: one a workgroup, for the shortest chain; many: 4 or 8, whose loads go together. 20 heads of 128 in bf16, us with
+  // 1 / 4 / 8: 1024 tokens 5.8 / 7.1 / 10.0, 1536 7.3 / 8.8 / 10.3, 2048 9.9 / 9.6 / 11.0, 4096 14.4 / 12.6 / 12.9, 8192
+  // 22.8 / 20.2 / 17.6, 16384 51.2 / 42.1 / 31.7
   const int tok = total <= 1024 ? 1 : total <= 8192 ? 4 : 8;
   const dim3 grid((unsigned)((total + tok - 1) / tok));
   if ((int64_t)grid.x >= (1 << 24)) return fail(PK_ERR_UNSUPPORTED, "%s: %lld tokens in one call (built: fewer than 2^27)", what, (long long)total);
@@ -1471,6 +1474,10 @@ struct AttendCut {
 AttendCut attend_cut(int dtype, int batch, int chunk, int heads, int kv_heads, int keys, bool narrow) {
   AttendCut c;
   const int64_t R = (int64_t)chunk * (heads / kv_heads), units = (int64_t)batch * kv_heads;
+  // From 33 rows on 128 a workgroup in 16 bits, for batches: 64 x 33 rows of 8 heads of 128 over 1500 states 82.8 us, 110.7
+  // with 32; 64 x 48 of 64 over the same 43.4 and 50.8; 64 x 36 of 4 heads of 128 over 3009 tokens 81.3 and 84.0. Few streams of up to
+  // 64 rows pay for it, whose keys it splits less: 4 x 48 rows of 8 heads of 64 over 1048 tokens 21.3 us, 13.8 with 32; 32 x 48
+  // 28.6 and 22.6; 8 x 36 of 4 heads of 128 over 3009 26.2 and 24.7; 32 x 96 24.3 and 27.5.
   c.rows = R <= 16 ? 16 : R <= 32 || dtype == PK_DTYPE_F32 || narrow ? 32 : 128;
   c.key_groups = c.rows == 128 && units * ((R + 127) / 128) < 512 ? 2 : 1;
   c.row_tiles = (int)((R + c.rows - 1) / c.rows);

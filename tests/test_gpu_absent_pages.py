@@ -101,3 +101,18 @@ def test_rows_made_again(cuda, dtype, T):
     assert not torch.isfinite(out[0, sees]).any()
     v[0][at - first[0]] = 0  # of no row that is compared
     _check(out, q, seen, k, v, heads, 1, hd, dtype, rows=[~sees])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gone", ["middle", "last"])
+def test_absent_pages_far_into_a_whole_window(cuda, dtype, gone):
+    """A window of hundreds of pages that one workgroup takes whole, since there are many streams (all on the same pages)."""
+    T, hd = 40, 64
+    _, q, pages, seen, k, v, _ = _absent(cuda, dtype, hd, 1, 1, 16, T, 9000, [20000], [gone])
+    n = 192
+    many = torch.randn(n, T, hd, generator=torch.Generator().manual_seed(1)).to(dtype)
+    many[-1] = q[0]
+    there = ops.PagedKV(pages.k_pool, pages.v_pool, pages.rows.repeat(n, 1), pages.max_pages)
+    out = ops.chunk_attn(many.to(cuda), there, 1, num_heads=1, left=9000).cpu()
+    for b in (0, 77, n - 1):
+        _check(out[b : b + 1], many[b : b + 1], seen, k, v, 1, 1, hd, dtype)
