@@ -230,6 +230,16 @@ __device__ static inline float quotient(float m, float l) { return l != 0.f ? 1.
 template <typename ST>
 constexpr float kTop = __is_same(ST, _Float16) ? 15.f : 0.f;
 
+// fp32's steps reach 1/2 at kFar: past it 2^(a score's exact product with the scale - a rounded maximum) may be anything, up to
+// infinity. Rows with such maxima are made again from scores that are rounded as their maximum is (attend_row), by parts
+// whose sum is NaN.
+constexpr float kFar = 4194304.f;
+__device__ static inline float2 part_of(float m, float l) { return float2{m, m != kNone && fabsf(m) >= kFar ? __builtin_nanf("") : l}; }
+__device__ static inline float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // what a workgroup needs of a stream
 struct StreamOf {
   int32_t A;     // position of token 0 (pages)
@@ -298,7 +308,7 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d = fmaf(x[e], q[c + e], d);
       }
-      s = d * p.scale;
+      s = rounded_product(d, p.scale);
     }
     float top = s;
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -489,18 +499,17 @@ __device__ static inline bool has_met(const AttendK<ST>& p, int b, const KeysOf&
 // WAVES parts of [rows][HD + 4] floats at `sums`.
 template <typename ST, int HD, bool PAGED, int ROWS, int WAVES, int THREADS, int KT>
 __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it, const StreamOf& s, const KeysOf& keys, const float* sums,
-                                         const float2* ml, uint32_t* bad, float* qs) {
+                                         const float2* ml, float* qs) {
   constexpr int VEC = 8, PER = HD / VEC, STRIDE = HD + 4, N = (ROWS * PER + THREADS - 1) / THREADS;
   static_assert(ROWS * PER % 64 == 0, "a wave has rows in all lanes or in none");
-  const bool check = PAGED && p.T > 1;
-  if (check) {
-    for (int i = threadIdx.x; i < (ROWS + 31) / 32; i += THREADS) bad[i] = 0;
-    __syncthreads();
-  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr uint64_t kRow = (1ull << PER) - 1;  // a row is PER neighbouring lanes
   float o[N][VEC], m[N], l[N];
+  uint64_t bad[N];
 #pragma unroll
   for (int y = 0; y < N; ++y) {
     const int x = y * THREADS + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC;
+    bad[y] = 0;
     if (r >= ROWS) continue;
     m[y] = kNone;
     l[y] = 0.f;
@@ -523,14 +532,13 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
       for (int w = 0; w < WAVES; ++w) o[y][e] += sums[(w * ROWS + r) * STRIDE + c + e];
       t = fmaf(o[y][e], 0.f, t);
     }
-    if (check && it.row0 + r < p.R && !(fabsf(t) < __builtin_inff())) atomicOr(&bad[r >> 5], 1u << (r & 31));
+    bad[y] = __ballot(it.row0 + r < p.R && !(fabsf(t) < __builtin_inff()));
   }
-  if (check) __syncthreads();
 #pragma unroll
   for (int y = 0; y < N; ++y) {
     const int x = y * THREADS + threadIdx.x, r = x / PER, c = (x - r * PER) * VEC, row = it.row0 + r;
     if (r >= ROWS || row >= p.R) continue;
-    if (check && (bad[r >> 5] >> (r & 31) & 1)) continue;
+    if (bad[y] >> (lane & -PER) & kRow) continue;
     const int i = row / p.G, h = it.hk * p.G + row - i * p.G;
     if (p.splits > 1) {
       const int64_t at = (((int64_t)it.b * p.Hkv + it.hk) * p.R + row) * p.splits + it.split;
@@ -547,14 +555,22 @@ __device__ static inline void attend_end(const AttendK<ST>& p, const ItemOf& it,
       if constexpr (sizeof(ST) == 4) st16(to + 4, Tr<ST>::pack(o[y] + 4));
     }
   }
-  if (!check) return;
-  // A row that is not finite may have met, as 0 times it, a value that it does not see: it is
-  // made again from the keys that it sees, one by one (rare). It is not written yet: out may be
-  // the query that is read again.
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int r = wave; r < ROWS; r += THREADS / 64) {
-    if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
-    const int row = it.row0 + r, i = row / p.G, h = it.hk * p.G + row % p.G;
+  // A row that is not finite may have met, as 0 times it, a value that it does not see, or scores past kFar: it is made again
+  // from the keys that it sees, one by one (rare). It is not written yet: out may be the query that is read again.
+  uint64_t some = bad[0];
+#pragma unroll
+  for (int y = 1; y < N; ++y) some |= bad[y];
+  if (__builtin_expect(some == 0, 1)) return;
+  for (int z = 0; z < N * (64 / PER); ++z) {
+    uint64_t rows = bad[0];
+#pragma unroll
+    for (int y = 1; y < N; ++y) rows = z / (64 / PER) == y ? bad[y] : rows;
+    if (rows == 0) {  // wave-uniform, as rows is: on to the next 64 / PER rows
+      z |= 64 / PER - 1;
+      continue;
+    }
+    if (!(rows >> (z % (64 / PER) * PER) & kRow)) continue;
+    const int r = (z / (64 / PER) * THREADS + wave * 64) / PER + z % (64 / PER), row = it.row0 + r, i = row / p.G, h = it.hk * p.G + row % p.G;
     const ST* const q = p.q + it.b * p.q_sb + i * p.q_st + (int64_t)h * HD;
     for (int c = lane; c < HD; c += 64) qs[wave * HD + c] = from_st(q[c]);
     wave_lds_sync();
@@ -604,8 +620,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
   constexpr int kStage = NW * KT * VROW, kSums = NW * ROWS * STRIDE * 4;
   __shared__ __align__(16) unsigned char smem[kStage > kSums ? kStage : kSums];
   __shared__ float2 ml[NW * ROWS];
-  __shared__ uint32_t bad[(ROWS + 31) / 32];
-  __shared__ float qs[PAGED ? NW * HD : 1];
+  __shared__ float qs[NW * HD];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   StreamOf s;
   const ItemOf it = item_of<ST, PAGED>(p, ROWS, s);
@@ -839,7 +854,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
       m[a] = kNone;
       l[a] = 0.f;
     }
-    if (g == 0) ml[wave * ROWS + 16 * a + r16] = float2{m[a], l[a]};
+    if (g == 0) ml[wave * ROWS + 16 * a + r16] = part_of(m[a], l[a]);
   }
   __syncthreads();  // and every wave is done with its staged rows
   float* const sums = reinterpret_cast<float*>(smem);
@@ -854,7 +869,7 @@ __global__ void __launch_bounds__(256, 2) attend_few_kernel(const AttendK<ST> p)
       *reinterpret_cast<f32x4_t*>(sums + (wave * ROWS + 16 * a + r16) * STRIDE + 16 * n + 4 * g) = live[a] ? o[a][n] * f : f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW, KT>(p, it, s, keys, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, NW, 64 * NW, KT>(p, it, s, keys, sums, ml, qs);
 }
 
 // ---- many rows
@@ -934,8 +949,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
   constexpr int kStage = KG * 2 * kBuf;
   __shared__ __align__(16) unsigned char smem[kStage > kSums ? kStage : kSums];
   __shared__ float2 ml[KG * ROWS];
-  __shared__ uint32_t bad[(ROWS + 31) / 32];
-  __shared__ float qs[PAGED ? 4 * KG * HD : 1];
+  __shared__ float qs[4 * KG * HD];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, wv = wave & 3, kg = wave >> 2;
   StreamOf s;
   const ItemOf it = item_of<ST, PAGED>(p, ROWS, s);
@@ -1039,7 +1053,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     // Pages of the split's keys that are not there (rare): the hardware's zeros would weigh as scores of 0, so their
     // 16 keys are taken out of each tile, by the ring again. Whether there are any is found while the first tiles are on
     // their way, by entries that are asked for before them, and sends each tile by way of the masks then: without absent pages
-    // the prompts above take 65.3 us, 65.0 without all of this (a loop that looks here, 65.7; a test of its own in each turn, 65.9).
+    // the prompts above take 0.3 us longer than without all of this (a loop that looks here 0.7, a test of its own in each turn 0.9).
     constexpr int LOOK = PAGED ? 4 : 1;
     int32_t look[LOOK];
     const int page0 = PAGED ? (int)(((uint32_t)keys.k0 + (uint32_t)max(keys.lo, keys.t0 * KT)) >> p.page_shift) : 0;
@@ -1234,7 +1248,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  if (h == 0) ml[kg * ROWS + 32 * wv + r32] = float2{m, l};
+  if (h == 0) ml[kg * ROWS + 32 * wv + r32] = part_of(m, l);
   __syncthreads();  // and every wave is done with the tiles
   float* const sums = reinterpret_cast<float*>(smem);
   float top = kNone;
@@ -1249,7 +1263,7 @@ __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<
       *reinterpret_cast<f32x4_t*>(sums + (kg * ROWS + 32 * wv + r32) * STRIDE + 32 * n + 8 * j + 4 * h) = v * f;
     }
   __syncthreads();
-  attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG, KT>(p, it, s, keys, sums, ml, bad, qs);
+  attend_end<ST, HD, PAGED, ROWS, KG, 256 * KG, KT>(p, it, s, keys, sums, ml, qs);
 }
 
 // where a row of a join goes

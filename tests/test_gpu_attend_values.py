@@ -1,4 +1,5 @@
-"""Attention over scores at the ends of a type's range: one key far above a long tail of others, scores of -inf."""
+"""Attention over scores at the ends of a type's range: one key far above a long tail of others, scores of -inf, scores
+of which fp32 knows large steps only."""
 
 import math
 
@@ -109,3 +110,64 @@ def test_scores_of_minus_infinity(cuda, dtype, n, T):
         v[-1] = math.inf
         tokens, _ = both(k)
         assert torch.isnan(tokens[:m]).all() and (tokens[m:] == 0).all()
+
+
+# fp16 ends at 2^16, and so do its products at 2^32
+@pytest.mark.parametrize("dtype,bits", [(t, b) for b in (12, 20, 24, 25, 27, 29, 30, 32, 34, 36, 60, 100) for t in (F32, F16, BF16) if t is not F16 or b <= 30])
+@pytest.mark.parametrize("n", [60, 3000])
+def test_scores_far_past_fp32s_steps(cuda, dtype, bits, n):
+    """Scores of up to 2^bits, of which fp32 knows steps of 2^(bits - 24) alone: the largest has the whole weight, two
+    that are equal have half of it each, whatever their sign. All products are exact in fp32, the others 2^(bits - 7) lower.
+
+    Halves are exact but for the output's rounding, u, the weights' and the sum's, 2 u, and fp32's: 2^-20."""
+    hd, heads, u = 64, 2, HALF[dtype]
+    g = torch.Generator().manual_seed(bits)
+    v = torch.randn(n, heads * hd, generator=g).to(dtype)
+    qd = 2.0 ** (bits // 2)
+    top, low = 2.0 ** (bits - bits // 2), 2.0 ** (bits - bits // 2) - 2.0 ** (bits - bits // 2 - 7)
+    for sign in (1, -1):
+        for best in ([0], [n - 1], [n // 2, n - 2], [3, n // 3]):
+            k = torch.zeros(n, heads * hd).to(dtype)
+            k[:, ::hd] = low if sign == 1 else -top
+            k[best, ::hd] = top if sign == 1 else -low
+            want = v[best].double().mean(0)
+            tol = (3 * u + 2.0**-20) * v[best].double().abs().mean(0) + 2.0**-30
+            for T in (1, 40):
+                q = torch.zeros(1, T, heads * hd).to(dtype)
+                q[..., ::hd] = qd
+                print(f"[far] {dtype} bits {bits} n {n} sign {sign} best {best} T {T}", flush=True)
+                out = ops.cross_attn(q.to(cuda), k[None].to(cuda), v[None].to(cuda), num_heads=heads, scale=1.0).double().cpu()
+                assert ((out - want).abs() <= tol).all(), f"states: {(out - want).abs().max()}"
+                more = T - 1
+                other = best[0] - 1 if best[0] else 1  # a key that is not one of the best: the step's own tokens have it, too
+                pages = _paged(cuda, torch.cat([k, k[other].expand(more, -1)]), torch.cat([v, v[:1].expand(more, -1)]), 16, T)
+                out = ops.chunk_attn(q.to(cuda), pages, 0, num_heads=heads, scale=1.0, left=n + T).double().cpu()
+                assert ((out - want).abs() <= tol).all(), f"tokens: {(out - want).abs().max()}"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [60, 700, 3000])
+@pytest.mark.parametrize("T", [1, 40])
+def test_scores_that_come_from_afar(cuda, dtype, n, T):
+    """A third of the keys, first, last or every third, score -2^30 (fp16) or -2^36, the others 0: the output is the others' mean.
+
+    Equal weights: the output's rounding, a weight's and the sum's, u each, fp32 sums over n keys in tiles of 16, 2^-18 as above."""
+    hd, heads, u = 64, 2, HALF[dtype]
+    g = torch.Generator().manual_seed(n)
+    v = torch.randn(n, heads * hd, generator=g).to(dtype)
+    q = torch.zeros(1, T, heads * hd).to(dtype)
+    q[..., ::hd] = 2.0 ** (15 if dtype is F16 else 18)
+    for away in (slice(0, n // 3), slice(n - n // 3, n), slice(0, n, 3)):
+        k = torch.zeros(n, heads * hd).to(dtype)
+        k[away, ::hd] = -q[0, 0, 0]
+        near = torch.ones(n, dtype=torch.bool)
+        near[away] = False
+        want = v[near].double().mean(0)
+        tol = (3 * u + 2.0**-18 + n / 16 * 2.0**-24) * v[near].double().abs().mean(0)
+        print(f"[afar] {dtype} n {n} T {T} away {away}", flush=True)
+        out = ops.cross_attn(q.to(cuda), k[None].to(cuda), v[None].to(cuda), num_heads=heads, scale=1.0).double().cpu()
+        assert ((out - want).abs() <= tol).all(), f"states: {((out - want).abs() / tol).max()}"
+        more = T - 1
+        kp, vp = torch.cat([k, -q[0, :more].abs()]), torch.cat([v, v[:1].expand(more, -1)])
+        out = ops.chunk_attn(q.to(cuda), _paged(cuda, kp, vp, 16, T), 0, num_heads=heads, scale=1.0, left=n + T).double().cpu()
+        assert ((out - want).abs() <= tol).all(), f"tokens: {((out - want).abs() / tol).max()}"
