@@ -935,11 +935,12 @@ __device__ static inline void stage_bytes(const u32x4 r, uint32_t lds, const uin
 // A group stages its tile of K and V in LDS, a tile ahead, straight from memory. As in
 // attend_few_kernel products are transposed, so that a lane has one query; the weights are rounded once to
 // the type for the second product (half a step of it relative to each; fp16: those below 2^-23 of the largest to 2^-34
-// of it; a low part as attend_few_kernel's would be half as many matrix instructions again, and there are no registers
-// for it). 4 x 512 tokens of 16 heads over 4 of 128 behind 3500 earlier ones, 58.7 GFLOP: 66 us (890 TFLOP/s). Bound by no
-// one thing: of 68.4 us, 61.6 are left without the weights (exp2, conversions), 63.1 without the operands' reads from LDS, 53.7
-// without both, where a large product's rate is 41.5; the other group's products hide a part of each. With one tile of registers between
-// the products 119, staged straight to LDS 113, two groups in turn 81, a wave's loads from one page 73. One group is enough
+// of it). A low part as attend_few_kernel's takes 85 us here instead of 65, for 1.66e-3 from the definition instead of 2.34e-3,
+// 1.65e-3 of which are the output's own rounding to bf16: within the type's half step, and not worth a third of the speed.
+// 4 x 512 tokens of 16 heads over 4 of 128 behind 3500 earlier ones, 58.7 GFLOP: 64 us (914 TFLOP/s). Bound by no one thing: of
+// 68.4 us (an earlier form of the end) 61.6 are left without the weights (exp2, conversions), 63.1 without the operands' reads
+// from LDS, 53.7 without both, where a large product's rate is 41.5; the other group's products hide a part of each. With one tile of
+// registers between the products 119, staged straight to LDS 113, two groups in turn 81, a wave's loads from one page 73. One group is enough
 // where there are 512 workgroups, two of which are on a CU.
 template <typename ST, int HD, bool PAGED, int KG>
 __global__ void __launch_bounds__(256 * KG, 2) attend_many_kernel(const AttendK<ST> p) {
