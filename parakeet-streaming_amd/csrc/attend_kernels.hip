@@ -298,6 +298,7 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
   for (int c = 0; c < HD / 64; ++c) acc[c] = 0.f;
   for (int d0 = 0; d0 < n; d0 += 64) {
     const int64_t at = d0 + lane < n ? key_at<ST, PAGED>(p, b, HD * E, h, first + d0 + lane, false) : -1;
+    const int64_t vat = PAGED || at < 0 ? at : key_at<ST, PAGED>(p, b, HD * E, h, first + d0 + lane, true);
     met = met || __any(at >= 0);
     float s = kNone;
     if (at >= 0) {
@@ -322,16 +323,35 @@ __device__ static inline void attend_row(const AttendK<ST>& p, int b, int h, con
     m = now;
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) acc[c] *= keep;
-    for (int u = 0; u < 64 && d0 + u < n; ++u) {
-      const float w = __shfl(e, u);
-      const int64_t va = key_at<ST, PAGED>(p, b, HD * E, h, first + d0 + u, true);
-      if (va < 0) continue;
+    if (l != l) {  // whatever follows
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const int col = lane + 64 * c;
-        acc[c] = fmaf(w, from_st(*reinterpret_cast<const ST*>(p.v + va + col / CB * step + col % CB * E)), acc[c]);
-      }
+      for (int c = 0; c < HD / 64; ++c) acc[c] = l;
+      break;
     }
+    // eight keys' values on their way at a time; of one that is not there, place 0's, which are not used
+    bool gone = true;
+    for (int u0 = 0; u0 < min(64, n - d0); u0 += 8) {
+      float x[8][HD / 64], w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int lo = __builtin_amdgcn_readlane((int)vat, u0 + u), hi = __builtin_amdgcn_readlane((int)(vat >> 32), u0 + u);
+        const int64_t va = (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+        w[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), u0 + u));
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+          const int col = lane + 64 * c;
+          const float y = from_st(*reinterpret_cast<const ST*>(p.v + max(va, (int64_t)0) + col / CB * step + col % CB * E));
+          x[u][c] = va < 0 ? 0.f : y;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) acc[c] = fmaf(w[u], x[u][c], acc[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) gone = gone && acc[c] != acc[c];
+    if (__all(gone)) break;
   }
   if (met) m = fmaxf(m, kLeast);
 }
